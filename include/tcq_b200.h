@@ -236,13 +236,80 @@ int tcq_chain(const void* acc, int acc_dtype, const float* s, const float* rs, c
 int tcq_rope(const uint16_t* x, uint16_t* out, const float* cos_t, const float* sin_t, int rows, int T, int heads, int D,
              int ldx, int ldo, void* stream);
 
+/* ------------------------------------------------------------------------------------------------ streaming memory
+ * Operators of a policy that keeps past frames (no counterpart in the reference, which recomputes its prefix for every
+ * action chunk): rotary positions with several axes, a paged key / value cache in 8 bits, and attention over it.
+ *
+ * Indices that only the device knows (positions, page numbers, lengths) are checked by the kernels: one out of range is
+ * replaced by the nearest valid one, nothing out of bounds is read or written, and tcq_device_error() reports flag 2. */
+
+/* Cosines and sines of a rotary embedding with 1 to 4 axes: cos_t / sin_t (positions, head_dim / 2) FP32; frequency j of a
+ * head belongs to the axis whose section holds j (section[0] frequencies on axis 0, then section[1] on axis 1, ...; they
+ * add up to head_dim / 2). pairs 0: element j turns with j + head_dim / 2 (half-split), 1: element 2 j with 2 j + 1. */
+typedef struct tcq_rope_plan {
+    const float* cos_t;
+    const float* sin_t;
+    int32_t positions, head_dim, axes, pairs;
+    int32_t section[4];
+} tcq_rope_plan;
+
+/* A key / value cache in 8 bits. A page is one block of TCQ_KV8_BLOCK tokens of one sequence: k (pages, kv_heads, 64,
+ * head_dim) int8, v (pages, kv_heads, head_dim, 64) int8 (values transposed, so that both operands of the attention's
+ * products run along their contraction), k_scale / v_scale (pages, kv_heads) FP32: a value is its integer times its
+ * block's scale. head_dim is 32, 48, 64, 80, 96 or 128; k and v are 16-byte aligned. A table (B, blocks) int32 names the
+ * page of each block of each sequence. */
+#define TCQ_KV8_BLOCK 64
+typedef struct tcq_kv8_cache {
+    int8_t* k;
+    int8_t* v;
+    float* k_scale;
+    float* v_scale;
+    int32_t pages, kv_heads, head_dim;
+} tcq_kv8_cache;
+
+/* out = rotary(x) for heads of plan->head_dim (even, at most 256): x (B, T, heads * head_dim) BF16 / F16 / F32 with strides
+ * x_sb (sequence) and x_st (token) in elements, out the same type with strides o_sb, o_st (out may be x). pos (axes, B, T)
+ * int32. Of a pair (a, b): a' = a c - b s, b' = a s + b c in FP32 with one rounding per operation and one to the type;
+ * inverse != 0 turns backwards (sin negated), which is also the gradient of the forward turn. */
+int tcq_rope_axes(const void* x, int dtype, int64_t x_sb, int64_t x_st, void* out, int64_t o_sb, int64_t o_st,
+                  const int32_t* pos, const tcq_rope_plan* plan, int B, int T, int heads, int inverse, void* stream);
+
+/* Write new tokens into the cache. k, v (B, T, kv_heads * head_dim) BF16 / F16 (both dtype), strides *_sb, *_st in elements
+ * (16-byte aligned rows); sequence b's tokens 0 .. count[b] - 1 (count NULL: T) become its tokens start[b] .. . With a
+ * plan, keys are first turned by pos (axes, B, T) in FP32 (no rounding to the input type in between). For the tokens of
+ * this call in one block and head, with amax over their finite values (infinities saturate, NaN is held as 0):
+ *   s = max(s_old, amax / 127), s_old = 0 when the call fills the block from its first token, inv = 1 / s;
+ *   q = clamp(rint(x * inv), -127, 127); if s > s_old the block's older tokens become rint(q * (s_old * inv));
+ *   s below 2^-120: the block is held as zeros with s = 0.
+ * Pages written by one call must be distinct. Tokens past the table's blocks are dropped (flag 2). */
+int tcq_kv8_append(const tcq_kv8_cache* cache, const void* k, int64_t k_sb, int64_t k_st, const void* v, int64_t v_sb,
+                   int64_t v_st, int dtype, const int32_t* table, int blocks, const int32_t* start, const int32_t* count,
+                   const int32_t* pos, const tcq_rope_plan* plan, int B, int T, void* stream);
+
+/* The values the cache stands for: tokens begin[b] .. begin[b] + T - 1 of each sequence as k, v (B, T, kv_heads *
+ * head_dim) of dtype (BF16 / F16 / F32; q * s in FP32, rounded once); zeros from token lens[b] on. */
+int tcq_kv8_read(const tcq_kv8_cache* cache, void* k, void* v, int dtype, const int32_t* table, int blocks,
+                 const int32_t* begin, const int32_t* lens, int B, int T, void* stream);
+
+/* Workspace of tcq_kv8_attention in bytes. Zero-filled before its first use; every call leaves it ready for the next. */
+size_t tcq_kv8_attention_workspace(int B, int T, int heads, int kv_heads, int head_dim, int blocks);
+
+/* out (B, T, heads * head_dim) = softmax(scale * q k^T) v over the cached tokens of each sequence. q BF16 / F16 with strides
+ * q_sb, q_st in elements (16-byte aligned rows), out contiguous, of q's type; query head h reads key head h / (heads /
+ * kv_heads). lens (B,): tokens in the cache, the new ones among them; count (B,) (NULL: T): queries of each sequence; query t
+ * sits at token lens[b] - count[b] + t and, with causal != 0, sees the tokens up to its own, else all lens[b]. Rows that see no
+ * token and rows past count[b] are zero. */
+int tcq_kv8_attention(const tcq_kv8_cache* cache, const void* q, int dtype, int64_t q_sb, int64_t q_st, void* out,
+                      const int32_t* table, int blocks, const int32_t* lens, const int32_t* count, int causal, float scale,
+                      int B, int T, int heads, void* workspace, size_t workspace_bytes, void* stream);
+
 /* Self-test of the failure path (no counterpart in the reference): one thread waits, through the same bounded wait the
  * tcgen05 kernels use, on a barrier that nothing arrives at; after limit_us (1 .. 1e6) microseconds the wait gives up,
  * raises device error flag 1 and the kernel returns. Nothing faults and the context stays usable. */
 int tcq_selftest_wait_expiry(unsigned limit_us, void* stream);
 
-/* Device error flags raised by bounded waits inside the kernels (1 = a pipeline wait expired and the kernel stopped
- * early). Synchronizes the current device. reset != 0 clears the flags. Returns -1 if the flags cannot be read. */
+/* Device error flags: 1 = a bounded pipeline wait expired and the kernel stopped early, 2 = a position, page number or
+ * length given to a streaming-memory operator was out of range (see there). Synchronizes the current device. reset != 0 clears the flags. Returns -1 if the flags cannot be read. */
 int tcq_device_error(int reset);
 
 #ifdef __cplusplus

@@ -14,6 +14,16 @@ P = ctypes.c_void_p
 I = ctypes.c_int
 SZ = ctypes.c_size_t
 F = ctypes.c_float
+L = ctypes.c_int64
+
+
+class RopePlan(ctypes.Structure):
+    _fields_ = [('cos_t', P), ('sin_t', P), ('positions', I), ('head_dim', I), ('axes', I), ('pairs', I), ('section', I * 4)]
+
+
+class Kv8Cache(ctypes.Structure):
+    _fields_ = [('k', P), ('v', P), ('k_scale', P), ('v_scale', P), ('pages', I), ('kv_heads', I), ('head_dim', I)]
+
 
 # name -> argument types (every function returns int, except where noted)
 SIGNATURES = {
@@ -47,10 +57,16 @@ SIGNATURES = {
     'tcq_add_norm': [P, P, P, P, P, P, I, P, P, I, I, F, I, I, I, P],
     'tcq_rope': [P, P, P, P, I, I, I, I, I, I, P],
     'tcq_chain': [P, I, P, P, P, P, I, I, P, P, P, P, P, P, I, P, P, I, I, F, I, P, P, P, P, I, I, I, P],
+    'tcq_rope_axes': [P, I, L, L, P, L, L, P, P, I, I, I, I, P],
+    'tcq_kv8_append': [P, P, L, L, P, L, L, I, P, I, P, P, P, P, I, I, P],
+    'tcq_kv8_read': [P, P, P, I, P, I, P, P, I, I, P],
+    'tcq_kv8_attention_workspace': [I, I, I, I, I, I],
+    'tcq_kv8_attention': [P, P, I, L, L, P, P, I, P, P, I, F, I, I, I, P, SZ, P],
     'tcq_selftest_wait_expiry': [ctypes.c_uint, P],
     'tcq_device_error': [I],
 }
-RESTYPES = {'tcq_status_string': ctypes.c_char_p, 'tcq_gemm_tcq_workspace': SZ, 'tcq_gemm_tcq_tc_workspace': SZ, 'tcq_gemm_tcq_noalloc_max_elements': SZ}
+RESTYPES = {'tcq_status_string': ctypes.c_char_p, 'tcq_gemm_tcq_workspace': SZ, 'tcq_gemm_tcq_tc_workspace': SZ, 'tcq_gemm_tcq_noalloc_max_elements': SZ,
+            'tcq_kv8_attention_workspace': SZ}
 
 
 def _load():

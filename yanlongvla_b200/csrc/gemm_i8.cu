@@ -1160,7 +1160,8 @@ int tcq_device_error(int reset) {
         const int z = 0;
         if (cudaMemcpyToSymbol(g_tcq_device_error, &z, sizeof(int)) != cudaSuccess) return -1;
     }
-    return v;
+    const int m = tcq_memory_error(reset), a = tcq_attention_error(reset);
+    return m < 0 || a < 0 ? -1 : v | m | a;
 }
 
 }  // extern "C"

@@ -1,0 +1,382 @@
+// Streaming-memory kernels around the attention: the rotary embedding with several axes, writing new tokens into the 8-bit
+// cache, and reading the cache back as values.
+#include <type_traits>
+
+#include "memory.cuh"
+
+__device__ int g_tcq_memory_error;
+
+int tcq_memory_error(int reset) {
+    int v = 0;
+    if (cudaMemcpyFromSymbol(&v, g_tcq_memory_error, sizeof(int)) != cudaSuccess) return -1;
+    if (reset && v) {
+        const int z = 0;
+        if (cudaMemcpyToSymbol(g_tcq_memory_error, &z, sizeof(int)) != cudaSuccess) return -1;
+    }
+    return v;
+}
+
+namespace {
+
+using namespace tcq;
+
+// ------------------------------------------------------------------------------------------------ rotary, several axes
+// A unit is V frequencies of one head: 2 V elements, as two V-element vectors (half-split: j and j + D/2; pairs: 2 V
+// neighbours). A thread keeps its V cosines and sines of one token in registers and turns that unit of every hp-th head,
+// so the tables are read once per token and 2 V / (heads / hp) elements. Bound by HBM (many tokens) or latency (few).
+template <int BYTES> struct Raw;
+template <> struct Raw<16> { typedef uint4 type; };
+template <> struct Raw<8> { typedef uint2 type; };
+template <> struct Raw<4> { typedef u32 type; };
+template <> struct Raw<2> { typedef u16 type; };
+
+template <int DT, int V>
+struct Vec {
+    static constexpr int BYTES = V * (DT == TCQ_DT_F32 ? 4 : 2);
+    typedef typename Raw<BYTES>::type R;
+    static TCQ_HD void load(const void* p, float* v) {
+        union { R r; u32 w[(BYTES + 3) / 4]; u16 h[BYTES / 2]; } u;
+        u.r = *reinterpret_cast<const R*>(p);
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[i] = DT == TCQ_DT_F32 ? __uint_as_float(u.w[i]) : elem_f<DT>(u.h[i]);
+    }
+    static TCQ_HD void store(void* p, const float* v) {
+        union { R r; u32 w[(BYTES + 3) / 4]; u16 h[BYTES / 2]; } u;
+        if (DT == TCQ_DT_F32) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) u.w[i] = __float_as_uint(v[i]);
+        } else if (V == 1) {
+            u.h[0] = (u16)pack2<DT>(v[0], 0.f);
+        } else {
+#pragma unroll
+            for (int i = 0; i < V / 2; ++i) u.w[i] = pack2<DT>(v[2 * i], v[2 * i + 1]);
+        }
+        *reinterpret_cast<R*>(p) = u.r;
+    }
+};
+
+template <int DT, int V, bool PAIRS>
+__global__ void __launch_bounds__(256) k_rope_axes(const char* __restrict__ x, char* __restrict__ out, RopeArgs r, i64 x_sb, i64 x_st,
+                                                   i64 o_sb, i64 o_st, i64 rows, int T, int heads, int C, int hp, float sign) {
+    constexpr int E = DT == TCQ_DT_F32 ? 4 : 2;
+    pdl_launch_dependents();
+    pdl_wait();
+    const int per = C * hp;
+    const i64 row = (i64)blockIdx.x * (blockDim.x / per) + threadIdx.x / per;
+    if (row >= rows) return;
+    const int u = threadIdx.x % per, c = u % C, h0 = u / C;
+    const i64 b = row / T, t = row - b * T;
+    const int D = 2 * r.half, first = PAIRS ? 2 * V * c : V * c, second = PAIRS ? first + V : first + r.half;
+    const char* xr = x + (b * x_sb + t * x_st) * E;
+    char* orow = out + (b * o_sb + t * o_st) * E;
+    float cs[V], sn[V];
+    rope_cs<V>(r, row, V * c, cs, sn, &g_tcq_memory_error);
+#pragma unroll
+    for (int i = 0; i < V; ++i) sn[i] *= sign;
+    for (int h = h0; h < heads; h += hp) {
+        float a[2 * V];
+        Vec<DT, V>::load(xr + (i64)(h * D + first) * E, a);
+        Vec<DT, V>::load(xr + (i64)(h * D + second) * E, a + V);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            if (PAIRS) turn(a[2 * i], a[2 * i + 1], cs[i], sn[i]);
+            else turn(a[i], a[V + i], cs[i], sn[i]);
+        }
+        Vec<DT, V>::store(orow + (i64)(h * D + first) * E, a);
+        Vec<DT, V>::store(orow + (i64)(h * D + second) * E, a + V);
+    }
+}
+
+template <int DT, int V>
+int launch_rope(const void* x, void* out, const RopeArgs& r, i64 x_sb, i64 x_st, i64 o_sb, i64 o_st, int B, int T, int heads, bool pairs,
+                float sign, void* stream) {
+    const int C = r.half / V;                      // units of a head (at most 128)
+    const int hp = heads < 256 / C ? heads : 256 / C;
+    const int tokens = 256 / (C * hp);             // tokens of a block
+    const i64 rows = (i64)B * T, blocks = (rows + tokens - 1) / tokens;
+    if (blocks > 0x7fffffff) return TCQ_ERR_SHAPE;
+    return launch_pdl(pairs ? k_rope_axes<DT, V, true> : k_rope_axes<DT, V, false>, dim3((unsigned)blocks), tokens * C * hp, 0, stream,
+                      (const char*)x, (char*)out, r, x_sb, x_st, o_sb, o_st, rows, T, heads, C, hp, sign);
+}
+
+// ------------------------------------------------------------------------------------------------ cache append
+TCQ_HD int q8(float x, float inv) {
+    float v = x * inv;
+    v = v == v ? v : 0.f;
+    return __float2int_rn(fminf(fmaxf(v, -127.f), 127.f));
+}
+TCQ_HD u32 q8x4(const float* x, float inv) {
+    u32 w = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w |= (u32)(q8(x[i], inv) & 255) << (8 * i);
+    return w;
+}
+TCQ_HD u32 requant4(u32 w, float ratio) {
+    u32 o = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o |= (u32)(__float2int_rn((float)(int)(i8)(w >> (8 * i)) * ratio) & 255) << (8 * i);
+    return o;
+}
+
+// One CTA writes one head of one block of one sequence, keys (blockIdx.y 0) or values (1). The new tokens stay in
+// registers between the block's largest magnitude and their quantization, so they are read once; values are turned into
+// rows of tokens through shared memory. The block's older tokens are touched only when its scale grows. Bound by HBM.
+template <int DT, int D>
+__global__ void __launch_bounds__(128) k_kv8_append(tcq_kv8_cache cache, const u16* __restrict__ k, i64 k_sb, i64 k_st,
+                                                    const u16* __restrict__ v, i64 v_sb, i64 v_st, const int* __restrict__ table,
+                                                    int blocks, const int* __restrict__ start, const int* __restrict__ count, RopeArgs r,
+                                                    int B, int T, int NB) {
+    constexpr int C = D / 16, NU = (kBlk * C + 127) / 128;      // units of 2 x 8 elements: per token, per thread
+    constexpr int VS = kBlk + 4;                                // row stride of the value tile (bytes)
+    __shared__ __align__(16) u32 tile32[D * VS / 4];
+    __shared__ float red[4];
+    i8* tile = reinterpret_cast<i8*>(tile32);
+    pdl_launch_dependents();
+    pdl_wait();
+    const int Hk = cache.kv_heads, h = blockIdx.x % Hk, bn = blockIdx.x / Hk, n = bn % NB, b = bn / NB;
+    const bool is_v = blockIdx.y != 0;
+    int st = start[b], cnt = count ? count[b] : T;
+    if (st < 0 || cnt < 0 || cnt > T) {
+        if (threadIdx.x == 0) atomicOr(&g_tcq_memory_error, 2);
+        st = max(st, 0), cnt = min(max(cnt, 0), T);
+    }
+    const int blk = st / kBlk + n, base = blk * kBlk;
+    const int lo = max(st - base, 0), hi = min(st + cnt - base, kBlk);       // new slots of the block
+    if (lo >= hi) return;
+    int page = blk < blocks ? table[(i64)b * blocks + blk] : -1;
+    if ((unsigned)page >= (unsigned)cache.pages) {
+        if (threadIdx.x == 0) atomicOr(&g_tcq_memory_error, 2);
+        return;
+    }
+    const u16* src = (is_v ? v + b * v_sb : k + b * k_sb) + h * D;
+    const i64 row_st = is_v ? v_st : k_st;
+    float x[NU][16];
+    float amax = 0.f;
+#pragma unroll
+    for (int i = 0; i < NU; ++i) {
+        const int u = threadIdx.x + 128 * i, slot = u / C, c = u - slot * C;
+        if (slot < lo || slot >= hi) continue;
+        const int t = base + slot - st;
+        Vec<DT, 8>::load(src + t * row_st + 8 * c, x[i]);
+        Vec<DT, 8>::load(src + t * row_st + 8 * c + D / 2, x[i] + 8);
+        if (!is_v && r.cos_t) {
+            float cs[8], sn[8];
+            rope_cs<8>(r, (i64)b * T + t, 8 * c, cs, sn, &g_tcq_memory_error);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) turn(x[i][j], x[i][8 + j], cs[j], sn[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            const float a = fabsf(x[i][j]);
+            amax = fmaxf(amax, a <= 3.402823466e38f ? a : 0.f);
+        }
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = amax;
+    float* scale = (is_v ? cache.v_scale : cache.k_scale) + (i64)page * Hk + h;
+    const float s_old = lo > 0 ? *scale : 0.f;
+    __syncthreads();
+    amax = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    float s = fmaxf(s_old, amax / 127.f);
+    if (s < 7.52316385e-37f) s = 0.f;                         // 2^-120
+    const float inv = s > 0.f ? 1.f / s : 0.f, ratio = s_old * inv;
+    const bool grown = lo > 0 && s > s_old;
+    if (threadIdx.x == 0) *scale = s;
+    const i64 off = ((i64)page * Hk + h) * (kBlk * D);
+    if (!is_v) {
+        i8* dst = cache.k + off;
+#pragma unroll
+        for (int i = 0; i < NU; ++i) {
+            const int u = threadIdx.x + 128 * i, slot = u / C, c = u - slot * C;
+            if (slot < lo || slot >= hi) continue;
+            uint2* p = reinterpret_cast<uint2*>(dst + slot * D + 8 * c);
+            p[0] = make_uint2(q8x4(x[i], inv), q8x4(x[i] + 4, inv));
+            p[D / 16] = make_uint2(q8x4(x[i] + 8, inv), q8x4(x[i] + 12, inv));
+        }
+        if (grown)
+            for (int i = threadIdx.x; i < lo * (D / 4); i += 128) {
+                u32* p = reinterpret_cast<u32*>(dst) + i;
+                *p = requant4(*p, ratio);
+            }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < NU; ++i) {
+        const int u = threadIdx.x + 128 * i, slot = u / C, c = u - slot * C;
+        if (slot < lo || slot >= hi) continue;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) tile[((j < 8 ? 8 * c : 8 * c + D / 2 - 8) + j) * VS + slot] = (i8)q8(x[i][j], inv);
+    }
+    __syncthreads();
+    i8* dst = cache.v + off;
+    for (int i = threadIdx.x; i < D * 4; i += 128) {          // 16-token pieces of the rows
+        const int d = i >> 2, t0 = (i & 3) * 16;
+        const bool any_new = t0 < hi && t0 + 16 > lo, any_old = grown && t0 < lo;
+        if (!any_new && !any_old) continue;
+        u32 w[4];
+        uint4* p = reinterpret_cast<uint4*>(dst + d * kBlk + t0);
+        if (t0 < lo || t0 + 16 > hi) {
+            const uint4 o = *p;
+            w[0] = o.x, w[1] = o.y, w[2] = o.z, w[3] = o.w;
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int t = t0 + 4 * j;
+            const u32 fresh = tile32[(d * VS + t) >> 2];
+            if (any_old) {
+                const u32 q = requant4(w[j], ratio);
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (t + e < lo) w[j] = (w[j] & ~(255u << (8 * e))) | (q & (255u << (8 * e)));
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (t + e >= lo && t + e < hi) w[j] = (w[j] & ~(255u << (8 * e))) | (fresh & (255u << (8 * e)));
+        }
+        *p = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ cache read
+// One CTA reads one head of one block, keys or values, and writes its tokens' rows. Values go through shared memory to
+// turn rows of tokens back into tokens. Bound by HBM.
+template <int DT, int D>
+__global__ void __launch_bounds__(128) k_kv8_read(tcq_kv8_cache cache, char* __restrict__ ko, char* __restrict__ vo,
+                                                  const int* __restrict__ table, int blocks, const int* __restrict__ begin,
+                                                  const int* __restrict__ lens, int T, int NB) {
+    constexpr int C = D / 8, E = DT == TCQ_DT_F32 ? 4 : 2, VS = kBlk + 4;
+    __shared__ __align__(16) u32 tile32[D * VS / 4];
+    pdl_launch_dependents();
+    pdl_wait();
+    const int Hk = cache.kv_heads, h = blockIdx.x % Hk, bn = blockIdx.x / Hk, n = bn % NB, b = bn / NB;
+    const bool is_v = blockIdx.y != 0;
+    int from = begin[b], len = lens[b];
+    if (from < 0 || len < 0 || (i64)len > (i64)blocks * kBlk) {
+        if (threadIdx.x == 0) atomicOr(&g_tcq_memory_error, 2);
+        from = max(from, 0), len = (int)min((i64)max(len, 0), (i64)blocks * kBlk);
+    }
+    const i64 blk = from / kBlk + n, base = blk * kBlk;
+    const int lo = (int)max((i64)from - base, (i64)0), hi = (int)min((i64)from + T - base, (i64)kBlk);
+    if (lo >= hi) return;
+    const int end = (int)min(max((i64)len - base, (i64)0), (i64)kBlk);        // slots that hold tokens
+    int page = 0;
+    if (end > lo) {
+        page = table[(i64)b * blocks + blk];
+        if ((unsigned)page >= (unsigned)cache.pages) {
+            if (threadIdx.x == 0) atomicOr(&g_tcq_memory_error, 2);
+            page = page < 0 ? 0 : cache.pages - 1;
+        }
+    }
+    const i64 off = ((i64)page * Hk + h) * (kBlk * D);
+    const float s = end > lo ? (is_v ? cache.v_scale : cache.k_scale)[(i64)page * Hk + h] : 0.f;
+    if (is_v && end > lo) {
+        const uint4* src = reinterpret_cast<const uint4*>(cache.v + off);
+        for (int i = threadIdx.x; i < D * 4; i += 128) {
+            const uint4 q = src[i];
+            u32* p = tile32 + ((i >> 2) * VS + (i & 3) * 16) / 4;
+            p[0] = q.x, p[1] = q.y, p[2] = q.z, p[3] = q.w;
+        }
+    }
+    __syncthreads();
+    char* out = (is_v ? vo : ko) + (((i64)b * T + base - from) * Hk + h) * D * E;
+    const i8* tile = reinterpret_cast<const i8*>(tile32);
+    for (int u = threadIdx.x; u < kBlk * C; u += 128) {
+        const int slot = u / C, c = u - slot * C;
+        if (slot < lo || slot >= hi) continue;
+        float y[8];
+        if (slot >= end) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) y[j] = 0.f;
+        } else if (is_v) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) y[j] = (float)(int)tile[(8 * c + j) * VS + slot] * s;
+        } else {
+            const uint2 q = *reinterpret_cast<const uint2*>(cache.k + off + slot * D + 8 * c);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) y[j] = (float)(int)(i8)((j < 4 ? q.x : q.y) >> (8 * (j & 3))) * s;
+        }
+        char* o = out + ((i64)slot * Hk * D + 8 * c) * E;
+        if (DT == TCQ_DT_F32) {
+            Vec<DT, 4>::store(o, y);
+            Vec<DT, 4>::store(o + 16, y + 4);
+        } else {
+            Vec<DT, DT == TCQ_DT_F32 ? 4 : 8>::store(o, y);
+        }
+    }
+}
+
+}  // namespace
+
+extern "C" {
+
+int tcq_rope_axes(const void* x, int dtype, int64_t x_sb, int64_t x_st, void* out, int64_t o_sb, int64_t o_st, const int32_t* pos,
+                  const tcq_rope_plan* plan, int B, int T, int heads, int inverse, void* stream) {
+    if (!x || !out || !pos || !plan) return TCQ_ERR_ARG;
+    if (dtype != TCQ_DT_BF16 && dtype != TCQ_DT_F16 && dtype != TCQ_DT_F32) return TCQ_ERR_DTYPE;
+    const int e = check_rope_plan(plan);
+    if (e) return e;
+    if (B < 1 || T < 1 || heads < 1) return TCQ_ERR_SHAPE;
+    const int es = dtype == TCQ_DT_F32 ? 4 : 2, half = plan->head_dim / 2;
+    // The widest vectors that the head width, the strides and the addresses allow.
+    int V = dtype == TCQ_DT_F32 ? 4 : 8;
+    const uintptr_t mix = (uintptr_t)x | (uintptr_t)out | (uintptr_t)((x_sb | x_st | o_sb | o_st) * es);
+    while (V > 1 && ((half % V) || (mix & (V * es - 1)))) V >>= 1;
+    if (mix & (es - 1)) return TCQ_ERR_ALIGN;
+    const RopeArgs r = rope_args(plan, pos, B, T);
+    const float sign = inverse ? -1.f : 1.f;
+#define TCQ_ROPE(DT, VV) launch_rope<DT, VV>(x, out, r, x_sb, x_st, o_sb, o_st, B, T, heads, plan->pairs != 0, sign, stream)
+#define TCQ_ROPE16(DT) (V == 8 ? TCQ_ROPE(DT, 8) : V == 4 ? TCQ_ROPE(DT, 4) : V == 2 ? TCQ_ROPE(DT, 2) : TCQ_ROPE(DT, 1))
+    if (dtype == TCQ_DT_BF16) return TCQ_ROPE16(TCQ_DT_BF16);
+    if (dtype == TCQ_DT_F16) return TCQ_ROPE16(TCQ_DT_F16);
+    return V == 4 ? TCQ_ROPE(TCQ_DT_F32, 4) : V == 2 ? TCQ_ROPE(TCQ_DT_F32, 2) : TCQ_ROPE(TCQ_DT_F32, 1);
+#undef TCQ_ROPE16
+#undef TCQ_ROPE
+}
+
+int tcq_kv8_append(const tcq_kv8_cache* cache, const void* k, int64_t k_sb, int64_t k_st, const void* v, int64_t v_sb, int64_t v_st,
+                   int dtype, const int32_t* table, int blocks, const int32_t* start, const int32_t* count, const int32_t* pos,
+                   const tcq_rope_plan* plan, int B, int T, void* stream) {
+    const int e = check_cache(cache);
+    if (e) return e;
+    if (!k || !v || !table || !start || (plan && !pos)) return TCQ_ERR_ARG;
+    if (dtype != TCQ_DT_BF16 && dtype != TCQ_DT_F16) return TCQ_ERR_DTYPE;
+    if (B < 1 || T < 1 || blocks < 1) return TCQ_ERR_SHAPE;
+    RopeArgs r = {};
+    if (plan) {
+        const int ep = check_rope_plan(plan);
+        if (ep) return ep;
+        if (plan->head_dim != cache->head_dim || plan->pairs) return TCQ_ERR_SHAPE;
+        r = rope_args(plan, pos, B, T);
+    }
+    if (!tcq_aligned(k, 16) || !tcq_aligned(v, 16) || ((k_sb | k_st | v_sb | v_st) & 7)) return TCQ_ERR_ALIGN;
+    const int NB = (int)(((i64)T + 2 * kBlk - 2) / kBlk);      // blocks that T tokens can touch
+    const i64 ctas = (i64)B * NB * cache->kv_heads;
+    if (ctas > 0x7fffffff) return TCQ_ERR_SHAPE;
+    return by_head_dim(cache->head_dim, [&](auto d) {
+        constexpr int D = decltype(d)::value;
+        return launch_pdl(dtype == TCQ_DT_BF16 ? k_kv8_append<TCQ_DT_BF16, D> : k_kv8_append<TCQ_DT_F16, D>, dim3((unsigned)ctas, 2), 128, 0,
+                          stream, *cache, (const u16*)k, (i64)k_sb, (i64)k_st, (const u16*)v, (i64)v_sb, (i64)v_st, table, blocks, start,
+                          count, r, B, T, NB);
+    });
+}
+
+int tcq_kv8_read(const tcq_kv8_cache* cache, void* k, void* v, int dtype, const int32_t* table, int blocks, const int32_t* begin,
+                 const int32_t* lens, int B, int T, void* stream) {
+    const int e = check_cache(cache);
+    if (e) return e;
+    if (!k || !v || !table || !begin || !lens) return TCQ_ERR_ARG;
+    if (dtype != TCQ_DT_BF16 && dtype != TCQ_DT_F16 && dtype != TCQ_DT_F32) return TCQ_ERR_DTYPE;
+    if (B < 1 || T < 1 || blocks < 1) return TCQ_ERR_SHAPE;
+    if (!tcq_aligned(k, 16) || !tcq_aligned(v, 16)) return TCQ_ERR_ALIGN;
+    const int NB = (int)(((i64)T + 2 * kBlk - 2) / kBlk);
+    const i64 ctas = (i64)B * NB * cache->kv_heads;
+    if (ctas > 0x7fffffff) return TCQ_ERR_SHAPE;
+    return by_head_dim(cache->head_dim, [&](auto d) {
+        constexpr int D = decltype(d)::value;
+        auto kern = dtype == TCQ_DT_BF16 ? k_kv8_read<TCQ_DT_BF16, D> : dtype == TCQ_DT_F16 ? k_kv8_read<TCQ_DT_F16, D> : k_kv8_read<TCQ_DT_F32, D>;
+        return launch_pdl(kern, dim3((unsigned)ctas, 2), 128, 0, stream, *cache, (char*)k, (char*)v, table, blocks, begin, lens, T, NB);
+    });
+}
+
+}  // extern "C"

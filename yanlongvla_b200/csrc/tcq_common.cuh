@@ -195,6 +195,11 @@ TCQ_HD const void* stage_const(char*& sp, const void* src, int bytes, bool on) {
         if (e_ != cudaSuccess) return TCQ_ERR_LAUNCH;             \
     } while (0)
 
+// Error flags of the streaming-memory kernels (kv8.cu, kv8_attention.cu), reported through tcq_device_error(); -1 if they
+// cannot be read.
+int tcq_memory_error(int reset);
+int tcq_attention_error(int reset);
+
 static inline bool tcq_aligned(const void* p, size_t a) { return (((uintptr_t)p) & (a - 1)) == 0; }
 
 // Streaming multiprocessors of the current device (queried once per translation unit; 148, a B200's, if the query
