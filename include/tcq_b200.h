@@ -256,7 +256,7 @@ typedef struct tcq_rope_plan {
 /* A key / value cache in 8 bits. A page is one block of TCQ_KV8_BLOCK tokens of one sequence: k (pages, kv_heads, 64,
  * head_dim) int8, v (pages, kv_heads, head_dim, 64) int8 (values transposed, so that both operands of the attention's
  * products run along their contraction), k_scale / v_scale (pages, kv_heads) FP32: a value is its integer times its
- * block's scale. head_dim is 32, 48, 64, 80, 96 or 128; k and v are 16-byte aligned. A table (B, blocks) int32 names the
+ * block's scale (the attention takes values of a block whose v_scale is below 2^-90 as zeros). head_dim is 32, 48, 64, 80, 96 or 128; k and v are 16-byte aligned. A table (B, blocks) int32 names the
  * page of each block of each sequence. */
 #define TCQ_KV8_BLOCK 64
 typedef struct tcq_kv8_cache {

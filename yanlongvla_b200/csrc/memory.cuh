@@ -3,6 +3,9 @@
 #pragma once
 #include <cuda_fp16.h>
 
+#include <atomic>
+#include <type_traits>
+
 #include "tcq_common.cuh"
 
 namespace tcq {
@@ -128,6 +131,19 @@ static inline int launch_pdl(void (*kern)(P...), dim3 grid, int threads, size_t 
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     return cudaLaunchKernelEx(&cfg, kern, P(args)...) == cudaSuccess ? TCQ_OK : TCQ_ERR_LAUNCH;
+}
+
+// The same for a kernel with more than 48 KB of dynamic shared memory; the attribute is set once per device.
+template <auto Kern, class A>
+static inline int launch_big(dim3 grid, int threads, size_t smem, void* stream, const A& args) {
+    static std::atomic<unsigned long long> set{0};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev > 63) return TCQ_ERR_DEVICE;
+    if (!(set.load(std::memory_order_relaxed) >> dev & 1)) {
+        if (cudaFuncSetAttribute(Kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) return TCQ_ERR_LAUNCH;
+        set.fetch_or(1ull << dev, std::memory_order_relaxed);
+    }
+    return launch_pdl(Kern, grid, threads, smem, stream, args);
 }
 
 static inline int check_cache(const tcq_kv8_cache* c) {
