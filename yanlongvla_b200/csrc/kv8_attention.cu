@@ -2,6 +2,7 @@
 #include <type_traits>
 
 #include "memory.cuh"
+#include "tma.cuh"
 
 __device__ int g_tcq_attention_error;
 
@@ -585,70 +586,539 @@ __global__ void __launch_bounds__(kWarps * 32, 1) k_attention_few(const AttnArgs
     asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
-// One warp per query row (sequence, query, head), 32 keys at a time: each lane forms one score (its key's row of D bytes),
-// the warp updates the running maximum and sum, and each lane then adds the keys' values into its own elements d = lane + 32 i.
-template <int DT, int D>
-__global__ void __launch_bounds__(128) k_attention_rows(tcq_kv8_cache cache, const u16* __restrict__ q, i64 q_sb, i64 q_st, u16* __restrict__ out,
-                                                        const int* __restrict__ table, int blocks, const int* __restrict__ lens,
-                                                        const int* __restrict__ count, int causal, float scale, i64 rows, int T, int heads) {
-    __shared__ float sq[4][D], sp[4][32];
+// ------------------------------------------------------------------------------------------------ many query rows
+// Frames and prompts: tensor-core products (tcgen05) on tiles of 128 query rows and 128 keys (two pages).
+//
+// The rows of a key head are its queries in token order, `group` heads to a token, so a causal limit never falls along the
+// rows. A CTA takes NG groups of up to 128 rows and one key head. Roles:
+//   softmax   128 threads per group, a row each: scores from TMEM, weights (FP16) back to TMEM over the scores;
+//   convert   128 threads: INT8 pages from global memory (requested one half tile ahead into registers) to FP16 tiles in
+//             shared memory, 128-byte swizzled, keys K-major along the head, values K-major along the tokens;
+//   product   one thread issues S = Q K^T (both operands in shared memory) and O += P V (P in TMEM).
+// The two groups alternate: while one's weights are formed, the other's products run. Mathematics, scaling of the queries and
+// handling of the scales are those of the few-row kernel; the reference m moves only when a score passes it by 2^4, and O (in
+// TMEM) is rescaled by its own row's thread. S of a tile is issued after O of the tile before it, and a commit covers every
+// product issued before it: scores that have arrived mean that O is complete up to the tile before.
+//
+// Few units (a frame of one robot): the tiles of a unit are divided over a cluster of CTAs, which add their parts through
+// distributed shared memory.
+
+constexpr int kTile = 128;            // keys of a tile, rows of a group
+
+template <int D, int NG>
+struct Many {
+    static constexpr int ATOMS = (D + 63) / 64;                       // 64-element columns of a K-major tile
+    static constexpr int QB = kTile * 128 * ATOMS;                    // bytes of a group's queries
+    static constexpr int KB = kTile * 128 * ATOMS;                    // of a tile's keys
+    static constexpr int VB = D * 128 * 2;                            // of its values
+    static constexpr int NS = 2;                                      // tiles of either in flight
+    static constexpr int Q0 = 0, K0 = NG * QB, V0 = K0 + NS * KB, BAR0 = V0 + NS * VB;
+    static constexpr int ML0 = BAR0 + 256;                            // m, l of every row (cluster sums)
+    static constexpr int BYTES = ML0 + NG * kTile * 8 + 1024;         // + slack to align the base to 1024
+    static constexpr int THREADS = NG * 128 + 160;
+    static constexpr u32 COLS = NG == 2 ? 512 : 256;
+    static constexpr int S0 = 0, O0 = NG * kTile;                     // TMEM columns: scores, outputs
+    static constexpr int PARTS = NG * kTile * D * 4;                  // a CTA's part of the outputs, over the tiles
+    static_assert(PARTS <= BAR0, "the parts overlay the tiles");
+};
+
+__device__ __forceinline__ u64 sw128_desc(u32 addr) {
+    return (u64)((addr >> 4) & 0x3FFF) | ((u64)1 << 16) | ((u64)(1024 >> 4) << 32) | ((u64)1 << 46) | ((u64)2 << 61);
+}
+// kind::f16: D FP32, A and B FP16, both K-major, M = 128.
+__host__ __device__ constexpr u32 idesc_f16(int n) { return (1u << 4) | ((u32)(n >> 3) << 17) | ((u32)(128 >> 4) << 24); }
+
+__device__ __forceinline__ void mma_ss(u32 d, u64 a, u64 b, u32 idesc, u32 acc) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a),
+                 "l"(b), "r"(idesc), "r"(acc) : "memory");
+}
+__device__ __forceinline__ void mma_ts(u32 d, u32 a, u64 b, u32 idesc, u32 acc) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a),
+                 "l"(b), "r"(idesc), "r"(acc) : "memory");
+}
+__device__ __forceinline__ void mma_commit(u32 bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+__device__ __forceinline__ void tmem_ld32(u32 addr, u32 (&v)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]),
+          "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]),
+          "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]),
+          "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+        : "r"(addr));
+}
+__device__ __forceinline__ void tmem_ld16(u32 addr, u32 (&v)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]),
+          "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+        : "r"(addr));
+}
+__device__ __forceinline__ void tmem_st16(u32 addr, const u32 (&v)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};" ::"r"(v[0]),
+        "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]),
+        "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(addr)
+        : "memory");
+}
+// Wait for this thread's TMEM loads; the registers they fill are not used before.
+template <int N>
+__device__ __forceinline__ void tmem_ld_wait(u32 (&v)[N]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int j = 0; j < N; ++j) asm volatile("" : "+r"(v[j]));
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void async_proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+__device__ __forceinline__ void cluster_barrier() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ u32 cluster_rank() {
+    u32 r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ u32 peer_addr(u32 addr, u32 rank) {
+    u32 r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ float4 peer_ld4(u32 addr) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ float2 peer_ld2(u32 addr) {
+    float2 v;
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+    return v;
+}
+
+// The barriers of a CTA, 8 bytes each from BAR0.
+enum { BAR_KFULL = 0, BAR_KEMPTY = 2, BAR_VFULL = 4, BAR_VEMPTY = 6, BAR_SFULL = 8, BAR_PFULL = 10, BAR_Q = 12, BAR_O = 13, BAR_COUNT = 14 };
+
+template <int DT, int D, int NG>
+__global__ void __launch_bounds__(Many<D, NG>::THREADS, NG == 1 && D <= 64 ? 2 : 1)
+k_attention_many(const AttnArgs A, int row_tiles, int tile_rows, int splits) {
+    typedef Many<D, NG> P;
+    constexpr int KS = D / 16, NC = D / 16;             // contraction steps; 16-byte chunks of a half tile per convert thread
+    extern __shared__ char smem_raw[];
+    char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    const u32 sbase = smem_u32(smem), bars = sbase + P::BAR0;
+    u32* tmem_slot = reinterpret_cast<u32*>(smem + P::BAR0 + 8 * BAR_COUNT);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    constexpr int W_CONV = NG * 4, W_MMA = W_CONV + 4;
+    auto bar = [&](int i) -> u32 { return bars + 8 * i; };
+    auto wait = [&](int i, u32 parity) -> bool { return mbar_wait_bounded(bar(i), parity & 1, abort_flag, &g_tcq_attention_error); };
+    if (tid == 0) {
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(bar(BAR_KFULL + i), 128);
+            mbar_init(bar(BAR_VFULL + i), 128);
+            mbar_init(bar(BAR_KEMPTY + i), 1);
+            mbar_init(bar(BAR_VEMPTY + i), 1);
+            mbar_init(bar(BAR_SFULL + i), 1);
+            mbar_init(bar(BAR_PFULL + i), 128);
+        }
+        mbar_init(bar(BAR_Q), NG * 128);
+        mbar_init(bar(BAR_O), 1);
+        *abort_flag = 0;
+        mbar_init_fence();
+    }
+    if (warp == W_MMA) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(P::COLS) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_before();
+    __syncthreads();
+    tc_after();
+    const u32 tmem = *tmem_slot;
     pdl_launch_dependents();
     pdl_wait();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const i64 row = (i64)blockIdx.x * 4 + warp;
-    if (row >= rows) return;
-    const int h = (int)(row % heads);
-    const i64 bt = row / heads, b = bt / T;
-    const int t = (int)(bt - b * T), Hk = cache.kv_heads, hk = h / (heads / Hk);
-    const int len = tokens_of(lens, b, blocks), cnt = queries_of(count, b, T);
-    const int limit = t >= cnt ? 0 : causal ? min(max(len - cnt + t + 1, 0), len) : len;
-    for (int d = lane; d < D; d += 32) sq[warp][d] = elem_f<DT>(q[b * q_sb + t * q_st + (i64)h * D + d]) * scale;
-    __syncwarp();
-    constexpr int ND = (D + 31) / 32;
-    float o[ND] = {}, m = -INFINITY, l = 0.f;
-    for (int k0 = 0; k0 < limit; k0 += 32) {
-        const i64 ph = (i64)page_of(table + b * blocks, k0 / kBlk, cache.pages) * Hk + hk, off = ph * (kBlk * D);
-        const int slot = k0 % kBlk;
-        const i8* kr = cache.k + off + (slot + lane) * D;
-        float s = 0.f;
-        for (int d = 0; d < D; d += 4) {
-            const u32 w = *reinterpret_cast<const u32*>(kr + d);
+
+    // ---- the unit: rows r0 .. r0 + tile_rows - 1 of key head h of sequence b (the heaviest row tiles of causal launches
+    // first), and this CTA's tiles [k0, k1) of its keys
+    const int Hk = A.cache.kv_heads, R = A.T * A.group;
+    const int sp = blockIdx.x % splits, unit = blockIdx.x / splits, bh = unit % (A.B * Hk), b = bh / Hk, h = bh - b * Hk;
+    const int rt = row_tiles - 1 - unit / (A.B * Hk), r0 = rt * tile_rows, r1 = min(R, r0 + tile_rows);
+    const int len = tokens_of(A.lens, b, A.blocks), cnt = queries_of(A.count, b, A.T);
+    const int last_q = min((r1 - 1) / A.group, cnt - 1), first_q = r0 / A.group;
+    const int upto = last_q < first_q ? 0 : A.causal ? min(max(len - cnt + last_q + 1, 0), len) : len;     // keys that some row sees
+    const int open = A.causal ? len - cnt + first_q + 1 : len;                                             // and that every row sees
+    const int tiles = (upto + kTile - 1) / kTile;
+    const int k0 = (int)((i64)tiles * sp / splits), k1 = (int)((i64)tiles * (sp + 1) / splits);
+    const int pages = (upto + kBlk - 1) / kBlk;
+    const int* trow = A.table + (i64)b * A.blocks;
+
+    float m = -INFINITY, l = 0.f;
+    if (warp < W_CONV) {
+        // ------------------------------------------------------------------------------------------------ softmax
+        const int g = warp >> 2, gl = tid & 127, r = r0 + g * kTile + gl, tq = r / A.group;
+        const bool live = r < r1 && tq < cnt;
+        const int limit = !live ? 0 : A.causal ? min(max(len - cnt + tq + 1, 0), len) : len;
+        float crow = 0.f;
+        if (k1 > k0) {
+            u32 qw[D / 2];
+            const u16* qr = A.q + b * A.q_sb + tq * A.q_st + (i64)(h * A.group + r - tq * A.group) * D;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s = fmaf((float)(int)(i8)(w >> (8 * e)), sq[warp][d + e], s);
-        }
-        s *= cache.k_scale[ph];
-        if (k0 + lane >= limit) s = -INFINITY;
-        float top = s;
-#pragma unroll
-        for (int w = 16; w; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
-        const float mn = fmaxf(m, top), f = expf(m - mn), p = expf(s - mn);
-        m = mn;
-        sp[warp][lane] = p * cache.v_scale[ph];
-        float sum = p;
-#pragma unroll
-        for (int w = 16; w; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
-        l = fmaf(l, f, sum);
-        __syncwarp();
-#pragma unroll
-        for (int i = 0; i < ND; ++i) {
-            const int d = lane + 32 * i;
-            if (d >= D) break;
-            const u32* vr = reinterpret_cast<const u32*>(cache.v + off + d * kBlk + slot);
-            float a = o[i] * f;
-            for (int j = 0; j < 8; ++j) {
-                const u32 w = vr[j];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) a = fmaf(sp[warp][4 * j + e], (float)(int)(i8)(w >> (8 * e)), a);
+            for (int i = 0; i < D / 8; ++i) {
+                const uint4 w = live ? reinterpret_cast<const uint4*>(qr)[i] : make_uint4(0, 0, 0, 0);
+                qw[4 * i] = w.x, qw[4 * i + 1] = w.y, qw[4 * i + 2] = w.z, qw[4 * i + 3] = w.w;
             }
-            o[i] = a;
-        }
-        __syncwarp();
-    }
+            float amax = 0.f, a, c;
 #pragma unroll
-    for (int i = 0; i < ND; ++i) {
-        const int d = lane + 32 * i;
-        if (d < D) out[(bt * heads + h) * D + d] = (u16)pack2<DT>(l > 0.f ? o[i] / l : 0.f, 0.f);
+            for (int i = 0; i < D / 2; ++i) {
+                unpack2<DT>(qw[i], a, c);
+                amax = fmaxf(amax, fmaxf(fabsf(a), fabsf(c)));
+            }
+            float back, up = row_scale(amax, back);
+            crow = back * fabsf(A.scale_log2);
+            if (A.scale_log2 < 0.f) up = -up;
+            char* q = smem + P::Q0 + g * P::QB + gl * 128;
+#pragma unroll
+            for (int i = 0; i < D / 8; ++i) {
+                u32 w[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    unpack2<DT>(qw[4 * i + j], a, c);
+                    w[j] = half2_of(a * up, c * up);
+                }
+                *reinterpret_cast<uint4*>(q + (i >> 3) * (kTile * 128) + (((i & 7) ^ (gl & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+            async_proxy_fence();
+            mbar_arrive(bar(BAR_Q));
+        }
+        const u32 lanes = (u32)((warp & 3) * 32) << 16, ts = tmem + lanes + P::S0 + g * kTile, to = tmem + lanes + P::O0 + g * D;
+        // the scales of the next tile's two pages are requested a tile ahead
+        auto page = [&](int p) -> i64 { return p < pages ? (i64)page_of(trow, p, A.cache.pages) * Hk + h : -1; };
+        i64 pg0 = -1, pg1 = -1;
+        float nk0 = 0.f, nk1 = 0.f, nv0 = 1.f, nv1 = 1.f;
+        auto request = [&](int i) {
+            if (i < k1) {
+                pg0 = page(2 * i), pg1 = page(2 * i + 1);
+                nk0 = A.cache.k_scale[pg0], nv0 = A.cache.v_scale[pg0];
+                nk1 = pg1 >= 0 ? A.cache.k_scale[pg1] : 0.f, nv1 = pg1 >= 0 ? A.cache.v_scale[pg1] : 1.f;
+            }
+        };
+        request(k0);
+#pragma unroll 1
+        for (int i = k0; i < k1; ++i) {
+            const float c[2] = {crow * nk0, crow * nk1}, vsc[2] = {nv0, nv1};
+            request(i + 1);
+            float bias[2], inv[2];
+#pragma unroll
+            for (int p = 0; p < 2; ++p) {
+                const float vs = safe_scale(vsc[p]);
+                bias[p] = lg2(vs), inv[p] = 1.f / vs;
+            }
+            if (!wait(BAR_SFULL + g, i - k0)) break;
+            tc_after();
+            const bool masked = (i + 1) * kTile > open;
+            const int lim = limit - i * kTile;
+            float top = -INFINITY;
+#pragma unroll
+            for (int p = 0; p < 2; ++p) {
+                float raw = -INFINITY;
+                u32 v[2][32];
+                tmem_ld32(ts + 64 * p, v[0]);
+                tmem_ld32(ts + 64 * p + 32, v[1]);
+                tmem_ld_wait(v[0]);
+                tmem_ld_wait(v[1]);
+                if (masked) {
+#pragma unroll
+                    for (int j = 0; j < 64; ++j)
+                        if (64 * p + j < lim) raw = fmaxf(raw, __uint_as_float(v[j >> 5][j & 31]));
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 64; ++j) raw = fmaxf(raw, __uint_as_float(v[j >> 5][j & 31]));
+                }
+                if (raw != -INFINITY) top = fmaxf(top, __fmaf_rn(raw, c[p], bias[p]));
+            }
+            const bool move = top > m + kSlack;
+            if (__any_sync(0xffffffffu, move)) {
+                const float f = move ? ex2(m - top) : 1.f;
+                if (move) m = top;
+                l *= f;
+                if (i > k0) {
+#pragma unroll 1
+                    for (int d = 0; d < D; d += 16) {
+                        u32 o[16];
+                        tmem_ld16(to + d, o);
+                        tmem_ld_wait(o);
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+                        tmem_st16(to + d, o);
+                    }
+                }
+            }
+            const float base = (m == -INFINITY ? 0.f : m) - kRef;
+#pragma unroll
+            for (int ch = 0; ch < 4; ++ch) {
+                const int p = ch >> 1;
+                u32 v[32], w[16];
+                tmem_ld32(ts + 32 * ch, v);
+                tmem_ld_wait(v);
+                const float add = bias[p] - base;
+                float sum = 0.f;
+#pragma unroll
+                for (int j = 0; j < 32; ++j) {
+                    float x = __fmaf_rn(__uint_as_float(v[j]), c[p], add);
+                    if (masked && 32 * ch + j >= lim) x = -INFINITY;
+                    x = ex2(x);
+                    sum += x;
+                    v[j] = __float_as_uint(x);
+                }
+                l = __fmaf_rn(sum, inv[p], l);
+                const bool mute = vsc[p] < kLeastScale;
+#pragma unroll
+                for (int j = 0; j < 16; ++j) w[j] = mute ? 0u : half2_of(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]));
+                tmem_st16(ts + 16 * ch, w);
+            }
+            tmem_st_wait();
+            tc_before();
+            mbar_arrive(bar(BAR_PFULL + g));
+        }
+        if (limit == 0) l = 0.f;
+        const bool got = k1 > k0 && wait(BAR_O, 0);
+        tc_after();
+        if (splits == 1) {
+            const float f = got && l != 0.f ? 1.f / l : 0.f;
+            u16* dst = A.out + (((i64)b * A.T + tq) * A.heads + h * A.group + r - tq * A.group) * D;
+#pragma unroll 1
+            for (int d = 0; d < D; d += 16) {
+                u32 o[16] = {};
+                if (got) {
+                    tmem_ld16(to + d, o);
+                    tmem_ld_wait(o);
+                }
+                if (r < r1) {
+                    u32 w[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        w[j] = f != 0.f || l != 0.f ? pack2<DT>(__uint_as_float(o[2 * j]) * f, __uint_as_float(o[2 * j + 1]) * f) : 0u;
+                    reinterpret_cast<uint4*>(dst + d)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+                    reinterpret_cast<uint4*>(dst + d)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+                }
+            }
+        } else {
+            // this CTA's part: rows of D floats over the tiles, 16-byte chunks permuted within a row
+            constexpr int X = (D / 4) % 8 == 0 ? 7 : 3;
+            const int row = g * kTile + gl;
+            float4* dst = reinterpret_cast<float4*>(smem) + row * (D / 4);
+#pragma unroll 1
+            for (int d = 0; d < D; d += 16) {
+                u32 o[16] = {};
+                if (got) {
+                    tmem_ld16(to + d, o);
+                    tmem_ld_wait(o);
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    dst[(d / 4 + j) ^ (row & X)] = make_float4(__uint_as_float(o[4 * j]), __uint_as_float(o[4 * j + 1]), __uint_as_float(o[4 * j + 2]),
+                                                               __uint_as_float(o[4 * j + 3]));
+            }
+            reinterpret_cast<float2*>(smem + P::ML0)[row] = make_float2(got ? m : -INFINITY, got ? l : 0.f);
+        }
+    } else if (warp < W_MMA) {
+        // ------------------------------------------------------------------------------------------------ convert
+        const int ct = tid - W_CONV * 32;
+        uint4 next[NC];
+        // half tile j: keys (even) or values (odd) of tile k0 + j / 2
+        auto request = [&](int j) {
+            const int i = k0 + (j >> 1);
+            if (i >= k1) return;
+            const int p1 = 2 * i + 1;
+            const i64 step = (i64)(kBlk * D);
+            const i8* src = (j & 1) ? A.cache.v : A.cache.k;
+            const i8* s0 = src + ((i64)page_of(trow, 2 * i, A.cache.pages) * Hk + h) * step;
+            const i8* s1 = p1 < pages ? src + ((i64)page_of(trow, p1, A.cache.pages) * Hk + h) * step : nullptr;
+#pragma unroll
+            for (int n = 0; n < NC; ++n) {
+                const int c = ct + 128 * n;
+                const i8* s = c < 4 * D ? s0 + c * 16 : s1 ? s1 + (c - 4 * D) * 16 : nullptr;
+                next[n] = s ? *reinterpret_cast<const uint4*>(s) : make_uint4(0, 0, 0, 0);
+            }
+        };
+        request(0);
+        const int halves = 2 * (k1 - k0);
+#pragma unroll 1
+        for (int j = 0; j < halves; ++j) {
+            const int it = j >> 1, s = it & 1, use = it >> 1;
+            uint4 cur[NC];
+#pragma unroll
+            for (int n = 0; n < NC; ++n) cur[n] = next[n];
+            request(j + 1);
+            if (!wait(((j & 1) ? BAR_VEMPTY : BAR_KEMPTY) + s, use + 1)) break;
+            char* dst = smem + ((j & 1) ? P::V0 + s * P::VB : P::K0 + s * P::KB);
+#pragma unroll
+            for (int n = 0; n < NC; ++n) {
+                const int c = ct + 128 * n, p = c >= 4 * D, cc = c - p * 4 * D;
+                int row, ch;
+                char* t;
+                if (j & 1) {
+                    row = cc >> 2, ch = 2 * (cc & 3);
+                    t = dst + p * (D * 128);
+                } else {
+                    row = cc / (D / 16);
+                    const int x = cc - row * (D / 16);
+                    row += 64 * p, ch = 2 * (x & 3);
+                    t = dst + (x >> 2) * (kTile * 128);
+                }
+                u32 w[8];
+                int8x4_to_half(cur[n].x, w[0], w[1]);
+                int8x4_to_half(cur[n].y, w[2], w[3]);
+                int8x4_to_half(cur[n].z, w[4], w[5]);
+                int8x4_to_half(cur[n].w, w[6], w[7]);
+                t += row * 128;
+                *reinterpret_cast<uint4*>(t + ((ch ^ (row & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+                *reinterpret_cast<uint4*>(t + (((ch + 1) ^ (row & 7)) << 4)) = make_uint4(w[4], w[5], w[6], w[7]);
+            }
+            async_proxy_fence();
+            mbar_arrive(bar(((j & 1) ? BAR_VFULL : BAR_KFULL) + s));
+        }
+    } else if (lane == 0 && k1 > k0) {
+        // ------------------------------------------------------------------------------------------------ product
+        auto scores = [&](int g, int s) {
+            const u32 qa = sbase + P::Q0 + g * P::QB, ka = sbase + P::K0 + s * P::KB;
+#pragma unroll
+            for (int k = 0; k < KS; ++k)
+                mma_ss(tmem + P::S0 + g * kTile, sw128_desc(qa + (k >> 2) * (kTile * 128) + 32 * (k & 3)),
+                       sw128_desc(ka + (k >> 2) * (kTile * 128) + 32 * (k & 3)), idesc_f16(kTile), k > 0);
+            mma_commit(bar(BAR_SFULL + g));
+        };
+        const int n = k1 - k0;
+        bool ok = wait(BAR_Q, 0) && wait(BAR_KFULL, 0);
+        if (ok) {
+            tc_after();
+            for (int g = 0; g < NG; ++g) scores(g, 0);
+            mma_commit(bar(BAR_KEMPTY));
+        }
+        for (int i = 0; i < n && ok; ++i) {
+            const int s = i & 1, s1 = (i + 1) & 1;
+            for (int g = 0; g < NG && ok; ++g) {
+                if (g == 0) ok = wait(BAR_VFULL + s, i >> 1);
+                ok = ok && wait(BAR_PFULL + g, i);
+                if (!ok) break;
+                tc_after();
+                const u32 va = sbase + P::V0 + s * P::VB;
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                    mma_ts(tmem + P::O0 + g * D, tmem + P::S0 + g * kTile + 8 * k, sw128_desc(va + (k >> 2) * (D * 128) + 32 * (k & 3)),
+                           idesc_f16(D), i > 0 || k > 0);
+                if (i + 1 < n) {
+                    if (g == 0) ok = wait(BAR_KFULL + s1, (i + 1) >> 1);
+                    if (!ok) break;
+                    tc_after();
+                    scores(g, s1);
+                }
+            }
+            if (!ok) break;
+            mma_commit(bar(BAR_VEMPTY + s));
+            if (i + 1 < n) mma_commit(bar(BAR_KEMPTY + s1));
+        }
+        mma_commit(bar(BAR_O));
+        // products in flight must end before TMEM is freed, also after an expired wait
+        volatile int never = 0;
+        mbar_wait_bounded(bar(BAR_O), 0, &never, &g_tcq_attention_error);
     }
+    tc_before();
+    __syncthreads();
+    tc_after();
+    if (warp == W_MMA) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(P::COLS) : "memory");
+    if (splits == 1) return;
+
+    // ---- the cluster's CTAs add their parts: each finishes a slice of the rows
+    cluster_barrier();
+    {
+        constexpr int X = (D / 4) % 8 == 0 ? 7 : 3;
+        const int rank = (int)cluster_rank(), rows = r1 - r0;
+        const int s0 = rows * rank / splits, s1 = rows * (rank + 1) / splits;
+        for (int e = tid; e < (s1 - s0) * (D / 8); e += P::THREADS) {
+            const int row = s0 + e / (D / 8), c8 = e % (D / 8);
+            float top = -INFINITY;
+            for (int k = 0; k < splits; ++k) top = fmaxf(top, peer_ld2(peer_addr(sbase + P::ML0 + row * 8, k)).x);
+            float acc[8] = {}, sum = 0.f;
+            for (int k = 0; k < splits; ++k) {
+                const float2 ml = peer_ld2(peer_addr(sbase + P::ML0 + row * 8, k));
+                const float f = top == -INFINITY ? 0.f : ex2(ml.x - top);
+                if (f == 0.f) continue;
+                sum += ml.y * f;
+                const u32 base = peer_addr(sbase, k) + row * (D * 4);
+                const float4 u = peer_ld4(base + (((2 * c8) ^ (row & X)) << 4)), v = peer_ld4(base + (((2 * c8 + 1) ^ (row & X)) << 4));
+                acc[0] += u.x * f, acc[1] += u.y * f, acc[2] += u.z * f, acc[3] += u.w * f;
+                acc[4] += v.x * f, acc[5] += v.y * f, acc[6] += v.z * f, acc[7] += v.w * f;
+            }
+            const float f = sum != 0.f ? 1.f / sum : 0.f;
+            u32 w[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[j] = sum != 0.f ? pack2<DT>(acc[2 * j] * f, acc[2 * j + 1] * f) : 0u;
+            const int r = r0 + row, tq = r / A.group;
+            u16* dst = A.out + (((i64)b * A.T + tq) * A.heads + h * A.group + r - tq * A.group) * D + 8 * c8;
+            *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+    }
+    cluster_barrier();
+}
+
+template <int DT, int D, int NG>
+int launch_many(const AttnArgs& A, void* stream) {
+    typedef Many<D, NG> P;
+    const auto kern = k_attention_many<DT, D, NG>;
+    constexpr int PER_SM = NG == 1 && D <= 64 ? 2 : 1;
+    const int R = A.T * A.group, row_tiles = (R + NG * kTile - 1) / (NG * kTile);
+    const int tile_rows = ((R + row_tiles - 1) / row_tiles + 31) & ~31;            // even shares, in warps
+    const i64 units = (i64)A.B * A.cache.kv_heads * row_tiles;
+    cudaLaunchConfig_t cfg = {};
+    cfg.blockDim = dim3(P::THREADS);
+    cfg.dynamicSmemBytes = P::BYTES;
+    cfg.stream = (cudaStream_t)stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    // What a device can hold of clusters of 1 .. 8 CTAs, asked once per device.
+    static std::atomic<int> held[64][9];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev > 63) return TCQ_ERR_DEVICE;
+    if (!held[dev][1].load(std::memory_order_acquire)) {
+        if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, P::BYTES) != cudaSuccess) return TCQ_ERR_LAUNCH;
+        for (int s = 8; s >= 1; --s) {
+            int n = 0;
+            cfg.gridDim = dim3(s);
+            attr[0].val.clusterDim.x = s;
+            cfg.numAttrs = 1;
+            if (s == 1) n = tcq_sm_count() * PER_SM;
+            else if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess) n = 0, cudaGetLastError();
+            held[dev][s].store(n, std::memory_order_release);
+        }
+    }
+    // Units that do not fill the device share their tiles among the CTAs of a cluster: the split with the least rounds of
+    // tiles, at least two tiles to a CTA of the longest sequence the table allows.
+    int splits = 1;
+    const i64 most = ((i64)A.blocks + 1) / 2;
+    if (units < held[dev][1].load(std::memory_order_relaxed)) {
+        double best = 1e30;
+        for (int s = 1; s <= 8 && (s == 1 || 2 * s <= most); ++s) {
+            const int n = held[dev][s].load(std::memory_order_relaxed);
+            if (n <= 0) continue;
+            const double cost = (double)((units + n - 1) / n) / s * (1 + 0.02 * (s - 1));
+            if (cost < best) best = cost, splits = s;
+        }
+    }
+    if (units * splits > 0x7fffffff) return TCQ_ERR_SHAPE;
+    cfg.gridDim = dim3((unsigned)(units * splits));
+    attr[0].val.clusterDim.x = splits;
+    cfg.numAttrs = 2;
+    return cudaLaunchKernelEx(&cfg, kern, A, row_tiles, tile_rows, splits) == cudaSuccess ? TCQ_OK : TCQ_ERR_LAUNCH;
 }
 
 // Arrival counters at the head of the workspace, one per worker.
@@ -707,13 +1177,11 @@ int tcq_kv8_attention(const tcq_kv8_cache* cache, const void* q, int dtype, int6
             return dtype == TCQ_DT_BF16 ? (alone ? go(yes, yes) : go(yes, no)) : (alone ? go(no, yes) : go(no, no));
         });
     }
-    const i64 all = (i64)B * T * heads;
-    if ((all + 3) / 4 > 0x7fffffff) return TCQ_ERR_SHAPE;
+    if (rows > 0x7fffffff) return TCQ_ERR_SHAPE;
     return by_head_dim(cache->head_dim, [&](auto d) {
         constexpr int D = decltype(d)::value;
-        return launch_pdl(dtype == TCQ_DT_BF16 ? k_attention_rows<TCQ_DT_BF16, D> : k_attention_rows<TCQ_DT_F16, D>,
-                          dim3((unsigned)((all + 3) / 4)), 128, 0, stream, *cache, (const u16*)q, (i64)q_sb, (i64)q_st, (u16*)out, table,
-                          blocks, lens, count, causal, scale, all, T, heads);
+        if (dtype == TCQ_DT_BF16) return rows <= kTile ? launch_many<TCQ_DT_BF16, D, 1>(A, stream) : launch_many<TCQ_DT_BF16, D, 2>(A, stream);
+        return rows <= kTile ? launch_many<TCQ_DT_F16, D, 1>(A, stream) : launch_many<TCQ_DT_F16, D, 2>(A, stream);
     });
 }
 
