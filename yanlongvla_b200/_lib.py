@@ -25,6 +25,16 @@ class Kv8Cache(ctypes.Structure):
     _fields_ = [('k', P), ('v', P), ('k_scale', P), ('v_scale', P), ('pages', I), ('kv_heads', I), ('head_dim', I)]
 
 
+
+# What the binding is handed: the C struct and the device its pointers belong to.
+class RopeHandle(ctypes.Structure):
+    _fields_ = [('plan', RopePlan), ('device', I)]
+
+
+class CacheHandle(ctypes.Structure):
+    _fields_ = [('cache', Kv8Cache), ('device', I)]
+
+
 # name -> argument types (every function returns int, except where noted)
 SIGNATURES = {
     'tcq_abi_version': [],

@@ -30,7 +30,7 @@ import ctypes
 
 import torch
 
-from . import _lib
+from . import _bind, _lib
 from ._lib import DT_BF16, DT_F16, DT_F32, DT_I32, TcqError, check, lib
 
 __all__ = ['quantize', 'pre', 'post', 'post3', 'postg', 'pre2', 'mid2', 'mid1', 'mid2_available', 'decode', 'decode_bf16', 'gemm_w8',
@@ -367,9 +367,9 @@ class RopeAxes:
             raise TcqError(f'RopeAxes: 1 to 4 sections that add up to {cos.shape[1]}, got {sections}')
         self.cos, self.sin, self.sections, self.pairs = cos, sin, sections, bool(pairs)
         self.axes, self.head_dim = len(sections), 2 * cos.shape[1]
-        self.plan = _lib.RopePlan(_p(cos), _p(sin), cos.shape[0], self.head_dim, self.axes, int(self.pairs),
-                                  (ctypes.c_int * 4)(*sections))
-        self.ref = ctypes.addressof(self.plan)
+        plan = _lib.RopePlan(_p(cos), _p(sin), cos.shape[0], self.head_dim, self.axes, int(self.pairs), (ctypes.c_int * 4)(*sections))
+        self._handle = _lib.RopeHandle(plan, cos.get_device())
+        self.ref = ctypes.addressof(self._handle)
 
     @staticmethod
     def tables(positions, head_dim, theta=10000.0, device='cuda'):
@@ -394,8 +394,8 @@ class KV8Cache:
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.pages, self.kv_heads, self.head_dim, self.width = pages, heads, D, heads * D
         self.device = k.device
-        self.cache = _lib.Kv8Cache(_p(k), _p(v), _p(k_scale), _p(v_scale), pages, heads, D)
-        self.ref = ctypes.addressof(self.cache)
+        self._handle = _lib.CacheHandle(_lib.Kv8Cache(_p(k), _p(v), _p(k_scale), _p(v_scale), pages, heads, D), k.get_device())
+        self.ref = ctypes.addressof(self._handle)
 
     @classmethod
     def empty(cls, pages, kv_heads, head_dim, device='cuda'):
@@ -404,36 +404,11 @@ class KV8Cache:
         return cls(k, torch.zeros(pages, kv_heads, head_dim, KV8_BLOCK, dtype=torch.int8, device=device), s[0], s[1])
 
 
-def _i32(what, t, *shape):
-    if t.dtype != torch.int32 or t.shape != shape or not t.is_cuda or not t.is_contiguous():
-        raise TcqError(f'{what} must be a contiguous int32 CUDA tensor of shape {shape}, got {t.dtype} {tuple(t.shape)}')
-    return t.data_ptr()
-
-
-def _rows(what, t, width=None):
-    """Type code and the (sequence, token) strides of t (B, T, width), whose rows are contiguous."""
-    if t.dim() != 3 or not t.is_cuda or t.stride(2) != 1 or (width is not None and t.shape[2] != width):
-        raise TcqError(f'{what} must be a CUDA tensor (B, T, {width or "heads * D"}) with contiguous rows, got {tuple(t.shape)}')
-    return t.stride(0), t.stride(1)
-
-
 def rope_axes(x, pos, rope, inverse=False, out=None):
     """Rotary embedding with several axes: x (B, T, heads * D) BF16 / F16 / F32 with contiguous rows, pos (axes, B, T) int32
     rows of the tables of `rope` (a RopeAxes). Of each pair a' = a c - b s, b' = a s + b c in FP32, one rounding per operation
     and one to the type. inverse=True turns back (the gradient of the forward turn). out may be x."""
-    B, T, W = x.shape
-    if W % rope.head_dim:
-        raise TcqError(f'rope_axes: rows of {W} are no multiple of the head width {rope.head_dim}')
-    if out is None:
-        out = torch.empty(B, T, W, dtype=x.dtype, device=x.device)
-    elif out.shape != x.shape or out.dtype != x.dtype:
-        raise TcqError('rope_axes: out must have the shape and type of x')
-    dt = _dt(x, (torch.bfloat16, torch.float16, torch.float32), 'rope_axes')
-    check(lib.tcq_rope_axes(_p(x), dt, *_rows('rope_axes: x', x), _p(out), *_rows('rope_axes: out', out),
-                            _i32('rope_axes: pos', pos, rope.axes, B, T), rope.ref, B, T, W // rope.head_dim, int(bool(inverse)),
-                            _stream()), 'tcq_rope_axes')
-    _count('rope_axes')
-    return out
+    return _bind.rope_axes(x, pos, rope, inverse, out)
 
 
 def kv8_append(cache, k, v, table, start, count=None, rope=None, pos=None):
@@ -441,35 +416,13 @@ def kv8_append(cache, k, v, table, start, count=None, rope=None, pos=None):
     start[b] + t of sequence b, in the pages of table (B, blocks) int32. With `rope` (a RopeAxes, half-split) and pos (axes, B, T),
     keys are first turned, in FP32. Per block and head s = max(s_old, max|x| / 127) over the call's tokens, q = rint(x * (1 / s));
     when s grows, the block's older tokens are rescaled. Pages written by one call must be distinct."""
-    B, T, _ = k.shape
-    dt = _dt(k, (torch.bfloat16, torch.float16), 'kv8_append')
-    if v.dtype != k.dtype or v.shape != k.shape:
-        raise TcqError('kv8_append: k and v must have the same shape and type')
-    if (rope is None) != (pos is None):
-        raise TcqError('kv8_append: give rope and pos, or neither')
-    check(lib.tcq_kv8_append(cache.ref, _p(k), *_rows('kv8_append: k', k, cache.width), _p(v), *_rows('kv8_append: v', v, cache.width), dt,
-                             _i32('kv8_append: table', table, B, table.shape[-1]), table.shape[-1], _i32('kv8_append: start', start, B),
-                             None if count is None else _i32('kv8_append: count', count, B),
-                             None if pos is None else _i32('kv8_append: pos', pos, rope.axes, B, T),
-                             None if rope is None else rope.ref, B, T, _stream()), 'tcq_kv8_append')
-    _count('kv8_append')
+    return _bind.kv8_append(cache, k, v, table, start, count, rope, pos)
 
 
 def kv8_read(cache, table, begin, lens, tokens, dtype=torch.bfloat16, out=None):
     """The values a cache stands for: tokens begin[b] .. begin[b] + tokens - 1 of each sequence as (k, v), each (B, tokens,
     kv_heads * D) of dtype (BF16 / F16 / F32), zero from token lens[b] on. out: a pair of tensors to write to."""
-    B, T = table.shape[0], int(tokens)
-    if out is None:
-        out = tuple(torch.empty(B, T, cache.width, dtype=dtype, device=cache.device) for _ in range(2))
-    k, v = out
-    _cuda(k, v)
-    if k.shape != (B, T, cache.width) or v.shape != k.shape or v.dtype != k.dtype:
-        raise TcqError(f'kv8_read: out must be two tensors ({B}, {T}, {cache.width}) of one type')
-    check(lib.tcq_kv8_read(cache.ref, _p(k), _p(v), _dt(k, (torch.bfloat16, torch.float16, torch.float32), 'kv8_read'),
-                           _i32('kv8_read: table', table, B, table.shape[-1]), table.shape[-1], _i32('kv8_read: begin', begin, B),
-                           _i32('kv8_read: lens', lens, B), B, T, _stream()), 'tcq_kv8_read')
-    _count('kv8_read')
-    return out
+    return _bind.kv8_read(cache, table, begin, lens, tokens, dtype, out)
 
 
 def kv8_attention(q, cache, table, lens, count=None, causal=True, scale=None, out=None):
@@ -477,37 +430,12 @@ def kv8_attention(q, cache, table, lens, count=None, causal=True, scale=None, ou
     head h reads key head h // (heads / kv_heads). lens (B,) int32: tokens in the cache, the new ones among them; query t of the
     count[b] (None: T) queries sits at token lens[b] - count[b] + t and, when causal, sees the tokens up to its own. scale None:
     D^-0.5. Returns out (B, T, heads * D) of q's type; rows that see no token, or past count[b], are zero."""
-    B, T, W = q.shape
-    D = cache.head_dim
-    heads = W // D
-    if W % D or heads % cache.kv_heads:
-        raise TcqError(f'kv8_attention: {W} columns are no multiple of {cache.kv_heads} key heads of {D}')
-    if out is None:
-        out = torch.empty(B, T, W, dtype=q.dtype, device=q.device)
-    elif out.shape != q.shape or out.dtype != q.dtype:
-        raise TcqError('kv8_attention: out must have the shape and type of q')
-    _cuda(out)
-    blocks = table.shape[-1]
-    ws = _memory_workspace(lib.tcq_kv8_attention_workspace(B, T, heads, cache.kv_heads, D, blocks), q.device)
-    check(lib.tcq_kv8_attention(cache.ref, _p(q), _dt(q, (torch.bfloat16, torch.float16), 'kv8_attention'),
-                                *_rows('kv8_attention: q', q), _p(out), _i32('kv8_attention: table', table, B, blocks), blocks,
-                                _i32('kv8_attention: lens', lens, B), None if count is None else _i32('kv8_attention: count', count, B),
-                                int(bool(causal)), D ** -0.5 if scale is None else float(scale), B, T, heads, _p(ws), ws.numel() * 4,
-                                _stream()), 'tcq_kv8_attention')
-    _count('kv8_attention')
-    return out
+    return _bind.kv8_attention(q, cache, table, lens, count, causal, scale, out)
 
 
-_MEMORY_WS = {}
-
-
-def _memory_workspace(need, device):
-    """Workspace of tcq_kv8_attention for the current stream (zero-filled once, left ready by every call; grown on demand)."""
-    key = (device, _stream())
-    ws = _MEMORY_WS.get(key)
-    if ws is None or ws.numel() * 4 < need:
-        ws = _MEMORY_WS[key] = torch.zeros((need + 3) // 4, dtype=torch.int32, device=device)
-    return ws
+_bind.init({name: ctypes.cast(getattr(lib, name), ctypes.c_void_p).value
+            for name in ('tcq_status_string', 'tcq_rope_axes', 'tcq_kv8_append', 'tcq_kv8_read', 'tcq_kv8_attention_workspace',
+                         'tcq_kv8_attention')}, TcqError, LAUNCHES, RopeAxes, KV8Cache)
 
 
 # ------------------------------------------------------------------------------------------------ trellis weights
