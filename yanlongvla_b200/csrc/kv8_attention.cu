@@ -40,14 +40,14 @@ TCQ_HD int queries_of(const int* count, i64 b, int T) {
     }
     return n;
 }
-TCQ_HD int page_of(const int* row, int blk, int pages) {
-    const int p = row[blk];
+TCQ_HD int page_in(int p, int pages) {
     if ((unsigned)p >= (unsigned)pages) {
         out_of_range();
         return p < 0 ? 0 : pages - 1;
     }
     return p;
 }
+TCQ_HD int page_of(const int* row, int blk, int pages) { return page_in(row[blk], pages); }
 
 // ------------------------------------------------------------------------------------------------ few query rows
 // T * group <= 16 MT query rows share a key head (single tokens, short action sequences): the kernel streams the pages once and
@@ -615,7 +615,10 @@ struct Many {
     static constexpr int Q0 = 0, K0 = NG * QB, V0 = K0 + NS * KB, BAR0 = V0 + NS * VB;
     static constexpr int ML0 = BAR0 + 256;                            // m, l of every row (cluster sums)
     static constexpr int BYTES = ML0 + NG * kTile * 8 + 1024;         // + slack to align the base to 1024
-    static constexpr int THREADS = NG * 128 + 160;
+    // Threads and registers. With two groups the CTA is launched with 128 registers a thread (512 x 128 = the SM's 65,536), of
+    // which the softmax warps take more and the others less: 256 x 168 + 256 x 88.
+    static constexpr int THREADS = NG == 2 ? 512 : 288;
+    static constexpr int POLY = D >= 96 ? 3 : 5;                      // of 16 pairs of weights, those formed by polynomial
     static constexpr u32 COLS = NG == 2 ? 512 : 256;
     static constexpr int S0 = 0, O0 = NG * kTile;                     // TMEM columns: scores, outputs
     static constexpr int PARTS = NG * kTile * D * 4;                  // a CTA's part of the outputs, over the tiles
@@ -673,6 +676,42 @@ __device__ __forceinline__ void tmem_ld_wait(u32 (&v)[N]) {
 #pragma unroll
     for (int j = 0; j < N; ++j) asm volatile("" : "+r"(v[j]));
 }
+// Pairs of FP32 values in one instruction.
+TCQ_HD u64 pair(float lo, float hi) {
+    u64 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+TCQ_HD void unpair(u64 v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+TCQ_HD u64 fma2(u64 a, u64 b, u64 c) {
+    u64 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+TCQ_HD u64 add2(u64 a, u64 b) {
+    u64 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
+// 2^x for a pair, x <= 126, values below 2^-126 as 2^-126 (zero once rounded to FP16), without the exponential unit, which
+// forms 16 results per clock and SM and is the kernel's narrowest pipe: x = n + f with |f| <= 1/2 (n by adding and
+// subtracting 1.5 * 2^23), a cubic fitted to 2^f for the least relative error (7.5e-5, against 4.9e-4 of the weight's
+// rounding to FP16), n added to its exponent.
+TCQ_HD u64 ex2_poly(u64 x) {
+    float lo, hi;
+    unpair(x, lo, hi);
+    x = pair(fmaxf(lo, -126.f), fmaxf(hi, -126.f));
+    const u64 t = add2(x, pair(12582912.f, 12582912.f)), n = add2(t, pair(-12582912.f, -12582912.f));
+    const u64 f = fma2(n, pair(-1.f, -1.f), x);
+    u64 p = fma2(f, pair(0.0551716685f, 0.0551716685f), pair(0.2426111251f, 0.2426111251f));
+    p = fma2(p, f, pair(0.6932609677f, 0.6932609677f));
+    p = fma2(p, f, pair(0.9999280572f, 0.9999280572f));
+    float tl, th;
+    unpair(t, tl, th);
+    unpair(p, lo, hi);
+    return pair(__uint_as_float(__float_as_uint(lo) + (__float_as_uint(tl) << 23)), __uint_as_float(__float_as_uint(hi) + (__float_as_uint(th) << 23)));
+}
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void async_proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
@@ -708,7 +747,7 @@ template <int DT, int D, int NG>
 __global__ void __launch_bounds__(Many<D, NG>::THREADS, NG == 1 && D <= 64 ? 2 : 1)
 k_attention_many(const AttnArgs A, int row_tiles, int tile_rows, int splits) {
     typedef Many<D, NG> P;
-    constexpr int KS = D / 16, NC = D / 16;             // contraction steps; 16-byte chunks of a half tile per convert thread
+    constexpr int KS = D / 16, NC = (4 * D + 127) / 128;      // contraction steps; 16-byte chunks of a page per convert thread
     extern __shared__ char smem_raw[];
     char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     const u32 sbase = smem_u32(smem), bars = sbase + P::BAR0;
@@ -758,6 +797,10 @@ k_attention_many(const AttnArgs A, int row_tiles, int tile_rows, int splits) {
     const int* trow = A.table + (i64)b * A.blocks;
 
     float m = -INFINITY, l = 0.f;
+    if (NG == 2) {
+        if (warp < W_CONV) asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
+        else asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    }
     if (warp < W_CONV) {
         // ------------------------------------------------------------------------------------------------ softmax
         const int g = warp >> 2, gl = tid & 127, r = r0 + g * kTile + gl, tq = r / A.group;
@@ -796,50 +839,58 @@ k_attention_many(const AttnArgs A, int row_tiles, int tile_rows, int splits) {
             mbar_arrive(bar(BAR_Q));
         }
         const u32 lanes = (u32)((warp & 3) * 32) << 16, ts = tmem + lanes + P::S0 + g * kTile, to = tmem + lanes + P::O0 + g * D;
-        // the scales of the next tile's two pages are requested a tile ahead
-        auto page = [&](int p) -> i64 { return p < pages ? (i64)page_of(trow, p, A.cache.pages) * Hk + h : -1; };
-        i64 pg0 = -1, pg1 = -1;
-        float nk0 = 0.f, nk1 = 0.f, nv0 = 1.f, nv1 = 1.f;
-        auto request = [&](int i) {
+        // the scales of the next tile's two pages are requested a tile ahead, the pages' numbers two
+        int id0 = 0, id1 = 0;
+        float nk[2] = {}, nv[2] = {1.f, 1.f};
+        auto request_ids = [&](int i) {
             if (i < k1) {
-                pg0 = page(2 * i), pg1 = page(2 * i + 1);
-                nk0 = A.cache.k_scale[pg0], nv0 = A.cache.v_scale[pg0];
-                nk1 = pg1 >= 0 ? A.cache.k_scale[pg1] : 0.f, nv1 = pg1 >= 0 ? A.cache.v_scale[pg1] : 1.f;
+                id0 = trow[2 * i];
+                id1 = trow[min(2 * i + 1, pages - 1)];
             }
         };
-        request(k0);
-#pragma unroll 1
-        for (int i = k0; i < k1; ++i) {
-            const float c[2] = {crow * nk0, crow * nk1}, vsc[2] = {nv0, nv1};
-            request(i + 1);
+        auto request_scales = [&](int i) {
+            if (i < k1) {
+                const i64 p0 = (i64)page_in(id0, A.cache.pages) * Hk + h, p1 = (i64)page_in(id1, A.cache.pages) * Hk + h;
+                nk[0] = A.cache.k_scale[p0], nv[0] = A.cache.v_scale[p0];
+                nk[1] = A.cache.k_scale[p1], nv[1] = A.cache.v_scale[p1];
+            }
+        };
+        request_ids(k0);
+        request_scales(k0);
+        request_ids(k0 + 1);
+        auto tile = [&](auto masked_c, int i, const float (&c)[2], const float (&vsc)[2]) {
+            constexpr bool MASKED = decltype(masked_c)::value;
             float bias[2], inv[2];
 #pragma unroll
             for (int p = 0; p < 2; ++p) {
                 const float vs = safe_scale(vsc[p]);
                 bias[p] = lg2(vs), inv[p] = 1.f / vs;
             }
-            if (!wait(BAR_SFULL + g, i - k0)) break;
-            tc_after();
-            const bool masked = (i + 1) * kTile > open;
             const int lim = limit - i * kTile;
+            // largest score of the row: four chains, the next 32 columns on their way
+            u32 v[2][32];
             float top = -INFINITY;
+            tmem_ld32(ts, v[0]);
 #pragma unroll
             for (int p = 0; p < 2; ++p) {
-                float raw = -INFINITY;
-                u32 v[2][32];
-                tmem_ld32(ts + 64 * p, v[0]);
-                tmem_ld32(ts + 64 * p + 32, v[1]);
-                tmem_ld_wait(v[0]);
-                tmem_ld_wait(v[1]);
-                if (masked) {
+                float raw[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                    for (int j = 0; j < 64; ++j)
-                        if (64 * p + j < lim) raw = fmaxf(raw, __uint_as_float(v[j >> 5][j & 31]));
-                } else {
+                for (int hf = 0; hf < 2; ++hf) {
+                    const int ch = 2 * p + hf;
+                    tmem_ld_wait(v[ch & 1]);
+                    tmem_ld32(ts + (ch < 3 ? 32 * (ch + 1) : 0), v[(ch + 1) & 1]);
 #pragma unroll
-                    for (int j = 0; j < 64; ++j) raw = fmaxf(raw, __uint_as_float(v[j >> 5][j & 31]));
+                    for (int j = 0; j < 32; j += 2) {
+                        float x = __uint_as_float(v[ch & 1][j]), y = __uint_as_float(v[ch & 1][j + 1]);
+                        if (MASKED) {
+                            x = 32 * ch + j < lim ? x : -INFINITY;
+                            y = 32 * ch + j + 1 < lim ? y : -INFINITY;
+                        }
+                        raw[(j >> 1) & 3] = fmaxf(raw[(j >> 1) & 3], fmaxf(x, y));
+                    }
                 }
-                if (raw != -INFINITY) top = fmaxf(top, __fmaf_rn(raw, c[p], bias[p]));
+                const float r = fmaxf(fmaxf(raw[0], raw[1]), fmaxf(raw[2], raw[3]));
+                if (!MASKED || r != -INFINITY) top = fmaxf(top, __fmaf_rn(r, c[p], bias[p]));
             }
             const bool move = top > m + kSlack;
             if (__any_sync(0xffffffffu, move)) {
@@ -862,25 +913,50 @@ k_attention_many(const AttnArgs A, int row_tiles, int tile_rows, int splits) {
 #pragma unroll
             for (int ch = 0; ch < 4; ++ch) {
                 const int p = ch >> 1;
-                u32 v[32], w[16];
-                tmem_ld32(ts + 32 * ch, v);
-                tmem_ld_wait(v);
-                const float add = bias[p] - base;
-                float sum = 0.f;
+                u32(&x)[32] = v[ch & 1];
+                tmem_ld_wait(x);
+                if (ch < 3) tmem_ld32(ts + 32 * (ch + 1), v[(ch + 1) & 1]);
+                const u64 c2 = pair(c[p], c[p]), a2 = pair(bias[p] - base, bias[p] - base);
+                u64 sum[2] = {0, 0};
+                u32 w[16];
 #pragma unroll
-                for (int j = 0; j < 32; ++j) {
-                    float x = __fmaf_rn(__uint_as_float(v[j]), c[p], add);
-                    if (masked && 32 * ch + j >= lim) x = -INFINITY;
-                    x = ex2(x);
-                    sum += x;
-                    v[j] = __float_as_uint(x);
+                for (int j = 0; j < 16; ++j) {
+                    u64 y = fma2(pair(__uint_as_float(x[2 * j]), __uint_as_float(x[2 * j + 1])), c2, a2);
+                    float lo, hi;
+                    if (!MASKED && j % 16 < P::POLY) {
+                        y = ex2_poly(y);
+                        unpair(y, lo, hi);
+                    } else {
+                        unpair(y, lo, hi);
+                        if (MASKED) {
+                            lo = 32 * ch + 2 * j < lim ? lo : -INFINITY;
+                            hi = 32 * ch + 2 * j + 1 < lim ? hi : -INFINITY;
+                        }
+                        lo = ex2(lo), hi = ex2(hi);
+                        y = pair(lo, hi);
+                    }
+                    sum[j & 1] = add2(sum[j & 1], y);
+                    w[j] = half2_of(lo, hi);
                 }
-                l = __fmaf_rn(sum, inv[p], l);
-                const bool mute = vsc[p] < kLeastScale;
+                float lo, hi;
+                unpair(add2(sum[0], sum[1]), lo, hi);
+                l = __fmaf_rn(lo + hi, inv[p], l);
+                if (vsc[p] < kLeastScale) {
 #pragma unroll
-                for (int j = 0; j < 16; ++j) w[j] = mute ? 0u : half2_of(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]));
+                    for (int j = 0; j < 16; ++j) w[j] = 0u;
+                }
                 tmem_st16(ts + 16 * ch, w);
             }
+        };
+#pragma unroll 1
+        for (int i = k0; i < k1; ++i) {
+            const float c[2] = {crow * nk[0], crow * nk[1]}, vsc[2] = {nv[0], nv[1]};
+            request_scales(i + 1);
+            request_ids(i + 2);
+            if (!wait(BAR_SFULL + g, i - k0)) break;
+            tc_after();
+            if ((i + 1) * kTile > open) tile(std::true_type(), i, c, vsc);
+            else tile(std::false_type(), i, c, vsc);
             tmem_st_wait();
             tc_before();
             mbar_arrive(bar(BAR_PFULL + g));
@@ -928,62 +1004,76 @@ k_attention_many(const AttnArgs A, int row_tiles, int tile_rows, int splits) {
         }
     } else if (warp < W_MMA) {
         // ------------------------------------------------------------------------------------------------ convert
+        // Steps of a tile: its two pages' keys, its two pages' values. A step's INT8 data is requested AHEAD steps before its
+        // use, the pages' numbers a tile before that.
         const int ct = tid - W_CONV * 32;
-        uint4 next[NC];
-        // half tile j: keys (even) or values (odd) of tile k0 + j / 2
-        auto request = [&](int j) {
-            const int i = k0 + (j >> 1);
+        int id[2] = {};
+        constexpr int AHEAD = D > 96 ? 2 : 4;            // steps between a request and its use
+        uint4 next[AHEAD][NC];
+        auto request_ids = [&](int i) {
+            if (i < k1) id[0] = trow[2 * i], id[1] = trow[min(2 * i + 1, pages - 1)];
+        };
+        auto request = [&](int i, int j, const int (&ids)[2]) {
             if (i >= k1) return;
-            const int p1 = 2 * i + 1;
-            const i64 step = (i64)(kBlk * D);
-            const i8* src = (j & 1) ? A.cache.v : A.cache.k;
-            const i8* s0 = src + ((i64)page_of(trow, 2 * i, A.cache.pages) * Hk + h) * step;
-            const i8* s1 = p1 < pages ? src + ((i64)page_of(trow, p1, A.cache.pages) * Hk + h) * step : nullptr;
+            const bool there = 2 * i + (j & 1) < pages;
+            const i8* src = (j & 2 ? A.cache.v : A.cache.k) + ((i64)page_in(ids[j & 1], A.cache.pages) * Hk + h) * (i64)(kBlk * D);
 #pragma unroll
             for (int n = 0; n < NC; ++n) {
                 const int c = ct + 128 * n;
-                const i8* s = c < 4 * D ? s0 + c * 16 : s1 ? s1 + (c - 4 * D) * 16 : nullptr;
-                next[n] = s ? *reinterpret_cast<const uint4*>(s) : make_uint4(0, 0, 0, 0);
+                next[j % AHEAD][n] = there && (NC * 128 == 4 * D || c < 4 * D) ? *reinterpret_cast<const uint4*>(src + c * 16) : make_uint4(0, 0, 0, 0);
             }
         };
-        request(0);
-        const int halves = 2 * (k1 - k0);
+        request_ids(k0);
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) request(k0, j, id);
+        int now[2] = {id[0], id[1]};
+        request_ids(k0 + 1);
 #pragma unroll 1
-        for (int j = 0; j < halves; ++j) {
-            const int it = j >> 1, s = it & 1, use = it >> 1;
-            uint4 cur[NC];
+        for (int i = k0; i < k1; ++i) {
+            const int it = i - k0, s = it & 1, use = it >> 1;
+            const int ids[2] = {id[0], id[1]};
+            request_ids(i + 2);
+            bool ok = true;
 #pragma unroll
-            for (int n = 0; n < NC; ++n) cur[n] = next[n];
-            request(j + 1);
-            if (!wait(((j & 1) ? BAR_VEMPTY : BAR_KEMPTY) + s, use + 1)) break;
-            char* dst = smem + ((j & 1) ? P::V0 + s * P::VB : P::K0 + s * P::KB);
+            for (int j = 0; j < 4; ++j) {
+                if (j == 0) ok = wait(BAR_KEMPTY + s, use + 1);
+                if (j == 2) ok = ok && wait(BAR_VEMPTY + s, use + 1);
+                if (!ok) break;
 #pragma unroll
-            for (int n = 0; n < NC; ++n) {
-                const int c = ct + 128 * n, p = c >= 4 * D, cc = c - p * 4 * D;
-                int row, ch;
-                char* t;
-                if (j & 1) {
-                    row = cc >> 2, ch = 2 * (cc & 3);
-                    t = dst + p * (D * 128);
-                } else {
-                    row = cc / (D / 16);
-                    const int x = cc - row * (D / 16);
-                    row += 64 * p, ch = 2 * (x & 3);
-                    t = dst + (x >> 2) * (kTile * 128);
+                for (int n = 0; n < NC; ++n) {
+                    const int c = ct + 128 * n;
+                    if (NC * 128 != 4 * D && c >= 4 * D) break;
+                    int row, ch;
+                    char* t;
+                    if (j & 2) {
+                        row = c >> 2, ch = 2 * (c & 3);
+                        t = smem + P::V0 + s * P::VB + (j & 1) * (D * 128);
+                    } else {
+                        row = c / (D / 16);
+                        const int x = c - row * (D / 16);
+                        row += 64 * (j & 1), ch = 2 * (x & 3);
+                        t = smem + P::K0 + s * P::KB + (x >> 2) * (kTile * 128);
+                    }
+                    u32 w[8];
+                    int8x4_to_half(next[j % AHEAD][n].x, w[0], w[1]);
+                    int8x4_to_half(next[j % AHEAD][n].y, w[2], w[3]);
+                    int8x4_to_half(next[j % AHEAD][n].z, w[4], w[5]);
+                    int8x4_to_half(next[j % AHEAD][n].w, w[6], w[7]);
+                    t += row * 128;
+                    *reinterpret_cast<uint4*>(t + ((ch ^ (row & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+                    *reinterpret_cast<uint4*>(t + (((ch + 1) ^ (row & 7)) << 4)) = make_uint4(w[4], w[5], w[6], w[7]);
                 }
-                u32 w[8];
-                int8x4_to_half(cur[n].x, w[0], w[1]);
-                int8x4_to_half(cur[n].y, w[2], w[3]);
-                int8x4_to_half(cur[n].z, w[4], w[5]);
-                int8x4_to_half(cur[n].w, w[6], w[7]);
-                t += row * 128;
-                *reinterpret_cast<uint4*>(t + ((ch ^ (row & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
-                *reinterpret_cast<uint4*>(t + (((ch + 1) ^ (row & 7)) << 4)) = make_uint4(w[4], w[5], w[6], w[7]);
+                if (j + AHEAD < 4) request(i, j + AHEAD, now);
+                else request(i + 1, j + AHEAD - 4, ids);
+                if (j & 1) {
+                    async_proxy_fence();
+                    mbar_arrive(bar((j & 2 ? BAR_VFULL : BAR_KFULL) + s));
+                }
             }
-            async_proxy_fence();
-            mbar_arrive(bar(((j & 1) ? BAR_VFULL : BAR_KFULL) + s));
+            if (!ok) break;
+            now[0] = ids[0], now[1] = ids[1];
         }
-    } else if (lane == 0 && k1 > k0) {
+    } else if (warp == W_MMA && lane == 0 && k1 > k0) {
         // ------------------------------------------------------------------------------------------------ product
         auto scores = [&](int g, int s) {
             const u32 qa = sbase + P::Q0 + g * P::QB, ka = sbase + P::K0 + s * P::KB;
@@ -1031,6 +1121,12 @@ k_attention_many(const AttnArgs A, int row_tiles, int tile_rows, int splits) {
     tc_before();
     __syncthreads();
     tc_after();
+    // Back to the launch's registers for the code that all warps share: only behind the barrier, when every softmax warp has
+    // had its larger share (a warp that took its registers back before could keep them from one forever).
+    if (NG == 2) {
+        if (warp < W_CONV) asm volatile("setmaxnreg.dec.sync.aligned.u32 128;");
+        else asm volatile("setmaxnreg.inc.sync.aligned.u32 128;");
+    }
     if (warp == W_MMA) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(P::COLS) : "memory");
     if (splits == 1) return;
 
