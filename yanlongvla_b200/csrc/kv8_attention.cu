@@ -53,12 +53,12 @@ TCQ_HD int page_of(const int* row, int blk, int pages) { return page_in(row[blk]
 // T * group <= 16 MT query rows share a key head (single tokens, short action sequences): the kernel streams the pages once and
 // is bound by HBM.
 //
-// Mathematics. With integers k, v and block scales ks, vs: score x = (q . k) ks scale log2(e) + log2(vs), reference m >= x - 4,
-// weight p = 2^(x - m + 10); out = sum p v / sum (p / vs). Folding vs into the exponent keeps every product operand an exact
+// Mathematics. With integers k, v and block scales ks, vs: score x = (q . k) ks scale log2(e) + log2(vs), reference
+// m >= x - 10.5, weight p = 2^(x - m + 5); out = sum p v / sum (p / vs). Folding vs into the exponent keeps every product operand an exact
 // small integer or one rounding of p, and the sum of p is formed before that rounding. m moves only when a score passes it
-// by more than 2^4, so the accumulators are rarely rescaled. Operands are FP16: an int8 is exact, a query row is scaled by a
+// by more than 10.5, so the accumulators are rarely rescaled. Operands are FP16: an int8 is exact, a query row is scaled by a
 // power of two so that its largest element lies in [2^14, 2^15) (elements below 2^-28 of it lose bits, those of BF16
-// inputs above that lose none), and p <= 2^14 keeps 11 bits down to 2^-28 of the largest and is dropped below 2^-38.
+// inputs above that lose none), and p <= 2^15.5 keeps 11 bits down to 2^-19 of the reference's and is dropped below 2^-30 of it.
 //
 // Layout. A warp takes whole pages. S = Q K^T and O = P V are m16n8k16 products. The order of a contraction is free, so lane
 // (n, t) reads 16 consecutive bytes of key row n (or of value row n: 16 tokens) and feeds them to four products: one 16-byte
@@ -68,8 +68,8 @@ TCQ_HD int page_of(const int* row, int blk, int pages) { return page_in(row[blk]
 // int8 -> FP16: u = byte ^ 0x80, 0x6400 | u is 1024 + u, minus 1152: five instructions for four elements.
 
 constexpr int kWarps = 8;
-constexpr float kRef = 10.f;          // log2 of the weight of a score equal to the reference
-constexpr float kSlack = 4.f;         // growth of the maximum that does not move the reference
+constexpr float kRef = 5.f;           // log2 of the weight of a score equal to the reference
+constexpr float kSlack = 10.5f;       // growth of the maximum that does not move the reference: weights up to 2^15.5
 
 TCQ_HD float ex2(float x) {
     float y;
@@ -131,7 +131,8 @@ struct Few {
     static constexpr int HDR = RING;                                       // ks, vs of each half page
     static constexpr int ML = HDR + kWarps * NH * 8;                       // m, l of every warp and row
     static constexpr int MERGE = ML + (W > 1 ? kWarps * 16 * MT * 8 : 0);  // one group of 8 rows of every warp
-    static constexpr int BYTES = MERGE + (W > 1 ? kWarps * 8 * (D + PAD) * 4 : 0);
+    static constexpr int SCAN = MERGE + (W > 1 ? kWarps * 8 * (D + PAD) * 4 : 0);
+    static constexpr int BYTES = SCAN + 64;
 };
 
 // 16-byte chunk c of key row r lies at chunk c ^ swap(r): rows of 128 bytes put their halves on alternating banks.
@@ -149,7 +150,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) k_attention_few(const AttnArgs
     typedef Few<D, MT, W> P;
     constexpr int NH = P::NH, KS = D / 16, ROWS = 16 * MT;
     extern __shared__ __align__(16) char smem[];
-    __shared__ int s_scan[kWarps + 4];
+    int* s_scan = reinterpret_cast<int*>(smem + P::SCAN);
     pdl_launch_dependents();
     pdl_wait();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, n = lane >> 2, t = lane & 3;
@@ -596,7 +597,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) k_attention_few(const AttnArgs
 //             shared memory, 128-byte swizzled, keys K-major along the head, values K-major along the tokens;
 //   product   one thread issues S = Q K^T (both operands in shared memory) and O += P V (P in TMEM).
 // The two groups alternate: while one's weights are formed, the other's products run. Mathematics, scaling of the queries and
-// handling of the scales are those of the few-row kernel; the reference m moves only when a score passes it by 2^4, and O (in
+// handling of the scales are those of the few-row kernel; the reference m moves only when a score passes it by 10.5, and O (in
 // TMEM) is rescaled by its own row's thread. S of a tile is issued after O of the tile before it, and a commit covers every
 // product issued before it: scores that have arrived mean that O is complete up to the tile before.
 //
@@ -612,13 +613,19 @@ struct Many {
     static constexpr int KB = kTile * 128 * ATOMS;                    // of a tile's keys
     static constexpr int VB = D * 128 * 2;                            // of its values
     static constexpr int NS = 2;                                      // tiles of either in flight
-    static constexpr int Q0 = 0, K0 = NG * QB, V0 = K0 + NS * KB, BAR0 = V0 + NS * VB;
+    static constexpr int PAGE = kBlk * D;                             // bytes of a page's keys or values
+    static constexpr int RING = 4;                                    // INT8 pages on their way (a tile's keys and values)
+    static constexpr int Q0 = 0, K0 = NG * QB, V0 = K0 + NS * KB, STAGE0 = V0 + NS * VB, BAR0 = STAGE0 + RING * PAGE;
     static constexpr int ML0 = BAR0 + 256;                            // m, l of every row (cluster sums)
-    static constexpr int BYTES = ML0 + NG * kTile * 8 + 1024;         // + slack to align the base to 1024
+    static constexpr int BYTES = ML0 + NG * kTile * 8;
     // Threads and registers. With two groups the CTA is launched with 128 registers a thread (512 x 128 = the SM's 65,536), of
-    // which the softmax warps take more and the others less: 256 x 168 + 256 x 88.
+    // which the softmax warps take more and the others less: 256 x 192 + 256 x 64.
     static constexpr int THREADS = NG == 2 ? 512 : 288;
-    static constexpr int POLY = D >= 96 ? 3 : 5;                      // of 16 pairs of weights, those formed by polynomial
+    static constexpr int CONV = THREADS - NG * 128 - 32;             // convert threads: what softmax and the product warp leave
+    #ifndef POLYN
+#define POLYN 5
+#endif
+    static constexpr int POLY = POLYN;                      // of 16 pairs of weights, those formed by polynomial
     static constexpr u32 COLS = NG == 2 ? 512 : 256;
     static constexpr int S0 = 0, O0 = NG * kTile;                     // TMEM columns: scores, outputs
     static constexpr int PARTS = NG * kTile * D * 4;                  // a CTA's part of the outputs, over the tiles
@@ -641,6 +648,12 @@ __device__ __forceinline__ void mma_ts(u32 d, u32 a, u64 b, u32 idesc, u32 acc) 
 }
 __device__ __forceinline__ void mma_commit(u32 bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+// True in one lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+    u32 r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+    return r != 0;
 }
 __device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -676,6 +689,12 @@ __device__ __forceinline__ void tmem_ld_wait(u32 (&v)[N]) {
 #pragma unroll
     for (int j = 0; j < N; ++j) asm volatile("" : "+r"(v[j]));
 }
+TCQ_HD float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
 // Pairs of FP32 values in one instruction.
 TCQ_HD u64 pair(float lo, float hi) {
     u64 r;
@@ -740,31 +759,37 @@ __device__ __forceinline__ float2 peer_ld2(u32 addr) {
     return v;
 }
 
+// 16 bytes to shared memory, zeros when !there.
+__device__ __forceinline__ void cp_async16_zfill(u32 dst, const void* src, bool there) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+
 // The barriers of a CTA, 8 bytes each from BAR0.
-enum { BAR_KFULL = 0, BAR_KEMPTY = 2, BAR_VFULL = 4, BAR_VEMPTY = 6, BAR_SFULL = 8, BAR_PFULL = 10, BAR_Q = 12, BAR_O = 13, BAR_COUNT = 14 };
+enum { BAR_KFULL = 0, BAR_KEMPTY = 2, BAR_VFULL = 4, BAR_VEMPTY = 6, BAR_SFULL = 8, BAR_PFULL = 10, BAR_Q = 14, BAR_O = 15, BAR_COUNT = 16 };
 
 template <int DT, int D, int NG>
 __global__ void __launch_bounds__(Many<D, NG>::THREADS, NG == 1 && D <= 64 ? 2 : 1)
 k_attention_many(const AttnArgs A, int row_tiles, int tile_rows, int splits) {
     typedef Many<D, NG> P;
-    constexpr int KS = D / 16, NC = (4 * D + 127) / 128;      // contraction steps; 16-byte chunks of a page per convert thread
-    extern __shared__ char smem_raw[];
-    char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    constexpr int KS = D / 16, NC = (8 * D + P::CONV - 1) / P::CONV;      // contraction steps; 16-byte chunks of half a tile per convert thread
+    extern __shared__ __align__(1024) char smem_tiles[];
+    char* const smem = smem_tiles;
     const u32 sbase = smem_u32(smem), bars = sbase + P::BAR0;
     u32* tmem_slot = reinterpret_cast<u32*>(smem + P::BAR0 + 8 * BAR_COUNT);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    constexpr int W_CONV = NG * 4, W_MMA = W_CONV + 4;
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+    constexpr int W_MMA = NG * 4, W_CONV = W_MMA + 1;
     auto bar = [&](int i) -> u32 { return bars + 8 * i; };
-    auto wait = [&](int i, u32 parity) -> bool { return mbar_wait_bounded(bar(i), parity & 1, abort_flag, &g_tcq_attention_error); };
+    auto wait = [&](int i, u32 parity) -> bool { return mbar_wait_suspended(bar(i), parity & 1, abort_flag, &g_tcq_attention_error); };
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) {
-            mbar_init(bar(BAR_KFULL + i), 128);
-            mbar_init(bar(BAR_VFULL + i), 128);
+            mbar_init(bar(BAR_KFULL + i), P::CONV / 32);    // one arrival per convert warp
+            mbar_init(bar(BAR_VFULL + i), P::CONV / 32);
             mbar_init(bar(BAR_KEMPTY + i), 1);
             mbar_init(bar(BAR_VEMPTY + i), 1);
             mbar_init(bar(BAR_SFULL + i), 1);
-            mbar_init(bar(BAR_PFULL + i), 128);
+            mbar_init(bar(BAR_PFULL + i), 4);               // per softmax warp; group and page at 2 g + p
+            mbar_init(bar(BAR_PFULL + 2 + i), 4);
         }
         mbar_init(bar(BAR_Q), NG * 128);
         mbar_init(bar(BAR_O), 1);
@@ -798,10 +823,10 @@ k_attention_many(const AttnArgs A, int row_tiles, int tile_rows, int splits) {
 
     float m = -INFINITY, l = 0.f;
     if (NG == 2) {
-        if (warp < W_CONV) asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
-        else asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+        if (warp < W_MMA) asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
+        else asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
     }
-    if (warp < W_CONV) {
+    if (warp < W_MMA) {
         // ------------------------------------------------------------------------------------------------ softmax
         const int g = warp >> 2, gl = tid & 127, r = r0 + g * kTile + gl, tq = r / A.group;
         const bool live = r < r1 && tq < cnt;
@@ -866,34 +891,29 @@ k_attention_many(const AttnArgs A, int row_tiles, int tile_rows, int splits) {
                 const float vs = safe_scale(vsc[p]);
                 bias[p] = lg2(vs), inv[p] = 1.f / vs;
             }
-            const int lim = limit - i * kTile;
-            // largest score of the row: four chains, the next 32 columns on their way
+            // A page's 64 scores at a time. The second page's are read, and the row's reference settled, before the first
+            // page's weights are handed over: until then no product reads or adds to this row.
             u32 v[2][32];
-            float top = -INFINITY;
-            tmem_ld32(ts, v[0]);
-#pragma unroll
-            for (int p = 0; p < 2; ++p) {
+            auto page_top = [&](int p, int lim) -> float {
                 float raw[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int hf = 0; hf < 2; ++hf) {
-                    const int ch = 2 * p + hf;
-                    tmem_ld_wait(v[ch & 1]);
-                    tmem_ld32(ts + (ch < 3 ? 32 * (ch + 1) : 0), v[(ch + 1) & 1]);
+                for (int hf = 0; hf < 2; ++hf)
 #pragma unroll
                     for (int j = 0; j < 32; j += 2) {
-                        float x = __uint_as_float(v[ch & 1][j]), y = __uint_as_float(v[ch & 1][j + 1]);
+                        float x = __uint_as_float(v[hf][j]), y = __uint_as_float(v[hf][j + 1]);
                         if (MASKED) {
-                            x = 32 * ch + j < lim ? x : -INFINITY;
-                            y = 32 * ch + j + 1 < lim ? y : -INFINITY;
+                            x = 32 * hf + j < lim ? x : -INFINITY;
+                            y = 32 * hf + j + 1 < lim ? y : -INFINITY;
                         }
-                        raw[(j >> 1) & 3] = fmaxf(raw[(j >> 1) & 3], fmaxf(x, y));
+                        raw[(j >> 1) & 3] = max3(raw[(j >> 1) & 3], x, y);
                     }
-                }
                 const float r = fmaxf(fmaxf(raw[0], raw[1]), fmaxf(raw[2], raw[3]));
-                if (!MASKED || r != -INFINITY) top = fmaxf(top, __fmaf_rn(r, c[p], bias[p]));
-            }
-            const bool move = top > m + kSlack;
-            if (__any_sync(0xffffffffu, move)) {
+                return MASKED && r == -INFINITY ? r : __fmaf_rn(r, p ? c[1] : c[0], p ? bias[1] : bias[0]);
+            };
+            // Move the reference up to `top` where it passed it by 2^kSlack: O, the sum and the weights already written follow.
+            auto settle = [&](float top, int written) {
+                const bool move = top > m + kSlack;
+                if (!__any_sync(0xffffffffu, move)) return;
                 const float f = move ? ex2(m - top) : 1.f;
                 if (move) m = top;
                 l *= f;
@@ -908,29 +928,41 @@ k_attention_many(const AttnArgs A, int row_tiles, int tile_rows, int splits) {
                         tmem_st16(to + d, o);
                     }
                 }
-            }
-            const float base = (m == -INFINITY ? 0.f : m) - kRef;
+                if (written) {
+                    tmem_st_wait();
+#pragma unroll 1
+                    for (int d = 0; d < 32; d += 16) {
+                        u32 o[16];
+                        tmem_ld16(ts + d, o);
+                        tmem_ld_wait(o);
 #pragma unroll
-            for (int ch = 0; ch < 4; ++ch) {
-                const int p = ch >> 1;
-                u32(&x)[32] = v[ch & 1];
-                tmem_ld_wait(x);
-                if (ch < 3) tmem_ld32(ts + 32 * (ch + 1), v[(ch + 1) & 1]);
-                const u64 c2 = pair(c[p], c[p]), a2 = pair(bias[p] - base, bias[p] - base);
+                        for (int j = 0; j < 16; ++j) {
+                            float lo, hi;
+                            unpack2<TCQ_DT_F16>(o[j], lo, hi);
+                            o[j] = half2_of(lo * f, hi * f);
+                        }
+                        tmem_st16(ts + d, o);
+                    }
+                }
+            };
+            auto weights = [&](int p, int hf, int lim) {
+                u32(&x)[32] = v[hf];
+                const float base = (m == -INFINITY ? 0.f : m) - kRef, cp = p ? c[1] : c[0], ap = (p ? bias[1] : bias[0]) - base;
+                const u64 c2 = pair(cp, cp), a2 = pair(ap, ap);
                 u64 sum[2] = {0, 0};
                 u32 w[16];
 #pragma unroll
                 for (int j = 0; j < 16; ++j) {
                     u64 y = fma2(pair(__uint_as_float(x[2 * j]), __uint_as_float(x[2 * j + 1])), c2, a2);
                     float lo, hi;
-                    if (!MASKED && j % 16 < P::POLY) {
+                    if (!MASKED && (j * P::POLY) % 16 < P::POLY) {
                         y = ex2_poly(y);
                         unpair(y, lo, hi);
                     } else {
                         unpair(y, lo, hi);
                         if (MASKED) {
-                            lo = 32 * ch + 2 * j < lim ? lo : -INFINITY;
-                            hi = 32 * ch + 2 * j + 1 < lim ? hi : -INFINITY;
+                            lo = 32 * hf + 2 * j < lim ? lo : -INFINITY;
+                            hi = 32 * hf + 2 * j + 1 < lim ? hi : -INFINITY;
                         }
                         lo = ex2(lo), hi = ex2(hi);
                         y = pair(lo, hi);
@@ -940,13 +972,31 @@ k_attention_many(const AttnArgs A, int row_tiles, int tile_rows, int splits) {
                 }
                 float lo, hi;
                 unpair(add2(sum[0], sum[1]), lo, hi);
-                l = __fmaf_rn(lo + hi, inv[p], l);
-                if (vsc[p] < kLeastScale) {
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) w[j] = 0u;
-                }
-                tmem_st16(ts + 16 * ch, w);
+                l = __fmaf_rn(lo + hi, p ? inv[1] : inv[0], l);
+                tmem_st16(ts + 32 * p + 16 * hf, w);
+            };
+            auto hand_over = [&](int p) {
+                tmem_st_wait();
+                tc_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar(BAR_PFULL + 2 * g + p));
+            };
+            // rolled: the code of all roles has to fit the SM's nearest instruction caches
+            tmem_ld32(ts, v[0]);
+            tmem_ld32(ts + 32, v[1]);
+#pragma unroll 1
+            for (int p = 0; p < 2; ++p) {
+                const int lim = limit - i * kTile - 64 * p;
+                tmem_ld_wait(v[0]);
+                tmem_ld_wait(v[1]);
+                settle(page_top(p, lim), p);
+                if (p) hand_over(0);
+                weights(p, 0, lim);
+                if (!p) tmem_ld32(ts + 64, v[0]);
+                weights(p, 1, lim);
+                if (!p) tmem_ld32(ts + 96, v[1]);
             }
+            hand_over(1);
         };
 #pragma unroll 1
         for (int i = k0; i < k1; ++i) {
@@ -957,9 +1007,6 @@ k_attention_many(const AttnArgs A, int row_tiles, int tile_rows, int splits) {
             tc_after();
             if ((i + 1) * kTile > open) tile(std::true_type(), i, c, vsc);
             else tile(std::false_type(), i, c, vsc);
-            tmem_st_wait();
-            tc_before();
-            mbar_arrive(bar(BAR_PFULL + g));
         }
         if (limit == 0) l = 0.f;
         const bool got = k1 > k0 && wait(BAR_O, 0);
@@ -1002,121 +1049,144 @@ k_attention_many(const AttnArgs A, int row_tiles, int tile_rows, int splits) {
             }
             reinterpret_cast<float2*>(smem + P::ML0)[row] = make_float2(got ? m : -INFINITY, got ? l : 0.f);
         }
-    } else if (warp < W_MMA) {
+    } else if (warp >= W_CONV) {
         // ------------------------------------------------------------------------------------------------ convert
-        // Steps of a tile: its two pages' keys, its two pages' values. A step's INT8 data is requested AHEAD steps before its
-        // use, the pages' numbers a tile before that.
+        // Halves of a tile: its two pages' keys, its two pages' values. A half's INT8 data is requested a tile ahead of its use
+        // (asynchronous copies of each thread's own 16-byte chunks), the pages' numbers two tiles.
         const int ct = tid - W_CONV * 32;
-        int id[2] = {};
-        constexpr int AHEAD = D > 96 ? 2 : 4;            // steps between a request and its use
-        uint4 next[AHEAD][NC];
+        int id[2] = {}, koff[NC], voff[NC];
+        float least[2] = {1.f, 1.f};                     // value scales of the tile last requested
+#pragma unroll
+        for (int n = 0; n < NC; ++n) {
+            // where chunk c of a half (16 elements) goes: 32 bytes of a key's row, of a value's row
+            const int c = ct + P::CONV * n, p = c >= 4 * D, cc = c - p * 4 * D, kr = cc / (D / 16), kx = cc - kr * (D / 16), vr = cc >> 2, vx = cc & 3;
+            koff[n] = P::K0 + (kx >> 2) * (kTile * 128) + (64 * p + kr) * 128 + (((2 * (kx & 3)) ^ (kr & 7)) << 4);
+            voff[n] = P::V0 + (p * D + vr) * 128 + (((2 * vx) ^ (vr & 7)) << 4);
+        }
         auto request_ids = [&](int i) {
             if (i < k1) id[0] = trow[2 * i], id[1] = trow[min(2 * i + 1, pages - 1)];
         };
-        auto request = [&](int i, int j, const int (&ids)[2]) {
-            if (i >= k1) return;
-            const bool there = 2 * i + (j & 1) < pages;
-            const i8* src = (j & 2 ? A.cache.v : A.cache.k) + ((i64)page_in(ids[j & 1], A.cache.pages) * Hk + h) * (i64)(kBlk * D);
+        auto request = [&](int i, int vals) {
+            if (i < k1) {
+                const bool two = 2 * i + 1 < pages;
+                const i64 p0 = (i64)page_in(id[0], A.cache.pages) * Hk + h, p1 = (i64)page_in(id[1], A.cache.pages) * Hk + h;
+                const i8* cells = vals ? A.cache.v : A.cache.k;
+                const i8 *s0 = cells + p0 * P::PAGE, *s1 = cells + (p1 - 1) * P::PAGE;
+                if (vals) least[0] = A.cache.v_scale[p0], least[1] = A.cache.v_scale[p1];
 #pragma unroll
-            for (int n = 0; n < NC; ++n) {
-                const int c = ct + 128 * n;
-                next[j % AHEAD][n] = there && (NC * 128 == 4 * D || c < 4 * D) ? *reinterpret_cast<const uint4*>(src + c * 16) : make_uint4(0, 0, 0, 0);
+                for (int n = 0; n < NC; ++n) {
+                    const int c = ct + P::CONV * n;
+                    const bool p = c >= 4 * D;
+                    if (NC * P::CONV == 8 * D || c < 8 * D)
+                        cp_async16_zfill(sbase + P::STAGE0 + vals * 2 * P::PAGE + c * 16, (p ? s1 : s0) + c * 16, two || !p);
+                }
             }
+            asm volatile("cp.async.commit_group;" ::: "memory");
         };
         request_ids(k0);
-#pragma unroll
-        for (int j = 0; j < AHEAD; ++j) request(k0, j, id);
-        int now[2] = {id[0], id[1]};
+        request(k0, 0);
+        request(k0, 1);
         request_ids(k0 + 1);
 #pragma unroll 1
         for (int i = k0; i < k1; ++i) {
             const int it = i - k0, s = it & 1, use = it >> 1;
-            const int ids[2] = {id[0], id[1]};
-            request_ids(i + 2);
             bool ok = true;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                if (j == 0) ok = wait(BAR_KEMPTY + s, use + 1);
-                if (j == 2) ok = ok && wait(BAR_VEMPTY + s, use + 1);
+#pragma unroll 1
+            for (int vals = 0; vals < 2; ++vals) {
+                ok = wait((vals ? BAR_VEMPTY : BAR_KEMPTY) + s, use + 1);
                 if (!ok) break;
+                asm volatile("cp.async.wait_group 1;" ::: "memory");
+                const int dst = s * (vals ? P::VB : P::KB);
 #pragma unroll
                 for (int n = 0; n < NC; ++n) {
-                    const int c = ct + 128 * n;
-                    if (NC * 128 != 4 * D && c >= 4 * D) break;
-                    int row, ch;
-                    char* t;
-                    if (j & 2) {
-                        row = c >> 2, ch = 2 * (c & 3);
-                        t = smem + P::V0 + s * P::VB + (j & 1) * (D * 128);
-                    } else {
-                        row = c / (D / 16);
-                        const int x = c - row * (D / 16);
-                        row += 64 * (j & 1), ch = 2 * (x & 3);
-                        t = smem + P::K0 + s * P::KB + (x >> 2) * (kTile * 128);
-                    }
+                    const int c = ct + P::CONV * n;
+                    if (NC * P::CONV != 8 * D && c >= 8 * D) break;
+                    uint4 q = *reinterpret_cast<const uint4*>(smem + P::STAGE0 + vals * 2 * P::PAGE + c * 16);
+                    if (vals && (c >= 4 * D ? least[1] : least[0]) < kLeastScale) q = make_uint4(0, 0, 0, 0);     // values that count as zero
                     u32 w[8];
-                    int8x4_to_half(next[j % AHEAD][n].x, w[0], w[1]);
-                    int8x4_to_half(next[j % AHEAD][n].y, w[2], w[3]);
-                    int8x4_to_half(next[j % AHEAD][n].z, w[4], w[5]);
-                    int8x4_to_half(next[j % AHEAD][n].w, w[6], w[7]);
-                    t += row * 128;
-                    *reinterpret_cast<uint4*>(t + ((ch ^ (row & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
-                    *reinterpret_cast<uint4*>(t + (((ch + 1) ^ (row & 7)) << 4)) = make_uint4(w[4], w[5], w[6], w[7]);
+                    int8x4_to_half(q.x, w[0], w[1]);
+                    int8x4_to_half(q.y, w[2], w[3]);
+                    int8x4_to_half(q.z, w[4], w[5]);
+                    int8x4_to_half(q.w, w[6], w[7]);
+                    const int o = (vals ? voff[n] : koff[n]) + dst;
+                    *reinterpret_cast<uint4*>(smem + o) = make_uint4(w[0], w[1], w[2], w[3]);
+                    *reinterpret_cast<uint4*>(smem + (o ^ 16)) = make_uint4(w[4], w[5], w[6], w[7]);
                 }
-                if (j + AHEAD < 4) request(i, j + AHEAD, now);
-                else request(i + 1, j + AHEAD - 4, ids);
-                if (j & 1) {
-                    async_proxy_fence();
-                    mbar_arrive(bar((j & 2 ? BAR_VFULL : BAR_KFULL) + s));
-                }
+                async_proxy_fence();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar((vals ? BAR_VFULL : BAR_KFULL) + s));
+                request(i + 1, vals);
             }
             if (!ok) break;
-            now[0] = ids[0], now[1] = ids[1];
+            request_ids(i + 2);
         }
-    } else if (warp == W_MMA && lane == 0 && k1 > k0) {
+        cp_async_wait_all();
+    } else if (k1 > k0) {
         // ------------------------------------------------------------------------------------------------ product
+        // The whole warp runs this loop, so that descriptors and addresses stay in uniform registers; one elected lane
+        // issues (issued from a single-lane branch, each product took about 130 clocks instead of the 64 of its arithmetic).
+        const u64 qd = sw128_desc(sbase + P::Q0), kd = sw128_desc(sbase + P::K0), vd = sw128_desc(sbase + P::V0);
         auto scores = [&](int g, int s) {
-            const u32 qa = sbase + P::Q0 + g * P::QB, ka = sbase + P::K0 + s * P::KB;
+            if (elect_one()) {
+                const u64 a = qd + (u32)(g * (P::QB >> 4)), b = kd + (u32)(s * (P::KB >> 4));
 #pragma unroll
-            for (int k = 0; k < KS; ++k)
-                mma_ss(tmem + P::S0 + g * kTile, sw128_desc(qa + (k >> 2) * (kTile * 128) + 32 * (k & 3)),
-                       sw128_desc(ka + (k >> 2) * (kTile * 128) + 32 * (k & 3)), idesc_f16(kTile), k > 0);
-            mma_commit(bar(BAR_SFULL + g));
+                for (int k = 0; k < KS; ++k) {
+                    constexpr u32 atom = kTile * 128 / 16;
+                    mma_ss(tmem + P::S0 + g * kTile, a + ((k >> 2) * atom + 2 * (k & 3)), b + ((k >> 2) * atom + 2 * (k & 3)), idesc_f16(kTile), k > 0);
+                }
+                mma_commit(bar(BAR_SFULL + g));
+            }
+            __syncwarp();
+        };
+        auto commit = [&](int i) {
+            if (elect_one()) mma_commit(bar(i));
+            __syncwarp();
         };
         const int n = k1 - k0;
         bool ok = wait(BAR_Q, 0) && wait(BAR_KFULL, 0);
         if (ok) {
             tc_after();
+#pragma unroll
             for (int g = 0; g < NG; ++g) scores(g, 0);
-            mma_commit(bar(BAR_KEMPTY));
+            commit(BAR_KEMPTY);
         }
+#pragma unroll 1
         for (int i = 0; i < n && ok; ++i) {
             const int s = i & 1, s1 = (i + 1) & 1;
-            for (int g = 0; g < NG && ok; ++g) {
-                if (g == 0) ok = wait(BAR_VFULL + s, i >> 1);
-                ok = ok && wait(BAR_PFULL + g, i);
-                if (!ok) break;
-                tc_after();
-                const u32 va = sbase + P::V0 + s * P::VB;
+            const bool more = i + 1 < n;
 #pragma unroll
-                for (int k = 0; k < 8; ++k)
-                    mma_ts(tmem + P::O0 + g * D, tmem + P::S0 + g * kTile + 8 * k, sw128_desc(va + (k >> 2) * (D * 128) + 32 * (k & 3)),
-                           idesc_f16(D), i > 0 || k > 0);
-                if (i + 1 < n) {
-                    if (g == 0) ok = wait(BAR_KFULL + s1, (i + 1) >> 1);
+            for (int g = 0; g < NG; ++g) {
+                if (g == 0) ok = wait(BAR_VFULL + s, i >> 1);
+#pragma unroll
+                for (int p = 0; p < 2; ++p) {
+                    ok = ok && wait(BAR_PFULL + 2 * g + p, i);
                     if (!ok) break;
                     tc_after();
-                    scores(g, s1);
+                    if (elect_one()) {
+                        const u64 b = vd + (u32)(s * (P::VB >> 4) + p * (D * 128 / 16));
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            mma_ts(tmem + P::O0 + g * D, tmem + P::S0 + g * kTile + 32 * p + 8 * k, b + 2 * k, idesc_f16(D), p > 0 || k > 0 ? 1u : (u32)(i > 0));
+                    }
+                    __syncwarp();
                 }
+                if (ok && more) {
+                    if (g == 0) ok = wait(BAR_KFULL + s1, (i + 1) >> 1);
+                    if (ok) {
+                        tc_after();
+                        scores(g, s1);
+                    }
+                }
+                if (!ok) break;
             }
             if (!ok) break;
-            mma_commit(bar(BAR_VEMPTY + s));
-            if (i + 1 < n) mma_commit(bar(BAR_KEMPTY + s1));
+            commit(BAR_VEMPTY + s);
+            if (more) commit(BAR_KEMPTY + s1);
         }
-        mma_commit(bar(BAR_O));
+        commit(BAR_O);
         // products in flight must end before TMEM is freed, also after an expired wait
         volatile int never = 0;
-        mbar_wait_bounded(bar(BAR_O), 0, &never, &g_tcq_attention_error);
+        mbar_wait_suspended(bar(BAR_O), 0, &never, &g_tcq_attention_error);
     }
     tc_before();
     __syncthreads();
@@ -1124,7 +1194,7 @@ k_attention_many(const AttnArgs A, int row_tiles, int tile_rows, int splits) {
     // Back to the launch's registers for the code that all warps share: only behind the barrier, when every softmax warp has
     // had its larger share (a warp that took its registers back before could keep them from one forever).
     if (NG == 2) {
-        if (warp < W_CONV) asm volatile("setmaxnreg.dec.sync.aligned.u32 128;");
+        if (warp < W_MMA) asm volatile("setmaxnreg.dec.sync.aligned.u32 128;");
         else asm volatile("setmaxnreg.inc.sync.aligned.u32 128;");
     }
     if (warp == W_MMA) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(P::COLS) : "memory");

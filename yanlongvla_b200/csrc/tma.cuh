@@ -63,6 +63,32 @@ __device__ __forceinline__ bool mbar_wait_bounded(u32 bar, u32 parity, volatile 
     }
 }
 
+// The same with the thread suspended by the hardware between its looks at the barrier (up to 100 us each), for waits of
+// microseconds next to warps that compute.
+__device__ __forceinline__ bool mbar_wait_suspended(u32 bar, u32 parity, volatile int* abort_flag, int* err,
+                                                    unsigned long long limit = kWaitNs) {
+    unsigned long long t0 = 0;
+    for (;;) {
+        u32 ok;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(ok)
+            : "r"(bar), "r"(parity), "r"(100000u)
+            : "memory");
+        if (ok) return true;
+        if (*abort_flag) return false;
+        const unsigned long long t = gtime();
+        if (!t0) t0 = t;
+        if (t - t0 > limit) {
+            atomicOr(err, 1);
+            *abort_flag = 1;
+            return false;
+        }
+    }
+}
+
 __device__ __forceinline__ void tma_load_2d(u32 dst, const CUtensorMap* map, u32 bar, int x, int y) {
     asm volatile(
         "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
