@@ -613,23 +613,25 @@ struct Many {
     static constexpr int KB = kTile * 128 * ATOMS;                    // of a tile's keys
     static constexpr int VB = D * 128 * 2;                            // of its values
     static constexpr int NS = 2;                                      // tiles of either in flight
+    // Threads and registers. With two groups the CTA is launched with 80 registers a thread (768 x 80), of which the softmax
+    // warps take more and the others less: 512 x 96 + 256 x 48 = 61,440.
+    static constexpr int SOFT = NG * 256;                            // softmax threads: two to a row, a page each
+    static constexpr int THREADS = NG == 2 ? 768 : 512;
+    static constexpr int CONV = THREADS - SOFT - 32;                 // convert threads: what softmax and the product warp leave
     static constexpr int PAGE = kBlk * D;                             // bytes of a page's keys or values
     static constexpr int RING = 4;                                    // INT8 pages on their way (a tile's keys and values)
     static constexpr int Q0 = 0, K0 = NG * QB, V0 = K0 + NS * KB, STAGE0 = V0 + NS * VB, BAR0 = STAGE0 + RING * PAGE;
-    static constexpr int ML0 = BAR0 + 256;                            // m, l of every row (cluster sums)
-    static constexpr int BYTES = ML0 + NG * kTile * 8;
-    // Threads and registers. With two groups the CTA is launched with 128 registers a thread (512 x 128 = the SM's 65,536), of
-    // which the softmax warps take more and the others less: 256 x 192 + 256 x 64.
-    static constexpr int THREADS = NG == 2 ? 512 : 288;
-    static constexpr int CONV = THREADS - NG * 128 - 32;             // convert threads: what softmax and the product warp leave
-    #ifndef POLYN
-#define POLYN 5
+    static constexpr int SWAP0 = BAR0 + 256;                          // a float of every softmax thread
+    static constexpr int BYTES = SWAP0 + SOFT * 4;
+    static constexpr int ML0 = STAGE0;                                // m, l of every row, over the stage (cluster sums)
+#ifndef POLYN
+#define POLYN 2
 #endif
     static constexpr int POLY = POLYN;                      // of 16 pairs of weights, those formed by polynomial
     static constexpr u32 COLS = NG == 2 ? 512 : 256;
     static constexpr int S0 = 0, O0 = NG * kTile;                     // TMEM columns: scores, outputs
     static constexpr int PARTS = NG * kTile * D * 4;                  // a CTA's part of the outputs, over the tiles
-    static_assert(PARTS <= BAR0, "the parts overlay the tiles");
+    static_assert(PARTS <= STAGE0 && NG * kTile * 8 <= RING * PAGE, "the parts overlay the tiles, their sums the stage");
 };
 
 __device__ __forceinline__ u64 sw128_desc(u32 addr) {
@@ -668,12 +670,15 @@ __device__ __forceinline__ void tmem_ld32(u32 addr, u32 (&v)[32]) {
           "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
         : "r"(addr));
 }
-__device__ __forceinline__ void tmem_ld16(u32 addr, u32 (&v)[16]) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]),
-          "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
-        : "r"(addr));
+__device__ __forceinline__ void tmem_ld8(u32 addr, u32 (&v)[8]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
+                 : "r"(addr));
+}
+__device__ __forceinline__ void tmem_st8(u32 addr, const u32 (&v)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};" ::"r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]),
+                 "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(addr)
+                 : "memory");
 }
 __device__ __forceinline__ void tmem_st16(u32 addr, const u32 (&v)[16]) {
     asm volatile(
@@ -734,6 +739,18 @@ TCQ_HD u64 ex2_poly(u64 x) {
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void async_proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
+// Two warps at a named barrier; pair_any: whether any of their threads says yes.
+__device__ __forceinline__ void pair_sync(int id) { asm volatile("barrier.cta.sync %0, 64;" ::"r"(id) : "memory"); }
+__device__ __forceinline__ bool pair_any(int id, bool yes) {
+    u32 r;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 q, %2, 0;\n\tbarrier.cta.red.or.pred p, %1, 64, q;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(r)
+        : "r"(id), "r"((u32)yes)
+        : "memory");
+    return r != 0;
+}
+
 __device__ __forceinline__ void cluster_barrier() {
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -768,7 +785,7 @@ __device__ __forceinline__ void cp_async16_zfill(u32 dst, const void* src, bool 
 enum { BAR_KFULL = 0, BAR_KEMPTY = 2, BAR_VFULL = 4, BAR_VEMPTY = 6, BAR_SFULL = 8, BAR_PFULL = 10, BAR_Q = 14, BAR_O = 15, BAR_COUNT = 16 };
 
 template <int DT, int D, int NG>
-__global__ void __launch_bounds__(Many<D, NG>::THREADS, NG == 1 && D <= 64 ? 2 : 1)
+__global__ void __launch_bounds__(Many<D, NG>::THREADS, 1)
 k_attention_many(const AttnArgs A, int row_tiles, int tile_rows, int splits) {
     typedef Many<D, NG> P;
     constexpr int KS = D / 16, NC = (8 * D + P::CONV - 1) / P::CONV;      // contraction steps; 16-byte chunks of half a tile per convert thread
@@ -778,7 +795,7 @@ k_attention_many(const AttnArgs A, int row_tiles, int tile_rows, int splits) {
     u32* tmem_slot = reinterpret_cast<u32*>(smem + P::BAR0 + 8 * BAR_COUNT);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
-    constexpr int W_MMA = NG * 4, W_CONV = W_MMA + 1;
+    constexpr int W_MMA = NG * 8, W_CONV = W_MMA + 1;
     auto bar = [&](int i) -> u32 { return bars + 8 * i; };
     auto wait = [&](int i, u32 parity) -> bool { return mbar_wait_suspended(bar(i), parity & 1, abort_flag, &g_tcq_attention_error); };
     if (tid == 0) {
@@ -791,7 +808,7 @@ k_attention_many(const AttnArgs A, int row_tiles, int tile_rows, int splits) {
             mbar_init(bar(BAR_PFULL + i), 4);               // per softmax warp; group and page at 2 g + p
             mbar_init(bar(BAR_PFULL + 2 + i), 4);
         }
-        mbar_init(bar(BAR_Q), NG * 128);
+        mbar_init(bar(BAR_Q), P::SOFT);
         mbar_init(bar(BAR_O), 1);
         *abort_flag = 0;
         mbar_init_fence();
@@ -823,133 +840,136 @@ k_attention_many(const AttnArgs A, int row_tiles, int tile_rows, int splits) {
 
     float m = -INFINITY, l = 0.f;
     if (NG == 2) {
-        if (warp < W_MMA) asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
-        else asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+        if (warp < W_MMA) asm volatile("setmaxnreg.inc.sync.aligned.u32 96;");
+        else asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
     }
     if (warp < W_MMA) {
         // ------------------------------------------------------------------------------------------------ softmax
-        const int g = warp >> 2, gl = tid & 127, r = r0 + g * kTile + gl, tq = r / A.group;
+        const int g = warp >> 3, p = (warp >> 2) & 1, gl = tid & 127, r = r0 + g * kTile + gl, tq = r / A.group;
+        const int pair_bar = 1 + g * 4 + (warp & 3);            // the two warps of 32 rows meet at a named barrier
         const bool live = r < r1 && tq < cnt;
         const int limit = !live ? 0 : A.causal ? min(max(len - cnt + tq + 1, 0), len) : len;
         float crow = 0.f;
+        float* swap = reinterpret_cast<float*>(smem + P::SWAP0);
+        const int mine = (g * 2 + p) * kTile + gl, other = mine ^ kTile;
         if (k1 > k0) {
-            u32 qw[D / 2];
-            const u16* qr = A.q + b * A.q_sb + tq * A.q_st + (i64)(h * A.group + r - tq * A.group) * D;
+            // Queries to shared memory: SEG lanes to a row (16 bytes each), a warp's 16 rows requested at once; each row scaled
+            // by a power of two, which its own threads then take from the swap area.
+            constexpr int LPR = D / 8, SEG = LPR <= 4 ? 4 : LPR <= 8 ? 8 : 16, RPP = 32 / SEG, NP = 16 / RPP;
+            const int sl = lane % SEG, w8 = warp & 7;
+            uint4 w[NP];
 #pragma unroll
-            for (int i = 0; i < D / 8; ++i) {
-                const uint4 w = live ? reinterpret_cast<const uint4*>(qr)[i] : make_uint4(0, 0, 0, 0);
-                qw[4 * i] = w.x, qw[4 * i + 1] = w.y, qw[4 * i + 2] = w.z, qw[4 * i + 3] = w.w;
+            for (int n = 0; n < NP; ++n) {
+                const int row = w8 * 16 + n * RPP + lane / SEG, rr = r0 + g * kTile + row, tt = rr / A.group;
+                const u16* qr = A.q + b * A.q_sb + tt * A.q_st + (i64)(h * A.group + rr - tt * A.group) * D;
+                w[n] = rr < r1 && tt < cnt && sl < LPR ? reinterpret_cast<const uint4*>(qr)[sl] : make_uint4(0, 0, 0, 0);
             }
-            float amax = 0.f, a, c;
 #pragma unroll
-            for (int i = 0; i < D / 2; ++i) {
-                unpack2<DT>(qw[i], a, c);
-                amax = fmaxf(amax, fmaxf(fabsf(a), fabsf(c)));
-            }
-            float back, up = row_scale(amax, back);
-            crow = back * fabsf(A.scale_log2);
-            if (A.scale_log2 < 0.f) up = -up;
-            char* q = smem + P::Q0 + g * P::QB + gl * 128;
-#pragma unroll
-            for (int i = 0; i < D / 8; ++i) {
-                u32 w[4];
+            for (int n = 0; n < NP; ++n) {
+                const int row = w8 * 16 + n * RPP + lane / SEG;
+                u32 ww[4] = {w[n].x, w[n].y, w[n].z, w[n].w};
+                float amax = 0.f, x, y;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    unpack2<DT>(qw[4 * i + j], a, c);
-                    w[j] = half2_of(a * up, c * up);
+                    unpack2<DT>(ww[j], x, y);
+                    amax = max3(amax, fabsf(x), fabsf(y));
                 }
-                *reinterpret_cast<uint4*>(q + (i >> 3) * (kTile * 128) + (((i & 7) ^ (gl & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+#pragma unroll
+                for (int o = 1; o < SEG; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+                float back, up = row_scale(amax, back);
+                if (A.scale_log2 < 0.f) up = -up;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    unpack2<DT>(ww[j], x, y);
+                    ww[j] = half2_of(x * up, y * up);
+                }
+                if (sl < LPR)
+                    *reinterpret_cast<uint4*>(smem + P::Q0 + g * P::QB + (sl >> 3) * (kTile * 128) + row * 128 + (((sl & 7) ^ (row & 7)) << 4)) =
+                        make_uint4(ww[0], ww[1], ww[2], ww[3]);
+                if (sl == 0) swap[g * 2 * kTile + row] = back;
             }
             async_proxy_fence();
+            asm volatile("barrier.cta.sync 15, %0;" ::"r"(P::SOFT) : "memory");
             mbar_arrive(bar(BAR_Q));
+            crow = swap[g * 2 * kTile + gl] * fabsf(A.scale_log2);
+            pair_sync(pair_bar);                              // both have read it before either swaps
         }
         const u32 lanes = (u32)((warp & 3) * 32) << 16, ts = tmem + lanes + P::S0 + g * kTile, to = tmem + lanes + P::O0 + g * D;
-        // the scales of the next tile's two pages are requested a tile ahead, the pages' numbers two
-        int id0 = 0, id1 = 0;
-        float nk[2] = {}, nv[2] = {1.f, 1.f};
-        auto request_ids = [&](int i) {
-            if (i < k1) {
-                id0 = trow[2 * i];
-                id1 = trow[min(2 * i + 1, pages - 1)];
-            }
+        // the scales of this thread's page of the next tile are requested a tile ahead, the page's number two
+        int id = 0;
+        float nk = 0.f, nv = 1.f;
+        auto request_id = [&](int i) {
+            if (i < k1) id = trow[min(2 * i + p, pages - 1)];
         };
         auto request_scales = [&](int i) {
             if (i < k1) {
-                const i64 p0 = (i64)page_in(id0, A.cache.pages) * Hk + h, p1 = (i64)page_in(id1, A.cache.pages) * Hk + h;
-                nk[0] = A.cache.k_scale[p0], nv[0] = A.cache.v_scale[p0];
-                nk[1] = A.cache.k_scale[p1], nv[1] = A.cache.v_scale[p1];
+                const i64 ph = (i64)page_in(id, A.cache.pages) * Hk + h;
+                nk = A.cache.k_scale[ph], nv = A.cache.v_scale[ph];
             }
         };
-        request_ids(k0);
+        request_id(k0);
         request_scales(k0);
-        request_ids(k0 + 1);
-        auto tile = [&](auto masked_c, int i, const float (&c)[2], const float (&vsc)[2]) {
+        request_id(k0 + 1);
+        // One page of a tile: its 64 scores into registers, their largest, weights back over the scores. The pair agrees on the
+        // row's reference before either writes a weight: nothing of S is read after that, and no product reads or adds to the
+        // rows before both pages' weights have been handed over. Returns false when a wait expired.
+        auto tile = [&](auto masked_c, int i, float c, float vsc) -> bool {
             constexpr bool MASKED = decltype(masked_c)::value;
-            float bias[2], inv[2];
-#pragma unroll
-            for (int p = 0; p < 2; ++p) {
-                const float vs = safe_scale(vsc[p]);
-                bias[p] = lg2(vs), inv[p] = 1.f / vs;
-            }
-            // A page's 64 scores at a time. The second page's are read, and the row's reference settled, before the first
-            // page's weights are handed over: until then no product reads or adds to this row.
+            const float vs = safe_scale(vsc), bias = lg2(vs), inv = 1.f / vs;
+            const int lim = limit - i * kTile - 64 * p;
+            const bool ok = wait(BAR_SFULL + g, i - k0);
+            tc_after();
             u32 v[2][32];
-            auto page_top = [&](int p, int lim) -> float {
-                float raw[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            tmem_ld32(ts + 64 * p, v[0]);
+            tmem_ld32(ts + 64 * p + 32, v[1]);
+            tmem_ld_wait(v[0]);
+            tmem_ld_wait(v[1]);
+            float raw[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int hf = 0; hf < 2; ++hf)
-#pragma unroll
-                    for (int j = 0; j < 32; j += 2) {
-                        float x = __uint_as_float(v[hf][j]), y = __uint_as_float(v[hf][j + 1]);
-                        if (MASKED) {
-                            x = 32 * hf + j < lim ? x : -INFINITY;
-                            y = 32 * hf + j + 1 < lim ? y : -INFINITY;
-                        }
-                        raw[(j >> 1) & 3] = max3(raw[(j >> 1) & 3], x, y);
-                    }
-                const float r = fmaxf(fmaxf(raw[0], raw[1]), fmaxf(raw[2], raw[3]));
-                return MASKED && r == -INFINITY ? r : __fmaf_rn(r, p ? c[1] : c[0], p ? bias[1] : bias[0]);
-            };
-            // Move the reference up to `top` where it passed it by 2^kSlack: O, the sum and the weights already written follow.
-            auto settle = [&](float top, int written) {
-                const bool move = top > m + kSlack;
-                if (!__any_sync(0xffffffffu, move)) return;
-                const float f = move ? ex2(m - top) : 1.f;
-                if (move) m = top;
+            for (int j = 0; j < 64; j += 2) {
+                float x = __uint_as_float(v[j >> 5][j & 31]), y = __uint_as_float(v[j >> 5][(j & 31) + 1]);
+                if (MASKED) {
+                    x = j < lim ? x : -INFINITY;
+                    y = j + 1 < lim ? y : -INFINITY;
+                }
+                raw[(j >> 1) & 3] = max3(raw[(j >> 1) & 3], x, y);
+            }
+            float top = fmaxf(fmaxf(raw[0], raw[1]), fmaxf(raw[2], raw[3]));
+            if (!MASKED || top != -INFINITY) top = __fmaf_rn(top, c, bias);
+            if (pair_any(pair_bar, top > m + kSlack || !ok)) {
+                // Move the reference up where a score passed it: O and the sum follow. An expired wait is told as a NaN that no
+                // arithmetic makes, so that both warps leave.
+                constexpr u32 gone = 0x7fffdeadu;
+                swap[mine] = ok ? top : __uint_as_float(gone);
+                pair_sync(pair_bar);
+                const float theirs = swap[other], both = fmaxf(top, theirs);
+                if (__any_sync(0xffffffffu, !ok || __float_as_uint(theirs) == gone)) return false;
+                const bool move = both > m + kSlack;
+                const float f = move ? ex2(m - both) : 1.f;
+                if (move) m = both;
                 l *= f;
                 if (i > k0) {
 #pragma unroll 1
-                    for (int d = 0; d < D; d += 16) {
-                        u32 o[16];
-                        tmem_ld16(to + d, o);
+                    for (int d = p * (D / 2); d < (p + 1) * (D / 2); d += 8) {
+                        u32 o[8];
+                        tmem_ld8(to + d, o);
                         tmem_ld_wait(o);
 #pragma unroll
-                        for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
-                        tmem_st16(to + d, o);
+                        for (int j = 0; j < 8; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+                        tmem_st8(to + d, o);
                     }
-                }
-                if (written) {
                     tmem_st_wait();
-#pragma unroll 1
-                    for (int d = 0; d < 32; d += 16) {
-                        u32 o[16];
-                        tmem_ld16(ts + d, o);
-                        tmem_ld_wait(o);
-#pragma unroll
-                        for (int j = 0; j < 16; ++j) {
-                            float lo, hi;
-                            unpack2<TCQ_DT_F16>(o[j], lo, hi);
-                            o[j] = half2_of(lo * f, hi * f);
-                        }
-                        tmem_st16(ts + d, o);
-                    }
+                    tc_before();
                 }
-            };
-            auto weights = [&](int p, int hf, int lim) {
+                pair_sync(pair_bar);
+                tc_after();
+            }
+            const float base = (m == -INFINITY ? 0.f : m) - kRef;
+            const u64 c2 = pair(c, c), a2 = pair(bias - base, bias - base);
+            u64 sum[2] = {0, 0};
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf) {
                 u32(&x)[32] = v[hf];
-                const float base = (m == -INFINITY ? 0.f : m) - kRef, cp = p ? c[1] : c[0], ap = (p ? bias[1] : bias[0]) - base;
-                const u64 c2 = pair(cp, cp), a2 = pair(ap, ap);
-                u64 sum[2] = {0, 0};
                 u32 w[16];
 #pragma unroll
                 for (int j = 0; j < 16; ++j) {
@@ -970,84 +990,65 @@ k_attention_many(const AttnArgs A, int row_tiles, int tile_rows, int splits) {
                     sum[j & 1] = add2(sum[j & 1], y);
                     w[j] = half2_of(lo, hi);
                 }
-                float lo, hi;
-                unpair(add2(sum[0], sum[1]), lo, hi);
-                l = __fmaf_rn(lo + hi, p ? inv[1] : inv[0], l);
                 tmem_st16(ts + 32 * p + 16 * hf, w);
-            };
-            auto hand_over = [&](int p) {
-                tmem_st_wait();
-                tc_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(bar(BAR_PFULL + 2 * g + p));
-            };
-            // rolled: the code of all roles has to fit the SM's nearest instruction caches
-            tmem_ld32(ts, v[0]);
-            tmem_ld32(ts + 32, v[1]);
-#pragma unroll 1
-            for (int p = 0; p < 2; ++p) {
-                const int lim = limit - i * kTile - 64 * p;
-                tmem_ld_wait(v[0]);
-                tmem_ld_wait(v[1]);
-                settle(page_top(p, lim), p);
-                if (p) hand_over(0);
-                weights(p, 0, lim);
-                if (!p) tmem_ld32(ts + 64, v[0]);
-                weights(p, 1, lim);
-                if (!p) tmem_ld32(ts + 96, v[1]);
             }
-            hand_over(1);
+            float lo, hi;
+            unpair(add2(sum[0], sum[1]), lo, hi);
+            l = __fmaf_rn(lo + hi, inv, l);
+            tmem_st_wait();
+            tc_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(BAR_PFULL + 2 * g + p));
+            return true;
         };
 #pragma unroll 1
         for (int i = k0; i < k1; ++i) {
-            const float c[2] = {crow * nk[0], crow * nk[1]}, vsc[2] = {nv[0], nv[1]};
+            const float c = crow * nk, vsc = nv;
             request_scales(i + 1);
-            request_ids(i + 2);
-            if (!wait(BAR_SFULL + g, i - k0)) break;
-            tc_after();
-            if ((i + 1) * kTile > open) tile(std::true_type(), i, c, vsc);
-            else tile(std::false_type(), i, c, vsc);
+            request_id(i + 2);
+            if (!((i + 1) * kTile > open ? tile(std::true_type(), i, c, vsc) : tile(std::false_type(), i, c, vsc))) break;
         }
-        if (limit == 0) l = 0.f;
+        // the row's sum from its two threads, its elements half by half
+        swap[mine] = limit == 0 ? 0.f : l;
+        pair_sync(pair_bar);
+        l = swap[mine & ~kTile] + swap[mine | kTile];
         const bool got = k1 > k0 && wait(BAR_O, 0);
         tc_after();
-        if (splits == 1) {
-            const float f = got && l != 0.f ? 1.f / l : 0.f;
-            u16* dst = A.out + (((i64)b * A.T + tq) * A.heads + h * A.group + r - tq * A.group) * D;
+        // Rows to shared memory, over the tiles (every product is done), 16-byte chunks permuted within a row: FP32 parts for
+        // the cluster's sum, or the output's values for stores of whole rows.
+        const float f = splits > 1 ? 1.f : l != 0.f ? 1.f / l : 0.f;
+        const int row = g * kTile + gl;
 #pragma unroll 1
-            for (int d = 0; d < D; d += 16) {
-                u32 o[16] = {};
-                if (got) {
-                    tmem_ld16(to + d, o);
-                    tmem_ld_wait(o);
-                }
-                if (r < r1) {
-                    u32 w[8];
-#pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        w[j] = f != 0.f || l != 0.f ? pack2<DT>(__uint_as_float(o[2 * j]) * f, __uint_as_float(o[2 * j + 1]) * f) : 0u;
-                    reinterpret_cast<uint4*>(dst + d)[0] = make_uint4(w[0], w[1], w[2], w[3]);
-                    reinterpret_cast<uint4*>(dst + d)[1] = make_uint4(w[4], w[5], w[6], w[7]);
-                }
+        for (int d = p * (D / 2); d < (p + 1) * (D / 2); d += 8) {
+            u32 o[8] = {};
+            if (got) {
+                tmem_ld8(to + d, o);
+                tmem_ld_wait(o);
             }
+            float y[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) y[j] = l != 0.f ? __uint_as_float(o[j]) * f : 0.f;
+            if (splits > 1) {
+                constexpr int X = (D / 4) % 8 == 0 ? 7 : 3;
+                float4* part = reinterpret_cast<float4*>(smem) + row * (D / 4);
+                part[(d / 4) ^ (row & X)] = make_float4(y[0], y[1], y[2], y[3]);
+                part[(d / 4 + 1) ^ (row & X)] = make_float4(y[4], y[5], y[6], y[7]);
+            } else {
+                constexpr int X = (D / 8) % 8 == 0 ? 7 : (D / 8) % 4 == 0 ? 3 : 1;
+                reinterpret_cast<uint4*>(smem)[row * (D / 8) + ((d / 8) ^ (row & X))] =
+                    make_uint4(pack2<DT>(y[0], y[1]), pack2<DT>(y[2], y[3]), pack2<DT>(y[4], y[5]), pack2<DT>(y[6], y[7]));
+            }
+        }
+        if (splits > 1) {
+            if (p == 0) reinterpret_cast<float2*>(smem + P::ML0)[row] = make_float2(got ? m : -INFINITY, got ? l : 0.f);
         } else {
-            // this CTA's part: rows of D floats over the tiles, 16-byte chunks permuted within a row
-            constexpr int X = (D / 4) % 8 == 0 ? 7 : 3;
-            const int row = g * kTile + gl;
-            float4* dst = reinterpret_cast<float4*>(smem) + row * (D / 4);
-#pragma unroll 1
-            for (int d = 0; d < D; d += 16) {
-                u32 o[16] = {};
-                if (got) {
-                    tmem_ld16(to + d, o);
-                    tmem_ld_wait(o);
-                }
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    dst[(d / 4 + j) ^ (row & X)] = make_float4(__uint_as_float(o[4 * j]), __uint_as_float(o[4 * j + 1]), __uint_as_float(o[4 * j + 2]),
-                                                               __uint_as_float(o[4 * j + 3]));
+            constexpr int X = (D / 8) % 8 == 0 ? 7 : (D / 8) % 4 == 0 ? 3 : 1;
+            asm volatile("barrier.cta.sync 15, %0;" ::"r"(P::SOFT) : "memory");
+            for (int e = tid; e < (r1 - r0) * (D / 8); e += P::SOFT) {
+                const int rr = e / (D / 8), ch = e - rr * (D / 8), t = (r0 + rr) / A.group;
+                u16* dst = A.out + (((i64)b * A.T + t) * A.heads + h * A.group + r0 + rr - t * A.group) * D;
+                reinterpret_cast<uint4*>(dst)[ch] = reinterpret_cast<const uint4*>(smem)[rr * (D / 8) + (ch ^ (rr & X))];
             }
-            reinterpret_cast<float2*>(smem + P::ML0)[row] = make_float2(got ? m : -INFINITY, got ? l : 0.f);
         }
     } else if (warp >= W_CONV) {
         // ------------------------------------------------------------------------------------------------ convert
@@ -1194,8 +1195,8 @@ k_attention_many(const AttnArgs A, int row_tiles, int tile_rows, int splits) {
     // Back to the launch's registers for the code that all warps share: only behind the barrier, when every softmax warp has
     // had its larger share (a warp that took its registers back before could keep them from one forever).
     if (NG == 2) {
-        if (warp < W_MMA) asm volatile("setmaxnreg.dec.sync.aligned.u32 128;");
-        else asm volatile("setmaxnreg.inc.sync.aligned.u32 128;");
+        if (warp < W_MMA) asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+        else asm volatile("setmaxnreg.inc.sync.aligned.u32 80;");
     }
     if (warp == W_MMA) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(P::COLS) : "memory");
     if (splits == 1) return;
@@ -1237,7 +1238,7 @@ template <int DT, int D, int NG>
 int launch_many(const AttnArgs& A, void* stream) {
     typedef Many<D, NG> P;
     const auto kern = k_attention_many<DT, D, NG>;
-    constexpr int PER_SM = NG == 1 && D <= 64 ? 2 : 1;
+    constexpr int PER_SM = 1;
     const int R = A.T * A.group, row_tiles = (R + NG * kTile - 1) / (NG * kTile);
     const int tile_rows = ((R + row_tiles - 1) / row_tiles + 31) & ~31;            // even shares, in warps
     const i64 units = (i64)A.B * A.cache.kv_heads * row_tiles;
