@@ -76,6 +76,11 @@ TCQ_HD float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+TCQ_HD float rcp(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 TCQ_HD float lg2(float x) {
     float y;
     asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -385,7 +390,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) k_attention_few(const AttnArgs
                 }
                 if (D % 32) step(D / 32 * 2, *reinterpret_cast<const u32*>(row + D / 32 * 32 + 4 * t));
             }
-            const float vs = safe_scale(sc.y), bias = lg2(vs), inv = 1.f / vs;
+            const float vs = safe_scale(sc.y), bias = lg2(vs), inv = rcp(vs);
             const bool masked = (pg + 1) * kBlk > open;
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt)
@@ -915,7 +920,7 @@ k_attention_many(const AttnArgs A, int row_tiles, int tile_rows, int splits) {
         // rows before both pages' weights have been handed over. Returns false when a wait expired.
         auto tile = [&](auto masked_c, int i, float c, float vsc) -> bool {
             constexpr bool MASKED = decltype(masked_c)::value;
-            const float vs = safe_scale(vsc), bias = lg2(vs), inv = 1.f / vs;
+            const float vs = safe_scale(vsc), bias = lg2(vs), inv = rcp(vs);
             const int lim = limit - i * kTile - 64 * p;
             const bool ok = wait(BAR_SFULL + g, i - k0);
             tc_after();
