@@ -67,7 +67,6 @@ TCQ_HD int page_of(const int* row, int blk, int pages) { return page_in(row[blk]
 //
 // int8 -> FP16: u = byte ^ 0x80, 0x6400 | u is 1024 + u, minus 1152: five instructions for four elements.
 
-constexpr int kWarps = 8;
 constexpr float kRef = 5.f;           // log2 of the weight of a score equal to the reference
 constexpr float kSlack = 10.5f;       // growth of the maximum that does not move the reference: weights up to 2^15.5
 
@@ -122,22 +121,20 @@ struct AttnArgs {
     const int* count;
     float* part;           // partial rows of segments that do not cover their unit
     int* counters;
-    int blocks, causal, B, T, heads, group, workers;
+    int blocks, causal, B, T, heads, group;
     float scale_log2;      // scale * log2(e)
 };
 
-// Shared-memory plan of the few-row kernel: a ring of NH half pages (64 D bytes: a block's keys or its values) per warp.
-template <int D, int MT, int W>
+// Plan of the few-row kernel. Every warp is a worker with a ring of NH half pages (64 D bytes: a block's keys or its values)
+// of its own. Twelve warps where their registers fit (a warp alone issues one instruction in about four clocks), else eight.
+template <int D, int MT>
 struct Few {
+    static constexpr int WARPS = D <= 64 && MT == 1 ? 12 : 8;
     static constexpr int HALF = kBlk * D;
-    static constexpr int NH = D <= 48 ? 8 : D == 64 ? 6 : D == 80 ? 5 : D == 96 ? 4 : 3;
-    static constexpr int PAD = D == 128 ? 4 : 8;
-    static constexpr int RING = kWarps * NH * HALF;
-    static constexpr int HDR = RING;                                       // ks, vs of each half page
-    static constexpr int ML = HDR + kWarps * NH * 8;                       // m, l of every warp and row
-    static constexpr int MERGE = ML + (W > 1 ? kWarps * 16 * MT * 8 : 0);  // one group of 8 rows of every warp
-    static constexpr int SCAN = MERGE + (W > 1 ? kWarps * 8 * (D + PAD) * 4 : 0);
-    static constexpr int BYTES = SCAN + 64;
+    static constexpr int NH = D == 32 ? 8 : D == 48 ? 6 : D == 64 ? (WARPS == 12 ? 4 : 6) : D == 80 ? 5 : D == 96 ? 4 : 3;
+    static constexpr int HDR = WARPS * NH * HALF;                          // ks, vs of each half page
+    static constexpr int SCAN = HDR + WARPS * NH * 8;                      // the block's scan of the lengths
+    static constexpr int BYTES = SCAN + 4 * WARPS * (int)sizeof(int);
 };
 
 // 16-byte chunk c of key row r lies at chunk c ^ swap(r): rows of 128 bytes put their halves on alternating banks.
@@ -150,48 +147,90 @@ struct Place {
     int b, h, ubeg, vp, np;
 };
 
-template <int DT, int D, int MT, int W>
-__global__ void __launch_bounds__(kWarps * 32, 1) k_attention_few(const AttnArgs A) {
-    typedef Few<D, MT, W> P;
-    constexpr int NH = P::NH, KS = D / 16, ROWS = 16 * MT;
+// One warp adds the parts of a unit (workers first .. last, in that order) and writes its R rows. Kept out of line: its many
+// loads in flight want registers of their own.
+template <int DT, int D>
+__device__ __noinline__ void add_parts(const float* parts, i64 size, int first, int last, int R, int group, u16* out, i64 token) {
+    constexpr int NI = 4, NB = 8;                 // pairs of elements of a lane, parts requested at once
+    const int lane = threadIdx.x & 31;
+#pragma unroll 1
+    for (int i0 = 0; i0 < R * (D / 2); i0 += 32 * NI) {
+        float2 acc[NI] = {};
+        float top[NI], sum[NI] = {};
+        int off[NI], ml[NI];
+#pragma unroll
+        for (int k = 0; k < NI; ++k) {
+            const int i = min(i0 + lane + 32 * k, R * (D / 2) - 1), r = i / (D / 2);
+            off[k] = r * (D + 2) + 2 * (i - r * (D / 2)), ml[k] = r * (D + 2) + D;
+            top[k] = -INFINITY;
+        }
+#pragma unroll 1
+        for (int w0 = first; w0 <= last; w0 += NB) {
+            float2 v[NB][NI], e[NB][NI];
+#pragma unroll
+            for (int w = 0; w < NB; ++w) {
+                const int at = min(w0 + w, last);
+                const float* part = parts + (2 * (i64)at + (at == first)) * size;
+#pragma unroll
+                for (int k = 0; k < NI; ++k) {
+                    v[w][k] = __ldcg(reinterpret_cast<const float2*>(part + off[k]));
+                    e[w][k] = __ldcg(reinterpret_cast<const float2*>(part + ml[k]));
+                }
+            }
+#pragma unroll
+            for (int w = 0; w < NB; ++w)
+                if (w0 + w <= last) {
+#pragma unroll
+                    for (int k = 0; k < NI; ++k) {
+                        const float nt = fmaxf(top[k], e[w][k].x), keep = nt == -INFINITY ? 0.f : ex2(top[k] - nt),
+                                    f = nt == -INFINITY ? 0.f : ex2(e[w][k].x - nt);
+                        top[k] = nt;
+                        sum[k] = __fmaf_rn(e[w][k].y, f, sum[k] * keep);
+                        acc[k].x = __fmaf_rn(v[w][k].x, f, acc[k].x * keep), acc[k].y = __fmaf_rn(v[w][k].y, f, acc[k].y * keep);
+                    }
+                }
+        }
+#pragma unroll
+        for (int k = 0; k < NI; ++k) {
+            const int i = i0 + lane + 32 * k, r = i / (D / 2), tq = r / group;
+            const float f = sum[k] != 0.f ? 1.f / sum[k] : 0.f;
+            if (i < R * (D / 2)) reinterpret_cast<u32*>(out + tq * token + (i64)(r - tq * group) * D)[i - r * (D / 2)] = pack2<DT>(acc[k].x * f, acc[k].y * f);
+        }
+    }
+}
+
+// Work. The pages of all sequences and heads form one list, cut into equal runs, one per warp (a unit is one head of one
+// sequence; an empty one takes a place without a page). A warp that holds a whole unit writes its output; parts of a unit go to
+// the workspace, and the last of its warps to arrive adds them in their order, so the result does not depend on timing.
+// whole != 0 (many short sequences): each warp takes whole units instead, one after the other.
+template <int DT, int D, int MT>
+__global__ void __launch_bounds__(Few<D, MT>::WARPS * 32, 1) k_attention_few(const AttnArgs A, int whole) {
+    typedef Few<D, MT> P;
+    constexpr int NH = P::NH, KS = D / 16, ROWS = 16 * MT, WARPS = P::WARPS;
     extern __shared__ __align__(16) char smem[];
     int* s_scan = reinterpret_cast<int*>(smem + P::SCAN);
     pdl_launch_dependents();
     pdl_wait();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, n = lane >> 2, t = lane & 3;
     const int Hk = A.cache.kv_heads, R = A.T * A.group;
+    // consecutive workers on different SMs
+    const int me = warp * gridDim.x + blockIdx.x, workers = WARPS * gridDim.x;
     char* ring = smem + warp * NH * P::HALF;
     float2* hdr = reinterpret_cast<float2*>(smem + P::HDR) + warp * NH;
 
     // ---- this worker's range [x0, x1) of places, and where it begins
-    int align = 1, chunk = 1, x0, x1;
+    int chunk = 1, x0, x1;
     Place at;
     auto places = [&](int len) { return max(1, (len + kBlk - 1) / kBlk); };
-    auto round_up = [&](int v) { return (v + align - 1) / align * align; };
-    if (W == 1) {
-        // whole units, one after the other
-        const int u = blockIdx.x * kWarps + warp;
-        if (u >= A.B * Hk) return;
-        at.b = u / Hk, at.h = u - at.b * Hk;
+    if (whole) {
+        if (me >= A.B * Hk) return;
+        at.b = me / Hk, at.h = me - at.b * Hk;
         x0 = 0, x1 = 1 << 30;
     } else {
         // all sequences' lengths: every thread a run of them, summed over the block
-        const int per = (A.B + kWarps * 32 - 1) / (kWarps * 32), b0 = min(A.B, tid * per), b1 = min(A.B, b0 + per);
-        int pages = 0, seqs = 0;
-        for (int b = b0; b < b1; ++b) pages += places(tokens_of(A.lens, b, A.blocks)), ++seqs;
-        int total = pages;
-#pragma unroll
-        for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-        if (lane == 0) s_scan[warp] = total;
-        __syncthreads();
-        total = 0;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) total += s_scan[w];
-        __syncthreads();
-        // few pages: places in groups of one page per warp, so that a worker serves one unit
-        if ((i64)total * Hk <= (i64)kWarps * A.workers) align = kWarps;
+        const int per = (A.B + WARPS * 32 - 1) / (WARPS * 32), b0 = min(A.B, tid * per), b1 = min(A.B, b0 + per);
         int mine = 0;
-        for (int b = b0; b < b1; ++b) mine += round_up(places(tokens_of(A.lens, b, A.blocks)));
+        for (int b = b0; b < b1; ++b) mine += places(tokens_of(A.lens, b, A.blocks));
         int scan = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -202,37 +241,41 @@ __global__ void __launch_bounds__(kWarps * 32, 1) k_attention_few(const AttnArgs
         __syncthreads();
         int before = scan - mine, all = 0;
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
+        for (int w = 0; w < WARPS; ++w) {
             before += w < warp ? s_scan[w] : 0;
             all += s_scan[w];
         }
         all *= Hk;
-        chunk = round_up((all + A.workers - 1) / A.workers);
-        x0 = min((i64)blockIdx.x * chunk, (i64)all), x1 = min(x0 + chunk, all);
-        if (x0 >= x1) return;                                             // the whole block
+        chunk = (all + workers - 1) / workers;
         int off = before * Hk;
         for (int b = b0; b < b1; ++b) {
-            const int w = round_up(places(tokens_of(A.lens, b, A.blocks))) * Hk;
-            if (x0 >= off && x0 < off + w) s_scan[kWarps] = b, s_scan[kWarps + 1] = off;
-            off += w;
+            const int v = places(tokens_of(A.lens, b, A.blocks)) * Hk;
+#pragma unroll 1
+            for (int w = 0; w < WARPS; ++w) {
+                const i64 x = (i64)(w * gridDim.x + blockIdx.x) * chunk;
+                if (x >= off && x < off + v) s_scan[WARPS + 2 * w] = b, s_scan[WARPS + 2 * w + 1] = off;
+            }
+            off += v;
         }
         __syncthreads();
-        at.b = s_scan[kWarps];
-        const int vp = round_up(places(tokens_of(A.lens, at.b, A.blocks)));
-        at.h = (x0 - s_scan[kWarps + 1]) / vp;
-        at.ubeg = s_scan[kWarps + 1] + at.h * vp;
+        if ((i64)me * chunk >= all) return;
+        x0 = me * chunk, x1 = min(x0 + chunk, all);
+        at.b = s_scan[WARPS + 2 * warp];
+        const int vp = places(tokens_of(A.lens, at.b, A.blocks));
+        at.h = (x0 - s_scan[WARPS + 2 * warp + 1]) / vp;
+        at.ubeg = s_scan[WARPS + 2 * warp + 1] + at.h * vp;
     }
     auto measure = [&](Place& p) {
         const int len = tokens_of(A.lens, p.b, A.blocks);
         p.np = (len + kBlk - 1) / kBlk;
-        p.vp = round_up(max(1, p.np));
+        p.vp = max(1, p.np);
     };
     measure(at);
-    if (W == 1) at.ubeg = 0, x1 = at.vp;
+    if (whole) at.ubeg = 0, x1 = at.vp;
     // The next unit of the range; false at its end.
     auto next_unit = [&](Place& p, int& end) -> bool {
-        if (W == 1) {
-            const int u = p.b * Hk + p.h + A.workers * kWarps;
+        if (whole) {
+            const int u = p.b * Hk + p.h + workers;
             if (u >= A.B * Hk) return false;
             p.b = u / Hk, p.h = u - p.b * Hk;
             measure(p);
@@ -251,7 +294,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) k_attention_few(const AttnArgs
 
     // ---- the producer: half pages of this warp's pages, in order, NH - 1 ahead of their use
     Place pat = at;
-    int px = x0 + (W == 1 ? 0 : warp), pend = x1, pid = 0, pslot = 0;
+    int px = x0, pend = x1, pid = 0, pslot = 0;
     bool pmore = true;
     auto p_settle = [&]() {                      // move px to the warp's next place that is a page
         for (;;) {
@@ -260,11 +303,11 @@ __global__ void __launch_bounds__(kWarps * 32, 1) k_attention_few(const AttnArgs
                     pmore = false;
                     return;
                 }
-                if (W == 1) px = 0;
+                if (whole) px = 0;
                 continue;
             }
             if (px - pat.ubeg < pat.np) break;
-            px += W;
+            ++px;
         }
         pid = page_of(A.table + (i64)pat.b * A.blocks, px - pat.ubeg, A.cache.pages);
     };
@@ -289,7 +332,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) k_attention_few(const AttnArgs
             } else {
 #pragma unroll
                 for (int i = 0; i < D / 8; ++i) cp_async16(dst + (lane + 32 * i) * 16, src + (lane + 32 * i) * 16);
-                px += W;
+                ++px;
                 p_settle();
             }
             p_values = !p_values;
@@ -310,7 +353,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) k_attention_few(const AttnArgs
 
     // ---- the consumer
     int end = x1;
-    int x = x0 + (W == 1 ? 0 : warp);
+    int x = x0;
     for (;;) {
         const int len = tokens_of(A.lens, at.b, A.blocks), cnt = queries_of(A.count, at.b, A.T);
         // query rows r = t * group + g of this head, as FP16 fragments scaled by a power of two
@@ -359,7 +402,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) k_attention_few(const AttnArgs
         }
         const int seg_end = min(at.ubeg + at.vp, end);
 #pragma unroll 1
-        for (; x < seg_end; x += W) {
+        for (; x < seg_end; ++x) {
             const int pg = x - at.ubeg;
             if (pg >= at.np) continue;
             const float2* sp = hdr + slot;
@@ -488,7 +531,8 @@ __global__ void __launch_bounds__(kWarps * 32, 1) k_attention_few(const AttnArgs
             const int tq = r / A.group;
             return A.out + (((i64)at.b * A.T + tq) * A.heads + at.h * A.group + r - tq * A.group) * D;
         };
-        if (W == 1) {
+        const bool all_of_it = at.ubeg >= (whole ? 0 : x0) && seg_end == at.ubeg + at.vp;
+        if (all_of_it) {
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -501,93 +545,34 @@ __global__ void __launch_bounds__(kWarps * 32, 1) k_attention_few(const AttnArgs
                     for (int i = 0; i < D / 8; ++i) dst[4 * i + t] = pack2<DT>(o[mt][i][2 * hf] * f, o[mt][i][2 * hf + 1] * f);
                 }
         } else {
-            float2* ml = reinterpret_cast<float2*>(smem + P::ML);
-            float* buf = reinterpret_cast<float*>(smem + P::MERGE);
-            constexpr int ST = D + P::PAD;
+            // a part: rows of D sums, the reference and the sum of weights; a worker has at most two, its first unit's and its last's
+            const int first = at.ubeg / chunk, last = (at.ubeg + at.vp - 1) / chunk;
+            auto record = [&](int w) -> float* { return A.part + (i64)(2 * w + (w == first ? 1 : 0)) * ROWS * (D + 2); };
+            float* part = record(me);
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-                for (int hf = 0; hf < 2; ++hf)
-                    if (t == 0) ml[warp * ROWS + 16 * mt + 8 * hf + n] = make_float2(m[mt][hf], l[mt][hf]);
-            __syncthreads();
-            const bool whole = max(at.ubeg, x0) == at.ubeg && seg_end == at.ubeg + at.vp;
-            const int first = at.ubeg / chunk, last = (at.ubeg + at.vp - 1) / chunk, me = blockIdx.x;
-            float* part = A.part + (i64)(2 * me + (me == first ? 1 : 0)) * ROWS * (D + 2);
-#pragma unroll
-            for (int grp = 0; grp < 2 * MT; ++grp) {
-                if (8 * grp >= R) break;
-                const int mt = grp >> 1, hf = grp & 1;
-                {
-                    float top = -INFINITY;
-#pragma unroll
-                    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, ml[w * ROWS + 8 * grp + n].x);
-                    const float f = top == -INFINITY ? 0.f : ex2(m[mt][hf] - top);
+                for (int hf = 0; hf < 2; ++hf) {
+                    const int r = 16 * mt + 8 * hf + n;
+                    if (r >= R) continue;
 #pragma unroll
                     for (int i = 0; i < D / 8; ++i)
-                        *reinterpret_cast<float2*>(buf + (warp * 8 + n) * ST + 8 * i + 2 * t) =
-                            make_float2(o[mt][i][2 * hf] * f, o[mt][i][2 * hf + 1] * f);
+                        *reinterpret_cast<float2*>(part + r * (D + 2) + 8 * i + 2 * t) = make_float2(o[mt][i][2 * hf], o[mt][i][2 * hf + 1]);
+                    if (t == 0) *reinterpret_cast<float2*>(part + r * (D + 2) + D) = make_float2(m[mt][hf], l[mt][hf]);
                 }
-                __syncthreads();
-                const int rows = min(8, R - 8 * grp);
-                for (int i = tid; i < rows * (D / 2); i += kWarps * 32) {
-                    const int rr = i / (D / 2), d = (i - rr * (D / 2)) * 2, r = 8 * grp + rr;
-                    float top = -INFINITY, sum = 0.f;
-#pragma unroll
-                    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, ml[w * ROWS + r].x);
-                    float2 acc = make_float2(0.f, 0.f);
-#pragma unroll
-                    for (int w = 0; w < kWarps; ++w) {
-                        const float2 v = *reinterpret_cast<const float2*>(buf + (w * 8 + rr) * ST + d), e = ml[w * ROWS + r];
-                        acc.x += v.x, acc.y += v.y;
-                        sum += e.y * (top == -INFINITY ? 0.f : ex2(e.x - top));
-                    }
-                    if (whole) {
-                        const float f = sum != 0.f ? 1.f / sum : 0.f;
-                        *reinterpret_cast<u32*>(out_row(r) + d) = pack2<DT>(acc.x * f, acc.y * f);
-                    } else {
-                        *reinterpret_cast<float2*>(part + r * (D + 2) + d) = acc;
-                        if (d == 0) *reinterpret_cast<float2*>(part + r * (D + 2) + D) = make_float2(top, sum);
-                    }
-                }
-                __syncthreads();
-            }
-            if (!whole) {
-                // the last of the unit's workers adds the parts in their order
+            __threadfence();
+            __syncwarp();
+            int seen = 0;
+            if (lane == 0) seen = atomicAdd(A.counters + first, 1);
+            seen = __shfl_sync(0xffffffffu, seen, 0);
+            if (seen == last - first) {
+                if (lane == 0) A.counters[first] = 0;
                 __threadfence();
-                __syncthreads();
-                if (tid == 0) {
-                    const int seen = atomicAdd(A.counters + first, 1);
-                    s_scan[kWarps + 3] = seen == last - first;
-                    if (seen == last - first) A.counters[first] = 0;
-                }
-                __syncthreads();
-                if (s_scan[kWarps + 3]) {
-                    __threadfence();
-                    for (int i = tid; i < R * (D / 2); i += kWarps * 32) {
-                        const int r = i / (D / 2), d = (i - r * (D / 2)) * 2;
-                        float top = -INFINITY;
-                        for (int w = first; w <= last; ++w) {
-                            const float* p = A.part + (i64)(2 * w + (w == first ? 1 : 0)) * ROWS * (D + 2) + r * (D + 2);
-                            top = fmaxf(top, __ldcg(p + D));
-                        }
-                        float sum = 0.f;
-                        float2 acc = make_float2(0.f, 0.f);
-                        for (int w = first; w <= last; ++w) {
-                            const float* p = A.part + (i64)(2 * w + (w == first ? 1 : 0)) * ROWS * (D + 2) + r * (D + 2);
-                            const float2 e = __ldcg(reinterpret_cast<const float2*>(p + D)), v = __ldcg(reinterpret_cast<const float2*>(p + d));
-                            const float f = top == -INFINITY ? 0.f : ex2(e.x - top);
-                            acc.x += v.x * f, acc.y += v.y * f;
-                            sum += e.y * f;
-                        }
-                        const float f = sum != 0.f ? 1.f / sum : 0.f;
-                        *reinterpret_cast<u32*>(out_row(r) + d) = pack2<DT>(acc.x * f, acc.y * f);
-                    }
-                }
-                __syncthreads();
+                add_parts<DT, D>(A.part, (i64)ROWS * (D + 2), first, last, R, A.group, out_row(0), (i64)A.heads * D);
             }
         }
         if (!next_unit(at, end)) break;
-        if (W == 1) x = 0;
+        if (whole) x = 0;
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
 }
@@ -1293,8 +1278,9 @@ int launch_many(const AttnArgs& A, void* stream) {
     return cudaLaunchKernelEx(&cfg, kern, A, row_tiles, tile_rows, splits) == cudaSuccess ? TCQ_OK : TCQ_ERR_LAUNCH;
 }
 
-// Arrival counters at the head of the workspace, one per worker.
-inline size_t counter_bytes(int workers) { return ((size_t)workers * sizeof(int) + 15) & ~(size_t)15; }
+// Arrival counters at the head of the workspace, one per worker of the few-row kernel.
+constexpr int kMostWarps = 12;
+inline size_t counter_bytes(int sms) { return ((size_t)kMostWarps * sms * sizeof(int) + 15) & ~(size_t)15; }
 
 // ------------------------------------------------------------------------------------------------ host side
 }  // namespace
@@ -1308,7 +1294,7 @@ size_t tcq_kv8_attention_workspace(int B, int T, int heads, int kv_heads, int he
     if (B < 1 || T < 1 || heads < 1 || kv_heads < 1 || head_dim < 1 || blocks < 1 || heads % kv_heads) return 0;
     const int sms = tcq_sm_count();
     const i64 rows = (i64)T * (heads / kv_heads);
-    if (few_rows(rows, head_dim)) return counter_bytes(sms) + (size_t)2 * sms * (rows <= 16 ? 16 : 32) * (head_dim + 2) * sizeof(float);
+    if (few_rows(rows, head_dim)) return counter_bytes(sms) + (size_t)2 * kMostWarps * sms * (rows <= 16 ? 16 : 32) * (head_dim + 2) * sizeof(float);
     return 16;
 }
 
@@ -1321,32 +1307,33 @@ int tcq_kv8_attention(const tcq_kv8_cache* cache, const void* q, int dtype, int6
     if (dtype != TCQ_DT_BF16 && dtype != TCQ_DT_F16) return TCQ_ERR_DTYPE;
     const int Hk = cache->kv_heads;
     if (B < 1 || T < 1 || blocks < 1 || heads < 1 || heads % Hk || blocks > (0x7fffffff / kBlk)) return TCQ_ERR_SHAPE;
-    if ((i64)B * Hk > 0x7fffffff || (i64)B * Hk * (blocks + kWarps) > 0x7fffffff) return TCQ_ERR_SHAPE;
+    if ((i64)B * Hk > 0x7fffffff || (i64)B * Hk * (blocks + 1) > 0x7fffffff) return TCQ_ERR_SHAPE;
     if (!tcq_aligned(q, 16) || !tcq_aligned(out, 16) || ((q_sb | q_st) & 7)) return TCQ_ERR_ALIGN;
     if (!workspace || workspace_bytes < tcq_kv8_attention_workspace(B, T, heads, Hk, cache->head_dim, blocks)) return TCQ_ERR_WORKSPACE;
     const int sms = tcq_sm_count();
     AttnArgs A = {*cache, (const u16*)q, q_sb, q_st, (u16*)out, table, lens, count, nullptr, (int*)workspace, blocks, causal, B, T, heads,
-                  heads / Hk, sms, scale * 1.4426950408889634f};
+                  heads / Hk, scale * 1.4426950408889634f};
     const i64 rows = (i64)T * A.group;
     if (few_rows(rows, cache->head_dim)) {
         A.part = reinterpret_cast<float*>((char*)workspace + counter_bytes(sms));
         const i64 units = (i64)B * Hk;
-        // Short sequences of many units: a warp per unit, nothing to merge.
-        const bool alone = blocks <= 8 && units >= 2 * sms;
-        const int grid = alone ? (int)((units + kWarps - 1) / kWarps < sms ? (units + kWarps - 1) / kWarps : sms) : sms;
-        if (alone) A.workers = grid;
+        // Many short sequences: whole units to a warp, nothing to add up (1024 units of three pages: see the kernel).
+        const int whole = blocks <= 8 && units >= 2 * sms;
         return by_head_dim(cache->head_dim, [&](auto d) {
             constexpr int D = decltype(d)::value;
-            auto go = [&](auto bf, auto one) {
-                constexpr int DT = decltype(bf)::value ? TCQ_DT_BF16 : TCQ_DT_F16, W = decltype(one)::value ? 1 : kWarps;
-                if constexpr (D <= 64) {
-                    if (rows > 16) return launch_big<k_attention_few<DT, D, 2, W>>(dim3(grid), kWarps * 32, Few<D, 2, W>::BYTES, stream, A);
-                }
-                return launch_big<k_attention_few<DT, D, 1, W>>(dim3(grid), kWarps * 32, Few<D, 1, W>::BYTES, stream, A);
+            auto go = [&](auto bf, auto two) {
+                constexpr int DT = decltype(bf)::value ? TCQ_DT_BF16 : TCQ_DT_F16, MT = decltype(two)::value;
+                typedef Few<D, MT> P;
+                return launch_big<k_attention_few<DT, D, MT>>(dim3(sms), P::WARPS * 32, P::BYTES, stream, A, whole);
             };
+            const std::integral_constant<int, 1> one{};
             const std::true_type yes{};
             const std::false_type no{};
-            return dtype == TCQ_DT_BF16 ? (alone ? go(yes, yes) : go(yes, no)) : (alone ? go(no, yes) : go(no, no));
+            if constexpr (D <= 64) {
+                const std::integral_constant<int, 2> two{};
+                if (rows > 16) return dtype == TCQ_DT_BF16 ? go(yes, two) : go(no, two);
+            }
+            return dtype == TCQ_DT_BF16 ? go(yes, one) : go(no, one);
         });
     }
     if (rows > 0x7fffffff) return TCQ_ERR_SHAPE;

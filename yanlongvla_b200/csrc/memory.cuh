@@ -134,8 +134,8 @@ static inline int launch_pdl(void (*kern)(P...), dim3 grid, int threads, size_t 
 }
 
 // The same for a kernel with more than 48 KB of dynamic shared memory; the attribute is set once per device.
-template <auto Kern, class A>
-static inline int launch_big(dim3 grid, int threads, size_t smem, void* stream, const A& args) {
+template <auto Kern, class... A>
+static inline int launch_big(dim3 grid, int threads, size_t smem, void* stream, const A&... args) {
     static std::atomic<unsigned long long> set{0};
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev > 63) return TCQ_ERR_DEVICE;
@@ -143,7 +143,7 @@ static inline int launch_big(dim3 grid, int threads, size_t smem, void* stream, 
         if (cudaFuncSetAttribute(Kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) return TCQ_ERR_LAUNCH;
         set.fetch_or(1ull << dev, std::memory_order_relaxed);
     }
-    return launch_pdl(Kern, grid, threads, smem, stream, args);
+    return launch_pdl(Kern, grid, threads, smem, stream, args...);
 }
 
 static inline int check_cache(const tcq_kv8_cache* c) {
