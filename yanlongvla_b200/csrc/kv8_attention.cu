@@ -60,10 +60,12 @@ TCQ_HD int page_of(const int* row, int blk, int pages) { return page_in(row[blk]
 // power of two so that its largest element lies in [2^14, 2^15) (elements below 2^-28 of it lose bits, those of BF16
 // inputs above that lose none), and p <= 2^15.5 keeps 11 bits down to 2^-19 of the reference's and is dropped below 2^-30 of it.
 //
-// Layout. A warp takes whole pages. S = Q K^T and O = P V are m16n8k16 products. The order of a contraction is free, so lane
-// (n, t) reads 16 consecutive bytes of key row n (or of value row n: 16 tokens) and feeds them to four products: one 16-byte
-// shared load per 16 elements and no transposition. Key columns are assigned to score columns so that a lane's scores are
-// exactly the tokens whose values it reads: key(block 2 i + h, column 2 t + e) = 16 t + 4 i + 2 h + e.
+// Layout. A warp takes whole pages. S^T = K Q^T and O^T = V^T P^T are m16n8k16 products with the 64 keys (or the D value
+// rows) as rows and NT tiles of 8 queries as columns, so that one token's few queries waste least. The order of a contraction is
+// free, so lane (n, t) reads 16 consecutive bytes of key row n (or of value row n: 16 tokens) and feeds them to four products:
+// one 16-byte shared load per 16 elements and no transposition. Keys are assigned to the rows of S^T so that a lane's
+// weights, turned by movmatrix, are exactly the tokens whose values it reads: row c = 2 t + e of block nb (8 rows) is
+// key 16 t + 2 nb + e.
 //
 // int8 -> FP16: u = byte ^ 0x80, 0x6400 | u is 1024 + u, minus 1152: five instructions for four elements.
 
@@ -103,6 +105,13 @@ TCQ_HD void mma16816(float (&d)[4], u32 a0, u32 a1, u32 a2, u32 a3, u32 b0, u32 
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// An 8 x 8 matrix of 16-bit elements, a row in four lanes, transposed.
+TCQ_HD u32 turned(u32 v) {
+    u32 r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+
 // Power of two that brings a row whose largest magnitude is amax into FP16's upper range, and its inverse.
 TCQ_HD float row_scale(float amax, float& back) {
     int e = (int)((__float_as_uint(amax) >> 23) & 255) - 127;           // floor(log2), -127 for zero and subnormals
@@ -125,16 +134,24 @@ struct AttnArgs {
     float scale_log2;      // scale * log2(e)
 };
 
-// Plan of the few-row kernel. Every warp is a worker with a ring of NH half pages (64 D bytes: a block's keys or its values)
-// of its own. Twelve warps where their registers fit (a warp alone issues one instruction in about four clocks), else eight.
-template <int D, int MT>
+// Plan of the few-row kernel. Every warp has a ring of NH half pages (64 D bytes: a block's keys or its values) of its own. As
+// many warps as their registers and rings allow: a warp alone issues one instruction in about four clocks.
+template <int D, int NT>
 struct Few {
-    static constexpr int WARPS = D <= 64 && MT == 1 ? 12 : 8;
     static constexpr int HALF = kBlk * D;
-    static constexpr int NH = D == 32 ? 8 : D == 48 ? 6 : D == 64 ? (WARPS == 12 ? 4 : 6) : D == 80 ? 5 : D == 96 ? 4 : 3;
+#ifndef FW
+#define FW 12
+#endif
+#ifndef FNB
+#define FNB 4
+#endif
+    static constexpr int WARPS = NT == 1 ? (D <= 64 ? FW : D < 128 ? 12 : 8) : NT == 2 && D <= 64 ? 12 : 8;
+    static constexpr int FIT = 216 * 1024 / (WARPS * HALF), NH = FIT < 8 ? FIT : 8;
+    static_assert(NH >= 3, "a half page in use and two on their way");
     static constexpr int HDR = WARPS * NH * HALF;                          // ks, vs of each half page
     static constexpr int SCAN = HDR + WARPS * NH * 8;                      // the block's scan of the lengths
     static constexpr int BYTES = SCAN + 4 * WARPS * (int)sizeof(int);
+    static_assert(8 * NT * (D + 2) * 4 <= NH * HALF, "a warp's part of a unit fits its ring");
 };
 
 // 16-byte chunk c of key row r lies at chunk c ^ swap(r): rows of 128 bytes put their halves on alternating banks.
@@ -151,7 +168,7 @@ struct Place {
 // loads in flight want registers of their own.
 template <int DT, int D>
 __device__ __noinline__ void add_parts(const float* parts, i64 size, int first, int last, int R, int group, u16* out, i64 token) {
-    constexpr int NI = 4, NB = 8;                 // pairs of elements of a lane, parts requested at once
+    constexpr int NI = 4, NB = FNB;                 // pairs of elements of a lane, parts requested at once
     const int lane = threadIdx.x & 31;
 #pragma unroll 1
     for (int i0 = 0; i0 < R * (D / 2); i0 += 32 * NI) {
@@ -199,14 +216,17 @@ __device__ __noinline__ void add_parts(const float* parts, i64 size, int first, 
     }
 }
 
-// Work. The pages of all sequences and heads form one list, cut into equal runs, one per warp (a unit is one head of one
-// sequence; an empty one takes a place without a page). A warp that holds a whole unit writes its output; parts of a unit go to
-// the workspace, and the last of its warps to arrive adds them in their order, so the result does not depend on timing.
-// whole != 0 (many short sequences): each warp takes whole units instead, one after the other.
-template <int DT, int D, int MT>
-__global__ void __launch_bounds__(Few<D, MT>::WARPS * 32, 1) k_attention_few(const AttnArgs A, int whole) {
-    typedef Few<D, MT> P;
-    constexpr int NH = P::NH, KS = D / 16, ROWS = 16 * MT, WARPS = P::WARPS;
+// Work, by what the lengths say:
+// - the pages of all sequences and heads form one list, cut into equal runs, one per warp (a unit is one head of one sequence;
+//   an empty one takes a place without a page). A warp that holds a whole unit writes its output; parts of a unit go to the
+//   workspace, and the last of its warps to arrive adds them in their order, so the result does not depend on timing;
+// - no more units than CTAs, of at most three pages per warp: a CTA takes a unit, its warps every WARPS-th page, and the parts are
+//   added in shared memory (one token over 203 keys of 8 heads: 5 us less than through the workspace);
+// - whole != 0 (many short sequences, told by the host): each warp takes whole units, one after the other.
+template <int DT, int D, int NT>
+__global__ void __launch_bounds__(Few<D, NT>::WARPS * 32, 1) k_attention_few(const AttnArgs A, int whole) {
+    typedef Few<D, NT> P;
+    constexpr int NH = P::NH, KS = D / 16, WARPS = P::WARPS;
     extern __shared__ __align__(16) char smem[];
     int* s_scan = reinterpret_cast<int*>(smem + P::SCAN);
     pdl_launch_dependents();
@@ -218,8 +238,8 @@ __global__ void __launch_bounds__(Few<D, MT>::WARPS * 32, 1) k_attention_few(con
     char* ring = smem + warp * NH * P::HALF;
     float2* hdr = reinterpret_cast<float2*>(smem + P::HDR) + warp * NH;
 
-    // ---- this worker's range [x0, x1) of places, and where it begins
-    int chunk = 1, x0, x1;
+    // ---- this worker's places x0, x0 + stride, .. below x1, and the unit they begin in
+    int chunk = 1, stride = 1, x0, x1;
     Place at;
     auto places = [&](int len) { return max(1, (len + kBlk - 1) / kBlk); };
     if (whole) {
@@ -229,8 +249,11 @@ __global__ void __launch_bounds__(Few<D, MT>::WARPS * 32, 1) k_attention_few(con
     } else {
         // all sequences' lengths: every thread a run of them, summed over the block
         const int per = (A.B + WARPS * 32 - 1) / (WARPS * 32), b0 = min(A.B, tid * per), b1 = min(A.B, b0 + per);
-        int mine = 0;
-        for (int b = b0; b < b1; ++b) mine += places(tokens_of(A.lens, b, A.blocks));
+        int mine = 0, most = 0;
+        for (int b = b0; b < b1; ++b) {
+            const int v = places(tokens_of(A.lens, b, A.blocks));
+            mine += v, most = max(most, v);
+        }
         int scan = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -238,32 +261,40 @@ __global__ void __launch_bounds__(Few<D, MT>::WARPS * 32, 1) k_attention_few(con
             if (lane >= o) scan += v;
         }
         if (lane == 31) s_scan[warp] = scan;
-        __syncthreads();
-        int before = scan - mine, all = 0;
+        const bool block = A.B * Hk <= gridDim.x && __syncthreads_and(most <= 3 * WARPS);
+        if (A.B * Hk > gridDim.x) __syncthreads();
+        if (block) {
+            if (blockIdx.x >= A.B * Hk) return;
+            stride = WARPS;
+            at.b = blockIdx.x / Hk, at.h = blockIdx.x - at.b * Hk, at.ubeg = 0;
+            x0 = warp, x1 = 1 << 30;
+        } else {
+            int before = scan - mine, all = 0;
 #pragma unroll
-        for (int w = 0; w < WARPS; ++w) {
-            before += w < warp ? s_scan[w] : 0;
-            all += s_scan[w];
-        }
-        all *= Hk;
-        chunk = (all + workers - 1) / workers;
-        int off = before * Hk;
-        for (int b = b0; b < b1; ++b) {
-            const int v = places(tokens_of(A.lens, b, A.blocks)) * Hk;
-#pragma unroll 1
             for (int w = 0; w < WARPS; ++w) {
-                const i64 x = (i64)(w * gridDim.x + blockIdx.x) * chunk;
-                if (x >= off && x < off + v) s_scan[WARPS + 2 * w] = b, s_scan[WARPS + 2 * w + 1] = off;
+                before += w < warp ? s_scan[w] : 0;
+                all += s_scan[w];
             }
-            off += v;
+            all *= Hk;
+            chunk = (all + workers - 1) / workers;
+            int off = before * Hk;
+            for (int b = b0; b < b1; ++b) {
+                const int v = places(tokens_of(A.lens, b, A.blocks)) * Hk;
+#pragma unroll 1
+                for (int w = 0; w < WARPS; ++w) {
+                    const i64 x = (i64)(w * gridDim.x + blockIdx.x) * chunk;
+                    if (x >= off && x < off + v) s_scan[WARPS + 2 * w] = b, s_scan[WARPS + 2 * w + 1] = off;
+                }
+                off += v;
+            }
+            __syncthreads();
+            if ((i64)me * chunk >= all) return;
+            x0 = me * chunk, x1 = min(x0 + chunk, all);
+            at.b = s_scan[WARPS + 2 * warp];
+            const int vp = places(tokens_of(A.lens, at.b, A.blocks));
+            at.h = (x0 - s_scan[WARPS + 2 * warp + 1]) / vp;
+            at.ubeg = s_scan[WARPS + 2 * warp + 1] + at.h * vp;
         }
-        __syncthreads();
-        if ((i64)me * chunk >= all) return;
-        x0 = me * chunk, x1 = min(x0 + chunk, all);
-        at.b = s_scan[WARPS + 2 * warp];
-        const int vp = places(tokens_of(A.lens, at.b, A.blocks));
-        at.h = (x0 - s_scan[WARPS + 2 * warp + 1]) / vp;
-        at.ubeg = s_scan[WARPS + 2 * warp + 1] + at.h * vp;
     }
     auto measure = [&](Place& p) {
         const int len = tokens_of(A.lens, p.b, A.blocks);
@@ -271,7 +302,8 @@ __global__ void __launch_bounds__(Few<D, MT>::WARPS * 32, 1) k_attention_few(con
         p.vp = max(1, p.np);
     };
     measure(at);
-    if (whole) at.ubeg = 0, x1 = at.vp;
+    if (whole) at.ubeg = 0;
+    if (whole || stride > 1) x1 = at.vp;
     // The next unit of the range; false at its end.
     auto next_unit = [&](Place& p, int& end) -> bool {
         if (whole) {
@@ -307,7 +339,7 @@ __global__ void __launch_bounds__(Few<D, MT>::WARPS * 32, 1) k_attention_few(con
                 continue;
             }
             if (px - pat.ubeg < pat.np) break;
-            ++px;
+            px += stride;
         }
         pid = page_of(A.table + (i64)pat.b * A.blocks, px - pat.ubeg, A.cache.pages);
     };
@@ -332,7 +364,7 @@ __global__ void __launch_bounds__(Few<D, MT>::WARPS * 32, 1) k_attention_few(con
             } else {
 #pragma unroll
                 for (int i = 0; i < D / 8; ++i) cp_async16(dst + (lane + 32 * i) * 16, src + (lane + 32 * i) * 16);
-                ++px;
+                px += stride;
                 p_settle();
             }
             p_values = !p_values;
@@ -356,210 +388,235 @@ __global__ void __launch_bounds__(Few<D, MT>::WARPS * 32, 1) k_attention_few(con
     int x = x0;
     for (;;) {
         const int len = tokens_of(A.lens, at.b, A.blocks), cnt = queries_of(A.count, at.b, A.T);
-        // query rows r = t * group + g of this head, as FP16 fragments scaled by a power of two
-        u32 qa[MT][KS][4];
-        float crow[MT][2];
-        int limit[MT][2];
+        // query rows r = t * group + g of this head, as FP16 columns scaled by a power of two; a lane loads row 8 nt + n and
+        // keeps the scores of rows 8 nt + 2 t + e
+        u32 qb[NT][KS][2];
+        float crow[NT][2];
+        int limit[NT][2];
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
+        for (int nt = 0; nt < NT; ++nt) {
+            const int r = 8 * nt + n, tq = r / A.group;
+            const bool live = r < R && tq < cnt;
+            const u16* qr = A.q + at.b * A.q_sb + tq * A.q_st + (i64)(at.h * A.group + r - tq * A.group) * D;
+            float v[KS][4], amax = 0.f;
 #pragma unroll
-            for (int hf = 0; hf < 2; ++hf) {
-                const int r = 16 * mt + 8 * hf + n, tq = r / A.group, g = r - tq * A.group;
-                const bool live = r < R && tq < cnt;
-                limit[mt][hf] = !live ? 0 : A.causal ? min(max(len - cnt + tq + 1, 0), len) : len;
-                const u16* qr = A.q + at.b * A.q_sb + tq * A.q_st + (i64)(at.h * A.group + g) * D;
-                float v[KS][4], amax = 0.f;
+            for (int s = 0; s < KS; ++s) {
+                // the four elements that lane t contributes to step s (see the key loads)
+                const int d = s < D / 64 * 4 ? 64 * (s / 4) + 16 * t + 4 * (s % 4)
+                            : s < D / 32 * 2 ? D / 64 * 64 + 8 * t + 4 * (s - D / 64 * 4) : D / 32 * 32 + 4 * t;
+                const uint2 w = live ? *reinterpret_cast<const uint2*>(qr + d) : make_uint2(0u, 0u);
+                unpack2<DT>(w.x, v[s][0], v[s][1]);
+                unpack2<DT>(w.y, v[s][2], v[s][3]);
 #pragma unroll
-                for (int s = 0; s < KS; ++s) {
-                    // the four elements that lane t contributes to step s (see the key loads)
-                    const int d = s < D / 64 * 4 ? 64 * (s / 4) + 16 * t + 4 * (s % 4)
-                                : s < D / 32 * 2 ? D / 64 * 64 + 8 * t + 4 * (s - D / 64 * 4) : D / 32 * 32 + 4 * t;
-                    uint2 w = live ? *reinterpret_cast<const uint2*>(qr + d) : make_uint2(0u, 0u);
-                    unpack2<DT>(w.x, v[s][0], v[s][1]);
-                    unpack2<DT>(w.y, v[s][2], v[s][3]);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) amax = fmaxf(amax, fabsf(v[s][e]));
-                }
-                amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-                amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-                float back;
-                const float up = row_scale(amax, back);
-                crow[mt][hf] = back * A.scale_log2;
-#pragma unroll
-                for (int s = 0; s < KS; ++s) {
-                    qa[mt][s][hf] = half2_of(v[s][0] * up, v[s][1] * up);
-                    qa[mt][s][2 + hf] = half2_of(v[s][2] * up, v[s][3] * up);
-                }
+                for (int e = 0; e < 4; ++e) amax = fmaxf(amax, fabsf(v[s][e]));
             }
+            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+            float back;
+            const float up = row_scale(amax, back);
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                qb[nt][s][0] = half2_of(v[s][0] * up, v[s][1] * up);
+                qb[nt][s][1] = half2_of(v[s][2] * up, v[s][3] * up);
+            }
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int rs = 8 * nt + 2 * t + e, ts = rs / A.group;
+                crow[nt][e] = __shfl_sync(0xffffffffu, back, 4 * (2 * t + e)) * A.scale_log2;
+                limit[nt][e] = rs >= R || ts >= cnt ? 0 : A.causal ? min(max(len - cnt + ts + 1, 0), len) : len;
+            }
+        }
         const int open = A.causal ? len - cnt + 1 : len;         // keys below this are seen by every query
-        float o[MT][D / 8][4], m[MT][2], l[MT][2];
+        float o[NT][D / 16][4], m[NT][2], l[NT][2];
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
+        for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-            for (int i = 0; i < D / 8; ++i) o[mt][i][0] = o[mt][i][1] = o[mt][i][2] = o[mt][i][3] = 0.f;
-            m[mt][0] = m[mt][1] = -INFINITY;
-            l[mt][0] = l[mt][1] = 0.f;
+            for (int i = 0; i < D / 16; ++i) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.f;
+            m[nt][0] = m[nt][1] = -INFINITY;
+            l[nt][0] = l[nt][1] = 0.f;
         }
         const int seg_end = min(at.ubeg + at.vp, end);
 #pragma unroll 1
-        for (; x < seg_end; ++x) {
+        for (; x < seg_end; x += stride) {
             const int pg = x - at.ubeg;
             if (pg >= at.np) continue;
             const float2* sp = hdr + slot;
             const char* kp = take();
             const float2 sc = *sp;
             slot = slot + 1 == NH ? 0 : slot + 1;
-            float s[MT][8][4];
+            // scores: tile j holds blocks 2 j (rows 0..7) and 2 j + 1
+            float s[NT][4][4];
 #pragma unroll
-            for (int nb = 0; nb < 8; ++nb) {
-                const int r = 16 * (n >> 1) + 2 * nb + (n & 1);           // nb = 2 i + h: 4 i + 2 h = 2 nb
-                const char* row = kp + r * D;
+            for (int j = 0; j < 4; ++j) {
+                const int r = 16 * (n >> 1) + 4 * j + (n & 1);
+                const char *ra = kp + r * D, *rb = ra + 2 * D;
 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt) s[mt][nb][0] = s[mt][nb][1] = s[mt][nb][2] = s[mt][nb][3] = 0.f;
-                auto step = [&](int ks, u32 w) {
-                    u32 b0, b1;
-                    int8x4_to_half(w, b0, b1);
+                for (int nt = 0; nt < NT; ++nt) s[nt][j][0] = s[nt][j][1] = s[nt][j][2] = s[nt][j][3] = 0.f;
+                auto step = [&](int ks, u32 wa, u32 wb) {
+                    u32 a0, a1, a2, a3;
+                    int8x4_to_half(wa, a0, a2);
+                    int8x4_to_half(wb, a1, a3);
 #pragma unroll
-                    for (int mt = 0; mt < MT; ++mt) mma16816(s[mt][nb], qa[mt][ks][0], qa[mt][ks][1], qa[mt][ks][2], qa[mt][ks][3], b0, b1);
+                    for (int nt = 0; nt < NT; ++nt) mma16816(s[nt][j], a0, a1, a2, a3, qb[nt][ks][0], qb[nt][ks][1]);
                 };
 #pragma unroll
                 for (int q4 = 0; q4 < D / 64; ++q4) {
-                    const uint4 w = *reinterpret_cast<const uint4*>(row + key_chunk<D>(r, 4 * q4 + t) * 16);
-                    step(4 * q4, w.x), step(4 * q4 + 1, w.y), step(4 * q4 + 2, w.z), step(4 * q4 + 3, w.w);
+                    const uint4 u = *reinterpret_cast<const uint4*>(ra + key_chunk<D>(r, 4 * q4 + t) * 16);
+                    const uint4 v = *reinterpret_cast<const uint4*>(rb + key_chunk<D>(r + 2, 4 * q4 + t) * 16);
+                    step(4 * q4, u.x, v.x), step(4 * q4 + 1, u.y, v.y), step(4 * q4 + 2, u.z, v.z), step(4 * q4 + 3, u.w, v.w);
                 }
                 if (D % 64 >= 32) {
-                    const uint2 w = *reinterpret_cast<const uint2*>(row + D / 64 * 64 + 8 * t);
-                    step(D / 64 * 4, w.x), step(D / 64 * 4 + 1, w.y);
+                    const uint2 u = *reinterpret_cast<const uint2*>(ra + D / 64 * 64 + 8 * t), v = *reinterpret_cast<const uint2*>(rb + D / 64 * 64 + 8 * t);
+                    step(D / 64 * 4, u.x, v.x), step(D / 64 * 4 + 1, u.y, v.y);
                 }
-                if (D % 32) step(D / 32 * 2, *reinterpret_cast<const u32*>(row + D / 32 * 32 + 4 * t));
+                if (D % 32)
+                    step(D / 32 * 2, *reinterpret_cast<const u32*>(ra + D / 32 * 32 + 4 * t), *reinterpret_cast<const u32*>(rb + D / 32 * 32 + 4 * t));
             }
             const float vs = safe_scale(sc.y), bias = lg2(vs), inv = rcp(vs);
             const bool masked = (pg + 1) * kBlk > open;
+            u32 pb[NT][4][2];
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
+            for (int nt = 0; nt < NT; ++nt) {
+                float top[2];
 #pragma unroll
-                for (int hf = 0; hf < 2; ++hf) {
-                    if (16 * mt + 8 * hf >= R) continue;
-                    const float c = crow[mt][hf] * sc.x;
-                    float top = -INFINITY;
+                for (int e = 0; e < 2; ++e) {
+                    const float c = crow[nt][e] * sc.x;
                     if (masked) {
-                        const int lim = limit[mt][hf] - pg * kBlk - 16 * t;
+                        const int lim = limit[nt][e] - pg * kBlk - 16 * (n >> 1) - (n & 1);
 #pragma unroll
-                        for (int nb = 0; nb < 8; ++nb)
-#pragma unroll
-                            for (int e = 0; e < 2; ++e) {
-                                float& v = s[mt][nb][2 * hf + e];
-                                v = 2 * nb + e < lim ? __fmaf_rn(v, c, bias) : -INFINITY;
-                                top = fmaxf(top, v);
-                            }
+                        for (int j = 0; j < 4; ++j) {
+                            s[nt][j][e] = 4 * j < lim ? __fmaf_rn(s[nt][j][e], c, bias) : -INFINITY;
+                            s[nt][j][2 + e] = 4 * j + 2 < lim ? __fmaf_rn(s[nt][j][2 + e], c, bias) : -INFINITY;
+                        }
                     } else {
 #pragma unroll
-                        for (int nb = 0; nb < 8; ++nb)
-#pragma unroll
-                            for (int e = 0; e < 2; ++e) {
-                                float& v = s[mt][nb][2 * hf + e];
-                                v = __fmaf_rn(v, c, bias);
-                                top = fmaxf(top, v);
-                            }
+                        for (int j = 0; j < 4; ++j) {
+                            s[nt][j][e] = __fmaf_rn(s[nt][j][e], c, bias);
+                            s[nt][j][2 + e] = __fmaf_rn(s[nt][j][2 + e], c, bias);
+                        }
                     }
-                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                    float& mr = m[mt][hf];
-                    const bool move = top > mr + kSlack;
-                    if (__any_sync(0xffffffffu, move)) {
-                        const float f = move ? ex2(mr - top) : 1.f;
-                        if (move) mr = top;
-                        l[mt][hf] *= f;
+                    top[e] = fmaxf(fmaxf(fmaxf(s[nt][0][e], s[nt][0][2 + e]), fmaxf(s[nt][1][e], s[nt][1][2 + e])),
+                                   fmaxf(fmaxf(s[nt][2][e], s[nt][2][2 + e]), fmaxf(s[nt][3][e], s[nt][3][2 + e])));
+                }
 #pragma unroll
-                        for (int i = 0; i < D / 8; ++i) o[mt][i][2 * hf] *= f, o[mt][i][2 * hf + 1] *= f;
-                    }
-                    const float base = (mr == -INFINITY ? 0.f : mr) - kRef;
+                for (int d = 4; d < 32; d <<= 1) {
+                    top[0] = fmaxf(top[0], __shfl_xor_sync(0xffffffffu, top[0], d));
+                    top[1] = fmaxf(top[1], __shfl_xor_sync(0xffffffffu, top[1], d));
+                }
+                const bool move0 = top[0] > m[nt][0] + kSlack, move1 = top[1] > m[nt][1] + kSlack;
+                if (__any_sync(0xffffffffu, move0 || move1)) {
+                    const float f0 = move0 ? ex2(m[nt][0] - top[0]) : 1.f, f1 = move1 ? ex2(m[nt][1] - top[1]) : 1.f;
+                    if (move0) m[nt][0] = top[0];
+                    if (move1) m[nt][1] = top[1];
+                    l[nt][0] *= f0, l[nt][1] *= f1;
+#pragma unroll
+                    for (int i = 0; i < D / 16; ++i) o[nt][i][0] *= f0, o[nt][i][1] *= f1, o[nt][i][2] *= f0, o[nt][i][3] *= f1;
+                }
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const float base = (m[nt][e] == -INFINITY ? 0.f : m[nt][e]) - kRef;
                     float sum = 0.f;
 #pragma unroll
-                    for (int nb = 0; nb < 8; ++nb)
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            float& v = s[mt][nb][2 * hf + e];
-                            v = ex2(v - base);
-                            sum += v;
-                        }
-                    l[mt][hf] = __fmaf_rn(sum, inv, l[mt][hf]);
+                    for (int j = 0; j < 4; ++j) {
+                        s[nt][j][e] = ex2(s[nt][j][e] - base), s[nt][j][2 + e] = ex2(s[nt][j][2 + e] - base);
+                        sum += s[nt][j][e] + s[nt][j][2 + e];
+                    }
+                    l[nt][e] = __fmaf_rn(sum, inv, l[nt][e]);
                 }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    pb[nt][j][0] = turned(half2_of(s[nt][j][0], s[nt][j][1]));
+                    pb[nt][j][1] = turned(half2_of(s[nt][j][2], s[nt][j][3]));
+                }
+            }
             if (sc.y < kLeastScale) {
 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt)
+                for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                    for (int nb = 0; nb < 8; ++nb) s[mt][nb][0] = s[mt][nb][1] = s[mt][nb][2] = s[mt][nb][3] = 0.f;
+                    for (int j = 0; j < 4; ++j) pb[nt][j][0] = pb[nt][j][1] = 0u;
             }
-            u32 pa[MT][4][4];
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const bool high = 16 * mt + 8 < R;
-                    pa[mt][i][0] = half2_of(s[mt][2 * i][0], s[mt][2 * i][1]);
-                    pa[mt][i][1] = high ? half2_of(s[mt][2 * i][2], s[mt][2 * i][3]) : 0u;
-                    pa[mt][i][2] = half2_of(s[mt][2 * i + 1][0], s[mt][2 * i + 1][1]);
-                    pa[mt][i][3] = high ? half2_of(s[mt][2 * i + 1][2], s[mt][2 * i + 1][3]) : 0u;
-                }
             const char* vp = take();
             slot = slot + 1 == NH ? 0 : slot + 1;
 #pragma unroll
-            for (int db = 0; db < D / 8; ++db) {
-                const uint4 w = *reinterpret_cast<const uint4*>(vp + (8 * db + n) * kBlk + 16 * t);
-                const u32 ww[4] = {w.x, w.y, w.z, w.w};
+            for (int i = 0; i < D / 16; ++i) {
+                const uint4 u = *reinterpret_cast<const uint4*>(vp + (16 * i + n) * kBlk + 16 * t);
+                const uint4 v = *reinterpret_cast<const uint4*>(vp + (16 * i + 8 + n) * kBlk + 16 * t);
+                const u32 uu[4] = {u.x, u.y, u.z, u.w}, vv[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    u32 b0, b1;
-                    int8x4_to_half(ww[i], b0, b1);
+                for (int j = 0; j < 4; ++j) {
+                    u32 a0, a1, a2, a3;
+                    int8x4_to_half(uu[j], a0, a2);
+                    int8x4_to_half(vv[j], a1, a3);
 #pragma unroll
-                    for (int mt = 0; mt < MT; ++mt) mma16816(o[mt][db], pa[mt][i][0], pa[mt][i][1], pa[mt][i][2], pa[mt][i][3], b0, b1);
+                    for (int nt = 0; nt < NT; ++nt) mma16816(o[nt][i], a0, a1, a2, a3, pb[nt][j][0], pb[nt][j][1]);
                 }
             }
         }
         // ---- the unit's rows, or this worker's part of them
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int hf = 0; hf < 2; ++hf) {
-                float& v = l[mt][hf];
-                v += __shfl_xor_sync(0xffffffffu, v, 1);
-                v += __shfl_xor_sync(0xffffffffu, v, 2);
-                if (limit[mt][hf] == 0) v = 0.f;              // a row that sees no token
+            for (int e = 0; e < 2; ++e) {
+                float& v = l[nt][e];
+#pragma unroll
+                for (int d = 4; d < 32; d <<= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+                if (limit[nt][e] == 0) v = 0.f;               // a row that sees no token
             }
         auto out_row = [&](int r) -> u16* {
             const int tq = r / A.group;
             return A.out + (((i64)at.b * A.T + tq) * A.heads + at.h * A.group + r - tq * A.group) * D;
         };
-        const bool all_of_it = at.ubeg >= (whole ? 0 : x0) && seg_end == at.ubeg + at.vp;
-        if (all_of_it) {
+        // a part: rows of D sums, the reference and the sum of weights
+        auto write_part = [&](float* part) {
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int hf = 0; hf < 2; ++hf) {
-                    const int r = 16 * mt + 8 * hf + n;
+                for (int e = 0; e < 2; ++e) {
+                    const int r = 8 * nt + 2 * t + e;
                     if (r >= R) continue;
-                    const float f = l[mt][hf] != 0.f ? 1.f / l[mt][hf] : 0.f;
-                    u32* dst = reinterpret_cast<u32*>(out_row(r));
+                    float* row = part + r * (D + 2);
 #pragma unroll
-                    for (int i = 0; i < D / 8; ++i) dst[4 * i + t] = pack2<DT>(o[mt][i][2 * hf] * f, o[mt][i][2 * hf + 1] * f);
+                    for (int i = 0; i < D / 16; ++i) row[16 * i + n] = o[nt][i][e], row[16 * i + 8 + n] = o[nt][i][2 + e];
+                    if (n == 0) row[D] = m[nt][e], row[D + 1] = l[nt][e];
                 }
+        };
+        if (stride > 1) {
+            __syncwarp();
+            write_part(reinterpret_cast<float*>(ring));
+            __syncthreads();
+            for (int i = tid; i < R * (D / 2); i += WARPS * 32) {
+                const int r = i / (D / 2), d = 2 * (i - r * (D / 2));
+                const char* part = smem + r * (D + 2) * 4;
+                float top = -INFINITY, sum = 0.f, a0 = 0.f, a1 = 0.f;
+#pragma unroll
+                for (int w = 0; w < WARPS; ++w) top = fmaxf(top, reinterpret_cast<const float*>(part + w * NH * P::HALF)[D]);
+#pragma unroll
+                for (int w = 0; w < WARPS; ++w) {
+                    const float* row = reinterpret_cast<const float*>(part + w * NH * P::HALF);
+                    const float f = top == -INFINITY ? 0.f : ex2(row[D] - top);
+                    sum = __fmaf_rn(row[D + 1], f, sum), a0 = __fmaf_rn(row[d], f, a0), a1 = __fmaf_rn(row[d + 1], f, a1);
+                }
+                const float f = sum != 0.f ? 1.f / sum : 0.f;
+                *reinterpret_cast<u32*>(out_row(r) + d) = pack2<DT>(a0 * f, a1 * f);
+            }
+            break;
+        }
+        if (at.ubeg >= (whole ? 0 : x0) && seg_end == at.ubeg + at.vp) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                const float f0 = l[nt][0] != 0.f ? 1.f / l[nt][0] : 0.f, f1 = l[nt][1] != 0.f ? 1.f / l[nt][1] : 0.f;
+                const int r = 8 * nt + n;                     // after the turn a lane holds row n, elements 2 t and 2 t + 1
+                u32* dst = reinterpret_cast<u32*>(out_row(r));
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i) {
+                    const u32 lo = turned(pack2<DT>(o[nt][i][0] * f0, o[nt][i][1] * f1)), hi = turned(pack2<DT>(o[nt][i][2] * f0, o[nt][i][3] * f1));
+                    if (r < R) dst[8 * i + t] = lo, dst[8 * i + 4 + t] = hi;
+                }
+            }
         } else {
-            // a part: rows of D sums, the reference and the sum of weights; a worker has at most two, its first unit's and its last's
+            // a worker has at most two parts, of its first unit and of its last
             const int first = at.ubeg / chunk, last = (at.ubeg + at.vp - 1) / chunk;
-            auto record = [&](int w) -> float* { return A.part + (i64)(2 * w + (w == first ? 1 : 0)) * ROWS * (D + 2); };
-            float* part = record(me);
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                for (int hf = 0; hf < 2; ++hf) {
-                    const int r = 16 * mt + 8 * hf + n;
-                    if (r >= R) continue;
-#pragma unroll
-                    for (int i = 0; i < D / 8; ++i)
-                        *reinterpret_cast<float2*>(part + r * (D + 2) + 8 * i + 2 * t) = make_float2(o[mt][i][2 * hf], o[mt][i][2 * hf + 1]);
-                    if (t == 0) *reinterpret_cast<float2*>(part + r * (D + 2) + D) = make_float2(m[mt][hf], l[mt][hf]);
-                }
+            write_part(A.part + (i64)(2 * me + (me == first ? 1 : 0)) * (8 * NT) * (D + 2));
             __threadfence();
             __syncwarp();
             int seen = 0;
@@ -568,7 +625,7 @@ __global__ void __launch_bounds__(Few<D, MT>::WARPS * 32, 1) k_attention_few(con
             if (seen == last - first) {
                 if (lane == 0) A.counters[first] = 0;
                 __threadfence();
-                add_parts<DT, D>(A.part, (i64)ROWS * (D + 2), first, last, R, A.group, out_row(0), (i64)A.heads * D);
+                add_parts<DT, D>(A.part, (i64)(8 * NT) * (D + 2), first, last, R, A.group, out_row(0), (i64)A.heads * D);
             }
         }
         if (!next_unit(at, end)) break;
@@ -1279,7 +1336,7 @@ int launch_many(const AttnArgs& A, void* stream) {
 }
 
 // Arrival counters at the head of the workspace, one per worker of the few-row kernel.
-constexpr int kMostWarps = 12;
+constexpr int kMostWarps = 16;
 inline size_t counter_bytes(int sms) { return ((size_t)kMostWarps * sms * sizeof(int) + 15) & ~(size_t)15; }
 
 // ------------------------------------------------------------------------------------------------ host side
@@ -1287,14 +1344,14 @@ inline size_t counter_bytes(int sms) { return ((size_t)kMostWarps * sms * sizeof
 
 extern "C" {
 
-// Rows that the few-row kernel takes: one m16 tile, or two where both fit the registers (head widths up to 64).
+// Rows that the few-row kernel takes: two tiles of 8, or four where they fit the registers (head widths up to 64).
 static inline bool few_rows(i64 rows, int head_dim) { return rows <= 16 || (rows <= 32 && head_dim <= 64); }
 
 size_t tcq_kv8_attention_workspace(int B, int T, int heads, int kv_heads, int head_dim, int blocks) {
     if (B < 1 || T < 1 || heads < 1 || kv_heads < 1 || head_dim < 1 || blocks < 1 || heads % kv_heads) return 0;
     const int sms = tcq_sm_count();
     const i64 rows = (i64)T * (heads / kv_heads);
-    if (few_rows(rows, head_dim)) return counter_bytes(sms) + (size_t)2 * kMostWarps * sms * (rows <= 16 ? 16 : 32) * (head_dim + 2) * sizeof(float);
+    if (few_rows(rows, head_dim)) return counter_bytes(sms) + (size_t)2 * kMostWarps * sms * ((rows + 7) / 8 * 8) * (head_dim + 2) * sizeof(float);
     return 16;
 }
 
@@ -1321,19 +1378,17 @@ int tcq_kv8_attention(const tcq_kv8_cache* cache, const void* q, int dtype, int6
         const int whole = blocks <= 8 && units >= 2 * sms;
         return by_head_dim(cache->head_dim, [&](auto d) {
             constexpr int D = decltype(d)::value;
-            auto go = [&](auto bf, auto two) {
-                constexpr int DT = decltype(bf)::value ? TCQ_DT_BF16 : TCQ_DT_F16, MT = decltype(two)::value;
-                typedef Few<D, MT> P;
-                return launch_big<k_attention_few<DT, D, MT>>(dim3(sms), P::WARPS * 32, P::BYTES, stream, A, whole);
+            auto go = [&](auto tiles) {
+                constexpr int NT = decltype(tiles)::value;
+                typedef Few<D, NT> P;
+                return dtype == TCQ_DT_BF16 ? launch_big<k_attention_few<TCQ_DT_BF16, D, NT>>(dim3(sms), P::WARPS * 32, P::BYTES, stream, A, whole)
+                                            : launch_big<k_attention_few<TCQ_DT_F16, D, NT>>(dim3(sms), P::WARPS * 32, P::BYTES, stream, A, whole);
             };
-            const std::integral_constant<int, 1> one{};
-            const std::true_type yes{};
-            const std::false_type no{};
             if constexpr (D <= 64) {
-                const std::integral_constant<int, 2> two{};
-                if (rows > 16) return dtype == TCQ_DT_BF16 ? go(yes, two) : go(no, two);
+                if (rows > 24) return go(std::integral_constant<int, 4>());
+                if (rows > 16) return go(std::integral_constant<int, 3>());
             }
-            return dtype == TCQ_DT_BF16 ? go(yes, one) : go(no, one);
+            return rows > 8 ? go(std::integral_constant<int, 2>()) : go(std::integral_constant<int, 1>());
         });
     }
     if (rows > 0x7fffffff) return TCQ_ERR_SHAPE;
