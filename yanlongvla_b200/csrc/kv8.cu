@@ -34,9 +34,10 @@ template <int DT, int V>
 struct Vec {
     static constexpr int BYTES = V * (DT == TCQ_DT_F32 ? 4 : 2);
     typedef typename Raw<BYTES>::type R;
-    static TCQ_HD void load(const void* p, float* v) {
+    static TCQ_HD void load(const void* p, float* v) { unpack(*reinterpret_cast<const R*>(p), v); }
+    static TCQ_HD void unpack(R r, float* v) {
         union { R r; u32 w[(BYTES + 3) / 4]; u16 h[BYTES / 2]; } u;
-        u.r = *reinterpret_cast<const R*>(p);
+        u.r = r;
 #pragma unroll
         for (int i = 0; i < V; ++i) v[i] = DT == TCQ_DT_F32 ? __uint_as_float(u.w[i]) : elem_f<DT>(u.h[i]);
     }
@@ -55,7 +56,7 @@ struct Vec {
     }
 };
 
-template <int DT, int V, bool PAIRS>
+template <int DT, int V, bool PAIRS, int HB>
 __global__ void __launch_bounds__(256) k_rope_axes(const char* __restrict__ x, char* __restrict__ out, RopeArgs r, i64 x_sb, i64 x_st,
                                                    i64 o_sb, i64 o_st, i64 rows, int T, int heads, int C, int hp, float sign) {
     constexpr int E = DT == TCQ_DT_F32 ? 4 : 2;
@@ -69,21 +70,39 @@ __global__ void __launch_bounds__(256) k_rope_axes(const char* __restrict__ x, c
     const int D = 2 * r.half, first = PAIRS ? 2 * V * c : V * c, second = PAIRS ? first + V : first + r.half;
     const char* xr = x + (b * x_sb + t * x_st) * E;
     char* orow = out + (b * o_sb + t * o_st) * E;
+    // HB > 1: that many heads are requested before the tables, whose loads wait for the positions
+    typedef typename Vec<DT, V>::R Rv;
     float cs[V], sn[V];
-    rope_cs<V>(r, row, V * c, cs, sn, &g_tcq_memory_error);
+    auto tables = [&]() {
+        rope_cs<V>(r, row, V * c, cs, sn, &g_tcq_memory_error);
 #pragma unroll
-    for (int i = 0; i < V; ++i) sn[i] *= sign;
-    for (int h = h0; h < heads; h += hp) {
-        float a[2 * V];
-        Vec<DT, V>::load(xr + (i64)(h * D + first) * E, a);
-        Vec<DT, V>::load(xr + (i64)(h * D + second) * E, a + V);
+        for (int i = 0; i < V; ++i) sn[i] *= sign;
+    };
+    if (HB == 1) tables();
+#pragma unroll 1
+    for (int hb = h0; hb < heads; hb += HB * hp) {
+        Rv lo[HB], hi[HB];
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            if (PAIRS) turn(a[2 * i], a[2 * i + 1], cs[i], sn[i]);
-            else turn(a[i], a[V + i], cs[i], sn[i]);
-        }
-        Vec<DT, V>::store(orow + (i64)(h * D + first) * E, a);
-        Vec<DT, V>::store(orow + (i64)(h * D + second) * E, a + V);
+        for (int k = 0; k < HB; ++k)
+            if (hb + k * hp < heads) {
+                lo[k] = *reinterpret_cast<const Rv*>(xr + (i64)((hb + k * hp) * D + first) * E);
+                hi[k] = *reinterpret_cast<const Rv*>(xr + (i64)((hb + k * hp) * D + second) * E);
+            }
+        if (HB > 1 && hb == h0) tables();
+#pragma unroll
+        for (int k = 0; k < HB; ++k)
+            if (hb + k * hp < heads) {
+                float a[2 * V];
+                Vec<DT, V>::unpack(lo[k], a);
+                Vec<DT, V>::unpack(hi[k], a + V);
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    if (PAIRS) turn(a[2 * i], a[2 * i + 1], cs[i], sn[i]);
+                    else turn(a[i], a[V + i], cs[i], sn[i]);
+                }
+                Vec<DT, V>::store(orow + (i64)((hb + k * hp) * D + first) * E, a);
+                Vec<DT, V>::store(orow + (i64)((hb + k * hp) * D + second) * E, a + V);
+            }
     }
 }
 
@@ -91,11 +110,18 @@ template <int DT, int V>
 int launch_rope(const void* x, void* out, const RopeArgs& r, i64 x_sb, i64 x_st, i64 o_sb, i64 o_st, int B, int T, int heads, bool pairs,
                 float sign, void* stream) {
     const int C = r.half / V;                      // units of a head (at most 128)
-    const int hp = heads < 256 / C ? heads : 256 / C;
+    const i64 rows = (i64)B * T;
+    // Heads side by side: all of them while the launch is short of threads (latency), a quarter of them when it has many
+    // (four heads share a thread's cosines and sines: 2 x 8191 x 32 x 128 F16 71 -> 59 us).
+    int hp = heads < 256 / C ? heads : 256 / C;
+    const bool four = heads >= 4 && rows * C * heads > (i64)tcq_sm_count() * 2048;
+    if (four && (heads + 3) / 4 < hp) hp = (heads + 3) / 4;
     const int tokens = 256 / (C * hp);             // tokens of a block
-    const i64 rows = (i64)B * T, blocks = (rows + tokens - 1) / tokens;
+    const i64 blocks = (rows + tokens - 1) / tokens;
     if (blocks > 0x7fffffff) return TCQ_ERR_SHAPE;
-    return launch_pdl(pairs ? k_rope_axes<DT, V, true> : k_rope_axes<DT, V, false>, dim3((unsigned)blocks), tokens * C * hp, 0, stream,
+    const auto kern = pairs ? (four ? k_rope_axes<DT, V, true, 4> : k_rope_axes<DT, V, true, 1>)
+                            : (four ? k_rope_axes<DT, V, false, 4> : k_rope_axes<DT, V, false, 1>);
+    return launch_pdl(kern, dim3((unsigned)blocks), tokens * C * hp, 0, stream,
                       (const char*)x, (char*)out, r, x_sb, x_st, o_sb, o_st, rows, T, heads, C, hp, sign);
 }
 
@@ -121,16 +147,18 @@ TCQ_HD u32 requant4(u32 w, float ratio) {
 // One CTA writes one head of one block of one sequence, keys (blockIdx.y 0) or values (1). The new tokens stay in
 // registers between the block's largest magnitude and their quantization, so they are read once; values are turned into
 // rows of tokens through shared memory. The block's older tokens are touched only when its scale grows. Bound by HBM.
+// Threads of an append CTA: at most 64 registers a thread, 1024 threads to an SM. A CTA passes through a chain of dependent loads
+// (start, page, tokens, positions, tables), so what counts is how many are under way.
+__host__ __device__ constexpr int append_threads(int D) { return D > 64 ? 256 : 128; }
+
 template <int DT, int D>
-__global__ void __launch_bounds__(128) k_kv8_append(tcq_kv8_cache cache, const u16* __restrict__ k, i64 k_sb, i64 k_st,
+__global__ void __launch_bounds__(append_threads(D), 1024 / append_threads(D)) k_kv8_append(tcq_kv8_cache cache, const u16* __restrict__ k, i64 k_sb, i64 k_st,
                                                     const u16* __restrict__ v, i64 v_sb, i64 v_st, const int* __restrict__ table,
                                                     int blocks, const int* __restrict__ start, const int* __restrict__ count, RopeArgs r,
                                                     int B, int T, int NB) {
-    constexpr int C = D / 16, NU = (kBlk * C + 127) / 128;      // units of 2 x 8 elements: per token, per thread
-    constexpr int VS = kBlk + 4;                                // row stride of the value tile (bytes)
-    __shared__ __align__(16) u32 tile32[D * VS / 4];
-    __shared__ float red[4];
-    i8* tile = reinterpret_cast<i8*>(tile32);
+    __shared__ __align__(16) u32 tile[D * 16];
+    constexpr int TH = append_threads(D);
+    __shared__ float red[TH / 32];
     pdl_launch_dependents();
     pdl_wait();
     const int Hk = cache.kv_heads, h = blockIdx.x % Hk, bn = blockIdx.x / Hk, n = bn % NB, b = bn / NB;
@@ -148,91 +176,142 @@ __global__ void __launch_bounds__(128) k_kv8_append(tcq_kv8_cache cache, const u
         if (threadIdx.x == 0) atomicOr(&g_tcq_memory_error, 2);
         return;
     }
-    const u16* src = (is_v ? v + b * v_sb : k + b * k_sb) + h * D;
-    const i64 row_st = is_v ? v_st : k_st;
-    float x[NU][16];
-    float amax = 0.f;
-#pragma unroll
-    for (int i = 0; i < NU; ++i) {
-        const int u = threadIdx.x + 128 * i, slot = u / C, c = u - slot * C;
-        if (slot < lo || slot >= hi) continue;
-        const int t = base + slot - st;
-        Vec<DT, 8>::load(src + t * row_st + 8 * c, x[i]);
-        Vec<DT, 8>::load(src + t * row_st + 8 * c + D / 2, x[i] + 8);
-        if (!is_v && r.cos_t) {
-            float cs[8], sn[8];
-            rope_cs<8>(r, (i64)b * T + t, 8 * c, cs, sn, &g_tcq_memory_error);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) turn(x[i][j], x[i][8 + j], cs[j], sn[j]);
-        }
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-            const float a = fabsf(x[i][j]);
-            amax = fmaxf(amax, a <= 3.402823466e38f ? a : 0.f);
-        }
-    }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = amax;
+    const i64 off = ((i64)page * Hk + h) * (kBlk * D);
     float* scale = (is_v ? cache.v_scale : cache.k_scale) + (i64)page * Hk + h;
     const float s_old = lo > 0 ? *scale : 0.f;
-    __syncthreads();
-    amax = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-    float s = fmaxf(s_old, amax / 127.f);
-    if (s < 7.52316385e-37f) s = 0.f;                         // 2^-120
-    const float inv = s > 0.f ? 1.f / s : 0.f, ratio = s_old * inv;
-    const bool grown = lo > 0 && s > s_old;
-    if (threadIdx.x == 0) *scale = s;
-    const i64 off = ((i64)page * Hk + h) * (kBlk * D);
+    float s, inv, ratio;
+    bool grown;
+    // the block's scale from this thread's largest magnitude
+    auto settle = [&](float amax) {
+#pragma unroll
+        for (int o = 16; o; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+        if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = amax;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < TH / 32; ++w) amax = fmaxf(amax, red[w]);
+        s = fmaxf(s_old, amax / 127.f);
+        if (s < 7.52316385e-37f) s = 0.f;                         // 2^-120
+        inv = s > 0.f ? 1.f / s : 0.f, ratio = s_old * inv;
+        grown = lo > 0 && s > s_old;
+        if (threadIdx.x == 0) *scale = s;
+    };
+    auto largest = [](float m, float x) {
+        const float a = fabsf(x);
+        return fmaxf(m, a <= 3.402823466e38f ? a : 0.f);
+    };
+    float amax = 0.f;
     if (!is_v) {
+        // units of 8 elements and their 8 partners of a turn: C per token, all of a thread's requested at once
+        constexpr int C = D / 16, NU = (kBlk * C + TH - 1) / TH;
+        const u16* src = k + b * k_sb + h * D;
+        uint4 raw[NU][2];
+#pragma unroll
+        for (int i = 0; i < NU; ++i) {
+            const int u = threadIdx.x + TH * i, slot = u / C, c = u - slot * C;
+            raw[i][0] = raw[i][1] = make_uint4(0, 0, 0, 0);
+            if (slot >= lo && slot < hi) {
+                const u16* p = src + (i64)(base + slot - st) * k_st + 8 * c;
+                raw[i][0] = *reinterpret_cast<const uint4*>(p), raw[i][1] = *reinterpret_cast<const uint4*>(p + D / 2);
+            }
+        }
+        float x[NU][16];
+#pragma unroll
+        for (int i = 0; i < NU; ++i) {
+            const int u = threadIdx.x + TH * i, slot = u / C, c = u - slot * C;
+            Vec<DT, 8>::unpack(raw[i][0], x[i]);
+            Vec<DT, 8>::unpack(raw[i][1], x[i] + 8);
+            if (r.cos_t && slot >= lo && slot < hi) {
+                float cs[8], sn[8];
+                rope_cs<8>(r, (i64)b * T + base + slot - st, 8 * c, cs, sn, &g_tcq_memory_error);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) turn(x[i][j], x[i][8 + j], cs[j], sn[j]);
+            }
+#pragma unroll
+            for (int j = 0; j < 16; ++j) amax = largest(amax, x[i][j]);
+        }
+        settle(amax);
         i8* dst = cache.k + off;
 #pragma unroll
         for (int i = 0; i < NU; ++i) {
-            const int u = threadIdx.x + 128 * i, slot = u / C, c = u - slot * C;
+            const int u = threadIdx.x + TH * i, slot = u / C, c = u - slot * C;
             if (slot < lo || slot >= hi) continue;
             uint2* p = reinterpret_cast<uint2*>(dst + slot * D + 8 * c);
             p[0] = make_uint2(q8x4(x[i], inv), q8x4(x[i] + 4, inv));
             p[D / 16] = make_uint2(q8x4(x[i] + 8, inv), q8x4(x[i] + 12, inv));
         }
         if (grown)
-            for (int i = threadIdx.x; i < lo * (D / 4); i += 128) {
+            for (int i = threadIdx.x; i < lo * (D / 4); i += TH) {
                 u32* p = reinterpret_cast<u32*>(dst) + i;
                 *p = requant4(*p, ratio);
             }
         return;
     }
+    // values: units of 4 tokens x 8 elements, so that four tokens of an element are one word of its row. The words meet in
+    // shared memory, word g of row d at g ^ (d / 8 mod 16): a warp's stores spread over the banks, and a 16-byte piece of a row
+    // keeps its four words, permuted.
+    constexpr int C = D / 8, NU = (16 * C + TH - 1) / TH;
+    const u16* src = v + b * v_sb + h * D;
+    uint4 raw[NU][4];
 #pragma unroll
     for (int i = 0; i < NU; ++i) {
-        const int u = threadIdx.x + 128 * i, slot = u / C, c = u - slot * C;
-        if (slot < lo || slot >= hi) continue;
+        const int u = threadIdx.x + TH * i, g = u / C, c = u - g * C;
 #pragma unroll
-        for (int j = 0; j < 16; ++j) tile[((j < 8 ? 8 * c : 8 * c + D / 2 - 8) + j) * VS + slot] = (i8)q8(x[i][j], inv);
+        for (int e = 0; e < 4; ++e) {
+            const int slot = 4 * g + e;
+            raw[i][e] = slot >= lo && slot < hi ? *reinterpret_cast<const uint4*>(src + (i64)(base + slot - st) * v_st + 8 * c) : make_uint4(0, 0, 0, 0);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < NU; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            float x[8];
+            Vec<DT, 8>::unpack(raw[i][e], x);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) amax = largest(amax, x[j]);
+        }
+    settle(amax);
+#pragma unroll
+    for (int i = 0; i < NU; ++i) {
+        const int u = threadIdx.x + TH * i, g = u / C, c = u - g * C;
+        if (16 * C % TH != 0 && u >= 16 * C) break;
+        float x[4][8];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) Vec<DT, 8>::unpack(raw[i][e], x[e]);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float y[4] = {x[0][j], x[1][j], x[2][j], x[3][j]};
+            tile[(8 * c + j) * 16 + (g ^ (c & 15))] = q8x4(y, inv);
+        }
     }
     __syncthreads();
     i8* dst = cache.v + off;
-    for (int i = threadIdx.x; i < D * 4; i += 128) {          // 16-token pieces of the rows
-        const int d = i >> 2, t0 = (i & 3) * 16;
+#pragma unroll
+    for (int i = threadIdx.x; i < D * 4; i += TH) {          // 16-token pieces of the rows
+        const int d = i >> 2, t0 = (i & 3) * 16, c = (d >> 3) & 15;
         const bool any_new = t0 < hi && t0 + 16 > lo, any_old = grown && t0 < lo;
         if (!any_new && !any_old) continue;
-        u32 w[4];
+        const uint4 f = reinterpret_cast<const uint4*>(tile)[d * 4 + ((i & 3) ^ (c >> 2))];
+        const bool x1 = c & 1, x2 = c & 2;
+        const u32 a0 = x1 ? f.y : f.x, a1 = x1 ? f.x : f.y, a2 = x1 ? f.w : f.z, a3 = x1 ? f.z : f.w;
+        const u32 fresh[4] = {x2 ? a2 : a0, x2 ? a3 : a1, x2 ? a0 : a2, x2 ? a1 : a3};
         uint4* p = reinterpret_cast<uint4*>(dst + d * kBlk + t0);
-        if (t0 < lo || t0 + 16 > hi) {
-            const uint4 o = *p;
-            w[0] = o.x, w[1] = o.y, w[2] = o.z, w[3] = o.w;
+        if (t0 >= lo && t0 + 16 <= hi) {
+            *p = make_uint4(fresh[0], fresh[1], fresh[2], fresh[3]);
+            continue;
         }
+        const uint4 o = *p;
+        u32 w[4] = {o.x, o.y, o.z, o.w};
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const int t = t0 + 4 * j;
-            const u32 fresh = tile32[(d * VS + t) >> 2];
-            if (any_old) {
-                const u32 q = requant4(w[j], ratio);
+            const u32 q = any_old ? requant4(w[j], ratio) : 0u;
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (t + e < lo) w[j] = (w[j] & ~(255u << (8 * e))) | (q & (255u << (8 * e)));
+            for (int e = 0; e < 4; ++e) {
+                const u32 m = 255u << (8 * e);
+                if (any_old && t + e < lo) w[j] = (w[j] & ~m) | (q & m);
+                if (t + e >= lo && t + e < hi) w[j] = (w[j] & ~m) | (fresh[j] & m);
             }
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (t + e >= lo && t + e < hi) w[j] = (w[j] & ~(255u << (8 * e))) | (fresh & (255u << (8 * e)));
         }
         *p = make_uint4(w[0], w[1], w[2], w[3]);
     }
@@ -245,8 +324,8 @@ template <int DT, int D>
 __global__ void __launch_bounds__(128) k_kv8_read(tcq_kv8_cache cache, char* __restrict__ ko, char* __restrict__ vo,
                                                   const int* __restrict__ table, int blocks, const int* __restrict__ begin,
                                                   const int* __restrict__ lens, int T, int NB) {
-    constexpr int C = D / 8, E = DT == TCQ_DT_F32 ? 4 : 2, VS = kBlk + 4;
-    __shared__ __align__(16) u32 tile32[D * VS / 4];
+    constexpr int E = DT == TCQ_DT_F32 ? 4 : 2;
+    __shared__ __align__(16) u32 tile[D * 16];
     pdl_launch_dependents();
     pdl_wait();
     const int Hk = cache.kv_heads, h = blockIdx.x % Hk, bn = blockIdx.x / Hk, n = bn % NB, b = bn / NB;
@@ -270,38 +349,72 @@ __global__ void __launch_bounds__(128) k_kv8_read(tcq_kv8_cache cache, char* __r
     }
     const i64 off = ((i64)page * Hk + h) * (kBlk * D);
     const float s = end > lo ? (is_v ? cache.v_scale : cache.k_scale)[(i64)page * Hk + h] : 0.f;
-    if (is_v && end > lo) {
-        const uint4* src = reinterpret_cast<const uint4*>(cache.v + off);
-        for (int i = threadIdx.x; i < D * 4; i += 128) {
-            const uint4 q = src[i];
-            u32* p = tile32 + ((i >> 2) * VS + (i & 3) * 16) / 4;
-            p[0] = q.x, p[1] = q.y, p[2] = q.z, p[3] = q.w;
-        }
-    }
-    __syncthreads();
     char* out = (is_v ? vo : ko) + (((i64)b * T + base - from) * Hk + h) * D * E;
-    const i8* tile = reinterpret_cast<const i8*>(tile32);
-    for (int u = threadIdx.x; u < kBlk * C; u += 128) {
-        const int slot = u / C, c = u - slot * C;
-        if (slot < lo || slot >= hi) continue;
-        float y[8];
-        if (slot >= end) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) y[j] = 0.f;
-        } else if (is_v) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) y[j] = (float)(int)tile[(8 * c + j) * VS + slot] * s;
-        } else {
-            const uint2 q = *reinterpret_cast<const uint2*>(cache.k + off + slot * D + 8 * c);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) y[j] = (float)(int)(i8)((j < 4 ? q.x : q.y) >> (8 * (j & 3))) * s;
-        }
-        char* o = out + ((i64)slot * Hk * D + 8 * c) * E;
+    const i64 row = (i64)Hk * D * E;
+    auto put = [&](int slot, int d, const float* y) {             // 8 elements of a token's row
+        char* o = out + slot * row + d * E;
         if (DT == TCQ_DT_F32) {
             Vec<DT, 4>::store(o, y);
             Vec<DT, 4>::store(o + 16, y + 4);
         } else {
             Vec<DT, DT == TCQ_DT_F32 ? 4 : 8>::store(o, y);
+        }
+    };
+    if (!is_v) {
+        constexpr int C = D / 8, NU = (kBlk * C + 127) / 128;
+        uint2 q[NU];
+#pragma unroll
+        for (int i = 0; i < NU; ++i) {
+            const int u = threadIdx.x + 128 * i, slot = u / C, c = u - slot * C;
+            q[i] = slot >= lo && slot < end ? *reinterpret_cast<const uint2*>(cache.k + off + slot * D + 8 * c) : make_uint2(0u, 0u);
+        }
+#pragma unroll
+        for (int i = 0; i < NU; ++i) {
+            const int u = threadIdx.x + 128 * i, slot = u / C, c = u - slot * C;
+            if (slot < lo || slot >= hi) continue;
+            float y[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) y[j] = (float)(int)(i8)((j < 4 ? q[i].x : q[i].y) >> (8 * (j & 3))) * s;
+            put(slot, 8 * c, y);
+        }
+        return;
+    }
+    // values: the rows of tokens through shared memory (words as in the append), then 4 tokens x 8 elements a thread
+    constexpr int C = D / 8, NP = D * 4 / 128, NU = (16 * C + 127) / 128;
+    if (end > lo) {
+        const uint4* src = reinterpret_cast<const uint4*>(cache.v + off);
+        uint4 q[NP + 1];
+#pragma unroll
+        for (int i = 0; i < NP + 1; ++i) {
+            const int u = threadIdx.x + 128 * i;
+            if (u < D * 4) q[i] = src[u];
+        }
+#pragma unroll
+        for (int i = 0; i < NP + 1; ++i) {
+            const int u = threadIdx.x + 128 * i, d = u >> 2, c = (d >> 3) & 15;
+            if (u >= D * 4) break;
+            const bool x1 = c & 1, x2 = c & 2;
+            const u32 a0 = x1 ? q[i].y : q[i].x, a1 = x1 ? q[i].x : q[i].y, a2 = x1 ? q[i].w : q[i].z, a3 = x1 ? q[i].z : q[i].w;
+            reinterpret_cast<uint4*>(tile)[d * 4 + ((u & 3) ^ (c >> 2))] = x2 ? make_uint4(a2, a3, a0, a1) : make_uint4(a0, a1, a2, a3);
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < NU; ++i) {
+        const int u = threadIdx.x + 128 * i, g = u / C, c = u - g * C;
+        if (16 * C % 128 != 0 && u >= 16 * C) break;
+        if (4 * g >= hi || 4 * g + 4 <= lo) continue;
+        u32 w[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) w[j] = tile[(8 * c + j) * 16 + (g ^ (c & 15))];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int slot = 4 * g + e;
+            if (slot < lo || slot >= hi) continue;
+            float y[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) y[j] = slot < end ? (float)(int)(i8)(w[j] >> (8 * e)) * s : 0.f;
+            put(slot, 8 * c, y);
         }
     }
 }
@@ -355,7 +468,7 @@ int tcq_kv8_append(const tcq_kv8_cache* cache, const void* k, int64_t k_sb, int6
     if (ctas > 0x7fffffff) return TCQ_ERR_SHAPE;
     return by_head_dim(cache->head_dim, [&](auto d) {
         constexpr int D = decltype(d)::value;
-        return launch_pdl(dtype == TCQ_DT_BF16 ? k_kv8_append<TCQ_DT_BF16, D> : k_kv8_append<TCQ_DT_F16, D>, dim3((unsigned)ctas, 2), 128, 0,
+        return launch_pdl(dtype == TCQ_DT_BF16 ? k_kv8_append<TCQ_DT_BF16, D> : k_kv8_append<TCQ_DT_F16, D>, dim3((unsigned)ctas, 2), append_threads(D), 0,
                           stream, *cache, (const u16*)k, (i64)k_sb, (i64)k_st, (const u16*)v, (i64)v_sb, (i64)v_st, table, blocks, start,
                           count, r, B, T, NB);
     });

@@ -139,13 +139,7 @@ struct AttnArgs {
 template <int D, int NT>
 struct Few {
     static constexpr int HALF = kBlk * D;
-#ifndef FW
-#define FW 12
-#endif
-#ifndef FNB
-#define FNB 4
-#endif
-    static constexpr int WARPS = NT == 1 ? (D <= 64 ? FW : D < 128 ? 12 : 8) : NT == 2 && D <= 64 ? 12 : 8;
+    static constexpr int WARPS = NT == 1 ? (D < 128 ? 12 : 8) : NT == 2 && D <= 64 ? 12 : 8;
     static constexpr int FIT = 216 * 1024 / (WARPS * HALF), NH = FIT < 8 ? FIT : 8;
     static_assert(NH >= 3, "a half page in use and two on their way");
     static constexpr int HDR = WARPS * NH * HALF;                          // ks, vs of each half page
@@ -168,7 +162,7 @@ struct Place {
 // loads in flight want registers of their own.
 template <int DT, int D>
 __device__ __noinline__ void add_parts(const float* parts, i64 size, int first, int last, int R, int group, u16* out, i64 token) {
-    constexpr int NI = 4, NB = FNB;                 // pairs of elements of a lane, parts requested at once
+    constexpr int NI = 4, NB = 4;                  // pairs of elements of a lane, parts requested at once
     const int lane = threadIdx.x & 31;
 #pragma unroll 1
     for (int i0 = 0; i0 < R * (D / 2); i0 += 32 * NI) {
@@ -671,10 +665,7 @@ struct Many {
     static constexpr int SWAP0 = BAR0 + 256;                          // a float of every softmax thread
     static constexpr int BYTES = SWAP0 + SOFT * 4;
     static constexpr int ML0 = STAGE0;                                // m, l of every row, over the stage (cluster sums)
-#ifndef POLYN
-#define POLYN 2
-#endif
-    static constexpr int POLY = POLYN;                      // of 16 pairs of weights, those formed by polynomial
+    static constexpr int POLY = 2;                      // of 16 pairs of weights, those formed by polynomial
     static constexpr u32 COLS = NG == 2 ? 512 : 256;
     static constexpr int S0 = 0, O0 = NG * kTile;                     // TMEM columns: scores, outputs
     static constexpr int PARTS = NG * kTile * D * 4;                  // a CTA's part of the outputs, over the tiles
