@@ -264,10 +264,16 @@ class LlmBlock(torch.nn.Module):
         self.mlp.down_proj = LinearSlot(c.llm_ffn, d)
         self.mlp.forward = lambda x: self.mlp.down_proj(F.silu(self.mlp.gate_proj(x)) * self.mlp.up_proj(x))
 
-    def forward(self, x, delta, rope):
+    def forward(self, x, delta, rope, memory=None, layer=0):
+        """rope: cos / sin tables of positions 0..T-1; with a memory (stream.StreamMemory) its own positions count instead, and
+        the attention reads the layer's cache of past frames and this one."""
         x, h = self.input_layernorm(x, delta)
         a = self.self_attn
         q, k, v = a.q_proj(h), a.k_proj(h), a.v_proj(h)
+        if memory is not None:
+            o = memory.attend(layer, q, k, v)
+            x, h = self.post_attention_layernorm(x, a.o_proj(o))
+            return x, self.mlp(h)
         cos, sin = rope
         if getattr(self, 'torch_ops', False):
             q, k = definition.rope(q, cos, sin, self.heads), definition.rope(k, cos, sin, self.kv_heads)
@@ -357,10 +363,17 @@ class GrootStylePolicy(torch.nn.Module):
         img = img.view(B, c.cameras * c.image_tokens, -1)
         return torch.cat((img, self.embed_tokens(lang_ids)), 1)
 
-    def backbone(self, prefix):
+    def backbone(self, prefix, memory=None):
+        """prefix (B, T, 2048) -> features of the same shape. memory: a stream.StreamMemory, to which the prefix is added as the
+        next frame and all of which its tokens attend to."""
         c = self.c
-        rope = rope_tables(prefix.shape[1], c.llm_hidden // c.llm_heads, prefix.device)
         x, d = prefix, None
+        if memory is not None:
+            memory.begin_frame()
+            for i, blk in enumerate(self.llm):
+                x, d = blk(x, d, None, memory, i)
+            return self.llm_norm(x, d)[1]
+        rope = rope_tables(prefix.shape[1], c.llm_hidden // c.llm_heads, prefix.device)
         for blk in self.llm:
             x, d = blk(x, d, rope)
         return self.llm_norm(x, d)[1]
@@ -391,8 +404,8 @@ class GrootStylePolicy(torch.nn.Module):
             a = a + dt * v.float()
         return a
 
-    def forward(self, images, lang_ids, state, noise):
-        return self.action_head(self.backbone(self.embed(images, lang_ids)), state, noise)
+    def forward(self, images, lang_ids, state, noise, memory=None):
+        return self.action_head(self.backbone(self.embed(images, lang_ids), memory), state, noise)
 
 
 # ---------------------------------------------------------------------------------------------------- weights

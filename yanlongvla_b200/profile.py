@@ -25,6 +25,7 @@ _FRAGMENTS = (
     ('MLP middles', ('k_mid',)),
     ('residual add + norm', ('k_addnorm', 'k_add_norm')),
     ('rotary embedding', ('k_rope',)),
+    ('8-bit cache', ('k_kv8', 'k_attention')),
     ('attention', ('flash', 'fmha', 'attention', 'softmax', 'sdpa', 'cudnn')),
     ('BF16 matrix product (cuBLAS)', ('gemm', 'Gemm', 'gemv', 'Gemv', 'cublas', 'nvjet', 'cutlass', 'matmul')),
     ('NCCL', ('nccl', 'Nccl')),
