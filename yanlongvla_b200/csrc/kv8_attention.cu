@@ -665,7 +665,6 @@ struct Many {
     static constexpr int SWAP0 = BAR0 + 256;                          // a float of every softmax thread
     static constexpr int BYTES = SWAP0 + SOFT * 4;
     static constexpr int ML0 = STAGE0;                                // m, l of every row, over the stage (cluster sums)
-    static constexpr int POLY = 2;                      // of 16 pairs of weights, those formed by polynomial
     static constexpr u32 COLS = NG == 2 ? 512 : 256;
     static constexpr int S0 = 0, O0 = NG * kTile;                     // TMEM columns: scores, outputs
     static constexpr int PARTS = NG * kTile * D * 4;                  // a CTA's part of the outputs, over the tiles
@@ -756,24 +755,6 @@ TCQ_HD u64 add2(u64 a, u64 b) {
     return r;
 }
 
-// 2^x for a pair, x <= 126, values below 2^-126 as 2^-126 (zero once rounded to FP16), without the exponential unit, which
-// forms 16 results per clock and SM and is the kernel's narrowest pipe: x = n + f with |f| <= 1/2 (n by adding and
-// subtracting 1.5 * 2^23), a cubic fitted to 2^f for the least relative error (7.5e-5, against 4.9e-4 of the weight's
-// rounding to FP16), n added to its exponent.
-TCQ_HD u64 ex2_poly(u64 x) {
-    float lo, hi;
-    unpair(x, lo, hi);
-    x = pair(fmaxf(lo, -126.f), fmaxf(hi, -126.f));
-    const u64 t = add2(x, pair(12582912.f, 12582912.f)), n = add2(t, pair(-12582912.f, -12582912.f));
-    const u64 f = fma2(n, pair(-1.f, -1.f), x);
-    u64 p = fma2(f, pair(0.0551716685f, 0.0551716685f), pair(0.2426111251f, 0.2426111251f));
-    p = fma2(p, f, pair(0.6932609677f, 0.6932609677f));
-    p = fma2(p, f, pair(0.9999280572f, 0.9999280572f));
-    float tl, th;
-    unpair(t, tl, th);
-    unpair(p, lo, hi);
-    return pair(__uint_as_float(__float_as_uint(lo) + (__float_as_uint(tl) << 23)), __uint_as_float(__float_as_uint(hi) + (__float_as_uint(th) << 23)));
-}
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void async_proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
@@ -1011,21 +992,15 @@ k_attention_many(const AttnArgs A, int row_tiles, int tile_rows, int splits) {
                 u32 w[16];
 #pragma unroll
                 for (int j = 0; j < 16; ++j) {
-                    u64 y = fma2(pair(__uint_as_float(x[2 * j]), __uint_as_float(x[2 * j + 1])), c2, a2);
+                    const u64 y = fma2(pair(__uint_as_float(x[2 * j]), __uint_as_float(x[2 * j + 1])), c2, a2);
                     float lo, hi;
-                    if (!MASKED && (j * P::POLY) % 16 < P::POLY) {
-                        y = ex2_poly(y);
-                        unpair(y, lo, hi);
-                    } else {
-                        unpair(y, lo, hi);
-                        if (MASKED) {
-                            lo = 32 * hf + 2 * j < lim ? lo : -INFINITY;
-                            hi = 32 * hf + 2 * j + 1 < lim ? hi : -INFINITY;
-                        }
-                        lo = ex2(lo), hi = ex2(hi);
-                        y = pair(lo, hi);
+                    unpair(y, lo, hi);
+                    if (MASKED) {
+                        lo = 32 * hf + 2 * j < lim ? lo : -INFINITY;
+                        hi = 32 * hf + 2 * j + 1 < lim ? hi : -INFINITY;
                     }
-                    sum[j & 1] = add2(sum[j & 1], y);
+                    lo = ex2(lo), hi = ex2(hi);
+                    sum[j & 1] = add2(sum[j & 1], pair(lo, hi));
                     w[j] = half2_of(lo, hi);
                 }
                 tmem_st16(ts + 32 * p + 16 * hf, w);

@@ -63,19 +63,26 @@ __device__ __forceinline__ bool mbar_wait_bounded(u32 bar, u32 parity, volatile 
     }
 }
 
-// The same with the thread suspended by the hardware between its looks at the barrier (up to 100 us each), for waits of
-// microseconds next to warps that compute.
+// The same for waits of microseconds next to warps that compute: up to 256 looks at the barrier, the thread suspended by the
+// hardware in each, before the abort flag and the timer are looked at (a look costs two to four instructions, which the
+// other warps of the scheduler would otherwise issue).
 __device__ __forceinline__ bool mbar_wait_suspended(u32 bar, u32 parity, volatile int* abort_flag, int* err,
                                                     unsigned long long limit = kWaitNs) {
     unsigned long long t0 = 0;
     for (;;) {
         u32 ok;
         asm volatile(
-            "{\n\t.reg .pred p;\n\t"
+            "{\n\t.reg .pred p, q;\n\t.reg .u32 n;\n\tmov.u32 n, 0;\n"
+            "LOOK:\n\t"
             "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+            "@p bra SEEN;\n\t"
+            "add.u32 n, n, 1;\n\t"
+            "setp.lt.u32 q, n, 256;\n\t"
+            "@q bra LOOK;\n"
+            "SEEN:\n\t"
             "selp.u32 %0, 1, 0, p;\n\t}"
             : "=r"(ok)
-            : "r"(bar), "r"(parity), "r"(100000u)
+            : "r"(bar), "r"(parity), "r"(20000u)
             : "memory");
         if (ok) return true;
         if (*abort_flag) return false;
