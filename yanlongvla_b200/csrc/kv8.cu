@@ -57,7 +57,7 @@ struct Vec {
 };
 
 template <int DT, int V, bool PAIRS, int HB>
-__global__ void __launch_bounds__(256) k_rope_axes(const char* __restrict__ x, char* __restrict__ out, RopeArgs r, i64 x_sb, i64 x_st,
+__global__ void __launch_bounds__(256, 3) k_rope_axes(const char* __restrict__ x, char* __restrict__ out, RopeArgs r, i64 x_sb, i64 x_st,
                                                    i64 o_sb, i64 o_st, i64 rows, int T, int heads, int C, int hp, float sign) {
     constexpr int E = DT == TCQ_DT_F32 ? 4 : 2;
     pdl_launch_dependents();
@@ -115,7 +115,7 @@ int launch_rope(const void* x, void* out, const RopeArgs& r, i64 x_sb, i64 x_st,
     // (four heads share a thread's cosines and sines: 2 x 8191 x 32 x 128 F16 71 -> 59 us).
     int hp = heads < 256 / C ? heads : 256 / C;
     const bool four = heads >= 4 && rows * C * heads > (i64)tcq_sm_count() * 2048;
-    if (four && (heads + 3) / 4 < hp) hp = (heads + 3) / 4;
+    if (four && (heads + 4 - 1) / 4 < hp) hp = (heads + 4 - 1) / 4;
     const int tokens = 256 / (C * hp);             // tokens of a block
     const i64 blocks = (rows + tokens - 1) / tokens;
     if (blocks > 0x7fffffff) return TCQ_ERR_SHAPE;
@@ -126,17 +126,23 @@ int launch_rope(const void* x, void* out, const RopeArgs& r, i64 x_sb, i64 x_st,
 }
 
 // ------------------------------------------------------------------------------------------------ cache append
-TCQ_HD int q8(float x, float inv) {
-    float v = x * inv;
-    v = v == v ? v : 0.f;
-    return __float2int_rn(fminf(fmaxf(v, -127.f), 127.f));
-}
+// Four quotients x * inv, |x * inv| < 127.5, rounded to nearest even and packed: 1.5 * 2^23 added leaves the integer in a
+// float's low bits.
 TCQ_HD u32 q8x4(const float* x, float inv) {
-    u32 w = 0;
+    u32 b[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) w |= (u32)(q8(x[i], inv) & 255) << (8 * i);
-    return w;
+    for (int i = 0; i < 4; ++i) b[i] = __float_as_uint(x[i] * inv + 12582912.f);
+    return __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
 }
+// The rare block with infinities or NaN: infinities become the block's largest value, NaN zero.
+TCQ_HD float tamed(float x, float s) { return x == x ? fminf(fmaxf(x, -127.f * s), 127.f * s) : 0.f; }
+
+// Largest magnitudes of 16-bit elements, two at a time: without their signs they order as unsigned integers, NaN above all.
+TCQ_HD u32 max2(u32 m, u32 w) { return __vmaxu2(m, w & 0x7fff7fffu); }
+TCQ_HD u32 max2(u32 m, const uint4& w) { return max2(max2(max2(max2(m, w.x), w.y), w.z), w.w); }
+template <int DT>
+TCQ_HD u32 max2_bits(u32 m) { return __float_as_uint(elem_f<DT>((u16)max(m & 0xffffu, m >> 16))); }
+
 TCQ_HD u32 requant4(u32 w, float ratio) {
     u32 o = 0;
 #pragma unroll
@@ -146,19 +152,17 @@ TCQ_HD u32 requant4(u32 w, float ratio) {
 
 // One CTA writes one head of one block of one sequence, keys (blockIdx.y 0) or values (1). The new tokens stay in
 // registers between the block's largest magnitude and their quantization, so they are read once; values are turned into
-// rows of tokens through shared memory. The block's older tokens are touched only when its scale grows. Bound by HBM.
-// Threads of an append CTA: at most 64 registers a thread, 1024 threads to an SM. A CTA passes through a chain of dependent loads
-// (start, page, tokens, positions, tables), so what counts is how many are under way.
-__host__ __device__ constexpr int append_threads(int D) { return D > 64 ? 256 : 128; }
-
+// rows of tokens through shared memory. The block's older tokens are touched only when its scale grows. A CTA passes through a
+// chain of dependent loads (start, tokens and page, positions, tables), so what counts is how many are under way: six CTAs of
+// 128 threads to an SM (4 x 8192 tokens of 8 heads of 128, F16 with rotary: 67 us, 3.0 TB/s; four of them 97 us, four of 256 threads 70 us).
 template <int DT, int D>
-__global__ void __launch_bounds__(append_threads(D), 1024 / append_threads(D)) k_kv8_append(tcq_kv8_cache cache, const u16* __restrict__ k, i64 k_sb, i64 k_st,
+__global__ void __launch_bounds__(128, 6) k_kv8_append(tcq_kv8_cache cache, const u16* __restrict__ k, i64 k_sb, i64 k_st,
                                                     const u16* __restrict__ v, i64 v_sb, i64 v_st, const int* __restrict__ table,
                                                     int blocks, const int* __restrict__ start, const int* __restrict__ count, RopeArgs r,
                                                     int B, int T, int NB) {
     __shared__ __align__(16) u32 tile[D * 16];
-    constexpr int TH = append_threads(D);
-    __shared__ float red[TH / 32];
+    constexpr int TH = 128;
+    __shared__ u32 red[TH / 32];
     pdl_launch_dependents();
     pdl_wait();
     const int Hk = cache.kv_heads, h = blockIdx.x % Hk, bn = blockIdx.x / Hk, n = bn % NB, b = bn / NB;
@@ -171,25 +175,38 @@ __global__ void __launch_bounds__(append_threads(D), 1024 / append_threads(D)) k
     const int blk = st / kBlk + n, base = blk * kBlk;
     const int lo = max(st - base, 0), hi = min(st + cnt - base, kBlk);       // new slots of the block
     if (lo >= hi) return;
-    int page = blk < blocks ? table[(i64)b * blocks + blk] : -1;
-    if ((unsigned)page >= (unsigned)cache.pages) {
-        if (threadIdx.x == 0) atomicOr(&g_tcq_memory_error, 2);
-        return;
-    }
-    const i64 off = ((i64)page * Hk + h) * (kBlk * D);
-    float* scale = (is_v ? cache.v_scale : cache.k_scale) + (i64)page * Hk + h;
-    const float s_old = lo > 0 ? *scale : 0.f;
+    const int page = blk < blocks ? table[(i64)b * blocks + blk] : -1;       // looked at once the tokens are on their way
+    i64 off = 0;
+    float* scale = nullptr;
+    float s_old = 0.f;
+    auto open_page = [&]() -> bool {
+        if ((unsigned)page >= (unsigned)cache.pages) {
+            if (threadIdx.x == 0) atomicOr(&g_tcq_memory_error, 2);
+            return false;
+        }
+        off = ((i64)page * Hk + h) * (kBlk * D);
+        scale = (is_v ? cache.v_scale : cache.k_scale) + (i64)page * Hk + h;
+        if (lo > 0) s_old = *scale;
+        return true;
+    };
     float s, inv, ratio;
     bool grown;
-    // the block's scale from this thread's largest magnitude
-    auto settle = [&](float amax) {
+    bool odd = false;
+    // the block's scale from this thread's largest magnitude (as FP32 bits); finite() is that of its finite values, asked for
+    // when the block holds others
+    auto settle = [&](u32 top, auto finite) {
+        for (;;) {
+            top = __reduce_max_sync(0xffffffffu, top);
+            if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = top;
+            __syncthreads();
 #pragma unroll
-        for (int o = 16; o; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-        if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = amax;
-        __syncthreads();
-#pragma unroll
-        for (int w = 0; w < TH / 32; ++w) amax = fmaxf(amax, red[w]);
-        s = fmaxf(s_old, amax / 127.f);
+            for (int w = 0; w < TH / 32; ++w) top = max(top, red[w]);
+            if (top < 0x7f800000u) break;
+            odd = true;
+            top = __float_as_uint(finite());
+            __syncthreads();
+        }
+        s = fmaxf(s_old, __uint_as_float(top) / 127.f);
         if (s < 7.52316385e-37f) s = 0.f;                         // 2^-120
         inv = s > 0.f ? 1.f / s : 0.f, ratio = s_old * inv;
         grown = lo > 0 && s > s_old;
@@ -199,7 +216,6 @@ __global__ void __launch_bounds__(append_threads(D), 1024 / append_threads(D)) k
         const float a = fabsf(x);
         return fmaxf(m, a <= 3.402823466e38f ? a : 0.f);
     };
-    float amax = 0.f;
     if (!is_v) {
         // units of 8 elements and their 8 partners of a turn: C per token, all of a thread's requested at once
         constexpr int C = D / 16, NU = (kBlk * C + TH - 1) / TH;
@@ -214,6 +230,8 @@ __global__ void __launch_bounds__(append_threads(D), 1024 / append_threads(D)) k
                 raw[i][0] = *reinterpret_cast<const uint4*>(p), raw[i][1] = *reinterpret_cast<const uint4*>(p + D / 2);
             }
         }
+        if (!open_page()) return;
+        u32 top = 0;
         float x[NU][16];
 #pragma unroll
         for (int i = 0; i < NU; ++i) {
@@ -226,10 +244,27 @@ __global__ void __launch_bounds__(append_threads(D), 1024 / append_threads(D)) k
 #pragma unroll
                 for (int j = 0; j < 8; ++j) turn(x[i][j], x[i][8 + j], cs[j], sn[j]);
             }
+            if (r.cos_t) {
 #pragma unroll
-            for (int j = 0; j < 16; ++j) amax = largest(amax, x[i][j]);
+                for (int j = 0; j < 16; ++j) top = max(top, __float_as_uint(x[i][j]) & 0x7fffffffu);
+            } else {
+                top = max(top, max2_bits<DT>(max2(max2(0u, raw[i][0]), raw[i][1])));
+            }
         }
-        settle(amax);
+        settle(top, [&] {
+            float m = 0.f;
+#pragma unroll
+            for (int i = 0; i < NU; ++i)
+#pragma unroll
+                for (int j = 0; j < 16; ++j) m = largest(m, x[i][j]);
+            return m;
+        });
+        if (odd) {
+#pragma unroll
+            for (int i = 0; i < NU; ++i)
+#pragma unroll
+                for (int j = 0; j < 16; ++j) x[i][j] = tamed(x[i][j], s);
+        }
         i8* dst = cache.k + off;
 #pragma unroll
         for (int i = 0; i < NU; ++i) {
@@ -261,16 +296,25 @@ __global__ void __launch_bounds__(append_threads(D), 1024 / append_threads(D)) k
             raw[i][e] = slot >= lo && slot < hi ? *reinterpret_cast<const uint4*>(src + (i64)(base + slot - st) * v_st + 8 * c) : make_uint4(0, 0, 0, 0);
         }
     }
+    if (!open_page()) return;
+    u32 top = 0;
 #pragma unroll
     for (int i = 0; i < NU; ++i)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            float x[8];
-            Vec<DT, 8>::unpack(raw[i][e], x);
+        for (int e = 0; e < 4; ++e) top = max2(top, raw[i][e]);
+    settle(max2_bits<DT>(top), [&] {
+        float m = 0.f;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) amax = largest(amax, x[j]);
-        }
-    settle(amax);
+        for (int i = 0; i < NU; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                float x[8];
+                Vec<DT, 8>::unpack(raw[i][e], x);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) m = largest(m, x[j]);
+            }
+        return m;
+    });
 #pragma unroll
     for (int i = 0; i < NU; ++i) {
         const int u = threadIdx.x + TH * i, g = u / C, c = u - g * C;
@@ -278,6 +322,10 @@ __global__ void __launch_bounds__(append_threads(D), 1024 / append_threads(D)) k
         float x[4][8];
 #pragma unroll
         for (int e = 0; e < 4; ++e) Vec<DT, 8>::unpack(raw[i][e], x[e]);
+        if (odd) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) x[j >> 3][j & 7] = tamed(x[j >> 3][j & 7], s);
+        }
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             const float y[4] = {x[0][j], x[1][j], x[2][j], x[3][j]};
@@ -468,7 +516,7 @@ int tcq_kv8_append(const tcq_kv8_cache* cache, const void* k, int64_t k_sb, int6
     if (ctas > 0x7fffffff) return TCQ_ERR_SHAPE;
     return by_head_dim(cache->head_dim, [&](auto d) {
         constexpr int D = decltype(d)::value;
-        return launch_pdl(dtype == TCQ_DT_BF16 ? k_kv8_append<TCQ_DT_BF16, D> : k_kv8_append<TCQ_DT_F16, D>, dim3((unsigned)ctas, 2), append_threads(D), 0,
+        return launch_pdl(dtype == TCQ_DT_BF16 ? k_kv8_append<TCQ_DT_BF16, D> : k_kv8_append<TCQ_DT_F16, D>, dim3((unsigned)ctas, 2), 128, 0,
                           stream, *cache, (const u16*)k, (i64)k_sb, (i64)k_st, (const u16*)v, (i64)v_sb, (i64)v_st, table, blocks, start,
                           count, r, B, T, NB);
     });

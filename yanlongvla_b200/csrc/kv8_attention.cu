@@ -131,6 +131,7 @@ struct AttnArgs {
     float* part;           // partial rows of segments that do not cover their unit
     int* counters;
     int blocks, causal, B, T, heads, group;
+    FastDiv by_group;
     float scale_log2;      // scale * log2(e)
 };
 
@@ -389,7 +390,7 @@ __global__ void __launch_bounds__(Few<D, NT>::WARPS * 32, 1) k_attention_few(con
         int limit[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-            const int r = 8 * nt + n, tq = r / A.group;
+            const int r = 8 * nt + n, tq = (int)fdiv((unsigned)r, A.by_group);
             const bool live = r < R && tq < cnt;
             const u16* qr = A.q + at.b * A.q_sb + tq * A.q_st + (i64)(at.h * A.group + r - tq * A.group) * D;
             float v[KS][4], amax = 0.f;
@@ -415,7 +416,7 @@ __global__ void __launch_bounds__(Few<D, NT>::WARPS * 32, 1) k_attention_few(con
             }
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                const int rs = 8 * nt + 2 * t + e, ts = rs / A.group;
+                const int rs = 8 * nt + 2 * t + e, ts = (int)fdiv((unsigned)rs, A.by_group);
                 crow[nt][e] = __shfl_sync(0xffffffffu, back, 4 * (2 * t + e)) * A.scale_log2;
                 limit[nt][e] = rs >= R || ts >= cnt ? 0 : A.causal ? min(max(len - cnt + ts + 1, 0), len) : len;
             }
@@ -557,7 +558,7 @@ __global__ void __launch_bounds__(Few<D, NT>::WARPS * 32, 1) k_attention_few(con
                 if (limit[nt][e] == 0) v = 0.f;               // a row that sees no token
             }
         auto out_row = [&](int r) -> u16* {
-            const int tq = r / A.group;
+            const int tq = (int)fdiv((unsigned)r, A.by_group);
             return A.out + (((i64)at.b * A.T + tq) * A.heads + at.h * A.group + r - tq * A.group) * D;
         };
         // a part: rows of D sums, the reference and the sum of weights
@@ -849,7 +850,7 @@ k_attention_many(const AttnArgs A, int row_tiles, int tile_rows, int splits) {
     const int sp = blockIdx.x % splits, unit = blockIdx.x / splits, bh = unit % (A.B * Hk), b = bh / Hk, h = bh - b * Hk;
     const int rt = row_tiles - 1 - unit / (A.B * Hk), r0 = rt * tile_rows, r1 = min(R, r0 + tile_rows);
     const int len = tokens_of(A.lens, b, A.blocks), cnt = queries_of(A.count, b, A.T);
-    const int last_q = min((r1 - 1) / A.group, cnt - 1), first_q = r0 / A.group;
+    const int last_q = min((int)fdiv((unsigned)(r1 - 1), A.by_group), cnt - 1), first_q = (int)fdiv((unsigned)r0, A.by_group);
     const int upto = last_q < first_q ? 0 : A.causal ? min(max(len - cnt + last_q + 1, 0), len) : len;     // keys that some row sees
     const int open = A.causal ? len - cnt + first_q + 1 : len;                                             // and that every row sees
     const int tiles = (upto + kTile - 1) / kTile;
@@ -864,7 +865,7 @@ k_attention_many(const AttnArgs A, int row_tiles, int tile_rows, int splits) {
     }
     if (warp < W_MMA) {
         // ------------------------------------------------------------------------------------------------ softmax
-        const int g = warp >> 3, p = (warp >> 2) & 1, gl = tid & 127, r = r0 + g * kTile + gl, tq = r / A.group;
+        const int g = warp >> 3, p = (warp >> 2) & 1, gl = tid & 127, r = r0 + g * kTile + gl, tq = (int)fdiv((unsigned)r, A.by_group);
         const int pair_bar = 1 + g * 4 + (warp & 3);            // the two warps of 32 rows meet at a named barrier
         const bool live = r < r1 && tq < cnt;
         const int limit = !live ? 0 : A.causal ? min(max(len - cnt + tq + 1, 0), len) : len;
@@ -879,7 +880,7 @@ k_attention_many(const AttnArgs A, int row_tiles, int tile_rows, int splits) {
             uint4 w[NP];
 #pragma unroll
             for (int n = 0; n < NP; ++n) {
-                const int row = w8 * 16 + n * RPP + lane / SEG, rr = r0 + g * kTile + row, tt = rr / A.group;
+                const int row = w8 * 16 + n * RPP + lane / SEG, rr = r0 + g * kTile + row, tt = (int)fdiv((unsigned)rr, A.by_group);
                 const u16* qr = A.q + b * A.q_sb + tt * A.q_st + (i64)(h * A.group + rr - tt * A.group) * D;
                 w[n] = rr < r1 && tt < cnt && sl < LPR ? reinterpret_cast<const uint4*>(qr)[sl] : make_uint4(0, 0, 0, 0);
             }
@@ -1058,7 +1059,7 @@ k_attention_many(const AttnArgs A, int row_tiles, int tile_rows, int splits) {
             constexpr int X = (D / 8) % 8 == 0 ? 7 : (D / 8) % 4 == 0 ? 3 : 1;
             asm volatile("barrier.cta.sync 15, %0;" ::"r"(P::SOFT) : "memory");
             for (int e = tid; e < (r1 - r0) * (D / 8); e += P::SOFT) {
-                const int rr = e / (D / 8), ch = e - rr * (D / 8), t = (r0 + rr) / A.group;
+                const int rr = e / (D / 8), ch = e - rr * (D / 8), t = (int)fdiv((unsigned)(r0 + rr), A.by_group);
                 u16* dst = A.out + (((i64)b * A.T + t) * A.heads + h * A.group + r0 + rr - t * A.group) * D;
                 reinterpret_cast<uint4*>(dst)[ch] = reinterpret_cast<const uint4*>(smem)[rr * (D / 8) + (ch ^ (rr & X))];
             }
@@ -1239,7 +1240,7 @@ k_attention_many(const AttnArgs A, int row_tiles, int tile_rows, int splits) {
             u32 w[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) w[j] = sum != 0.f ? pack2<DT>(acc[2 * j] * f, acc[2 * j + 1] * f) : 0u;
-            const int r = r0 + row, tq = r / A.group;
+            const int r = r0 + row, tq = (int)fdiv((unsigned)r, A.by_group);
             u16* dst = A.out + (((i64)b * A.T + tq) * A.heads + h * A.group + r - tq * A.group) * D + 8 * c8;
             *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
         }
@@ -1335,7 +1336,7 @@ int tcq_kv8_attention(const tcq_kv8_cache* cache, const void* q, int dtype, int6
     if (!workspace || workspace_bytes < tcq_kv8_attention_workspace(B, T, heads, Hk, cache->head_dim, blocks)) return TCQ_ERR_WORKSPACE;
     const int sms = tcq_sm_count();
     AttnArgs A = {*cache, (const u16*)q, q_sb, q_st, (u16*)out, table, lens, count, nullptr, (int*)workspace, blocks, causal, B, T, heads,
-                  heads / Hk, scale * 1.4426950408889634f};
+                  heads / Hk, make_fastdiv((unsigned)(heads / Hk)), scale * 1.4426950408889634f};
     const i64 rows = (i64)T * A.group;
     if (few_rows(rows, cache->head_dim)) {
         A.part = reinterpret_cast<float*>((char*)workspace + counter_bytes(sms));
