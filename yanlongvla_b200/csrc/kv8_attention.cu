@@ -50,15 +50,17 @@ TCQ_HD int page_in(int p, int pages) {
 TCQ_HD int page_of(const int* row, int blk, int pages) { return page_in(row[blk], pages); }
 
 // ------------------------------------------------------------------------------------------------ few query rows
-// T * group <= 16 MT query rows share a key head (single tokens, short action sequences): the kernel streams the pages once and
-// is bound by HBM.
+// T * group <= 32 query rows share a key head (single tokens, short action sequences; 16 rows above head width 64): the kernel
+// streams the pages once. Bound by HBM for long sequences (4 x 131037 keys of 8 heads of 64: 107 us, 5.0 TB/s), by the latency of a
+// warp's page (about 1.5 us) for short ones (one token over 203 keys: 4.6 us a call).
 //
 // Mathematics. With integers k, v and block scales ks, vs: score x = (q . k) ks scale log2(e) + log2(vs), reference
-// m >= x - 10.5, weight p = 2^(x - m + 5); out = sum p v / sum (p / vs). Folding vs into the exponent keeps every product operand an exact
-// small integer or one rounding of p, and the sum of p is formed before that rounding. m moves only when a score passes it
-// by more than 10.5, so the accumulators are rarely rescaled. Operands are FP16: an int8 is exact, a query row is scaled by a
-// power of two so that its largest element lies in [2^14, 2^15) (elements below 2^-28 of it lose bits, those of BF16
-// inputs above that lose none), and p <= 2^15.5 keeps 11 bits down to 2^-19 of the reference's and is dropped below 2^-30 of it.
+// m >= x - 10.5, weight p = 2^(x - m + 5); out = sum p v / sum (p / vs). Folding vs into the exponent keeps every operand of a
+// product an exact small integer or one rounding of p, and the sum of p is formed in FP32 before that rounding. m moves only
+// when a score passes it by more than 10.5, so the accumulators are rarely rescaled. Operands are FP16, accumulators FP32: an
+// int8 is exact, a query row is scaled by a power of two so that its largest element lies in [2^14, 2^15) (elements below 2^-28
+// of it lose bits, those of BF16 inputs above that lose none), and p <= 2^15.5 keeps 11 bits down to 2^-19 of the reference's
+// and is dropped below 2^-30 of it. BF16 in its place would keep 8 bits of p.
 //
 // Layout. A warp takes whole pages. S^T = K Q^T and O^T = V^T P^T are m16n8k16 products with the 64 keys (or the D value
 // rows) as rows and NT tiles of 8 queries as columns, so that one token's few queries waste least. The order of a contraction is
@@ -136,7 +138,8 @@ struct AttnArgs {
 };
 
 // Plan of the few-row kernel. Every warp has a ring of NH half pages (64 D bytes: a block's keys or its values) of its own. As
-// many warps as their registers and rings allow: a warp alone issues one instruction in about four clocks.
+// many warps as their registers and rings allow: a warp alone issues one instruction in about four clocks (32 ragged sequences
+// and 4 x 131037 keys: 39 and 107 us with 12 warps, 40 and 109 with 8; 16 spill registers: 50 and 125).
 template <int D, int NT>
 struct Few {
     static constexpr int HALF = kBlk * D;
@@ -159,12 +162,17 @@ struct Place {
     int b, h, ubeg, vp, np;
 };
 
-// One warp adds the parts of a unit (workers first .. last, in that order) and writes its R rows. Kept out of line: its many
-// loads in flight want registers of their own.
+// The part of a unit that worker w wrote: a worker has at most two, of its first unit and (as that unit's first worker) its last.
+TCQ_HD i64 part_slot(int w, int first) { return 2 * (i64)w + (w == first ? 1 : 0); }
+
+// One warp adds parts of a unit, those of workers from, from + step, .. to, in that order: to the unit's R output rows, or, with
+// out NULL, to the part of worker `from`. Kept out of line, four parts at a time: its loads in flight want registers, and eight
+// parts made the caller spill (107 -> 124 us at 4 x 131037 keys).
 template <int DT, int D>
-__device__ __noinline__ void add_parts(const float* parts, i64 size, int first, int last, int R, int group, u16* out, i64 token) {
-    constexpr int NI = 4, NB = 4;                  // pairs of elements of a lane, parts requested at once
+__device__ __noinline__ void add_parts(float* parts, i64 size, int first, int from, int to, int step, int R, int group, u16* out, i64 token) {
+    constexpr int NI = 4, NB = 4;                 // pairs of elements of a lane, parts requested at once
     const int lane = threadIdx.x & 31;
+    float* target = parts + part_slot(from, first) * size;
 #pragma unroll 1
     for (int i0 = 0; i0 < R * (D / 2); i0 += 32 * NI) {
         float2 acc[NI] = {};
@@ -177,12 +185,12 @@ __device__ __noinline__ void add_parts(const float* parts, i64 size, int first, 
             top[k] = -INFINITY;
         }
 #pragma unroll 1
-        for (int w0 = first; w0 <= last; w0 += NB) {
+        for (int w0 = from; w0 <= to; w0 += NB * step) {
             float2 v[NB][NI], e[NB][NI];
 #pragma unroll
             for (int w = 0; w < NB; ++w) {
-                const int at = min(w0 + w, last);
-                const float* part = parts + (2 * (i64)at + (at == first)) * size;
+                const int at = w0 + w * step <= to ? w0 + w * step : w0;
+                const float* part = parts + part_slot(at, first) * size;
 #pragma unroll
                 for (int k = 0; k < NI; ++k) {
                     v[w][k] = __ldcg(reinterpret_cast<const float2*>(part + off[k]));
@@ -191,7 +199,7 @@ __device__ __noinline__ void add_parts(const float* parts, i64 size, int first, 
             }
 #pragma unroll
             for (int w = 0; w < NB; ++w)
-                if (w0 + w <= last) {
+                if (w0 + w * step <= to) {
 #pragma unroll
                     for (int k = 0; k < NI; ++k) {
                         const float nt = fmaxf(top[k], e[w][k].x), keep = nt == -INFINITY ? 0.f : ex2(top[k] - nt),
@@ -205,10 +213,25 @@ __device__ __noinline__ void add_parts(const float* parts, i64 size, int first, 
 #pragma unroll
         for (int k = 0; k < NI; ++k) {
             const int i = i0 + lane + 32 * k, r = i / (D / 2), tq = r / group;
+            if (i >= R * (D / 2)) continue;
             const float f = sum[k] != 0.f ? 1.f / sum[k] : 0.f;
-            if (i < R * (D / 2)) reinterpret_cast<u32*>(out + tq * token + (i64)(r - tq * group) * D)[i - r * (D / 2)] = pack2<DT>(acc[k].x * f, acc[k].y * f);
+            if (out) reinterpret_cast<u32*>(out + tq * token + (i64)(r - tq * group) * D)[i - r * (D / 2)] = pack2<DT>(acc[k].x * f, acc[k].y * f);
+            else *reinterpret_cast<float2*>(target + off[k]) = acc[k];
         }
     }
+    if (out) return;
+    // references and sums last: every lane has read them by now
+    float top = -INFINITY, sum = 0.f;
+    if (lane < R)
+        for (int w = from; w <= to; w += step) {
+            const float2 e = __ldcg(reinterpret_cast<const float2*>(parts + part_slot(w, first) * size + lane * (D + 2) + D));
+            const float nt = fmaxf(top, e.x);
+            if (nt == -INFINITY) continue;
+            sum = __fmaf_rn(e.y, ex2(e.x - nt), sum * ex2(top - nt));
+            top = nt;
+        }
+    __syncwarp();
+    if (lane < R) *reinterpret_cast<float2*>(target + lane * (D + 2) + D) = make_float2(top, sum);
 }
 
 // Work, by what the lengths say:
@@ -216,7 +239,7 @@ __device__ __noinline__ void add_parts(const float* parts, i64 size, int first, 
 //   an empty one takes a place without a page). A warp that holds a whole unit writes its output; parts of a unit go to the
 //   workspace, and the last of its warps to arrive adds them in their order, so the result does not depend on timing;
 // - no more units than CTAs, of at most three pages per warp: a CTA takes a unit, its warps every WARPS-th page, and the parts are
-//   added in shared memory (one token over 203 keys of 8 heads: 5 us less than through the workspace);
+//   added in shared memory (one token over 203 keys of 8 heads: 4.9 us a call, through the workspace 10.8);
 // - whole != 0 (many short sequences, told by the host): each warp takes whole units, one after the other.
 template <int DT, int D, int NT>
 __global__ void __launch_bounds__(Few<D, NT>::WARPS * 32, 1) k_attention_few(const AttnArgs A, int whole) {
@@ -609,19 +632,33 @@ __global__ void __launch_bounds__(Few<D, NT>::WARPS * 32, 1) k_attention_few(con
                 }
             }
         } else {
-            // a worker has at most two parts, of its first unit and of its last
+            // More than 16 parts are added in two steps, sixteen neighbours first (one warp over 222 parts of one token and
+            // 131037 keys took as long as the pages: 84 -> 47 us).
             const int first = at.ubeg / chunk, last = (at.ubeg + at.vp - 1) / chunk;
-            write_part(A.part + (i64)(2 * me + (me == first ? 1 : 0)) * (8 * NT) * (D + 2));
-            __threadfence();
-            __syncwarp();
-            int seen = 0;
-            if (lane == 0) seen = atomicAdd(A.counters + first, 1);
-            seen = __shfl_sync(0xffffffffu, seen, 0);
-            if (seen == last - first) {
-                if (lane == 0) A.counters[first] = 0;
+            constexpr i64 SIZE = (i64)(8 * NT) * (D + 2);
+            write_part(A.part + part_slot(me, first) * SIZE);
+            // true in the warp that arrives last
+            auto arrive = [&](int* counter, int expected) -> bool {
                 __threadfence();
-                add_parts<DT, D>(A.part, (i64)(8 * NT) * (D + 2), first, last, R, A.group, out_row(0), (i64)A.heads * D);
+                __syncwarp();
+                int seen = 0;
+                if (lane == 0) seen = atomicAdd(counter, 1);
+                seen = __shfl_sync(0xffffffffu, seen, 0);
+                if (seen != expected - 1) return false;
+                if (lane == 0) *counter = 0;
+                __threadfence();
+                return true;
+            };
+            int step = 1;
+            bool add = true;
+            if (last - first >= 16) {
+                const int lead = first + (me - first) / 16 * 16, end16 = min(lead + 15, last);
+                add = arrive(A.counters + workers + part_slot(lead, first), end16 - lead + 1);
+                if (add) add_parts<DT, D>(A.part, SIZE, first, lead, end16, 1, R, A.group, nullptr, 0);
+                step = 16;
             }
+            if (add && arrive(A.counters + first, (last - first) / step + 1))
+                add_parts<DT, D>(A.part, SIZE, first, first, last, step, R, A.group, out_row(0), (i64)A.heads * D);
         }
         if (!next_unit(at, end)) break;
         if (whole) x = 0;
@@ -634,14 +671,23 @@ __global__ void __launch_bounds__(Few<D, NT>::WARPS * 32, 1) k_attention_few(con
 //
 // The rows of a key head are its queries in token order, `group` heads to a token, so a causal limit never falls along the
 // rows. A CTA takes NG groups of up to 128 rows and one key head. Roles:
-//   softmax   128 threads per group, a row each: scores from TMEM, weights (FP16) back to TMEM over the scores;
-//   convert   128 threads: INT8 pages from global memory (requested one half tile ahead into registers) to FP16 tiles in
-//             shared memory, 128-byte swizzled, keys K-major along the head, values K-major along the tokens;
-//   product   one thread issues S = Q K^T (both operands in shared memory) and O += P V (P in TMEM).
+//   softmax   256 threads per group, two to a row, a page of the tile each: 64 scores from TMEM, weights (FP16) back to TMEM
+//             over the scores. The two agree on the row's reference at a named barrier before either writes;
+//   product   one warp, an elected lane of which issues S = Q K^T (both operands in shared memory) and O += P V (P in TMEM);
+//   convert   what is left: INT8 pages, copied asynchronously a tile ahead, to FP16 tiles in shared memory, 128-byte swizzled,
+//             keys K-major along the head, values K-major along the tokens.
 // The two groups alternate: while one's weights are formed, the other's products run. Mathematics, scaling of the queries and
 // handling of the scales are those of the few-row kernel; the reference m moves only when a score passes it by 10.5, and O (in
-// TMEM) is rescaled by its own row's thread. S of a tile is issued after O of the tile before it, and a commit covers every
+// TMEM) is rescaled by its own row's threads. S of a tile is issued after O of the tile before it, and a commit covers every
 // product issued before it: scores that have arrived mean that O is complete up to the tile before.
+//
+// Bound by the softmax warps' chain per tile (about 3,700 clocks at head width 64, 4,000 at 128: scores 500 .. 900, load 200,
+// maximum and barrier 500, weights 1,400 .. 1,950, of which the exponential unit alone needs 2,048 for both groups, handing over
+// and the loop 700), not by the products (1,024 and 2,048 clocks): 2 x 4096 queries of 32 heads of 128, 8 key heads, 4200 keys: 330 us,
+// 880 TFLOP/s; 160 queries over 16411 keys, heads of 64: 61 us. Measured on the way to this shape, same two cases: one thread to a row with two
+// passes over the scores 423 and 73 us; products issued from a single-lane branch (130 clocks each instead of 64) 448 and 74;
+// a row per lane for loads and stores of Q and O 376 and 67 us; scores a tile ahead in TMEM columns of their own (heads up to 64)
+// 64 us at the second; an eighth to a third of the exponentials by polynomial: no faster.
 //
 // Few units (a frame of one robot): the tiles of a unit are divided over a cluster of CTAs, which add their parts through
 // distributed shared memory.
@@ -656,7 +702,8 @@ struct Many {
     static constexpr int VB = D * 128 * 2;                            // of its values
     static constexpr int NS = 2;                                      // tiles of either in flight
     // Threads and registers. With two groups the CTA is launched with 80 registers a thread (768 x 80), of which the softmax
-    // warps take more and the others less: 512 x 96 + 256 x 48 = 61,440.
+    // warps take more and the others less: 512 x 96 + 256 x 48 = 61,440 (launch_many checks the 80).
+    static constexpr int LAUNCH_REGS = 80;
     static constexpr int SOFT = NG * 256;                            // softmax threads: two to a row, a page each
     static constexpr int THREADS = NG == 2 ? 768 : 512;
     static constexpr int CONV = THREADS - SOFT - 32;                 // convert threads: what softmax and the product warp leave
@@ -1252,7 +1299,6 @@ template <int DT, int D, int NG>
 int launch_many(const AttnArgs& A, void* stream) {
     typedef Many<D, NG> P;
     const auto kern = k_attention_many<DT, D, NG>;
-    constexpr int PER_SM = 1;
     const int R = A.T * A.group, row_tiles = (R + NG * kTile - 1) / (NG * kTile);
     const int tile_rows = ((R + row_tiles - 1) / row_tiles + 31) & ~31;            // even shares, in warps
     const i64 units = (i64)A.B * A.cache.kv_heads * row_tiles;
@@ -1272,12 +1318,15 @@ int launch_many(const AttnArgs& A, void* stream) {
     if (cudaGetDevice(&dev) != cudaSuccess || dev > 63) return TCQ_ERR_DEVICE;
     if (!held[dev][1].load(std::memory_order_acquire)) {
         if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, P::BYTES) != cudaSuccess) return TCQ_ERR_LAUNCH;
+        // the register shares of the roles are taken from what the launch gives the CTA: less would leave them waiting
+        cudaFuncAttributes fa;
+        if (cudaFuncGetAttributes(&fa, kern) != cudaSuccess || (NG == 2 && fa.numRegs != P::LAUNCH_REGS)) return TCQ_ERR_LAUNCH;
         for (int s = 8; s >= 1; --s) {
             int n = 0;
             cfg.gridDim = dim3(s);
             attr[0].val.clusterDim.x = s;
             cfg.numAttrs = 1;
-            if (s == 1) n = tcq_sm_count() * PER_SM;
+            if (s == 1) n = tcq_sm_count();
             else if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess) n = 0, cudaGetLastError();
             held[dev][s].store(n, std::memory_order_release);
         }
@@ -1302,9 +1351,9 @@ int launch_many(const AttnArgs& A, void* stream) {
     return cudaLaunchKernelEx(&cfg, kern, A, row_tiles, tile_rows, splits) == cudaSuccess ? TCQ_OK : TCQ_ERR_LAUNCH;
 }
 
-// Arrival counters at the head of the workspace, one per worker of the few-row kernel.
-constexpr int kMostWarps = 16;
-inline size_t counter_bytes(int sms) { return ((size_t)kMostWarps * sms * sizeof(int) + 15) & ~(size_t)15; }
+// Arrival counters at the head of the workspace, three per worker of the few-row kernel (its unit, and its two parts' groups).
+constexpr int kMostWarps = 12;
+inline size_t counter_bytes(int sms) { return ((size_t)3 * kMostWarps * sms * sizeof(int) + 15) & ~(size_t)15; }
 
 // ------------------------------------------------------------------------------------------------ host side
 }  // namespace

@@ -184,6 +184,33 @@ def _case_chain(m, n, launches):
         K.chain(x, 'rms', w, None, 1e-6, acc=z, sv=sv, su=su, q=q, scale=s, want_n=False)
 
 
+def _case_memory(kind, robots, tokens, length, width, launches):
+    """The streaming memory's kernels on `robots` sequences of 32 query and 8 key heads of `width`: 'attend' (tokens queries of each
+    over length cached tokens), 'append' (tokens new ones, keys turned) or 'read'."""
+    from . import kernels as K
+    dev = torch.device('cuda')
+    g = torch.Generator(device=dev).manual_seed(16)
+    blocks = -(-max(length, tokens) // K.KV8_BLOCK)
+    cache = K.KV8Cache.empty(robots * blocks, 8, width)
+    cache.k.copy_(torch.randint(-127, 128, cache.k.shape, device=dev, generator=g, dtype=torch.int8))
+    cache.v.copy_(torch.randint(-127, 128, cache.v.shape, device=dev, generator=g, dtype=torch.int8))
+    cache.k_scale.fill_(0.01)
+    cache.v_scale.fill_(0.01)
+    table = torch.randperm(robots * blocks, device=dev, generator=g).to(torch.int32).view(robots, blocks)
+    zero, lens = (torch.full((robots,), n, dtype=torch.int32, device=dev) for n in (0, length))
+    q = torch.randn(robots, tokens, 32 * width, device=dev, generator=g).bfloat16()
+    k = torch.randn(robots, tokens, 8 * width, device=dev, generator=g).bfloat16()
+    rope = K.RopeAxes(*K.RopeAxes.tables(max(tokens, 64), width), (width // 2,))
+    pos = torch.arange(tokens, dtype=torch.int32, device=dev).expand(1, robots, tokens).contiguous()
+    for _ in range(launches):
+        if kind == 'attend':
+            K.kv8_attention(q, cache, table, lens)
+        elif kind == 'append':
+            K.kv8_append(cache, k, k, table, zero, rope=rope, pos=pos)
+        else:
+            K.kv8_read(cache, table, zero, lens, length)
+
+
 def _case_policy(batch):
     """replay_breakdown of one CUDA-graph replay of the fly policy's action chunk for `batch` observations."""
     import json
@@ -206,12 +233,15 @@ def _case_policy(batch):
 def main(argv=None):
     import argparse
     ap = argparse.ArgumentParser(description='one kernel case for a profiler')
-    ap.add_argument('case', choices=['gemv', 'gemv_tc', 'gemm', 'pre', 'rotate', 'chain', 'policy'])
+    ap.add_argument('case', choices=['gemv', 'gemv_tc', 'gemm', 'pre', 'rotate', 'chain', 'attend', 'append', 'read', 'policy'])
     ap.add_argument('--m', type=int, default=4096)
     ap.add_argument('--n', type=int, default=None)
     ap.add_argument('--k', type=int, default=None)
     ap.add_argument('--tokens', type=int, default=1)
     ap.add_argument('--launches', type=int, default=4)
+    ap.add_argument('--robots', type=int, default=1, help='attend / append / read: sequences')
+    ap.add_argument('--length', type=int, default=4096, help='attend / read: cached tokens of a sequence')
+    ap.add_argument('--width', type=int, default=64, help='attend / append / read: head width')
     ap.add_argument('--out', choices=['i32', 'bf16'], default='i32', help='gemm case: INT32 or BF16 (scaled) output')
     a = ap.parse_args(argv)
     if a.case == 'gemv':
@@ -222,6 +252,8 @@ def main(argv=None):
         _case_gemm(a.m, a.k or 2048, a.n or 8192, a.launches, a.out)
     elif a.case == 'policy':
         _case_policy(a.tokens)
+    elif a.case in ('attend', 'append', 'read'):
+        _case_memory(a.case, a.robots, a.tokens, a.length, a.width, a.launches)
     elif a.case == 'chain':
         _case_chain(a.m, a.k or 1536, a.launches)
     else:
