@@ -351,6 +351,35 @@ def test_attention_long(K, T, D):
     check_attention(K, q, cache, table, lens)
 
 
+@pytest.mark.parametrize('most', [300, 1500])
+@pytest.mark.parametrize('T,heads,kv_heads,D', [(1, 8, 8, 64), (1, 16, 8, 128), (9, 8, 8, 48), (17, 8, 8, 48), (25, 8, 8, 32), (3, 40, 8, 80),
+                                                (20, 16, 8, 64)])
+def test_attention_many_units(K, T, heads, kv_heads, D, most):
+    """More heads of more sequences than the device has SMs, short (whole units to a warp) and longer ones, some empty."""
+    lens = [0 if b % 13 == 5 else max(T if b % 7 else 1, (b * 37 + 11) % most) for b in range(41)]
+    q, cache, table = attention_case(K, 41, T, heads, kv_heads, D, lens)
+    check_attention(K, q, cache, table, lens)
+    count = [(b * 5) % (T + 1) for b in range(41)]
+    check_attention(K, q, cache, table, lens, count=count, causal=False)
+
+
+@pytest.mark.parametrize('lens', [[3000], [9000, 64]])
+def test_attention_few_units(K, lens):
+    """One key head: every part of a sequence in another warp, on one CTA and over the device."""
+    for T, D in ((1, 64), (2, 128), (6, 48)):
+        q, cache, table = attention_case(K, len(lens), T, 4, 1, D, lens)
+        want = check_attention(K, q, cache, table, lens)
+        for _ in range(3):
+            assert torch.equal(K.kv8_attention(q, cache, table, i32(lens)), want)
+
+
+@pytest.mark.parametrize('T', [1, 20, 300])
+def test_attention_negative_scale(K, T):
+    lens = [260]
+    q, cache, table = attention_case(K, 1, T, 4, 2, 64, lens)
+    check_attention(K, q, cache, table, lens, scale=-0.2)
+
+
 @pytest.mark.parametrize('T', [1, 20, 300])
 def test_attention_loud_and_quiet_scores(K, T):
     """Scores of several hundred (one key takes all the weight), none at all, and blocks of very different scales."""
