@@ -38,8 +38,15 @@ struct Vec {
     static TCQ_HD void unpack(R r, float* v) {
         union { R r; u32 w[(BYTES + 3) / 4]; u16 h[BYTES / 2]; } u;
         u.r = r;
+        if (DT == TCQ_DT_F32) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) v[i] = DT == TCQ_DT_F32 ? __uint_as_float(u.w[i]) : elem_f<DT>(u.h[i]);
+            for (int i = 0; i < V; ++i) v[i] = __uint_as_float(u.w[i]);
+        } else if (V == 1) {
+            v[0] = elem_f<DT>(u.h[0]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < V / 2; ++i) unpack2<DT>(u.w[i], v[2 * i], v[2 * i + 1]);
+        }
     }
     static TCQ_HD void store(void* p, const float* v) {
         union { R r; u32 w[(BYTES + 3) / 4]; u16 h[BYTES / 2]; } u;

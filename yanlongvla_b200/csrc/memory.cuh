@@ -31,8 +31,14 @@ TCQ_HD u32 pack2(float lo, float hi) {
 
 template <int DT>
 TCQ_HD void unpack2(u32 w, float& lo, float& hi) {
-    lo = elem_f<DT>((u16)(w & 0xffffu));
-    hi = elem_f<DT>((u16)(w >> 16));
+    if (DT == TCQ_DT_F16) {
+        __half2 h;
+        memcpy(&h, &w, 4);
+        const float2 f = __half22float2(h);
+        lo = f.x, hi = f.y;
+    } else {
+        lo = __uint_as_float(w << 16), hi = __uint_as_float(w & 0xffff0000u);
+    }
 }
 
 // ---------------------------------------------------------------------------------------------------- rotary tables
