@@ -2,8 +2,8 @@
 
 Mirrors deploy/tcq_kernels/kernels.py of the reference (ForeverBlue816/yanlongvla): the same function names, argument
 meaning and buffer layouts, so callers written against the reference work unchanged. Every call launches on
-torch.cuda.current_stream(), allocates nothing except the cached per-stream workspace of gemm_tcq, and therefore
-works inside torch.cuda.graph() captures. A non-zero status from the library raises TcqError.
+torch.cuda.current_stream(), allocates nothing except outputs it is not given and the cached per-stream workspaces of
+gemm_tcq and kv8_attention, and therefore works inside torch.cuda.graph() captures. A non-zero status from the library raises TcqError.
 
   pre      x (M, K) BF16/F16/F32 -> q (M, K) int8 and/or q4 (K/4, ld) int32, scale (M,)     (kernels.py:602-606)
   post     acc (M, lda) I32 / F32 / BF16 columns col0.. -> y (M, N) BF16                    (kernels.py:612-615)
@@ -355,8 +355,8 @@ KV8_BLOCK = 64           # tokens of a cache block
 
 class RopeAxes:
     """Tables of a rotary embedding with 1 to 4 axes. cos, sin (positions, D / 2) FP32; sections: how many of the D / 2
-    frequencies turn by each axis' position, in order (Sum = D / 2). pairs False: element j turns with j + D / 2 (as `rope`),
-    True: 2 j with 2 j + 1. `rope_axes` tables for a plain geometric progression come from RopeAxes.tables."""
+    frequencies turn by each axis' position, in order (their sum is D / 2). pairs False: element j turns with j + D / 2 (as `rope`),
+    True: 2 j with 2 j + 1. RopeAxes.tables makes the tables of the usual geometric progression."""
 
     def __init__(self, cos, sin, sections, pairs=False):
         _cuda(cos, sin)
