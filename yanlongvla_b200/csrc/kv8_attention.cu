@@ -1062,8 +1062,16 @@ k_attention_many(const AttnArgs A, int row_tiles, int tile_rows, int splits) {
             if (lane == 0) mbar_arrive(bar(BAR_PFULL + 2 * g + p));
             return true;
         };
+        // Warps without a query (the last rows of a tile, sequences with fewer queries) only keep the barriers going: what their
+        // TMEM lanes hold stays in their own rows.
+        const bool idle = !__any_sync(0xffffffffu, live);
 #pragma unroll 1
         for (int i = k0; i < k1; ++i) {
+            if (idle) {
+                if (!wait(BAR_SFULL + g, i - k0)) break;
+                if (lane == 0) mbar_arrive(bar(BAR_PFULL + 2 * g + p));
+                continue;
+            }
             const float c = crow * nk, vsc = nv;
             request_scales(i + 1);
             request_id(i + 2);
