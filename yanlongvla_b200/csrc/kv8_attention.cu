@@ -1284,7 +1284,9 @@ k_attention_many(const AttnArgs A, int row_tiles, int tile_rows, int splits) {
             for (int k = 0; k < splits; ++k) {
                 const float2 ml = peer_ld2(peer_addr(sbase + P::ML0 + row * 8, k));
                 const float f = top == -INFINITY ? 0.f : ex2(ml.x - top);
-                if (f == 0.f) continue;
+                // Nothing of this part remains, unless its sum is NaN: scores that are NaN move no reference (a part of a NaN query
+                // has -inf and a NaN sum), and the row has to say so.
+                if (f == 0.f && ml.y == ml.y) continue;
                 sum += ml.y * f;
                 const u32 base = peer_addr(sbase, k) + row * (D * 4);
                 const float4 u = peer_ld4(base + (((2 * c8) ^ (row & X)) << 4)), v = peer_ld4(base + (((2 * c8 + 1) ^ (row & X)) << 4));
