@@ -291,7 +291,10 @@ int tcq_kv8_append(const tcq_kv8_cache* cache, const void* k, int64_t k_sb, int6
 int tcq_kv8_read(const tcq_kv8_cache* cache, void* k, void* v, int dtype, const int32_t* table, int blocks,
                  const int32_t* begin, const int32_t* lens, int B, int T, void* stream);
 
-/* Workspace of tcq_kv8_attention in bytes. Zero-filled before its first use; every call leaves it ready for the next. */
+/* Workspace of tcq_kv8_attention in bytes. Zero-filled before its first use (the first TCQ_KV8_ZEROED_BYTES of it, or all of a
+ * smaller one, are enough); every call leaves it ready for the next. Calls that can run at the same time want a workspace
+ * each, and a captured graph one that no other graph and no call outside it uses, zero-filled by a node of the graph. */
+#define TCQ_KV8_ZEROED_BYTES 65536
 size_t tcq_kv8_attention_workspace(int B, int T, int heads, int kv_heads, int head_dim, int blocks);
 
 /* out (B, T, heads * head_dim) = softmax(scale * q k^T) v over the cached tokens of each sequence. q BF16 / F16 with strides
@@ -307,6 +310,9 @@ int tcq_kv8_attention(const tcq_kv8_cache* cache, const void* q, int dtype, int6
  * tcgen05 kernels use, on a barrier that nothing arrives at; after limit_us (1 .. 1e6) microseconds the wait gives up,
  * raises device error flag 1 and the kernel returns. Nothing faults and the context stays usable. */
 int tcq_selftest_wait_expiry(unsigned limit_us, void* stream);
+
+/* The stream capture that `stream` is part of: *id is its number, unique in the process, or 0 when the stream is not capturing. */
+int tcq_capture_id(void* stream, unsigned long long* id);
 
 /* Device error flags: 1 = a bounded pipeline wait expired and the kernel stopped early, 2 = a position, page number or
  * length given to a streaming-memory operator was out of range (see there). Synchronizes the current device. reset != 0 clears the flags. Returns -1 if the flags cannot be read. */

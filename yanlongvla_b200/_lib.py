@@ -73,6 +73,7 @@ SIGNATURES = {
     'tcq_kv8_attention_workspace': [I, I, I, I, I, I],
     'tcq_kv8_attention': [P, P, I, L, L, P, P, I, P, P, I, F, I, I, I, P, SZ, P],
     'tcq_selftest_wait_expiry': [ctypes.c_uint, P],
+    'tcq_capture_id': [P, ctypes.POINTER(ctypes.c_uint64)],
     'tcq_device_error': [I],
 }
 RESTYPES = {'tcq_status_string': ctypes.c_char_p, 'tcq_gemm_tcq_workspace': SZ, 'tcq_gemm_tcq_tc_workspace': SZ, 'tcq_gemm_tcq_noalloc_max_elements': SZ,

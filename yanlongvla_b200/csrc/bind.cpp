@@ -7,7 +7,6 @@
 
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
-#include <ATen/ops/zeros.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
@@ -24,6 +23,7 @@ decltype(&tcq_kv8_append) f_append;
 decltype(&tcq_kv8_read) f_read;
 decltype(&tcq_kv8_attention_workspace) f_workspace;
 decltype(&tcq_kv8_attention) f_attention;
+decltype(&tcq_capture_id) f_capture;
 PyObject *g_error, *g_launches, *g_rope_class, *g_cache_class, *s_ref;
 
 struct Refused {};                         // a Python error is set
@@ -225,26 +225,41 @@ PyObject* kv8_read(PyObject*, PyObject* const* a, Py_ssize_t n) {
     });
 }
 
-// Workspace of the attention for a stream: zero-filled once, left ready by every call, grown on demand. Kept until the process
-// ends (a destructor would run after the CUDA context is gone).
+// Workspace of the attention for a stream. Outside captures: one per device and stream, grown on demand, replaced in the stream's
+// order. In a capture the graph gets one of its own: allocated in the capture, so that it lives in the graph's memory pool, with
+// its counters cleared by a node of the graph, so that the graph may be replayed before, after or (on another stream) next to any
+// other call. A graph is never handed the stream's own workspace, whose address a later call may change. The capture's is let go by
+// the first call on the stream that belongs to another capture or to none; the memory stays with the pool.
+// Entries are kept until the process ends (a destructor would run after the CUDA context is gone).
 void* workspace(int dev, void* stream, size_t need, size_t& have) {
     struct Entry {
         int dev;
         void* stream;
-        at::Tensor t;
+        unsigned long long capture;
+        at::Tensor own, captured;
     };
     static auto* all = new std::vector<Entry>();
     Entry* e = nullptr;
     for (auto& x : *all)
         if (x.dev == dev && x.stream == stream) e = &x;
     if (!e) {
-        all->push_back({dev, stream, at::Tensor()});
+        all->push_back({dev, stream, 0, at::Tensor(), at::Tensor()});
         e = &all->back();
     }
-    if (!e->t.defined() || static_cast<size_t>(e->t.numel()) < need)
-        e->t = at::zeros({static_cast<int64_t>(need)}, at::TensorOptions().dtype(at::kByte).device(at::kCUDA, static_cast<c10::DeviceIndex>(dev)));
-    have = static_cast<size_t>(e->t.numel());
-    return e->t.data_ptr();
+    unsigned long long capture = 0;
+    f_capture(stream, &capture);
+    if (e->capture != capture) {
+        e->captured.reset();
+        e->capture = capture;
+    }
+    at::Tensor& t = capture ? e->captured : e->own;
+    if (!t.defined() || static_cast<size_t>(t.numel()) < need) {
+        t.reset();
+        t = at::empty({static_cast<int64_t>(need)}, at::TensorOptions().dtype(at::kByte).device(at::kCUDA, static_cast<c10::DeviceIndex>(dev)));
+        t.narrow(0, 0, std::min<int64_t>(t.numel(), TCQ_KV8_ZEROED_BYTES)).zero_();
+    }
+    have = static_cast<size_t>(t.numel());
+    return t.data_ptr();
 }
 
 // kv8_attention(q, cache, table, lens, count, causal, scale, out)
@@ -294,7 +309,8 @@ PyObject* init(PyObject*, PyObject* args) {
         return at != nullptr;
     };
     if (!take("tcq_status_string", f_status) || !take("tcq_rope_axes", f_rope) || !take("tcq_kv8_append", f_append) || !take("tcq_kv8_read", f_read) ||
-        !take("tcq_kv8_attention_workspace", f_workspace) || !take("tcq_kv8_attention", f_attention)) {
+        !take("tcq_kv8_attention_workspace", f_workspace) || !take("tcq_kv8_attention", f_attention) ||
+        !take("tcq_capture_id", f_capture)) {
         if (!PyErr_Occurred()) PyErr_SetString(PyExc_KeyError, "a function address is missing");
         return nullptr;
     }

@@ -1153,6 +1153,17 @@ int tcq_selftest_wait_expiry(unsigned limit_us, void* stream) {
     return cudaGetLastError() == cudaSuccess ? TCQ_OK : TCQ_ERR_LAUNCH;
 }
 
+int tcq_capture_id(void* stream, unsigned long long* id) {
+    if (!id) return TCQ_ERR_ARG;
+    *id = 0;
+    cudaStreamCaptureStatus st;
+    unsigned long long n = 0;
+    // The default stream has no answer while a stream that it waits for is capturing; itself it captures nothing.
+    if (cudaStreamGetCaptureInfo((cudaStream_t)stream, &st, &n) != cudaSuccess) cudaGetLastError();
+    else if (st != cudaStreamCaptureStatusNone) *id = n;
+    return TCQ_OK;
+}
+
 int tcq_device_error(int reset) {
     int v = 0;
     if (cudaMemcpyFromSymbol(&v, g_tcq_device_error, sizeof(int)) != cudaSuccess) return -1;

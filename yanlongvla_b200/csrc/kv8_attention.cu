@@ -1362,6 +1362,7 @@ int launch_many(const AttnArgs& A, void* stream) {
 }
 
 // Arrival counters at the head of the workspace, three per worker of the few-row kernel (its unit, and its two parts' groups).
+// They are what has to be zero before the first call; TCQ_KV8_ZEROED_BYTES holds those of 455 SMs.
 constexpr int kMostWarps = 12;
 inline size_t counter_bytes(int sms) { return ((size_t)3 * kMostWarps * sms * sizeof(int) + 15) & ~(size_t)15; }
 
@@ -1392,6 +1393,7 @@ int tcq_kv8_attention(const tcq_kv8_cache* cache, const void* q, int dtype, int6
     if (B < 1 || T < 1 || blocks < 1 || heads < 1 || heads % Hk || blocks > (0x7fffffff / kBlk)) return TCQ_ERR_SHAPE;
     if ((i64)B * Hk > 0x7fffffff || (i64)B * Hk * (blocks + 1) > 0x7fffffff) return TCQ_ERR_SHAPE;
     if (!tcq_aligned(q, 16) || !tcq_aligned(out, 16) || ((q_sb | q_st) & 7)) return TCQ_ERR_ALIGN;
+    if (counter_bytes(tcq_sm_count()) > TCQ_KV8_ZEROED_BYTES) return TCQ_ERR_DEVICE;
     if (!workspace || workspace_bytes < tcq_kv8_attention_workspace(B, T, heads, Hk, cache->head_dim, blocks)) return TCQ_ERR_WORKSPACE;
     const int sms = tcq_sm_count();
     AttnArgs A = {*cache, (const u16*)q, q_sb, q_st, (u16*)out, table, lens, count, nullptr, (int*)workspace, blocks, causal, B, T, heads,

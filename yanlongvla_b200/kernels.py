@@ -3,7 +3,8 @@
 Mirrors deploy/tcq_kernels/kernels.py of the reference (ForeverBlue816/yanlongvla): the same function names, argument
 meaning and buffer layouts, so callers written against the reference work unchanged. Every call launches on
 torch.cuda.current_stream(), allocates nothing except outputs it is not given and the cached per-stream workspaces of
-gemm_tcq and kv8_attention, and therefore works inside torch.cuda.graph() captures. A non-zero status from the library raises TcqError.
+gemm_tcq and kv8_attention, and therefore works inside torch.cuda.graph() captures (kv8_attention gives each graph a workspace of its
+own, from the graph's memory pool, cleared by a node of the graph). A non-zero status from the library raises TcqError.
 
   pre      x (M, K) BF16/F16/F32 -> q (M, K) int8 and/or q4 (K/4, ld) int32, scale (M,)     (kernels.py:602-606)
   post     acc (M, lda) I32 / F32 / BF16 columns col0.. -> y (M, N) BF16                    (kernels.py:612-615)
@@ -435,7 +436,7 @@ def kv8_attention(q, cache, table, lens, count=None, causal=True, scale=None, ou
 
 _bind.init({name: ctypes.cast(getattr(lib, name), ctypes.c_void_p).value
             for name in ('tcq_status_string', 'tcq_rope_axes', 'tcq_kv8_append', 'tcq_kv8_read', 'tcq_kv8_attention_workspace',
-                         'tcq_kv8_attention')}, TcqError, LAUNCHES, RopeAxes, KV8Cache)
+                         'tcq_kv8_attention', 'tcq_capture_id')}, TcqError, LAUNCHES, RopeAxes, KV8Cache)
 
 
 # ------------------------------------------------------------------------------------------------ trellis weights
