@@ -3,8 +3,8 @@
 Mirrors deploy/tcq_kernels/kernels.py of the reference (ForeverBlue816/yanlongvla): the same function names, argument
 meaning and buffer layouts, so callers written against the reference work unchanged. Every call launches on
 torch.cuda.current_stream(), allocates nothing except outputs it is not given and the cached per-stream workspaces of
-gemm_tcq and kv8_attention, and therefore works inside torch.cuda.graph() captures (kv8_attention gives each graph a workspace of its
-own, from the graph's memory pool, cleared by a node of the graph). A non-zero status from the library raises TcqError.
+gemm_tcq and kv8_attention, and therefore works inside torch.cuda.graph() captures (both give each graph a workspace of its own,
+from the graph's memory pool, cleared by a node of the graph). A non-zero status from the library raises TcqError.
 
   pre      x (M, K) BF16/F16/F32 -> q (M, K) int8 and/or q4 (K/4, ld) int32, scale (M,)     (kernels.py:602-606)
   post     acc (M, lda) I32 / F32 / BF16 columns col0.. -> y (M, N) BF16                    (kernels.py:612-615)
@@ -464,18 +464,31 @@ def gemm_w8(W, q4, s, rs, z):
     _count('gemm_w8')
 
 
-_WS = {}
+_WS = {}                 # (device, stream) -> the stream's workspace
+_WS_CAPTURED = {}        # (device, stream) -> (capture, workspace) of the last capture on the stream
 
 
 def workspace(M, N, device):
     """Zero-filled workspace of tcq_gemm_tcq / tcq_gemm_tcq_tc for the current stream (every call leaves it zero;
-    grown on demand)."""
+    grown on demand). A graph that is being captured gets one of its own, from its memory pool and zero-filled by a node of the
+    graph (one for all its calls): the stream's may be replaced by a later call, and other graphs may run at the same time."""
     need = max(int(lib.tcq_gemm_tcq_workspace(M, N)), int(lib.tcq_gemm_tcq_tc_workspace(M, N)))
     key = (str(device), _stream())
-    ws = _WS.get(key)
+    captured = None
+    if torch.cuda.is_current_stream_capturing():
+        number = ctypes.c_uint64()
+        check(lib.tcq_capture_id(key[1], ctypes.byref(number)), 'tcq_capture_id')
+        captured = number.value
+        ws = _WS_CAPTURED[key][1] if key in _WS_CAPTURED and _WS_CAPTURED[key][0] == captured else None
+    else:
+        ws = _WS.get(key)
+        _WS_CAPTURED.pop(key, None)                  # that capture is over: its memory stays with the graph's pool
     if ws is None or ws.numel() * 4 < need:
         ws = torch.zeros(max(need // 4, 1 << 16), dtype=torch.int32, device=device)
-        _WS[key] = ws
+        if captured is None:
+            _WS[key] = ws
+        else:
+            _WS_CAPTURED[key] = captured, ws
     return ws
 
 
