@@ -3,7 +3,7 @@ without a truth value."""
 import pytest
 import torch
 
-from test_memory_gpu import K, attention_case, gen, i32, make_cache, rope_case  # noqa: F401  (K is the module's fixture)
+from test_memory_gpu import K, attention_case, check_attention, gen, i32, make_cache, rope_case  # noqa: F401  (K is the module's fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -25,3 +25,19 @@ def test_attention_nan_query_stays_in_its_row(K, T, heads, kv_heads, D, n, causa
         assert row.isnan().all()
         row.copy_(want[0, t, h * D:(h + 1) * D])
         assert torch.equal(o, want)
+
+
+@pytest.mark.parametrize('D', [48, 64, 128])
+def test_attention_scores_are_read_before_weights_replace_them(K, D):
+    """The weights of one page of a tile take the place of scores of both pages. With many tiles, most of which move no reference,
+    every run gives the same bits and the definition's values, also next to other work on the device."""
+    lens = [1500, 1411]
+    q, cache, table = attention_case(K, 2, 700, 32, 8, D, lens)
+    want = check_attention(K, q, cache, table, lens)
+    other, a = torch.cuda.Stream(), torch.randn(2048, 2048, device='cuda')
+    for i in range(20):
+        with torch.cuda.stream(other):
+            for _ in range(i % 4):
+                a @ a
+        assert torch.equal(K.kv8_attention(q, cache, table, i32(lens)), want)
+    torch.cuda.synchronize()

@@ -1003,7 +1003,12 @@ k_attention_many(const AttnArgs A, int row_tiles, int tile_rows, int splits) {
             }
             float top = fmaxf(fmaxf(raw[0], raw[1]), fmaxf(raw[2], raw[3]));
             if (!MASKED || top != -INFINITY) top = __fmaf_rn(top, c, bias);
-            if (pair_any(pair_bar, top > m + kSlack || !ok)) {
+            // The pair's barrier stands between this warp's loads of the scores and the other's weights over the same columns:
+            // with a fence on either side it orders them.
+            tc_before();
+            const bool moves = pair_any(pair_bar, top > m + kSlack || !ok);
+            tc_after();
+            if (moves) {
                 // Move the reference up where a score passed it: O and the sum follow. An expired wait is told as a NaN that no
                 // arithmetic makes, so that both warps leave.
                 constexpr u32 gone = 0x7fffdeadu;
