@@ -369,7 +369,7 @@ class GrootStylePolicy(torch.nn.Module):
         c = self.c
         x, d = prefix, None
         if memory is not None:
-            memory.begin_frame()
+            memory.begin_frame(prefix)
             for i, blk in enumerate(self.llm):
                 x, d = blk(x, d, None, memory, i)
             return self.llm_norm(x, d)[1]

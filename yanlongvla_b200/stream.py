@@ -40,9 +40,12 @@ class StreamMemory:
         pos = torch.stack((torch.zeros_like(rows), rows, cols)).to(device)
         self.pos = pos[:, None].expand(3, robots, pos.shape[1]).contiguous()
 
-    def begin_frame(self):
-        """Make room for the next frame: its tokens follow those remembered. On the device but for the check of the capacity."""
+    def begin_frame(self, frame=None):
+        """Make room for the next frame: its tokens follow those remembered. On the device but for the check of the capacity.
+        frame: the (B, T, ...) tensor that the layers will get; one of another batch or length is refused before anything moves."""
         n = self.pos.shape[2]
+        if frame is not None and tuple(frame.shape[:2]) != (self.robots, n):
+            raise K.TcqError(f'StreamMemory: a frame of {self.robots} robots with {n} tokens each expected, got {tuple(frame.shape[:2])}')
         if self.tokens + n > self.max_tokens or self.frames >= self.max_frames:
             raise K.TcqError(f'StreamMemory: a frame of {n} tokens does not fit behind {self.tokens} of {self.max_tokens} tokens, {self.frames} frames')
         if self.frames:
