@@ -4,8 +4,9 @@
     python -m yanlongvla_b200.stream --robots 2 --frames 8 [--llm-layers 24]
 
 runs the policy of `policy` (random weights, synthetic frames) with a memory and prints the time per frame. The kernels:
-rope_axes turns the queries, kv8_append turns and stores the keys and stores the values, kv8_attention reads the cache; all
-lengths and positions live on the device, so a step can be captured in a CUDA graph.
+rope_axes turns the queries, kv8_append turns and stores the keys and stores the values, kv8_attention reads the cache. All
+lengths and positions live on the device, so a step can be captured in a CUDA graph: what a capture records moves them on at each
+replay, and StreamMemory.reserve(), called before each replay, keeps the host's count and checks the capacity.
 """
 import argparse
 
@@ -37,8 +38,17 @@ class StreamMemory:
         i = torch.arange(c.image_tokens, dtype=torch.int32)
         rows = torch.cat([i // side] * c.cameras + [side + torch.arange(c.lang_tokens, dtype=torch.int32)])
         cols = torch.cat([i % side + side * k for k in range(c.cameras)] + [side * c.cameras + torch.arange(c.lang_tokens, dtype=torch.int32)])
-        pos = torch.stack((torch.zeros_like(rows), rows, cols)).to(device)
+        pos = torch.stack((torch.full_like(rows, -1), rows, cols)).to(device)          # begin_frame moves the time on
         self.pos = pos[:, None].expand(3, robots, pos.shape[1]).contiguous()
+
+    def reserve(self):
+        """Count the next frame in on the host; refused where it does not fit. begin_frame calls it, except in a capture, which runs
+        nothing: call it before each replay of a captured step."""
+        n = self.pos.shape[2]
+        if self.tokens + n > self.max_tokens or self.frames >= self.max_frames:
+            raise K.TcqError(f'StreamMemory: a frame of {n} tokens does not fit behind {self.tokens} of {self.max_tokens} tokens, {self.frames} frames')
+        self.frames += 1
+        self.tokens += n
 
     def begin_frame(self, frame=None):
         """Make room for the next frame: its tokens follow those remembered. On the device but for the check of the capacity.
@@ -46,12 +56,9 @@ class StreamMemory:
         n = self.pos.shape[2]
         if frame is not None and tuple(frame.shape[:2]) != (self.robots, n):
             raise K.TcqError(f'StreamMemory: a frame of {self.robots} robots with {n} tokens each expected, got {tuple(frame.shape[:2])}')
-        if self.tokens + n > self.max_tokens or self.frames >= self.max_frames:
-            raise K.TcqError(f'StreamMemory: a frame of {n} tokens does not fit behind {self.tokens} of {self.max_tokens} tokens, {self.frames} frames')
-        if self.frames:
-            self.pos[0] += 1
-        self.frames += 1
-        self.tokens += n
+        if not torch.cuda.is_current_stream_capturing():
+            self.reserve()
+        self.pos[0] += 1
         self.start.copy_(self.lens)
         self.lens += n
 
@@ -67,7 +74,7 @@ class StreamMemory:
         self.tokens = self.frames = 0
         self.lens.zero_()
         self.start.zero_()
-        self.pos[0].zero_()
+        self.pos[0].fill_(-1)
 
     @property
     def bytes(self):
