@@ -41,3 +41,30 @@ def test_attention_scores_are_read_before_weights_replace_them(K, D):
                 a @ a
         assert torch.equal(K.kv8_attention(q, cache, table, i32(lens)), want)
     torch.cuda.synchronize()
+
+
+def odd_rows(x):
+    """x (1, 1, W) as a view whose strides of the two dimensions of size one are odd."""
+    W = x.shape[2]
+    flat = torch.zeros(W + 17, device='cuda', dtype=x.dtype)
+    flat[8:8 + W] = x[0, 0]
+    y = flat[None, None, 8:8 + W]
+    assert y.stride() == (W + 17, W + 17, 1) and (W + 17) % 2 == 1
+    return y
+
+
+def test_strides_of_dimensions_of_size_one_do_not_count(K):
+    """One token of one sequence, cut from a buffer of odd length: the strides that nothing steps by are no reason to refuse it."""
+    g = gen(21)
+    heads, D = 2, 64
+    rope, pos, _ = rope_case(K, D, 3, 1, 1, g, False)
+    k, v = (torch.randn(1, 1, heads * D, device='cuda', generator=g).bfloat16() for _ in range(2))
+    q = torch.randn(1, 1, 4 * heads * D, device='cuda', generator=g).bfloat16()
+    table = i32([[2, 0]])
+    caches = [make_cache(K, 3, heads, D, gen(22)) for _ in range(2)]
+    K.kv8_append(caches[0], k, v, table, i32([70]), rope=rope, pos=pos)
+    K.kv8_append(caches[1], odd_rows(k), odd_rows(v), table, i32([70]), rope=rope, pos=pos)
+    for name in ('k', 'v', 'k_scale', 'v_scale'):
+        assert torch.equal(getattr(caches[0], name), getattr(caches[1], name))
+    assert torch.equal(K.rope_axes(odd_rows(q), pos, rope), K.rope_axes(q, pos, rope))
+    assert torch.equal(K.kv8_attention(odd_rows(q), caches[0], table, i32([71])), K.kv8_attention(q, caches[0], table, i32([71])))

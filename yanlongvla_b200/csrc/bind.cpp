@@ -115,6 +115,9 @@ void done(int status, const char* what, const char* name) {
     if (bad) throw Refused();
 }
 
+// Distance of a dimension's steps in elements; nothing steps along one of size one, whatever stride its tensor states.
+int64_t step(const at::Tensor& t, int dim) { return t.size(dim) > 1 ? t.stride(dim) : 0; }
+
 int extent(const char* what, int64_t n) {
     if (n > INT32_MAX) refuse(what, "a size passes 31 bits");
     return static_cast<int>(n);
@@ -152,7 +155,7 @@ PyObject* rope_axes(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const at::Tensor& out = a[4] == Py_None ? made : tensor(me, a[4], "out");
         rows(me, "out", out, dev);
         if (out.sizes() != x.sizes() || out.scalar_type() != x.scalar_type()) refuse(me, "out must have the shape and type of x");
-        done(f_rope(x.const_data_ptr(), dt, x.stride(0), x.stride(1), out.data_ptr(), out.stride(0), out.stride(1), p, plan, extent(me, B),
+        done(f_rope(x.const_data_ptr(), dt, step(x, 0), step(x, 1), out.data_ptr(), step(out, 0), step(out, 1), p, plan, extent(me, B),
                     extent(me, T), extent(me, W / plan->head_dim), inverse, stream_of(me, dev)),
              "tcq_rope_axes", me);
         if (a[4] == Py_None) return THPVariable_Wrap(made);
@@ -180,7 +183,7 @@ PyObject* kv8_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const int32_t* cp = a[5] == Py_None ? nullptr : ints(me, "count", tensor(me, a[5], "count"), {B}, dev);
         const auto* plan = a[6] == Py_None ? nullptr : handle<tcq_rope_plan>(me, a[6], g_rope_class, dev);
         const int32_t* pp = plan ? ints(me, "pos", tensor(me, a[7], "pos"), {plan->axes, B, T}, dev) : nullptr;
-        done(f_append(c, k.const_data_ptr(), k.stride(0), k.stride(1), v.const_data_ptr(), v.stride(0), v.stride(1), dt, tp, extent(me, blocks), sp,
+        done(f_append(c, k.const_data_ptr(), step(k, 0), step(k, 1), v.const_data_ptr(), step(v, 0), step(v, 1), dt, tp, extent(me, blocks), sp,
                       cp, pp, plan, extent(me, B), extent(me, T), stream_of(me, dev)),
              "tcq_kv8_append", me);
         Py_RETURN_NONE;
@@ -289,7 +292,7 @@ PyObject* kv8_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const int b = extent(me, B), t = extent(me, T), h = extent(me, heads), bl = extent(me, blocks);
         size_t have = 0;
         void* ws = workspace(dev, st, f_workspace(b, t, h, c->kv_heads, c->head_dim, bl), have);
-        done(f_attention(c, q.const_data_ptr(), dt, q.stride(0), q.stride(1), out.data_ptr(), tp, bl, lp, cp, causal, (float)scale, b, t, h, ws,
+        done(f_attention(c, q.const_data_ptr(), dt, step(q, 0), step(q, 1), out.data_ptr(), tp, bl, lp, cp, causal, (float)scale, b, t, h, ws,
                          have, st),
              "tcq_kv8_attention", me);
         if (a[7] == Py_None) return THPVariable_Wrap(made);
