@@ -68,3 +68,16 @@ def test_strides_of_dimensions_of_size_one_do_not_count(K):
         assert torch.equal(getattr(caches[0], name), getattr(caches[1], name))
     assert torch.equal(K.rope_axes(odd_rows(q), pos, rope), K.rope_axes(q, pos, rope))
     assert torch.equal(K.kv8_attention(odd_rows(q), caches[0], table, i32([71])), K.kv8_attention(q, caches[0], table, i32([71])))
+
+
+def test_flags_without_a_truth_value_are_refused(K):
+    """causal and inverse are asked for their truth; an object that has none raises its own error and nothing is launched."""
+    q, cache, table = attention_case(K, 1, 3, 4, 2, 64, [70])
+    rope, pos, _ = rope_case(K, 64, 2, 3, 1, gen(1), False)
+    launches = dict(K.LAUNCHES)
+    with pytest.raises(RuntimeError, match='ambiguous'):
+        K.kv8_attention(q, cache, table, i32([70]), causal=torch.ones(2))
+    with pytest.raises(RuntimeError, match='ambiguous'):
+        K.rope_axes(q, pos, rope, inverse=torch.ones(2))
+    assert K.LAUNCHES == launches
+    assert torch.equal(K.kv8_attention(q, cache, table, i32([70]), causal=1), K.kv8_attention(q, cache, table, i32([70])))

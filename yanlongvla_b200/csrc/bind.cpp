@@ -115,6 +115,13 @@ void done(int status, const char* what, const char* name) {
     if (bad) throw Refused();
 }
 
+// Truth of an argument; what has none raises its own error.
+int flag(PyObject* o) {
+    const int t = PyObject_IsTrue(o);
+    if (t < 0) throw Refused();
+    return t;
+}
+
 // Distance of a dimension's steps in elements; nothing steps along one of size one, whatever stride its tensor states.
 int64_t step(const at::Tensor& t, int dim) { return t.size(dim) > 1 ? t.stride(dim) : 0; }
 
@@ -143,7 +150,7 @@ PyObject* rope_axes(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return guarded(n, 5, [&]() -> PyObject* {
         const char* me = "rope_axes";
         const at::Tensor &x = tensor(me, a[0], "x"), &pos = tensor(me, a[1], "pos");
-        const int inverse = PyObject_IsTrue(a[3]), dev = x.is_cuda() ? x.get_device() : -1;
+        const int inverse = flag(a[3]), dev = x.is_cuda() ? x.get_device() : -1;
         const auto* plan = handle<tcq_rope_plan>(me, a[2], g_rope_class, dev);
         rows(me, "x", x, dev);
         const int64_t B = x.size(0), T = x.size(1), W = x.size(2);
@@ -280,7 +287,7 @@ PyObject* kv8_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const int32_t* tp = ints(me, "table", table, {B, blocks}, dev);
         const int32_t* lp = ints(me, "lens", lens, {B}, dev);
         const int32_t* cp = a[4] == Py_None ? nullptr : ints(me, "count", tensor(me, a[4], "count"), {B}, dev);
-        const int causal = PyObject_IsTrue(a[5]);
+        const int causal = flag(a[5]);
         const double scale = a[6] == Py_None ? 1.0 / std::sqrt((double)D) : PyFloat_AsDouble(a[6]);
         if (scale == -1.0 && PyErr_Occurred()) return nullptr;
         at::Tensor made;
