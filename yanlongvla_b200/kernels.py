@@ -67,6 +67,11 @@ def _cuda(*ts):
             raise TcqError('all tensors must be contiguous CUDA tensors')
 
 
+def _one_device(what, *ts):
+    if any(t.device != ts[0].device for t in ts):
+        raise TcqError(f'{what}: tensors on several devices: {", ".join(str(t.device) for t in ts)}')
+
+
 # ------------------------------------------------------------------------------------------------ activation tables
 _TABLES = {}
 
@@ -361,6 +366,7 @@ class RopeAxes:
 
     def __init__(self, cos, sin, sections, pairs=False):
         _cuda(cos, sin)
+        _one_device('RopeAxes', cos, sin)
         if cos.dtype != torch.float32 or sin.dtype != torch.float32 or cos.dim() != 2 or cos.shape != sin.shape:
             raise TcqError('RopeAxes: cos and sin must be float32 (positions, D / 2)')
         sections = tuple(int(n) for n in sections)
@@ -387,6 +393,7 @@ class KV8Cache:
 
     def __init__(self, k, v, k_scale, v_scale):
         _cuda(k, v, k_scale, v_scale)
+        _one_device('KV8Cache', k, v, k_scale, v_scale)
         pages, heads, _, D = k.shape
         if k.dtype != torch.int8 or v.dtype != torch.int8 or k.shape[2] != KV8_BLOCK or v.shape != (pages, heads, D, KV8_BLOCK):
             raise TcqError(f'KV8Cache: k (pages, heads, {KV8_BLOCK}, D) and v (pages, heads, D, {KV8_BLOCK}) int8')
