@@ -1,4 +1,4 @@
-"""The streaming-memory operators' host side without a GPU: handles over several devices."""
+"""The streaming-memory operators' host side without a GPU: what the handles refuse."""
 import pytest
 import torch
 
@@ -42,3 +42,11 @@ def test_tables_are_on_one_device():
     with pytest.raises(K.TcqError, match='several devices'):
         K.RopeAxes(OnDevice((9, 32), torch.float32, 0), OnDevice((9, 32), torch.float32, 1), (32,))
     assert K.RopeAxes(*(OnDevice((9, 32), torch.float32, 1) for _ in range(2)), (16, 16))._handle.device == 1
+
+
+def test_a_cache_of_another_rank_is_refused():
+    from yanlongvla_b200 import kernels as K
+    k, v, ks, vs = cache_parts((0, 0, 0, 0))
+    for shape in ((3, 64, 64), (3, 2, 1, 64, 64)):
+        with pytest.raises(K.TcqError, match='must be'):
+            K.KV8Cache(OnDevice(shape, torch.int8, 0), v, ks, vs)

@@ -394,6 +394,8 @@ class KV8Cache:
     def __init__(self, k, v, k_scale, v_scale):
         _cuda(k, v, k_scale, v_scale)
         _one_device('KV8Cache', k, v, k_scale, v_scale)
+        if k.dim() != 4:
+            raise TcqError(f'KV8Cache: k must be (pages, heads, {KV8_BLOCK}, D), got {tuple(k.shape)}')
         pages, heads, _, D = k.shape
         if k.dtype != torch.int8 or v.dtype != torch.int8 or k.shape[2] != KV8_BLOCK or v.shape != (pages, heads, D, KV8_BLOCK):
             raise TcqError(f'KV8Cache: k (pages, heads, {KV8_BLOCK}, D) and v (pages, heads, D, {KV8_BLOCK}) int8')
