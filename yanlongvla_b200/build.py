@@ -59,6 +59,7 @@ def build_bind(force=False, verbose=False):
     cuda = Path(os.environ.get('CUDA_HOME', '/usr/local/cuda'))
     libs = cpp_extension.library_paths()
     cmd = [os.environ.get('CXX', 'g++'), '-O2', '-std=c++17', '-fPIC', '-shared', f'-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}',
+           f'-DTCQ_TORCH_VERSION="{torch.__version__}"',
            *(f'-I{p}' for p in cpp_extension.include_paths()), f'-I{cuda / "include"}', f'-I{sysconfig.get_paths()["include"]}',
            f'-I{ROOT / "include"}', str(src), '-o', str(BIND), *(f'-L{p}' for p in libs), *(f'-Wl,-rpath,{p}' for p in libs),
            '-ltorch_python', '-ltorch', '-ltorch_cpu', '-lc10', '-lc10_cuda']
@@ -73,20 +74,19 @@ def build_bind(force=False, verbose=False):
 
 def build(force=False, verbose=False, extra=()):
     OBJ.mkdir(exist_ok=True)
-    build_bind(force, verbose)
     if force:
         for o in OBJ.glob('*.o'):
             o.unlink()
     srcs = sorted(CSRC.glob('*.cu'))
     with ThreadPoolExecutor(max_workers=min(8, len(srcs))) as ex:
         objs = [o for o, _ in ex.map(lambda s: _compile(s, verbose, extra), srcs)]
-    if LIB.exists() and LIB.stat().st_mtime >= max(o.stat().st_mtime for o in objs) and not force:
-        return LIB
-    cmd = [NVCC, *ARCH, '-shared', '-o', str(LIB), *map(str, objs)]
-    r = subprocess.run(cmd, capture_output=True, text=True)
-    if r.returncode:
-        sys.stderr.write(' '.join(cmd) + '\n' + r.stdout + r.stderr)
-        raise RuntimeError('link failed')
+    if force or not LIB.exists() or LIB.stat().st_mtime < max(o.stat().st_mtime for o in objs):
+        cmd = [NVCC, *ARCH, '-shared', '-o', str(LIB), *map(str, objs)]
+        r = subprocess.run(cmd, capture_output=True, text=True)
+        if r.returncode:
+            sys.stderr.write(' '.join(cmd) + '\n' + r.stdout + r.stderr)
+            raise RuntimeError('link failed')
+    build_bind(force, verbose)                       # last: without it all operators but the streaming memory's work
     return LIB
 
 

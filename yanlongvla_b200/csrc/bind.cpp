@@ -341,6 +341,12 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_bind", "Binding of the streaming-
 }  // namespace
 
 PyMODINIT_FUNC PyInit__bind() {
+    if (Py_Version >> 16 != PY_VERSION_HEX >> 16) {
+        PyErr_Format(PyExc_ImportError, "it is built for Python %d.%d", PY_MAJOR_VERSION, PY_MINOR_VERSION);
+        return nullptr;
+    }
     s_ref = PyUnicode_InternFromString("ref");
-    return PyModule_Create(&module);
+    PyObject* m = PyModule_Create(&module);
+    if (m && PyModule_AddStringConstant(m, "torch_version", TCQ_TORCH_VERSION) < 0) Py_CLEAR(m);
+    return m;
 }

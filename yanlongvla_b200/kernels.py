@@ -31,8 +31,26 @@ import ctypes
 
 import torch
 
-from . import _bind, _lib
+from . import _lib
 from ._lib import DT_BF16, DT_F16, DT_F32, DT_I32, TcqError, check, lib
+
+try:
+    from . import _bind
+    if getattr(_bind, 'torch_version', None) != torch.__version__:
+        raise ImportError(f'it is built for PyTorch {getattr(_bind, "torch_version", "?")}, this is {torch.__version__}')
+except ImportError as e:
+    class _bind:
+        """In place of a binding that is not there, or not for this Python and PyTorch: the streaming-memory operators say so when
+        they are called; all others go through the C library alone."""
+        why = f'the binding of the streaming-memory operators cannot be used ({e}): build it with `python -m yanlongvla_b200.build`'
+
+        def _missing(*args):
+            raise ImportError(_bind.why)
+
+        def init(*args):
+            pass
+
+        rope_axes = kv8_append = kv8_read = kv8_attention = _missing
 
 __all__ = ['quantize', 'pre', 'post', 'post3', 'postg', 'pre2', 'mid2', 'mid1', 'mid2_available', 'decode', 'decode_bf16', 'gemm_w8',
            'gemm_tcq', 'gemm_tcq_x', 'gemm_tcq_tc', 'gemmf_tcq', 'gemmf_w8', 'add_norm', 'chain', 'rope', 'workspace',
