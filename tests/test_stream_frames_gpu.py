@@ -94,3 +94,25 @@ def test_a_captured_step_moves_the_memory_on(P, B, captured_at):
         eager.forget()
         graphed.forget()
     assert K.device_error() == 0
+
+
+def test_the_whole_policy_in_a_graph(P, setup):
+    """A chunk with a memory, captured as the first frame: every replay gives the actions of the run outside a graph."""
+    from yanlongvla_b200.stream import StreamMemory
+    c, model = setup
+    eager, graphed = (StreamMemory(c, 1, 4 * c.prefix_tokens) for _ in range(2))
+    held = [t.clone() for t in frames(P, c, 1, 1)[0]]
+    graph = torch.cuda.CUDAGraph()
+    with torch.no_grad():
+        wants = [model(*obs, memory=eager).clone() for obs in frames(P, c, 1, 4)]
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph):
+            actions = model(*held, memory=graphed)
+        for obs, want in zip(frames(P, c, 1, 4), wants):
+            for to, x in zip(held, obs):
+                to.copy_(x)
+            graphed.reserve()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(actions, want)
+    assert torch.equal(graphed.lens, eager.lens) and graphed.tokens == eager.tokens
