@@ -162,6 +162,8 @@ TCQ_HD u32 requant4(u32 w, float ratio) {
 // rows of tokens through shared memory. The block's older tokens are touched only when its scale grows. A CTA passes through a
 // chain of dependent loads (start, tokens and page, positions, tables), so what counts is how many are under way: six CTAs of
 // 128 threads to an SM (4 x 8192 tokens of 8 heads of 128, F16 with rotary: 67 us, 3.0 TB/s; four of them 97 us, four of 256 threads 70 us).
+// Their 80 registers do not hold the turned keys of the wider heads: at head widths 80 and 96 a thread stores 248 (F16) or 380 bytes
+// (BF16) to local memory, at 128 500 or 736, and loads somewhat more; up to 64 at most 16.
 template <int DT, int D>
 __global__ void __launch_bounds__(128, 6) k_kv8_append(tcq_kv8_cache cache, const u16* __restrict__ k, i64 k_sb, i64 k_st,
                                                     const u16* __restrict__ v, i64 v_sb, i64 v_st, const int* __restrict__ table,

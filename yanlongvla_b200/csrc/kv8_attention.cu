@@ -51,7 +51,7 @@ TCQ_HD int page_of(const int* row, int blk, int pages) { return page_in(row[blk]
 
 // ------------------------------------------------------------------------------------------------ few query rows
 // T * group <= 32 query rows share a key head (single tokens, short action sequences; 16 rows above head width 64): the kernel
-// streams the pages once. Bound by HBM for long sequences (4 x 131037 keys of 8 heads of 64: 107 us, 5.0 TB/s), by the latency of a
+// streams the pages once. Bound by HBM for long sequences (4 x 131037 keys of 8 heads of 64: 104 us, 5.1 TB/s), by the latency of a
 // warp's page (about 1.5 us) for short ones (one token over 203 keys: 4.6 us a call).
 //
 // Mathematics. With integers k, v and block scales ks, vs: score x = (q . k) ks scale log2(e) + log2(vs), reference
@@ -60,7 +60,8 @@ TCQ_HD int page_of(const int* row, int blk, int pages) { return page_in(row[blk]
 // when a score passes it by more than 10.5, so the accumulators are rarely rescaled. Operands are FP16, accumulators FP32: an
 // int8 is exact, a query row is scaled by a power of two so that its largest element lies in [2^14, 2^15) (elements below 2^-28
 // of it lose bits, those of BF16 inputs above that lose none), and p <= 2^15.5 keeps 11 bits down to 2^-19 of the reference's
-// and is dropped below 2^-30 of it. BF16 in its place would keep 8 bits of p.
+// and is dropped below 2^-30 of it: with n keys a row is off by at most 2^-11 sum p |v| + 2^-30 n max |v| for it (p normed here;
+// F16 outputs of two 4096-token prompts are 2.8e-4 from 64 bits, 2.1e-4 with FP32 weights). BF16 in its place would keep 8 bits of p.
 //
 // Layout. A warp takes whole pages. S^T = K Q^T and O^T = V^T P^T are m16n8k16 products with the 64 keys (or the D value
 // rows) as rows and NT tiles of 8 queries as columns, so that one token's few queries waste least. The order of a contraction is
@@ -683,14 +684,15 @@ __global__ void __launch_bounds__(Few<D, NT>::WARPS * 32, 1) k_attention_few(con
 //
 // Bound by the softmax warps' chain per tile (about 3,700 clocks at head width 64, 4,000 at 128: scores 500 .. 900, load 200,
 // maximum and barrier 500, weights 1,400 .. 1,950, of which the exponential unit alone needs 2,048 for both groups, handing over
-// and the loop 700), not by the products (1,024 and 2,048 clocks): 2 x 4096 queries of 32 heads of 128, 8 key heads, 4200 keys: 330 us,
-// 880 TFLOP/s; 160 queries over 16411 keys, heads of 64: 61 us. Measured on the way to this shape, same two cases: one thread to a row with two
+// and the loop 700), not by the products (1,024 and 2,048 clocks): 2 x 4096 queries of 32 heads of 128, 8 key heads, 4200 keys: 345 to
+// 351 us, 823 to 838 TFLOP/s; 160 queries over 16411 keys, heads of 64: 60.5 us. Measured on the way to this shape, same two cases: one thread to a row with two
 // passes over the scores 423 and 73 us; products issued from a single-lane branch (130 clocks each instead of 64) 448 and 74;
 // a row per lane for loads and stores of Q and O 376 and 67 us; scores a tile ahead in TMEM columns of their own (heads up to 64)
 // 64 us at the second; an eighth to a third of the exponentials by polynomial: no faster.
 //
 // Few units (a frame of one robot): the tiles of a unit are divided over a cluster of CTAs, which add their parts through
-// distributed shared memory.
+// distributed shared memory. Into how many goes by the table's width, the host's bound on the lengths: a table of another
+// width may add the parts in another order.
 
 constexpr int kTile = 128;            // keys of a tile, rows of a group
 

@@ -457,7 +457,8 @@ def kv8_attention(q, cache, table, lens, count=None, causal=True, scale=None, ou
     """softmax(scale q k^T) v over the cached tokens of each sequence. q (B, T, heads * D) BF16 / F16 with contiguous rows; query
     head h reads key head h // (heads / kv_heads). lens (B,) int32: tokens in the cache, the new ones among them; query t of the
     count[b] (None: T) queries sits at token lens[b] - count[b] + t and, when causal, sees the tokens up to its own. scale None:
-    D^-0.5. Returns out (B, T, heads * D) of q's type; rows that see no token, or past count[b], are zero."""
+    D^-0.5. Returns out (B, T, heads * D) of q's type; rows that see no token, or past count[b], are zero. The same call gives the
+    same bits every time; sums may be formed in another order for a table of another width or another number of sequences."""
     return _bind.kv8_attention(q, cache, table, lens, count, causal, scale, out)
 
 

@@ -17,7 +17,8 @@ from . import kernels as K
 
 class StreamMemory:
     """Caches of every LLM layer for `robots` sequences of up to `max_tokens` tokens. Pages are assigned once: block i of robot b
-    is page b * blocks + i of each layer."""
+    is page b * blocks + i of each layer. Its operators are the kernels in every runtime of the policy, the one of PyTorch
+    operations among them."""
 
     def __init__(self, c, robots, max_tokens, device='cuda', theta=10000.0, max_frames=4096):
         D = c.llm_hidden // c.llm_heads
@@ -25,7 +26,7 @@ class StreamMemory:
         blocks = -(-max_tokens // K.KV8_BLOCK)
         self.caches = [K.KV8Cache.empty(robots * blocks, c.llm_kv_heads, D, device) for _ in range(c.llm_layers)]
         self.table = torch.arange(robots * blocks, dtype=torch.int32, device=device).view(robots, blocks)
-        # half of the frequencies' share for time, the rest split between rows and columns
+        # a quarter of the frequencies for time, the rest split between rows and columns
         time = D // 8
         row = (D // 2 - time + 1) // 2
         side = int(c.image_tokens ** 0.5)
