@@ -267,11 +267,13 @@ def _refer(refs, table, by):
 
 def _plain_branch(s):
     c = s.case
-    # fork: sequence b becomes what parent[b] was
+    # fork: sequence b becomes what parent[b] was, with the pages that hold its tokens
     old, lens = s.table.clone(), s.lens.clone()
     take = s.parent.clamp(min=0).long()
-    s.table.copy_(torch.where(s.parent[:, None] >= 0, old[take], -1))
-    s.lens.copy_(torch.where(s.parent >= 0, lens[take], 0))
+    new_lens = torch.where(s.parent >= 0, lens[take], 0)
+    stays = (s.parent == torch.arange(len(take), device='cuda'))[:, None]
+    s.table.copy_(torch.where(stays, old, torch.where(s.block < (new_lens[:, None] + BLOCK - 1) // BLOCK, old[take], -1)))
+    s.lens.copy_(new_lens)
     _refer(s.refs, old, -1)
     _refer(s.refs, s.table, 1)
     # reserve: pages for the new tokens, and for a begun block that others share
@@ -285,12 +287,12 @@ def _plain_branch(s):
     held = s.refs[at.clamp(min=0).long()]
     own_page = begun & (held == writers) & is_last                                    # the last of them keeps a page no one else names
     copied = begun & ~own_page
-    need = ((s.block >= first[:, None] + begun[:, None].int()) & (s.block < last[:, None]) & (s.count > 0)[:, None]) \
+    need = ((s.block >= first[:, None]) & (s.block < last[:, None]) & (s.table < 0) & (s.count > 0)[:, None]) \
         | ((s.block == first[:, None]) & copied[:, None])
     each = need.sum(1)
     upto = each.cumsum(0)
     free = (s.refs == 0).cumsum(0)
-    fits = (each == 0) | (upto <= free[-1])
+    fits = upto <= free[-1]                                                          # behind a sequence that does not fit, none does
     granted = torch.where(fits, s.count, 0).to(torch.int32)
     need &= fits[:, None]
     copied &= fits
