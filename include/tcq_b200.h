@@ -306,6 +306,40 @@ int tcq_kv8_attention(const tcq_kv8_cache* cache, const void* q, int dtype, int6
                       const int32_t* table, int blocks, const int32_t* lens, const int32_t* count, int causal, float scale,
                       int B, int T, int heads, void* workspace, size_t workspace_bytes, void* stream);
 
+/* Pages of the cache shared by several sequences. refs (pages,) int32 counts the table entries that name a page (0: the page is
+ * free); a row of a table names its sequence's pages from block 0 on and holds -1 behind them. pages is below 2^30, the
+ * sequences of a table number at most TCQ_KV8_MAX_SEQUENCES. Results do not depend on timing. */
+#define TCQ_KV8_MAX_SEQUENCES 8192
+
+/* Sequence b becomes what sequence parent[b] was, all at once: row b names parent[b]'s pages of its lens tokens (pages it had only
+ * reserved are not shared), lens[b] is its length. parent[b] = b: unchanged; below 0: empty. Pages that are named no more become free. */
+int tcq_kv8_fork(int32_t* refs, int pages, int32_t* table, int blocks, int32_t* lens, const int32_t* parent, int B, void* stream);
+
+/* Room for count[b] new tokens behind each sequence's lens[b]: missing pages are taken from the free ones, from the lowest number
+ * on, by sequence and block. A begun block whose page others name too is replaced by a page of its own; copies (2, B) int32 gives the
+ * source and the new page, -1 elsewhere (tcq_kv8_copy moves what they hold). Where the call's own sequences are all that name a
+ * page, the last of them keeps it. granted (B,) int32: count[b], or 0 for a sequence that the free pages do not serve, for
+ * all behind it, and for one that does not fit the table (flag 2); such a sequence is left as it was. lens is only read. */
+int tcq_kv8_reserve(int32_t* refs, int pages, int32_t* table, int blocks, const int32_t* lens, const int32_t* count, int32_t* granted,
+                    int32_t* copies, int B, void* stream);
+
+/* Sequence b keeps its first min(keep[b], lens[b]) tokens and the pages that hold them; lens[b] is lowered to that, the row's other
+ * entries become -1, and pages that are named no more become free. */
+int tcq_kv8_free(int32_t* refs, int pages, int32_t* table, int blocks, int32_t* lens, const int32_t* keep, int B, void* stream);
+
+/* Copy pages in each of `layers` caches (an array in host memory, all of one shape): copies (2, n) int32, page copies[n + i] becomes
+ * what page copies[i] is; a pair with a negative number is passed over. No page may be written by two pairs, nor be read by
+ * one and written by another. */
+#define TCQ_KV8_MAX_LAYERS 64            /* caches that one launch takes */
+int tcq_kv8_copy(const tcq_kv8_cache* caches, int layers, const int32_t* copies, int n, void* stream);
+
+/* Pack tokens into other pages, in each of `layers` caches: token j < kept[b] (NULL: tokens) of a new sequence is token
+ * index[b * tokens + j] of sequence b, in any order. table (B, blocks) and lens name the old tokens, new_table (B, new_blocks) the
+ * pages that are written, none of which may be among those read. A new block's scale is the largest of the scales its tokens
+ * come with, q' = rint(q * (s_old / s)); its unused slots are zero. A number past the sequence gives a token of zeros (flag 2). */
+int tcq_kv8_compact(const tcq_kv8_cache* caches, int layers, const int32_t* table, int blocks, const int32_t* lens, const int32_t* index,
+                    int tokens, const int32_t* kept, const int32_t* new_table, int new_blocks, int B, void* stream);
+
 /* Self-test of the failure path (no counterpart in the reference): one thread waits, through the same bounded wait the
  * tcgen05 kernels use, on a barrier that nothing arrives at; after limit_us (1 .. 1e6) microseconds the wait gives up,
  * raises device error flag 1 and the kernel returns. Nothing faults and the context stays usable. */

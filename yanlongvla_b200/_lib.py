@@ -72,6 +72,11 @@ SIGNATURES = {
     'tcq_kv8_read': [P, P, P, I, P, I, P, P, I, I, P],
     'tcq_kv8_attention_workspace': [I, I, I, I, I, I],
     'tcq_kv8_attention': [P, P, I, L, L, P, P, I, P, P, I, F, I, I, I, P, SZ, P],
+    'tcq_kv8_fork': [P, I, P, I, P, P, I, P],
+    'tcq_kv8_reserve': [P, I, P, I, P, P, P, P, I, P],
+    'tcq_kv8_free': [P, I, P, I, P, P, I, P],
+    'tcq_kv8_copy': [P, I, P, I, P],
+    'tcq_kv8_compact': [P, I, P, I, P, P, I, P, P, I, I, P],
     'tcq_selftest_wait_expiry': [ctypes.c_uint, P],
     'tcq_capture_id': [P, ctypes.POINTER(ctypes.c_uint64)],
     'tcq_device_error': [I],

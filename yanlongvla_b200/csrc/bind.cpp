@@ -24,7 +24,12 @@ decltype(&tcq_kv8_read) f_read;
 decltype(&tcq_kv8_attention_workspace) f_workspace;
 decltype(&tcq_kv8_attention) f_attention;
 decltype(&tcq_capture_id) f_capture;
-PyObject *g_error, *g_launches, *g_rope_class, *g_cache_class, *s_ref;
+decltype(&tcq_kv8_fork) f_fork;
+decltype(&tcq_kv8_reserve) f_reserve;
+decltype(&tcq_kv8_free) f_free;
+decltype(&tcq_kv8_copy) f_copy;
+decltype(&tcq_kv8_compact) f_compact;
+PyObject *g_error, *g_launches, *g_rope_class, *g_cache_class, *g_pages_class, *s_ref, *s_refs;
 
 struct Refused {};                         // a Python error is set
 
@@ -307,11 +312,129 @@ PyObject* kv8_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     });
 }
 
-// init(addresses of the C functions by name, error class, launch counts, RopeAxes, KV8Cache)
+// The reference counts of a KV8Pages (checked when it was made).
+const at::Tensor& refs_of(const char* what, PyObject* o, int dev) {
+    if (!PyObject_TypeCheck(o, reinterpret_cast<PyTypeObject*>(g_pages_class))) {
+        PyErr_Format(PyExc_TypeError, "%s: expected a KV8Pages", what);
+        throw Refused();
+    }
+    PyObject* r = PyObject_GetAttr(o, s_refs);
+    if (!r) throw Refused();
+    Py_DECREF(r);                          // the object keeps it
+    const at::Tensor& t = tensor(what, r, "refs");
+    if (t.dim() != 1) refuse(what, "refs must be a (pages,) tensor");
+    ints(what, "refs", t, {t.size(0)}, dev);
+    return t;
+}
+
+// table (B, blocks), lens (B,) and one more (B,) tensor of ints that come with a KV8Pages.
+struct Rows {
+    int dev, pages, B, blocks;
+    int32_t *refs, *table, *lens;
+    const int32_t* more;
+    at::TensorOptions options;
+};
+Rows paged(const char* what, PyObject* owner, PyObject* table_o, PyObject* lens_o, PyObject* more_o, const char* more) {
+    const at::Tensor &table = tensor(what, table_o, "table"), &lens = tensor(what, lens_o, "lens");
+    const int dev = table.is_cuda() ? table.get_device() : -1;
+    const at::Tensor& refs = refs_of(what, owner, dev);
+    const int64_t B = table.dim() == 2 ? table.size(0) : 0, blocks = table.dim() == 2 ? table.size(1) : 0;
+    ints(what, "table", table, {B, blocks}, dev);
+    ints(what, "lens", lens, {B}, dev);
+    const int32_t* m = ints(what, more, tensor(what, more_o, more), {B}, dev);
+    return {dev, extent(what, refs.size(0)), extent(what, B), extent(what, blocks), refs.data_ptr<int32_t>(), table.data_ptr<int32_t>(),
+            lens.data_ptr<int32_t>(), m, table.options()};
+}
+
+// kv8_fork(pages, table, lens, parent)
+PyObject* kv8_fork(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded(n, 4, [&]() -> PyObject* {
+        const char* me = "kv8_fork";
+        const Rows r = paged(me, a[0], a[1], a[2], a[3], "parent");
+        done(f_fork(r.refs, r.pages, r.table, r.blocks, r.lens, r.more, r.B, stream_of(me, r.dev)), "tcq_kv8_fork", me);
+        Py_RETURN_NONE;
+    });
+}
+
+// kv8_reserve(pages, table, lens, count)
+PyObject* kv8_reserve(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded(n, 4, [&]() -> PyObject* {
+        const char* me = "kv8_reserve";
+        const Rows r = paged(me, a[0], a[1], a[2], a[3], "count");
+        void* st = stream_of(me, r.dev);
+        at::Tensor granted = at::empty({r.B}, r.options), copies = at::empty({2, r.B}, r.options);
+        done(f_reserve(r.refs, r.pages, r.table, r.blocks, r.lens, r.more, granted.data_ptr<int32_t>(), copies.data_ptr<int32_t>(), r.B, st),
+             "tcq_kv8_reserve", me);
+        return Py_BuildValue("(NN)", THPVariable_Wrap(granted), THPVariable_Wrap(copies));
+    });
+}
+
+// kv8_free(pages, table, lens, keep)
+PyObject* kv8_free(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded(n, 4, [&]() -> PyObject* {
+        const char* me = "kv8_free";
+        const Rows r = paged(me, a[0], a[1], a[2], a[3], "keep");
+        done(f_free(r.refs, r.pages, r.table, r.blocks, r.lens, r.more, r.B, stream_of(me, r.dev)), "tcq_kv8_free", me);
+        Py_RETURN_NONE;
+    });
+}
+
+// The C structs of a KV8Cache, or of a list or tuple of them.
+std::vector<tcq_kv8_cache> layers_of(const char* what, PyObject* o, int dev) {
+    std::vector<tcq_kv8_cache> c;
+    if (!PyList_Check(o) && !PyTuple_Check(o)) {
+        c.push_back(*handle<tcq_kv8_cache>(what, o, g_cache_class, dev));
+        return c;
+    }
+    const Py_ssize_t n = PySequence_Fast_GET_SIZE(o);
+    if (n < 1 || n > INT32_MAX) refuse(what, "no cache given");
+    c.reserve(static_cast<size_t>(n));
+    for (Py_ssize_t i = 0; i < n; ++i) c.push_back(*handle<tcq_kv8_cache>(what, PySequence_Fast_GET_ITEM(o, i), g_cache_class, dev));
+    for (const auto& x : c)
+        if (x.pages != c[0].pages || x.kv_heads != c[0].kv_heads || x.head_dim != c[0].head_dim) refuse(what, "the caches must be of one shape");
+    return c;
+}
+
+// kv8_copy(caches, copies)
+PyObject* kv8_copy(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded(n, 2, [&]() -> PyObject* {
+        const char* me = "kv8_copy";
+        const at::Tensor& copies = tensor(me, a[1], "copies");
+        const int dev = copies.is_cuda() ? copies.get_device() : -1;
+        const auto c = layers_of(me, a[0], dev);
+        const int64_t pairs = copies.dim() == 2 ? copies.size(1) : 0;
+        const int32_t* p = ints(me, "copies", copies, {2, pairs}, dev);
+        done(f_copy(c.data(), extent(me, c.size()), p, extent(me, pairs), stream_of(me, dev)), "tcq_kv8_copy", me);
+        Py_RETURN_NONE;
+    });
+}
+
+// kv8_compact(caches, table, lens, index, new_table, kept)
+PyObject* kv8_compact(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded(n, 6, [&]() -> PyObject* {
+        const char* me = "kv8_compact";
+        const at::Tensor &table = tensor(me, a[1], "table"), &lens = tensor(me, a[2], "lens"), &index = tensor(me, a[3], "index"),
+                         &to = tensor(me, a[4], "new_table");
+        const int dev = table.is_cuda() ? table.get_device() : -1;
+        const auto c = layers_of(me, a[0], dev);
+        const int64_t B = table.dim() == 2 ? table.size(0) : 0, blocks = table.dim() == 2 ? table.size(1) : 0;
+        const int64_t M = index.dim() == 2 ? index.size(1) : 0, new_blocks = to.dim() == 2 ? to.size(1) : 0;
+        const int32_t *tp = ints(me, "table", table, {B, blocks}, dev), *lp = ints(me, "lens", lens, {B}, dev),
+                      *ip = ints(me, "index", index, {B, M}, dev), *np = ints(me, "new_table", to, {B, new_blocks}, dev);
+        const int32_t* kp = a[5] == Py_None ? nullptr : ints(me, "kept", tensor(me, a[5], "kept"), {B}, dev);
+        done(f_compact(c.data(), extent(me, c.size()), tp, extent(me, blocks), lp, ip, extent(me, M), kp, np, extent(me, new_blocks),
+                       extent(me, B), stream_of(me, dev)),
+             "tcq_kv8_compact", me);
+        Py_RETURN_NONE;
+    });
+}
+
+// init(addresses of the C functions by name, error class, launch counts, RopeAxes, KV8Cache, KV8Pages)
 PyObject* init(PyObject*, PyObject* args) {
     PyObject* f;
-    if (!PyArg_ParseTuple(args, "O!OO!OO", &PyDict_Type, &f, &g_error, &PyDict_Type, &g_launches, &g_rope_class, &g_cache_class)) return nullptr;
-    for (PyObject* o : {g_error, g_launches, g_rope_class, g_cache_class}) Py_INCREF(o);
+    if (!PyArg_ParseTuple(args, "O!OO!OOO", &PyDict_Type, &f, &g_error, &PyDict_Type, &g_launches, &g_rope_class, &g_cache_class, &g_pages_class))
+        return nullptr;
+    for (PyObject* o : {g_error, g_launches, g_rope_class, g_cache_class, g_pages_class}) Py_INCREF(o);
     auto take = [&](const char* name, auto& fn) {
         PyObject* p = PyDict_GetItemString(f, name);
         void* at = p ? PyLong_AsVoidPtr(p) : nullptr;
@@ -320,7 +443,8 @@ PyObject* init(PyObject*, PyObject* args) {
     };
     if (!take("tcq_status_string", f_status) || !take("tcq_rope_axes", f_rope) || !take("tcq_kv8_append", f_append) || !take("tcq_kv8_read", f_read) ||
         !take("tcq_kv8_attention_workspace", f_workspace) || !take("tcq_kv8_attention", f_attention) ||
-        !take("tcq_capture_id", f_capture)) {
+        !take("tcq_capture_id", f_capture) || !take("tcq_kv8_fork", f_fork) || !take("tcq_kv8_reserve", f_reserve) ||
+        !take("tcq_kv8_free", f_free) || !take("tcq_kv8_copy", f_copy) || !take("tcq_kv8_compact", f_compact)) {
         if (!PyErr_Occurred()) PyErr_SetString(PyExc_KeyError, "a function address is missing");
         return nullptr;
     }
@@ -333,6 +457,11 @@ PyMethodDef methods[] = {
     {"kv8_append", reinterpret_cast<PyCFunction>(kv8_append), METH_FASTCALL, nullptr},
     {"kv8_read", reinterpret_cast<PyCFunction>(kv8_read), METH_FASTCALL, nullptr},
     {"kv8_attention", reinterpret_cast<PyCFunction>(kv8_attention), METH_FASTCALL, nullptr},
+    {"kv8_fork", reinterpret_cast<PyCFunction>(kv8_fork), METH_FASTCALL, nullptr},
+    {"kv8_reserve", reinterpret_cast<PyCFunction>(kv8_reserve), METH_FASTCALL, nullptr},
+    {"kv8_free", reinterpret_cast<PyCFunction>(kv8_free), METH_FASTCALL, nullptr},
+    {"kv8_copy", reinterpret_cast<PyCFunction>(kv8_copy), METH_FASTCALL, nullptr},
+    {"kv8_compact", reinterpret_cast<PyCFunction>(kv8_compact), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
 
@@ -346,6 +475,7 @@ PyMODINIT_FUNC PyInit__bind() {
         return nullptr;
     }
     s_ref = PyUnicode_InternFromString("ref");
+    s_refs = PyUnicode_InternFromString("refs");
     PyObject* m = PyModule_Create(&module);
     if (m && PyModule_AddStringConstant(m, "torch_version", TCQ_TORCH_VERSION) < 0) Py_CLEAR(m);
     return m;

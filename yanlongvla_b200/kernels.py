@@ -26,6 +26,8 @@ Streaming memory (no counterpart in the reference, which recomputes its prefix f
   kv8_append     new keys (turned on the way) and values into a KV8Cache: INT8, one scale per 64 tokens and head, paged
   kv8_read       the values a cache stands for
   kv8_attention  attention over a cache, for single tokens, frames and prompts
+  kv8_fork, kv8_reserve, kv8_free   sequences that share a cache's pages (reference counts in a KV8Pages), pages for new tokens
+  kv8_copy, kv8_compact             pages copied, tokens packed into other pages, in every layer by one launch
 """
 import ctypes
 
@@ -51,11 +53,13 @@ except ImportError as e:
             pass
 
         rope_axes = kv8_append = kv8_read = kv8_attention = _missing
+        kv8_fork = kv8_reserve = kv8_free = kv8_copy = kv8_compact = _missing
 
 __all__ = ['quantize', 'pre', 'post', 'post3', 'postg', 'pre2', 'mid2', 'mid1', 'mid2_available', 'decode', 'decode_bf16', 'gemm_w8',
            'gemm_tcq', 'gemm_tcq_x', 'gemm_tcq_tc', 'gemmf_tcq', 'gemmf_w8', 'add_norm', 'chain', 'rope', 'workspace',
            'selftest_wait_expiry', 'pre_h', 'rotate', 'int_mm', 'int8_gemm', 'int8_gemm_bias', 'device_error', 'gelu_table', 'silu_table', 'act_table',
-           'RopeAxes', 'KV8Cache', 'KV8_BLOCK', 'rope_axes', 'kv8_append', 'kv8_read', 'kv8_attention', 'TcqError', 'LAUNCHES']
+           'RopeAxes', 'KV8Cache', 'KV8_BLOCK', 'rope_axes', 'kv8_append', 'kv8_read', 'kv8_attention', 'KV8Pages', 'kv8_fork', 'kv8_reserve',
+           'kv8_free', 'kv8_copy', 'kv8_compact', 'TcqError', 'LAUNCHES']
 
 _DT = {torch.bfloat16: DT_BF16, torch.float32: DT_F32, torch.float16: DT_F16, torch.int32: DT_I32}
 LAUNCHES = {}            # entry point -> number of calls (launch accounting for the benchmark)
@@ -432,6 +436,25 @@ class KV8Cache:
         return cls(k, torch.zeros(pages, kv_heads, head_dim, KV8_BLOCK, dtype=torch.int8, device=device), s[0], s[1])
 
 
+class KV8Pages:
+    """Which of a cache's pages are in use: refs (pages,) int32 counts the table entries that name a page, 0 is a free page. One KV8Pages
+    serves the caches of all layers that share a table. A table's rows name pages from block 0 on and hold -1 behind them."""
+
+    def __init__(self, refs):
+        _cuda(refs)
+        if refs.dtype != torch.int32 or refs.dim() != 1 or not 1 <= refs.shape[0] < 1 << 30:
+            raise TcqError(f'KV8Pages: refs must be int32 (pages,), got {refs.dtype} {tuple(refs.shape)}')
+        self.refs, self.pages, self.device = refs, refs.shape[0], refs.device
+
+    @classmethod
+    def empty(cls, pages, device='cuda'):
+        return cls(torch.zeros(pages, dtype=torch.int32, device=device))
+
+    def table(self, sequences, blocks):
+        """A table (sequences, blocks) of sequences without pages."""
+        return torch.full((sequences, blocks), -1, dtype=torch.int32, device=self.device)
+
+
 def rope_axes(x, pos, rope, inverse=False, out=None):
     """Rotary embedding with several axes: x (B, T, heads * D) BF16 / F16 / F32 with contiguous rows, pos (axes, B, T) int32
     rows of the tables of `rope` (a RopeAxes). Of each pair a' = a c - b s, b' = a s + b c in FP32, one rounding per operation
@@ -462,9 +485,48 @@ def kv8_attention(q, cache, table, lens, count=None, causal=True, scale=None, ou
     return _bind.kv8_attention(q, cache, table, lens, count, causal, scale, out)
 
 
+def kv8_fork(pages, table, lens, parent):
+    """Sequence b becomes what sequence parent[b] was, all at once and without copying a token: table (B, blocks) and lens (B,) are
+    changed in place, pages (a KV8Pages) counts who names what. parent (B,) int32; parent[b] == b leaves b as it is, a negative
+    one empties it. Pages that were only reserved (behind lens) are not shared. A shared page that is begun is replaced at the next
+    kv8_reserve of one of its sequences: call that before kv8_append."""
+    return _bind.kv8_fork(pages, table, lens, parent)
+
+
+def kv8_reserve(pages, table, lens, count):
+    """Pages for count[b] (B,) int32 new tokens behind each sequence's lens[b], the lowest free ones first; table is filled in. Returns
+    (granted, copies): granted (B,) int32 is count, or 0 for a sequence that the free pages do not serve and for all behind it
+    (those are left as they were; device_error reports flag 2); hand it to kv8_append as its count and add it to lens. copies
+    (2, B) int32 names the begun pages that others share and what replaces them, -1 elsewhere: kv8_copy(caches, copies) moves
+    their contents before the append."""
+    return _bind.kv8_reserve(pages, table, lens, count)
+
+
+def kv8_free(pages, table, lens, keep):
+    """Sequence b keeps its first min(keep[b], lens[b]) tokens (keep (B,) int32; 0: none) and the pages that hold them; table and lens are
+    changed in place, pages that no sequence names any more are free."""
+    return _bind.kv8_free(pages, table, lens, keep)
+
+
+def kv8_copy(caches, copies):
+    """Page copies[1, i] becomes what page copies[0, i] is in every cache of `caches` (a KV8Cache, or a list of them of one shape: the
+    layers); copies (2, n) int32, pairs with a negative number are passed over. No page may be written twice, nor read and written."""
+    return _bind.kv8_copy(caches, copies)
+
+
+def kv8_compact(caches, table, lens, index, new_table, kept=None):
+    """Tokens packed into other pages, in every cache of `caches`: token j < kept[b] (None: all) of a new sequence is token index[b, j]
+    (B, n) int32 of sequence b, in any order; new_table (B, blocks) int32 names the pages that are written, none of which may be
+    among those that table names. A new block's scale is the largest its tokens come with, q' = rint(q * (s_old / s)): a
+    token that comes with that scale keeps its integers, any other is off by at most half of it more. Positions turned into
+    the keys stay what they were. kv8_reserve gives the pages, kv8_free takes the old ones back."""
+    return _bind.kv8_compact(caches, table, lens, index, new_table, kept)
+
+
 _bind.init({name: ctypes.cast(getattr(lib, name), ctypes.c_void_p).value
             for name in ('tcq_status_string', 'tcq_rope_axes', 'tcq_kv8_append', 'tcq_kv8_read', 'tcq_kv8_attention_workspace',
-                         'tcq_kv8_attention', 'tcq_capture_id')}, TcqError, LAUNCHES, RopeAxes, KV8Cache)
+                         'tcq_kv8_attention', 'tcq_capture_id', 'tcq_kv8_fork', 'tcq_kv8_reserve', 'tcq_kv8_free', 'tcq_kv8_copy',
+                         'tcq_kv8_compact')}, TcqError, LAUNCHES, RopeAxes, KV8Cache, KV8Pages)
 
 
 # ------------------------------------------------------------------------------------------------ trellis weights
