@@ -340,6 +340,18 @@ int tcq_kv8_copy(const tcq_kv8_cache* caches, int layers, const int32_t* copies,
 int tcq_kv8_compact(const tcq_kv8_cache* caches, int layers, const int32_t* table, int blocks, const int32_t* lens, const int32_t* index,
                     int tokens, const int32_t* kept, const int32_t* new_table, int new_blocks, int B, void* stream);
 
+/* ------------------------------------------------------------------------------------------------ cross attention
+ * out (B S, T, heads * head_dim) = softmax(scale * q k^T) v over an encoder's states (the action head's attention to the backbone's
+ * features, in the reference a library call of its model code). q (B S, T, heads * head_dim): the S batches b S .. b S + S - 1 read the states of
+ * sequence b, S candidates that share them; k, v (B, N, kv_heads * head_dim); all BF16 or all F16, strides *_sb, *_st in elements (rows
+ * 16-byte aligned; a k_sb or v_sb of 0 shares one batch of states), out contiguous. Query head h reads key head h / (heads /
+ * kv_heads); head_dim is a multiple of 8, at most 128. State j of sequence b is there if j < lens[b] (lens NULL: N) and
+ * mask[b * mask_sb + j] != 0 (mask NULL: yes); what lies in k and v where none is has no effect, NaN neither. Rows that see no
+ * state are zero. Scores, sums and maxima are FP32; weights are rounded to the type once. No workspace; the same call gives the same bits. */
+int tcq_cross_attention(const void* q, int64_t q_sb, int64_t q_st, const void* k, int64_t k_sb, int64_t k_st, const void* v, int64_t v_sb,
+                        int64_t v_st, int dtype, void* out, const int32_t* lens, const uint8_t* mask, int64_t mask_sb, float scale, int B,
+                        int S, int T, int N, int heads, int kv_heads, int head_dim, void* stream);
+
 /* Self-test of the failure path (no counterpart in the reference): one thread waits, through the same bounded wait the
  * tcgen05 kernels use, on a barrier that nothing arrives at; after limit_us (1 .. 1e6) microseconds the wait gives up,
  * raises device error flag 1 and the kernel returns. Nothing faults and the context stays usable. */
@@ -349,7 +361,7 @@ int tcq_selftest_wait_expiry(unsigned limit_us, void* stream);
 int tcq_capture_id(void* stream, unsigned long long* id);
 
 /* Device error flags: 1 = a bounded pipeline wait expired and the kernel stopped early, 2 = a position, page number or
- * length given to a streaming-memory operator was out of range (see there). Synchronizes the current device. reset != 0 clears the flags. Returns -1 if the flags cannot be read. */
+ * length given to a streaming-memory operator or to the cross attention was out of range (see there). Synchronizes the current device. reset != 0 clears the flags. Returns -1 if the flags cannot be read. */
 int tcq_device_error(int reset);
 
 #ifdef __cplusplus

@@ -77,6 +77,7 @@ SIGNATURES = {
     'tcq_kv8_free': [P, I, P, I, P, P, I, P],
     'tcq_kv8_copy': [P, I, P, I, P],
     'tcq_kv8_compact': [P, I, P, I, P, P, I, P, P, I, I, P],
+    'tcq_cross_attention': [P, L, L, P, L, L, P, L, L, I, P, P, P, L, F, I, I, I, I, I, I, I, P],
     'tcq_selftest_wait_expiry': [ctypes.c_uint, P],
     'tcq_capture_id': [P, ctypes.POINTER(ctypes.c_uint64)],
     'tcq_device_error': [I],

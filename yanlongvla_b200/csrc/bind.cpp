@@ -1,4 +1,4 @@
-// Python binding of the streaming-memory entry points (tcq_rope_axes, tcq_kv8_*) of libtcq_b200.so.
+// Python binding of the streaming-memory entry points (tcq_rope_axes, tcq_kv8_*) and of tcq_cross_attention of libtcq_b200.so.
 //
 // These run once per token and layer, and a call's own work takes a few microseconds: the checks of the arguments and the
 // launch are made here rather than through ctypes. The C ABI stays the only interface to the kernels: kernels.py passes the
@@ -29,6 +29,7 @@ decltype(&tcq_kv8_reserve) f_reserve;
 decltype(&tcq_kv8_free) f_free;
 decltype(&tcq_kv8_copy) f_copy;
 decltype(&tcq_kv8_compact) f_compact;
+decltype(&tcq_cross_attention) f_cross;
 PyObject *g_error, *g_launches, *g_rope_class, *g_cache_class, *g_pages_class, *s_ref, *s_refs;
 
 struct Refused {};                         // a Python error is set
@@ -429,6 +430,55 @@ PyObject* kv8_compact(PyObject*, PyObject* const* a, Py_ssize_t n) {
     });
 }
 
+// cross_attention(q, k, v, heads, kv_heads, lens, mask, scale, out)
+PyObject* cross_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded(n, 9, [&]() -> PyObject* {
+        const char* me = "cross_attention";
+        const at::Tensor &q = tensor(me, a[0], "q"), &k = tensor(me, a[1], "k"), &v = tensor(me, a[2], "v");
+        const int64_t heads = PyLong_AsLongLong(a[3]);
+        if (heads == -1 && PyErr_Occurred()) return nullptr;
+        const int64_t kv_heads = a[4] == Py_None ? heads : PyLong_AsLongLong(a[4]);
+        if (kv_heads == -1 && PyErr_Occurred()) return nullptr;
+        const int dev = q.is_cuda() ? q.get_device() : -1;
+        rows(me, "q", q, dev);
+        rows(me, "k", k, dev);
+        rows(me, "v", v, dev);
+        const int64_t B = k.size(0), N = k.size(1), W = q.size(2);
+        if (heads < 1 || kv_heads < 1 || heads % kv_heads || W % heads) refuse(me, "heads must divide q's rows, kv_heads the heads");
+        const int64_t D = W / heads;
+        if (k.size(2) != kv_heads * D) refuse(me, "k's rows are not kv_heads heads of q's width");
+        if (v.sizes() != k.sizes()) refuse(me, "k and v must have the same shape");
+        if (k.scalar_type() != q.scalar_type() || v.scalar_type() != q.scalar_type()) refuse(me, "q, k and v must have one type");
+        if (B < 1 || q.size(0) < 1 || q.size(0) % B) refuse(me, "q must have a multiple of the batches of k and v");
+        const int dt = dtype_code(me, q, false);
+        const int32_t* lp = a[5] == Py_None ? nullptr : ints(me, "lens", tensor(me, a[5], "lens"), {B}, dev);
+        const uint8_t* mp = nullptr;
+        int64_t mask_sb = 0;
+        if (a[6] != Py_None) {
+            const at::Tensor& mask = tensor(me, a[6], "mask");
+            const std::array<int64_t, 2> want{B, N};
+            if (mask.scalar_type() != at::kBool || !mask.is_cuda() || mask.get_device() != dev || mask.sizes() != at::IntArrayRef(want) ||
+                (N > 1 && mask.stride(1) != 1))
+                refuse(me, "mask must be a bool CUDA tensor (B, N) with contiguous rows, on one device with the others");
+            mp = static_cast<const uint8_t*>(mask.const_data_ptr());
+            mask_sb = step(mask, 0);
+        }
+        const double scale = a[7] == Py_None ? 1.0 / std::sqrt((double)D) : PyFloat_AsDouble(a[7]);
+        if (scale == -1.0 && PyErr_Occurred()) return nullptr;
+        at::Tensor made;
+        if (a[8] == Py_None) made = at::empty(q.sizes(), q.options());
+        const at::Tensor& out = a[8] == Py_None ? made : tensor(me, a[8], "out");
+        if (out.sizes() != q.sizes() || out.scalar_type() != q.scalar_type() || !out.is_contiguous() || !out.is_cuda() || out.get_device() != dev)
+            refuse(me, "out must be contiguous and have the shape, type and device of q");
+        done(f_cross(q.const_data_ptr(), step(q, 0), step(q, 1), k.const_data_ptr(), step(k, 0), step(k, 1), v.const_data_ptr(), step(v, 0),
+                     step(v, 1), dt, out.data_ptr(), lp, mp, mask_sb, (float)scale, extent(me, B), extent(me, q.size(0) / B),
+                     extent(me, q.size(1)), extent(me, N), extent(me, heads), extent(me, kv_heads), extent(me, D), stream_of(me, dev)),
+             "tcq_cross_attention", me);
+        if (a[8] == Py_None) return THPVariable_Wrap(made);
+        return Py_NewRef(a[8]);
+    });
+}
+
 // init(addresses of the C functions by name, error class, launch counts, RopeAxes, KV8Cache, KV8Pages)
 PyObject* init(PyObject*, PyObject* args) {
     PyObject* f;
@@ -444,7 +494,8 @@ PyObject* init(PyObject*, PyObject* args) {
     if (!take("tcq_status_string", f_status) || !take("tcq_rope_axes", f_rope) || !take("tcq_kv8_append", f_append) || !take("tcq_kv8_read", f_read) ||
         !take("tcq_kv8_attention_workspace", f_workspace) || !take("tcq_kv8_attention", f_attention) ||
         !take("tcq_capture_id", f_capture) || !take("tcq_kv8_fork", f_fork) || !take("tcq_kv8_reserve", f_reserve) ||
-        !take("tcq_kv8_free", f_free) || !take("tcq_kv8_copy", f_copy) || !take("tcq_kv8_compact", f_compact)) {
+        !take("tcq_kv8_free", f_free) || !take("tcq_kv8_copy", f_copy) || !take("tcq_kv8_compact", f_compact) ||
+        !take("tcq_cross_attention", f_cross)) {
         if (!PyErr_Occurred()) PyErr_SetString(PyExc_KeyError, "a function address is missing");
         return nullptr;
     }
@@ -461,6 +512,7 @@ PyMethodDef methods[] = {
     {"kv8_reserve", reinterpret_cast<PyCFunction>(kv8_reserve), METH_FASTCALL, nullptr},
     {"kv8_free", reinterpret_cast<PyCFunction>(kv8_free), METH_FASTCALL, nullptr},
     {"kv8_copy", reinterpret_cast<PyCFunction>(kv8_copy), METH_FASTCALL, nullptr},
+    {"cross_attention", reinterpret_cast<PyCFunction>(cross_attention), METH_FASTCALL, nullptr},
     {"kv8_compact", reinterpret_cast<PyCFunction>(kv8_compact), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };

@@ -1171,8 +1171,8 @@ int tcq_device_error(int reset) {
         const int z = 0;
         if (cudaMemcpyToSymbol(g_tcq_device_error, &z, sizeof(int)) != cudaSuccess) return -1;
     }
-    const int m = tcq_memory_error(reset), a = tcq_attention_error(reset), p = tcq_pages_error(reset);
-    return m < 0 || a < 0 || p < 0 ? -1 : v | m | a | p;
+    const int m = tcq_memory_error(reset), a = tcq_attention_error(reset), p = tcq_pages_error(reset), c = tcq_cross_error(reset);
+    return m < 0 || a < 0 || p < 0 || c < 0 ? -1 : v | m | a | p | c;
 }
 
 }  // extern "C"

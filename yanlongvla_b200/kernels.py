@@ -28,6 +28,9 @@ Streaming memory (no counterpart in the reference, which recomputes its prefix f
   kv8_attention  attention over a cache, for single tokens, frames and prompts
   kv8_fork, kv8_reserve, kv8_free   sequences that share a cache's pages (reference counts in a KV8Pages), pages for new tokens
   kv8_copy, kv8_compact             pages copied, tokens packed into other pages, in every layer by one launch
+
+Model glue without a kernel of its own in the reference (its model code calls PyTorch):
+  cross_attention  attention to an encoder's states of another length: ragged, masked, shared by several candidates
 """
 import ctypes
 
@@ -44,7 +47,7 @@ except ImportError as e:
     class _bind:
         """In place of a binding that is not there, or not for this Python and PyTorch: the streaming-memory operators say so when
         they are called; all others go through the C library alone."""
-        why = f'the binding of the streaming-memory operators cannot be used ({e}): build it with `python -m yanlongvla_b200.build`'
+        why = f'the binding of the streaming-memory operators and the cross attention cannot be used ({e}): build it with `python -m yanlongvla_b200.build`'
 
         def _missing(*args):
             raise ImportError(_bind.why)
@@ -53,13 +56,13 @@ except ImportError as e:
             pass
 
         rope_axes = kv8_append = kv8_read = kv8_attention = _missing
-        kv8_fork = kv8_reserve = kv8_free = kv8_copy = kv8_compact = _missing
+        kv8_fork = kv8_reserve = kv8_free = kv8_copy = kv8_compact = cross_attention = _missing
 
 __all__ = ['quantize', 'pre', 'post', 'post3', 'postg', 'pre2', 'mid2', 'mid1', 'mid2_available', 'decode', 'decode_bf16', 'gemm_w8',
            'gemm_tcq', 'gemm_tcq_x', 'gemm_tcq_tc', 'gemmf_tcq', 'gemmf_w8', 'add_norm', 'chain', 'rope', 'workspace',
            'selftest_wait_expiry', 'pre_h', 'rotate', 'int_mm', 'int8_gemm', 'int8_gemm_bias', 'device_error', 'gelu_table', 'silu_table', 'act_table',
            'RopeAxes', 'KV8Cache', 'KV8_BLOCK', 'rope_axes', 'kv8_append', 'kv8_read', 'kv8_attention', 'KV8Pages', 'kv8_fork', 'kv8_reserve',
-           'kv8_free', 'kv8_copy', 'kv8_compact', 'TcqError', 'LAUNCHES']
+           'kv8_free', 'kv8_copy', 'kv8_compact', 'cross_attention', 'TcqError', 'LAUNCHES']
 
 _DT = {torch.bfloat16: DT_BF16, torch.float32: DT_F32, torch.float16: DT_F16, torch.int32: DT_I32}
 LAUNCHES = {}            # entry point -> number of calls (launch accounting for the benchmark)
@@ -523,10 +526,20 @@ def kv8_compact(caches, table, lens, index, new_table, kept=None):
     return _bind.kv8_compact(caches, table, lens, index, new_table, kept)
 
 
+def cross_attention(q, k, v, heads, kv_heads=None, lens=None, mask=None, scale=None, out=None):
+    """softmax(scale q k^T) v over an encoder's states. q (B * S, T, heads * D), k, v (B, N, kv_heads * D), all BF16 or all F16, with
+    contiguous rows (column views of wider tensors will do: rows 16-byte aligned); D a multiple of 8, at most 128. The S batches b * S ..
+    of q read the states of sequence b (S candidates that share them); query head h reads key head h // (heads / kv_heads). A
+    state j is there if j < lens[b] ((B,) int32; None: all N) and mask[b, j] ((B, N) bool; None: yes); what lies elsewhere in k
+    and v has no effect. scale None: D^-0.5. Returns out (B * S, T, heads * D) of q's type; rows that see no state are zero. No
+    gradient; the same call gives the same bits every time."""
+    return _bind.cross_attention(q, k, v, heads, kv_heads, lens, mask, scale, out)
+
+
 _bind.init({name: ctypes.cast(getattr(lib, name), ctypes.c_void_p).value
             for name in ('tcq_status_string', 'tcq_rope_axes', 'tcq_kv8_append', 'tcq_kv8_read', 'tcq_kv8_attention_workspace',
                          'tcq_kv8_attention', 'tcq_capture_id', 'tcq_kv8_fork', 'tcq_kv8_reserve', 'tcq_kv8_free', 'tcq_kv8_copy',
-                         'tcq_kv8_compact')}, TcqError, LAUNCHES, RopeAxes, KV8Cache, KV8Pages)
+                         'tcq_kv8_compact', 'tcq_cross_attention')}, TcqError, LAUNCHES, RopeAxes, KV8Cache, KV8Pages)
 
 
 # ------------------------------------------------------------------------------------------------ trellis weights
