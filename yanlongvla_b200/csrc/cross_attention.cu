@@ -4,7 +4,7 @@
 // (B, N) say which states are there. The rows that read one key head of one sequence are its R = S T group queries, token by
 // token, `group` heads to a token: they share every load of K and V.
 #include "memory.cuh"
-#include "tma.cuh"
+#include "tc.cuh"
 
 __device__ int g_tcq_cross_error;
 
@@ -35,12 +35,6 @@ struct CrossArgs {
     float scale_log2;                                     // scale * log2(e)
 };
 
-TCQ_HD float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
 TCQ_HD int states_of(const CrossArgs& A, int b) {
     if (!A.lens) return A.N;
     const int n = A.lens[b];
@@ -63,6 +57,21 @@ __device__ __forceinline__ void tma_load_4d(u32 dst, const CUtensorMap* map, u32
         "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
         "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(w)
         : "memory");
+}
+
+// Scores come as (q k) c with c > 0, so that their order is known before the scaling: a negative scale turns the queries, a scale of zero
+// makes them zero.
+TCQ_HD float score_scale(const CrossArgs& A) { return A.scale_log2 == 0.f ? 1.f : fabsf(A.scale_log2); }
+TCQ_HD u32 query_flip(const CrossArgs& A) { return A.scale_log2 < 0.f ? 0x80008000u : 0u; }
+TCQ_HD u32 query_keep(const CrossArgs& A) { return A.scale_log2 == 0.f ? 0u : ~0u; }
+
+// Two weights, rounded to nearest even (a NaN of any kind stays one); lo in the low half.
+template <int DT>
+TCQ_HD u32 weights2(float lo, float hi) {
+    u32 r;
+    if (DT == TCQ_DT_F16) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
 }
 
 // Weights are 2^(x - m + kRef), m the row's reference, moved only when a score passes it by more than kSlack: below 2^13, so
@@ -106,26 +115,11 @@ struct Rows {
     }
 };
 
-__device__ __forceinline__ void cluster_barrier() {
-    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ u32 peer_addr(u32 addr, u32 rank) {
-    u32 r;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
-    return r;
-}
 __device__ __forceinline__ float peer_ld(u32 addr) {
     float v;
     asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
     return v;
 }
-__device__ __forceinline__ float2 peer_ld2(u32 addr) {
-    float2 v;
-    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
-    return v;
-}
-
 template <int DT, int DP>
 __global__ void __launch_bounds__(kRowWarps * 32, DP <= 64 ? 2 : 1)
 k_cross_rows(const CrossArgs A, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, int wm_log2, int stages,
@@ -210,18 +204,18 @@ k_cross_rows(const CrossArgs A, const __grid_constant__ CUtensorMap kmap, const 
         const int ra = r0 + 16 * wm + g, rc = ra + 8;
         const u16* qa = A.q + row_at(A, b, h, min(ra, A.rows - 1), A.q_sb, A.q_st);
         const u16* qc = A.q + row_at(A, b, h, min(rc, A.rows - 1), A.q_sb, A.q_st);
-        const u32 flip = A.scale_log2 < 0.f ? 0x80008000u : 0u;    // a negative scale turns the queries
+        const u32 flip = query_flip(A), keep = query_keep(A);
 #pragma unroll
         for (int k = 0; k < KS; ++k)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const int d = 16 * k + 8 * e + 2 * t;
-                const bool in = DP % 16 == 0 && d < A.D;
-                q[k][2 * e] = in && ra < r1 ? *reinterpret_cast<const u32*>(qa + d) ^ flip : 0u;
-                q[k][2 * e + 1] = in && rc < r1 ? *reinterpret_cast<const u32*>(qc + d) ^ flip : 0u;
+                const bool in = d < A.D;
+                q[k][2 * e] = in && ra < r1 ? *reinterpret_cast<const u32*>(qa + d) & keep ^ flip : 0u;
+                q[k][2 * e + 1] = in && rc < r1 ? *reinterpret_cast<const u32*>(qc + d) & keep ^ flip : 0u;
             }
     }
-    const float c = fabsf(A.scale_log2);
+    const float c = score_scale(A);
     float o[NT][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < NT; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
@@ -259,12 +253,7 @@ k_cross_rows(const CrossArgs A, const __grid_constant__ CUtensorMap kmap, const 
 #pragma unroll
             for (int n = 1; n < NK; ++n) top[e] = fmaxf(top[e], fmaxf(s[n][2 * e], s[n][2 * e + 1]));
         }
-        if (MASKED) {                                              // c may be zero: -inf stays -inf
-            top[0] = top[0] == -INFINITY ? top[0] : top[0] * c;
-            top[1] = top[1] == -INFINITY ? top[1] : top[1] * c;
-        } else {
-            top[0] *= c, top[1] *= c;
-        }
+        top[0] *= c, top[1] *= c;
         if (__any_sync(0xffffffffu, top[0] > m[0] + kSlack || top[1] > m[1] + kSlack)) {
             float f[2];
 #pragma unroll
@@ -283,10 +272,7 @@ k_cross_rows(const CrossArgs A, const __grid_constant__ CUtensorMap kmap, const 
 #pragma unroll
         for (int n = 0; n < NK; ++n)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float x = MASKED && s[n][e] == -INFINITY ? -INFINITY : __fmaf_rn(s[n][e], c, base[e >> 1]);
-                s[n][e] = ex2(x);
-            }
+            for (int e = 0; e < 4; ++e) s[n][e] = ex2(__fmaf_rn(s[n][e], c, base[e >> 1]));
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
             float sum = 0.f;
@@ -296,8 +282,8 @@ k_cross_rows(const CrossArgs A, const __grid_constant__ CUtensorMap kmap, const 
         }
 #pragma unroll
         for (int k = 0; k < NK / 2; ++k) {
-            const u32 a0 = pack2<DT>(s[2 * k][0], s[2 * k][1]), a1 = pack2<DT>(s[2 * k][2], s[2 * k][3]), a2 = pack2<DT>(s[2 * k + 1][0], s[2 * k + 1][1]),
-                      a3 = pack2<DT>(s[2 * k + 1][2], s[2 * k + 1][3]);
+            const u32 a0 = weights2<DT>(s[2 * k][0], s[2 * k][1]), a1 = weights2<DT>(s[2 * k][2], s[2 * k][3]),
+                      a2 = weights2<DT>(s[2 * k + 1][0], s[2 * k + 1][1]), a3 = weights2<DT>(s[2 * k + 1][2], s[2 * k + 1][3]);
             // what lies where no state is may be anything, NaN too: this lane's keys 16 k + 2 t, + 1 and 8 further
             u32 z0 = 0xffffffffu, z1 = 0xffffffffu;
             if (MASKED) {
@@ -394,6 +380,499 @@ k_cross_rows(const CrossArgs A, const __grid_constant__ CUtensorMap kmap, const 
     if (splits > 1) cluster_barrier();                             // a part may be read until here
 }
 
+// ------------------------------------------------------------------------------------------------ tiles of 128 rows
+// Tensor-core products (tcgen05) on tiles of 128 query rows and 128 states, for many rows over many states. A CTA has two groups
+// of softmax warps, 128 threads each, a row to a thread. ROWS: the groups take 128 rows each of one unit (up to 256 rows of one key
+// head) and every tile of states serves both. Otherwise (up to 128 rows) both groups take the same rows and every other tile each, and
+// their parts are added at the end. Roles:
+//   softmax   scores from TMEM into registers, weights back over the scores (16 bits, 64 of the 128 columns), half a tile at a time;
+//   product   one warp, an elected lane of which issues S = Q K^T (Q, K in shared memory) and O += P V (P in TMEM, V as it lies in
+//             memory: the states along the contraction, MN-major);
+//   load      one warp: which tiles hold a state, their truth values as bits, K and V into a ring of tiles (TMA);
+//   clean     one warp, only where lens or a mask may leave states out: rows of V without a state become zero before a product reads
+//             them (a weight of zero times NaN is NaN). Keys need no such care: their scores are replaced.
+// The groups alternate: while one's weights are formed, the other's products run. A group's S of a tile is issued after its O
+// of the tile before, and a commit covers every product issued before it: scores that have arrived mean that O is complete
+// up to the tile before. The reference m of a row moves only when a score passes it by kSlack; O (in TMEM) is then
+// rescaled by its own row's thread.
+constexpr int kTile = 128;
+
+template <int DP, bool ROWS>
+struct Tiles {
+    static constexpr int ATOMS = (DP + 63) / 64;                       // 64-element columns of a tile
+    static constexpr int TB = ATOMS * kTile * 128;                     // bytes of a tile: a group's queries, keys, values
+    static constexpr int QN = ROWS ? 2 : 1;
+    static constexpr int FIT = (226 * 1024 - QN * TB) / TB, RING = FIT < 8 ? FIT : 8;      // tiles of keys and values on their way
+    static constexpr int THREADS = 11 * 32;                            // eight softmax warps, product, load, clean
+    static constexpr int Q0 = 0, RING0 = QN * TB, BAR0 = RING0 + RING * TB;
+    static constexpr int META = 8;                                     // tiles whose truth values are kept
+    static constexpr int META0 = BAR0 + 288, ML0 = META0 + META * 32;  // m, l of every row
+    static constexpr int BYTES = ML0 + 2 * kTile * 8;
+    static constexpr u32 COLS = 512, S0 = 0, O0 = 256;                 // TMEM columns: scores (128 each), outputs
+    static constexpr int PARTS = 2 * kTile * DP * 4;
+    static_assert(RING >= 5, "two tiles in use, the next keys on their way");
+    static_assert(PARTS <= BAR0 && BYTES <= 227 * 1024, "the parts overlay the tiles");
+};
+// What is kept of a tile: its number (below 0: the end), whether all its states are there, its truth values.
+struct TileMeta {
+    int at, whole, pad[2];
+    u32 bits[4];
+};
+// Barriers, 8 bytes each from BAR0: ring slot i full and empty, values of tile t cleaned (t mod META), of group g scores and weights (two
+// halves), queries, the end.
+enum { TBAR_FULL = 0, TBAR_EMPTY = 8, TBAR_CLEAN = 16, TBAR_S = 24, TBAR_P = 26, TBAR_Q = 30, TBAR_END = 31, TBAR_COUNT = 32 };
+
+template <int DT, int DP, bool ROWS>
+__global__ void __launch_bounds__(Tiles<DP, ROWS>::THREADS, 1)
+k_cross_tiles(const CrossArgs A, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, int row_tiles, int tile_rows,
+              int splits) {
+    typedef Tiles<DP, ROWS> P;
+    constexpr int KS = DP / 16;
+    constexpr u32 IDESC = DT == TCQ_DT_BF16 ? kIdescBf16 : 0u;
+    extern __shared__ __align__(1024) char smem_tiles[];
+    char* const smem = smem_tiles;
+    const u32 sbase = smem_u32(smem), bars = sbase + P::BAR0;
+    u32* tmem_slot = reinterpret_cast<u32*>(smem + P::BAR0 + 8 * TBAR_COUNT);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + P::META0) + 2;      // in the first entry's padding
+    TileMeta* meta = reinterpret_cast<TileMeta*>(smem + P::META0);
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+    constexpr int W_MMA = 8, W_LOAD = 9, W_CLEAN = 10;
+    auto bar = [&](int i) -> u32 { return bars + 8 * i; };
+    auto wait = [&](int i, u32 parity) -> bool { return mbar_wait_suspended(bar(i), parity & 1, abort_flag, &g_tcq_cross_error); };
+    if (tid == 0) {
+        for (int i = 0; i < P::RING; ++i) {
+            mbar_init(bar(TBAR_FULL + i), 1);
+            mbar_init(bar(TBAR_EMPTY + i), 1);
+        }
+        for (int i = 0; i < P::META; ++i) mbar_init(bar(TBAR_CLEAN + i), 1);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(bar(TBAR_S + i), 1);
+            mbar_init(bar(TBAR_P + i), 4);                    // per softmax warp; group and half at 2 g + half
+            mbar_init(bar(TBAR_P + 2 + i), 4);
+        }
+        mbar_init(bar(TBAR_Q), 256);
+        mbar_init(bar(TBAR_END), 1);
+        *abort_flag = 0;
+        mbar_init_fence();
+    }
+    if (warp == W_MMA) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(P::COLS) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_before();
+    __syncthreads();
+    tc_after();
+    const u32 tmem = *tmem_slot;
+    pdl_launch_dependents();
+    pdl_wait();
+
+    // ---- the unit: rows r0 .. r1 - 1 of key head h of sequence b, and this CTA's tiles [k0, k1) of its states
+    const int sp = blockIdx.x % splits, unit = blockIdx.x / splits, rt = unit % row_tiles, bh = unit / row_tiles, b = bh / A.kv_heads,
+              h = bh - b * A.kv_heads;
+    const int r0 = rt * tile_rows, r1 = min(A.rows, r0 + tile_rows);
+    const int len = states_of(A, b), tiles = (len + kTile - 1) / kTile;
+    const int k0 = (int)((i64)tiles * sp / splits), k1 = (int)((i64)tiles * (sp + 1) / splits);
+    const bool parts = splits > 1 || !ROWS;                   // rows have more than one part
+    const bool ragged = A.lens || A.mask;
+
+    if (warp < W_MMA) {
+        // ------------------------------------------------------------------------------------------------ softmax
+        const int g = warp >> 2, gl = tid & 127, row = ROWS ? g * kTile + gl : gl;
+        const bool idle = r0 + (row & ~31) >= r1;             // a warp without a row only keeps the barriers going
+        const float c = score_scale(A);
+        if (k1 > k0) {
+            // Queries to shared memory: SEG lanes to a row, 16 bytes each
+            constexpr int SEG = DP <= 32 ? 4 : DP <= 64 ? 8 : 16, RPP = 32 / SEG, WROWS = ROWS ? 32 : 16, NP = WROWS / RPP;
+            const int sl = lane % SEG, first = warp * WROWS;
+            const u32 flip = query_flip(A), keep = query_keep(A);
+            uint4 w[NP];
+#pragma unroll
+            for (int n = 0; n < NP; ++n) {
+                const int rr = r0 + first + n * RPP + lane / SEG;
+                w[n] = make_uint4(0, 0, 0, 0);
+                if (rr < r1 && 8 * sl < A.D) {
+                    w[n] = *reinterpret_cast<const uint4*>(A.q + row_at(A, b, h, rr, A.q_sb, A.q_st) + 8 * sl);
+                    w[n].x = w[n].x & keep ^ flip, w[n].y = w[n].y & keep ^ flip, w[n].z = w[n].z & keep ^ flip, w[n].w = w[n].w & keep ^ flip;
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < NP; ++n) {
+                const int q = first + n * RPP + lane / SEG, qg = q >> 7, qr = q & 127;
+                if (8 * sl < DP)
+                    *reinterpret_cast<uint4*>(smem + P::Q0 + qg * P::TB + (sl >> 3) * (kTile * 128) + qr * 128 + (((sl & 7) ^ (qr & 7)) << 4)) = w[n];
+            }
+            async_proxy_fence();
+        }
+        mbar_arrive(bar(TBAR_Q));
+        const u32 lanes = (u32)((warp & 3) * 32) << 16, ts = tmem + lanes + P::S0 + g * kTile, to = tmem + lanes + P::O0 + g * kTile;
+        float m = -INFINITY, l = 0.f;
+        // One tile: 128 scores of this thread's row, their largest, weights over them. Nothing of the scores is read after the first
+        // store; the product of a half is issued when its four warps have handed it over.
+        auto tile = [&](auto masked_c, int i, const u32 (&bits)[4]) {
+            constexpr bool MASKED = decltype(masked_c)::value;
+            u32 v[4][32];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) tmem_ld32(ts + 32 * j, v[j]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) tmem_ld_wait(v[j]);
+            if (MASKED) {
+#pragma unroll
+                for (int j = 0; j < 128; ++j)
+                    if (!(bits[j >> 5] >> (j & 31) & 1)) v[j >> 5][j & 31] = 0xff800000u;
+            }
+            float raw[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int j = 0; j < 128; j += 2)
+                raw[(j >> 1) & 3] = max3(raw[(j >> 1) & 3], __uint_as_float(v[j >> 5][j & 31]), __uint_as_float(v[j >> 5][(j & 31) + 1]));
+            float top = fmaxf(fmaxf(raw[0], raw[1]), fmaxf(raw[2], raw[3]));
+            top *= c;
+            if (__any_sync(0xffffffffu, top > m + kSlack)) {
+                const bool move = top > m + kSlack;
+                const float f = move ? ex2(m - top) : 1.f;
+                if (move) m = top;
+                l *= f;
+                if (i > 0) {
+#pragma unroll 1
+                    for (int d = 0; d < DP; d += 16) {
+                        u32 o[2][8];
+                        tmem_ld8(to + d, o[0]);
+                        tmem_ld8(to + d + 8, o[1]);
+                        tmem_ld_wait(o[0]);
+                        tmem_ld_wait(o[1]);
+#pragma unroll
+                        for (int j = 0; j < 8; ++j)
+                            o[0][j] = __float_as_uint(__uint_as_float(o[0][j]) * f), o[1][j] = __float_as_uint(__uint_as_float(o[1][j]) * f);
+                        tmem_st8(to + d, o[0]);
+                        tmem_st8(to + d + 8, o[1]);
+                    }
+                }
+            }
+            const float base = kRef - (m == -INFINITY ? 0.f : m);
+            const u64 c2 = pair(c, c), a2 = pair(base, base);
+            u64 sum[2] = {0, 0};
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                u32 w[16];
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    const u32 x = v[q][2 * j], y = v[q][2 * j + 1];
+                    float lo, hi;
+                    unpair(fma2(pair(__uint_as_float(x), __uint_as_float(y)), c2, a2), lo, hi);
+                    lo = ex2(lo), hi = ex2(hi);
+                    sum[j & 1] = add2(sum[j & 1], pair(lo, hi));
+                    w[j] = weights2<DT>(lo, hi);
+                }
+                tmem_st16(ts + 16 * q, w);
+                if (q & 1) {
+                    tmem_st_wait();
+                    tc_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(bar(TBAR_P + 2 * g + (q >> 1)));
+                }
+            }
+            float lo, hi;
+            unpair(add2(sum[0], sum[1]), lo, hi);
+            l += lo + hi;
+        };
+        bool ok = true;
+        for (int i = 0; k1 > k0; ++i) {
+            ok = wait(TBAR_S + g, i);
+            tc_after();
+            if (!ok) break;
+            const TileMeta& t = meta[(ROWS ? i : 2 * i + g) & (P::META - 1)];
+            const int4 head = *reinterpret_cast<const int4*>(&t);
+            if (head.x < 0) break;
+            if (idle) {
+                if (lane == 0) mbar_arrive(bar(TBAR_P + 2 * g)), mbar_arrive(bar(TBAR_P + 2 * g + 1));
+                continue;
+            }
+            u32 bits[4] = {};
+            if (head.y) {
+                tile(std::false_type(), i, bits);
+            } else {
+                const uint4 w = *reinterpret_cast<const uint4*>(t.bits);
+                bits[0] = w.x, bits[1] = w.y, bits[2] = w.z, bits[3] = w.w;
+                tile(std::true_type(), i, bits);
+            }
+        }
+        // every product has ended: the rows' outputs, or their parts, over the tiles, 16-byte pieces permuted within a row
+        const bool got = ok && l != 0.f;
+        const float f = parts ? 1.f : got ? 1.f / l : 0.f;
+        if (parts) asm volatile("barrier.cta.sync 15, 256;" ::: "memory");
+        constexpr int XP = (DP / 4) % 8 == 0 ? 7 : 3, XO = (DP / 8) % 8 == 0 ? 7 : (DP / 8) % 4 == 0 ? 3 : 1;
+        if (!idle) {
+#pragma unroll 1
+            for (int d = 0; d < DP; d += 8) {
+                u32 o[8] = {};
+                if (ok && k1 > k0) {
+                    tmem_ld8(to + d, o);
+                    tmem_ld_wait(o);
+                }
+                float y[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) y[j] = got ? __uint_as_float(o[j]) * f : 0.f;
+                if (parts) {
+                    float4* part = reinterpret_cast<float4*>(smem) + (g * kTile + gl) * (DP / 4);
+                    part[(d / 4) ^ (gl & XP)] = make_float4(y[0], y[1], y[2], y[3]);
+                    part[(d / 4 + 1) ^ (gl & XP)] = make_float4(y[4], y[5], y[6], y[7]);
+                } else {
+                    reinterpret_cast<uint4*>(smem + P::Q0 + g * P::TB)[gl * (DP / 8) + ((d / 8) ^ (gl & XO))] =
+                        make_uint4(pack2<DT>(y[0], y[1]), pack2<DT>(y[2], y[3]), pack2<DT>(y[4], y[5]), pack2<DT>(y[6], y[7]));
+                }
+            }
+        }
+        if (parts) {
+            reinterpret_cast<float2*>(smem + P::ML0)[g * kTile + gl] = make_float2(ok && !idle ? m : -INFINITY, ok && !idle ? l : 0.f);
+        } else if (!idle) {
+            __syncwarp();
+            const int w0 = gl & ~31, rows = min(32, r1 - r0 - (row & ~31)), pieces = A.D / 8;
+            for (int e = lane; e < rows * pieces; e += 32) {
+                const int rr = e / pieces, ch = e - rr * pieces;
+                u16* dst = A.out + row_at(A, b, h, r0 + (row & ~31) + rr, (i64)A.T * A.heads * A.D, (i64)A.heads * A.D);
+                reinterpret_cast<uint4*>(dst)[ch] =
+                    reinterpret_cast<const uint4*>(smem + P::Q0 + g * P::TB)[(w0 + rr) * (DP / 8) + (ch ^ ((w0 + rr) & XO))];
+            }
+        }
+    } else if (k1 > k0 && warp == W_LOAD) {
+        // ------------------------------------------------------------------------------------------------ load
+        // Item 2 t of the ring is the keys of the t-th tile that holds a state, item 2 t + 1 its values.
+        const unsigned char* mrow = A.mask ? A.mask + b * A.mask_sb : nullptr;
+        unsigned char mb[4] = {};
+        auto look = [&](int i) {
+            if (mrow && i < k1)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) mb[j] = i * kTile + 32 * j + lane < len ? mrow[i * kTile + 32 * j + lane] : 0;
+        };
+        look(k0);
+        bool ok = true;
+        int t = 0;
+        auto slot_free = [&](int item) { return item < P::RING || wait(TBAR_EMPTY + item % P::RING, item / P::RING - 1); };
+        for (int i = k0; i < k1 && ok; ++i) {
+            u32 bits[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int n = len - i * kTile - 32 * j;
+                bits[j] = mrow ? __ballot_sync(0xffffffffu, mb[j] != 0) : n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u;
+            }
+            look(i + 1);
+            if (!(bits[0] | bits[1] | bits[2] | bits[3])) continue;
+            const bool whole = (bits[0] & bits[1] & bits[2] & bits[3]) == 0xffffffffu;
+            ok = slot_free(2 * t);
+            if (ok && lane == 0) {
+                TileMeta& e = meta[t & (P::META - 1)];
+                e.at = i, e.whole = whole;
+                e.bits[0] = bits[0], e.bits[1] = bits[1], e.bits[2] = bits[2], e.bits[3] = bits[3];
+            }
+            for (int vals = 0; vals < 2 && ok; ++vals) {
+                const int item = 2 * t + vals, s = item % P::RING;
+                if (vals) ok = slot_free(item);
+                if (ok && lane == 0) {
+                    mbar_expect_tx(bar(TBAR_FULL + s), P::TB);
+#pragma unroll
+                    for (int a = 0; a < P::ATOMS; ++a)
+                        tma_load_4d(sbase + P::RING0 + s * P::TB + a * (kTile * 128), vals ? &vmap : &kmap, bar(TBAR_FULL + s), 64 * a, i * kTile, h,
+                                    b * (vals ? A.vb : A.kb));
+                }
+                __syncwarp();
+            }
+            if (ok) ++t;
+        }
+        // the end, for the product and clean warps: in place of the next keys (and, where the groups take turns, of those behind them)
+        for (int e = 0; e < (ROWS ? 1 : 2) && ok; ++e) {
+            ok = slot_free(2 * (t + e)) && slot_free(2 * (t + e) + 1);
+            if (ok && lane == 0) {
+                meta[(t + e) & (P::META - 1)].at = -1;
+                mbar_arrive(bar(TBAR_FULL + 2 * (t + e) % P::RING));
+                mbar_arrive(bar(TBAR_FULL + (2 * (t + e) + 1) % P::RING));
+            }
+            __syncwarp();
+        }
+        if (*abort_flag) {                                    // copies on their way land before the CTA ends
+            volatile int never = 0;
+            for (int item = max(0, 2 * t - P::RING); item < 2 * t; ++item)
+                mbar_wait_suspended(bar(TBAR_FULL + item % P::RING), (item / P::RING) & 1, &never, &g_tcq_cross_error, kWaitNs / 20);
+        }
+    } else if (k1 > k0 && warp == W_CLEAN && ragged) {
+        // ------------------------------------------------------------------------------------------------ clean
+        for (int t = 0;; ++t) {
+            const int item = 2 * t + 1, s = item % P::RING;
+            if (!wait(TBAR_FULL + s, item / P::RING)) break;
+            const TileMeta& e = meta[t & (P::META - 1)];
+            if (e.at < 0) break;
+            if (!e.whole) {
+                char* v = smem + P::RING0 + s * P::TB;
+                for (int j = 0; j < kTile; j += 4) {
+                    const int key = j + (lane >> 3);             // eight lanes to a row of 128 bytes
+                    if (!(e.bits[key >> 5] >> (key & 31) & 1))
+#pragma unroll
+                        for (int a = 0; a < P::ATOMS; ++a) *reinterpret_cast<uint4*>(v + a * (kTile * 128) + key * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
+                }
+                async_proxy_fence();
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(TBAR_CLEAN + (t & (P::META - 1))));
+        }
+    } else if (k1 > k0 && warp == W_MMA) {
+        // ------------------------------------------------------------------------------------------------ product
+        const u64 qd = sw128_desc(sbase + P::Q0), kd = sw128_desc(sbase + P::RING0), vd = sw128_desc_mn(sbase + P::RING0, kTile * 128);
+        constexpr u32 atom = kTile * 128 / 16, tb = P::TB >> 4;
+        bool ended[2] = {false, false};
+        // S of group g's i-th tile; false: there is none, or a wait expired
+        bool ok = true;
+        auto scores = [&](int g, int i) {
+            const int t = ROWS ? i : 2 * i + g, item = 2 * t, s = item % P::RING;
+            ok = ok && wait(TBAR_FULL + s, item / P::RING);
+            if (!ok) return;
+            if (meta[t & (P::META - 1)].at < 0) {
+                ended[g] = true;
+                return;
+            }
+            tc_after();
+            if (elect_one()) {
+                const u64 a = qd + (u32)((ROWS ? g : 0) * tb), bb = kd + (u32)(s * tb);
+#pragma unroll
+                for (int k = 0; k < KS; ++k)
+                    mma_ss(tmem + P::S0 + g * kTile, a + ((k >> 2) * atom + 2 * (k & 3)), bb + ((k >> 2) * atom + 2 * (k & 3)), idesc_f16(kTile) | IDESC, k > 0);
+                mma_commit(bar(TBAR_S + g));
+                if (!ROWS || g == 1) mma_commit(bar(TBAR_EMPTY + s));
+            }
+            __syncwarp();
+        };
+        auto outputs = [&](int g, int i) {
+            const int t = ROWS ? i : 2 * i + g, item = 2 * t + 1, s = item % P::RING;
+            ok = ok && (ragged ? wait(TBAR_CLEAN + (t & (P::META - 1)), t / P::META) : wait(TBAR_FULL + s, item / P::RING));
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                ok = ok && wait(TBAR_P + 2 * g + half, i);
+                if (!ok) return;
+                tc_after();
+                if (elect_one()) {
+#pragma unroll
+                    for (int k = 4 * half; k < 4 * half + 4; ++k)
+                        mma_ts(tmem + P::O0 + g * kTile, tmem + P::S0 + g * kTile + 8 * k, vd + (u32)(s * tb + k * (16 * 128 / 16)), idesc_f16(DP) | IDESC | kIdescBAlongN,
+                               k > 0 ? 1u : (u32)(i > 0));
+                }
+                __syncwarp();
+            }
+            if (!ROWS || g == 1) {
+                if (elect_one()) mma_commit(bar(TBAR_EMPTY + s));
+                __syncwarp();
+            }
+        };
+        ok = wait(TBAR_Q, 0);
+        scores(0, 0);
+        scores(1, 0);
+        for (int i = 0; ok && !(ended[0] && ended[1]); ++i)
+#pragma unroll
+            for (int g = 0; g < 2; ++g)
+                if (ok && !ended[g]) {
+                    outputs(g, i);
+                    scores(g, i + 1);
+                }
+        // The end of both groups: complete when every product is. After an expired wait too, products in flight end before TMEM is
+        // freed.
+        if (elect_one()) mma_commit(bar(TBAR_S)), mma_commit(bar(TBAR_S + 1)), mma_commit(bar(TBAR_END));
+        __syncwarp();
+        if (!ok) {
+            volatile int never = 0;
+            mbar_wait_suspended(bar(TBAR_END), 0, &never, &g_tcq_cross_error);
+        }
+    }
+    tc_before();
+    __syncthreads();
+    tc_after();
+    if (warp == W_MMA) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(P::COLS) : "memory");
+    if (!parts) return;
+
+    // ---- parts are added: those of the two groups where they share rows, those of a cluster's CTAs, each CTA a slice of the rows
+    if (splits > 1) cluster_barrier();
+    {
+        constexpr int XP = (DP / 4) % 8 == 0 ? 7 : 3;
+        const int rows = r1 - r0, s0 = rows * sp / splits, s1 = rows * (sp + 1) / splits, pieces = A.D / 8;
+        for (int e = tid; e < (s1 - s0) * pieces; e += P::THREADS) {
+            const int row = s0 + e / pieces, c8 = e % pieces;
+            float top = -INFINITY;
+            for (int k = 0; k < splits; ++k)
+#pragma unroll
+                for (int g = 0; g < (ROWS ? 1 : 2); ++g) top = fmaxf(top, peer_ld2(peer_addr(sbase + P::ML0 + (g * kTile + row) * 8, k)).x);
+            float acc[8] = {}, sum = 0.f;
+            for (int k = 0; k < splits; ++k)
+#pragma unroll
+                for (int g = 0; g < (ROWS ? 1 : 2); ++g) {
+                    const float2 ml = peer_ld2(peer_addr(sbase + P::ML0 + (g * kTile + row) * 8, k));
+                    const float f = top == -INFINITY ? (ml.y == ml.y ? 0.f : 1.f) : ex2(ml.x - top);
+                    // a part without weight adds nothing, unless its sum is NaN: the row has to say so
+                    if (f == 0.f && ml.y == ml.y) continue;
+                    sum += ml.y * f;
+                    const u32 base = peer_addr(sbase, k) + (g * kTile + row) * (DP * 4);
+                    const float4 u = peer_ld4(base + (((2 * c8) ^ (row & XP)) << 4)), v = peer_ld4(base + (((2 * c8 + 1) ^ (row & XP)) << 4));
+                    acc[0] += u.x * f, acc[1] += u.y * f, acc[2] += u.z * f, acc[3] += u.w * f;
+                    acc[4] += v.x * f, acc[5] += v.y * f, acc[6] += v.z * f, acc[7] += v.w * f;
+                }
+            const float f = sum != 0.f ? 1.f / sum : 0.f;
+            u32 w[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[j] = sum != 0.f ? pack2<DT>(acc[2 * j] * f, acc[2 * j + 1] * f) : 0u;
+            u16* dst = A.out + row_at(A, b, h, r0 + row, (i64)A.T * A.heads * A.D, (i64)A.heads * A.D) + 8 * c8;
+            *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+    }
+    if (splits > 1) cluster_barrier();                        // a part may be read until here
+}
+
+template <int DT, int DP, bool ROWS>
+int launch_tiles(const CrossArgs& A, const CUtensorMap& km, const CUtensorMap& vm, void* stream) {
+    typedef Tiles<DP, ROWS> P;
+    const auto kern = k_cross_tiles<DT, DP, ROWS>;
+    const int most = ROWS ? 2 * kTile : kTile, row_tiles = (A.rows + most - 1) / most;
+    const int tile_rows = (((A.rows + row_tiles - 1) / row_tiles) + 31) & ~31;     // even shares, in warps
+    const i64 units = (i64)A.B * A.kv_heads * row_tiles;
+    cudaLaunchConfig_t cfg = {};
+    cfg.blockDim = dim3(P::THREADS);
+    cfg.dynamicSmemBytes = P::BYTES;
+    cfg.stream = (cudaStream_t)stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    // what a device can hold of clusters of 1 .. 8 CTAs, asked once per device
+    static std::atomic<int> held[64][9];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev > 63) return TCQ_ERR_DEVICE;
+    if (!held[dev][1].load(std::memory_order_acquire)) {
+        if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, P::BYTES) != cudaSuccess) return TCQ_ERR_LAUNCH;
+        for (int s = 8; s >= 1; --s) {
+            int n = 0;
+            cfg.gridDim = dim3(s);
+            attr[0].val.clusterDim.x = s;
+            cfg.numAttrs = 1;
+            if (s == 1) n = tcq_sm_count();
+            else if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess) n = 0, cudaGetLastError();
+            held[dev][s].store(n, std::memory_order_release);
+        }
+    }
+    // Units that do not fill the device share their tiles among the CTAs of a cluster: the split with the least rounds of
+    // tiles, at least two tiles to a group of a CTA.
+    int splits = 1;
+    const i64 tiles = ((i64)A.N + kTile - 1) / kTile;
+    if (units < held[dev][1].load(std::memory_order_relaxed)) {
+        double best = 1e30;
+        for (int s = 1; s <= 8 && (s == 1 || (ROWS ? 2 : 4) * s <= tiles); ++s) {
+            const int n = held[dev][s].load(std::memory_order_relaxed);
+            if (n <= 0) continue;
+            const double cost = (double)((units + n - 1) / n) / s * (1 + 0.02 * (s - 1));
+            if (cost < best) best = cost, splits = s;
+        }
+    }
+    if (units * splits > 0x7fffffff) return TCQ_ERR_SHAPE;
+    cfg.gridDim = dim3((unsigned)(units * splits));
+    attr[0].val.clusterDim.x = splits;
+    cfg.numAttrs = 2;
+    return cudaLaunchKernelEx(&cfg, kern, A, km, vm, row_tiles, tile_rows, splits) == cudaSuccess ? TCQ_OK : TCQ_ERR_LAUNCH;
+}
+
 // Zeros for queries without states (N = 0).
 __global__ void __launch_bounds__(256) k_cross_none(uint4* out, i64 n) {
     pdl_launch_dependents();
@@ -487,7 +966,9 @@ int tcq_cross_attention(const void* q, int64_t q_sb, int64_t q_st, const void* k
     // sequences that share one batch of states (stride 0) have one in the tensor map
     if (B == 1) k_sb = v_sb = 0;
     CUtensorMap km, vm;
-    const int box = by_width(head_dim, [](auto d) { return Rows<decltype(d)::value>::CHUNK; });
+    // few rows or few states: products of 16 rows; else tiles of 128 rows and 128 states
+    const bool tiles = rows > 32 && N >= 512;
+    const int box = tiles ? kTile : by_width(head_dim, [](auto d) { return Rows<decltype(d)::value>::CHUNK; });
     if (!encode(&km, k, dtype, head_dim, N, kv_heads, B, k_st, k_sb, box) || !encode(&vm, v, dtype, head_dim, N, kv_heads, B, v_st, v_sb, box))
         return TCQ_ERR_DEVICE;
     const int group = heads / kv_heads;
@@ -495,6 +976,10 @@ int tcq_cross_attention(const void* q, int64_t q_sb, int64_t q_st, const void* k
                          k_sb != 0, v_sb != 0, make_fastdiv((unsigned)group), make_fastdiv((unsigned)T), scale * 1.4426950408889634f};
     return by_width(head_dim, [&](auto d) {
         constexpr int DP = decltype(d)::value;
+        if (tiles) {
+            if (dtype == TCQ_DT_BF16) return rows <= kTile ? launch_tiles<TCQ_DT_BF16, DP, false>(A, km, vm, stream) : launch_tiles<TCQ_DT_BF16, DP, true>(A, km, vm, stream);
+            return rows <= kTile ? launch_tiles<TCQ_DT_F16, DP, false>(A, km, vm, stream) : launch_tiles<TCQ_DT_F16, DP, true>(A, km, vm, stream);
+        }
         return dtype == TCQ_DT_BF16 ? launch_rows<TCQ_DT_BF16, DP>(A, km, vm, stream) : launch_rows<TCQ_DT_F16, DP>(A, km, vm, stream);
     });
 }
