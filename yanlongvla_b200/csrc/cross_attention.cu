@@ -80,11 +80,14 @@ constexpr float kRef = 5.f, kSlack = 8.f;
 
 // ------------------------------------------------------------------------------------------------ products of 16 rows
 // Warps of 16 query rows on m16n8k16 products, for few rows or few states: bound by HBM where the states are many, by latency where
-// they are few. A CTA of eight warps takes WM groups of 16 rows and divides the keys among its 8 / WM key groups, and those
-// of a cluster of CTAs: each key group streams chunks of 32 states (16 above head width 64) through a ring of its own (TMA, 128-byte swizzle, zeros past D and N).
-// The first warp of a key group requests them and skips chunks of which the mask leaves nothing. The parts of a row are
-// added in shared memory, a cluster's through distributed shared memory, always in the same order.
-constexpr int kRowWarps = 8;
+// they are few. A CTA has four such warps and one that requests the states. WM of the warps take 16 rows each of one unit (the rows
+// of a key head of a sequence, in blocks of 16 WM); the 4 / WM rings of states serve
+//   - whole: a unit each (many units: nothing to add up), or
+//   - the same unit, its states divided among the rings of a cluster's CTAs (few units). A row's parts are added in shared memory, a
+//     cluster's through distributed shared memory, always in the same order.
+// A ring holds chunks of 32 states (16 above head width 64): TMA, 128-byte swizzle, zeros past D and N. The requesting warp
+// passes over chunks of which the mask leaves nothing, and tells what each stage holds.
+constexpr int kRowWarps = 4, kRowThreads = 32 * (kRowWarps + 1);
 
 TCQ_HD void ldsm4(u32 addr, u32 (&r)[4]) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
@@ -106,99 +109,134 @@ TCQ_HD void mma16816(float (&d)[4], u32 a0, u32 a1, u32 a2, u32 a3, u32 b0, u32 
 template <int DP>
 struct Rows {
     static constexpr int CHUNK = DP <= 64 ? 32 : 16;                                                 // states
-    static constexpr int ATOMS = (DP + 63) / 64, HALF = ATOMS * CHUNK * 128, STAGE = 2 * HALF;       // bytes of a chunk's keys, of both
+    static constexpr int ATOMS = (DP + 63) / 64, HALF = ATOMS * CHUNK * 128, STAGE = 2 * HALF;       // bytes of a chunk's keys, of both: 8 KB
     static constexpr int PITCH = DP + 4;                                                             // floats of a part's row
-    static constexpr int PARTS = kRowWarps * 16 * PITCH * 4;
-    static constexpr int bytes(int rings, int stages) {                                             // 3 stages of 8 rings: 197 KB
-        const int ring = rings * stages * STAGE;
-        return (ring > PARTS ? ring : PARTS) + rings * stages * 24 + 16;
+    static constexpr int PARTS = kRowWarps * 16 * PITCH * 4, ML = 16 * kRowWarps * 8;                // parts, then m and l of the CTA's rows
+    static constexpr int MOST = 6;                                                                   // stages of a ring, at most
+    static constexpr int ring_bytes(int rings, int stages) {
+        return rings * stages * STAGE > PARTS + ML ? rings * stages * STAGE : PARTS + ML;
     }
+    static constexpr int bytes(int rings, int stages) { return ring_bytes(rings, stages) + rings * stages * 24 + 16; }
+};
+struct RowsPlan {
+    int wm_log2, stages, splits, whole, row_blocks, block_rows, units;
+    FastDiv by_blocks, by_heads, by_splits;
 };
 
-__device__ __forceinline__ float peer_ld(u32 addr) {
-    float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
-    return v;
-}
 template <int DT, int DP>
-__global__ void __launch_bounds__(kRowWarps * 32, DP <= 64 ? 2 : 1)
-k_cross_rows(const CrossArgs A, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, int wm_log2, int stages,
-             int splits, int row_blocks, int block_rows) {
+__global__ void __launch_bounds__(kRowThreads, DP <= 64 ? 3 : 2)
+k_cross_rows(const CrossArgs A, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const RowsPlan R) {
     typedef Rows<DP> P;
-    constexpr int KS = DP / 16, NT = DP / 8, kChunk = P::CHUNK, NK = kChunk / 8;
-    constexpr u32 kAll = (u32)((1ull << kChunk) - 1);
+    constexpr int KS = DP / 16, NT = DP / 8, NK = P::CHUNK / 8, RINGS = kRowWarps;
+    constexpr u32 kAll = (u32)((1ull << P::CHUNK) - 1);
     extern __shared__ __align__(1024) char smem_rows[];
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, g = lane >> 2, t = lane & 3;
-    const int WM = 1 << wm_log2, rings = kRowWarps >> wm_log2, wm = warp & (WM - 1), kg = warp >> wm_log2;
+    const int WM = 1 << R.wm_log2, rings = kRowWarps >> R.wm_log2, wm = warp & (WM - 1), kg = warp >> R.wm_log2, stages = R.stages;
     const u32 sbase = smem_u32(smem_rows);
-    const int ring_bytes = max(rings * stages * P::STAGE, P::PARTS);
+    const int ring_bytes = P::ring_bytes(rings, stages);
     const u32 bars = sbase + ring_bytes;                           // full, empty of each stage of each ring
     int2* meta = reinterpret_cast<int2*>(smem_rows + ring_bytes + rings * stages * 16);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(smem_rows + ring_bytes + rings * stages * 24);
-    auto full = [&](int s) -> u32 { return bars + 16 * (kg * stages + s); };
-    auto empty = [&](int s) -> u32 { return bars + 16 * (kg * stages + s) + 8; };
     if (tid < rings * stages) {
         mbar_init(bars + 16 * tid, 1);
         mbar_init(bars + 16 * tid + 8, WM);
         if (tid == 0) *abort_flag = 0;
         mbar_init_fence();
     }
+    const int rank = (int)(blockIdx.x - fdiv(blockIdx.x, R.by_splits) * R.splits);
+    // the unit of ring k: row block, sequence and key head
+    auto unit_of = [&](int k, int& rb, int& b, int& h) {
+        const int u = R.whole ? blockIdx.x * rings + k : (int)fdiv(blockIdx.x, R.by_splits);
+        const int bh = (int)fdiv((unsigned)u, R.by_blocks);
+        rb = u - bh * R.row_blocks;
+        b = (int)fdiv((unsigned)bh, R.by_heads), h = bh - b * A.kv_heads;
+        return u < R.units;
+    };
     __syncthreads();
     pdl_launch_dependents();
     pdl_wait();
 
-    const int rank = blockIdx.x % splits, unit = blockIdx.x / splits, rb = unit % row_blocks, bh = unit / row_blocks;
-    const int b = bh / A.kv_heads, h = bh - b * A.kv_heads, r0 = rb * block_rows, r1 = min(A.rows, r0 + block_rows);
-    const int len = states_of(A, b);
-    // this key group's chunks [c0, c1)
-    const int chunks = (len + kChunk - 1) / kChunk, worker = rank * rings + kg, workers = splits * rings;
-    const int c0 = (int)((i64)chunks * worker / workers), c1 = (int)((i64)chunks * (worker + 1) / workers);
-
-    // ---- the producer: the next chunk that holds a state, its truth values as bits
-    const unsigned char* mrow = A.mask ? A.mask + b * A.mask_sb : nullptr;
-    int pc = c0, ps = 0, puse = 0;
-    unsigned char pm = 0;
-    auto look = [&]() {                                            // request the mask of chunk pc
-        if (mrow && pc < c1) pm = lane < kChunk && pc * kChunk + lane < len ? mrow[pc * kChunk + lane] : 0;
-    };
-    bool pend = false;
-    auto issue = [&]() {
-        if (pend) return;
-        u32 bits = 0;
-        int at = -1;
-        while (pc < c1) {
-            const int n = len - pc * kChunk;
-            bits = mrow ? __ballot_sync(0xffffffffu, pm != 0) : n >= kChunk ? kAll : (1u << n) - 1u;
-            at = pc++;
-            look();
-            if (bits) break;
-        }
-        if (!bits) at = -1, pend = true;
-        if (puse && !mbar_wait_suspended(empty(ps), (puse - 1) & 1, abort_flag, &g_tcq_cross_error)) pend = true, at = -1;
-        if (lane == 0) {
-            meta[kg * stages + ps] = make_int2(at, (int)bits);
-            if (at < 0) {
-                mbar_arrive(full(ps));
-            } else {
-                const u32 dst = sbase + (kg * stages + ps) * P::STAGE;
-                mbar_expect_tx(full(ps), P::STAGE);
+    if (warp == kRowWarps) {
+        // ------------------------------------------------------------------------------------------------ the requests
+        int pc[RINGS] = {}, c1[RINGS] = {}, ub[RINGS] = {}, uh[RINGS] = {}, ulen[RINGS] = {};
+        unsigned char pm[RINGS] = {};
+        auto look = [&](int k) {                                   // the truth values of chunk pc
+            if (A.mask && pc[k] < c1[k]) {
+                const int j = pc[k] * P::CHUNK + lane;
+                pm[k] = lane < P::CHUNK && j < ulen[k] ? A.mask[ub[k] * A.mask_sb + j] : 0;
+            }
+        };
 #pragma unroll
-                for (int a = 0; a < P::ATOMS; ++a) {
-                    tma_load_4d(dst + a * (kChunk * 128), &kmap, full(ps), 64 * a, at * kChunk, h, b * A.kb);
-                    tma_load_4d(dst + P::HALF + a * (kChunk * 128), &vmap, full(ps), 64 * a, at * kChunk, h, b * A.vb);
+        for (int k = 0; k < RINGS; ++k) {
+            int rb;
+            const bool there = k < rings && unit_of(k, rb, ub[k], uh[k]);
+            ulen[k] = there ? states_of(A, ub[k]) : 0;
+        }
+#pragma unroll
+        for (int k = 0; k < RINGS; ++k) {
+            // this ring's chunks: all, or its run of the cluster's
+            const int chunks = (ulen[k] + P::CHUNK - 1) / P::CHUNK, workers = R.whole ? 1 : R.splits * rings, w = R.whole ? 0 : rank * rings + k;
+            const int each = chunks / workers, more = chunks - each * workers;
+            pc[k] = w * each + min(w, more), c1[k] = k < rings ? pc[k] + each + (w < more) : pc[k];
+            look(k);
+        }
+        u32 ended = 0;
+        bool ok = true;
+        int slot = 0, use = 0;
+        for (; ok && ended != (1u << rings) - 1; ++slot) {
+            if (slot == stages) slot = 0, ++use;
+#pragma unroll
+            for (int k = 0; k < RINGS; ++k) {
+                if (k >= rings || (ended >> k & 1) || !ok) continue;
+                const int s = k * stages + slot;
+                u32 bits = 0;
+                int at = -1;
+                while (pc[k] < c1[k]) {
+                    const int n = ulen[k] - pc[k] * P::CHUNK;
+                    bits = A.mask ? __ballot_sync(0xffffffffu, pm[k] != 0) : n >= P::CHUNK ? kAll : (1u << n) - 1u;
+                    at = pc[k]++;
+                    look(k);
+                    if (bits) break;
                 }
+                if (!bits) at = -1, ended |= 1u << k;
+                if (use) ok = mbar_wait_suspended(bars + 16 * s + 8, (use - 1) & 1, abort_flag, &g_tcq_cross_error);
+                if (ok && elect_one()) {
+                    meta[s] = make_int2(at, (int)bits);
+                    if (at < 0) {
+                        mbar_arrive(bars + 16 * s);
+                    } else {
+                        const u32 dst = sbase + s * P::STAGE;
+                        mbar_expect_tx(bars + 16 * s, P::STAGE);
+#pragma unroll
+                        for (int a = 0; a < P::ATOMS; ++a)
+                            tma_load_4d(dst + a * (P::CHUNK * 128), &kmap, bars + 16 * s, 64 * a, at * P::CHUNK, uh[k], ub[k] * A.kb);
+#pragma unroll
+                        for (int a = 0; a < P::ATOMS; ++a)
+                            tma_load_4d(dst + P::HALF + a * (P::CHUNK * 128), &vmap, bars + 16 * s, 64 * a, at * P::CHUNK, uh[k], ub[k] * A.vb);
+                    }
+                }
+                __syncwarp();
             }
         }
-        __syncwarp();
-        if (++ps == stages) ps = 0, ++puse;
-    };
-    const bool live = r0 + 16 * wm < r1;                           // a warp without a row only keeps the barriers going
-    if (wm == 0) {
-        look();
-        for (int i = 0; i + 1 < stages; ++i) issue();
+        if (*abort_flag) {                                         // copies on their way land before their stages are left
+            volatile int never = 0;
+            for (int k = 0; k < rings; ++k)
+                for (int s = 0; s < stages; ++s) {
+                    const int uses = use + (s < slot);             // at most: a barrier that saw fewer is waited for in vain, within the limit
+                    if (uses) mbar_wait_suspended(bars + 16 * (k * stages + s), (uses - 1) & 1, &never, &g_tcq_cross_error, kWaitNs / 100);
+                }
+        }
+        if (R.whole || rings * R.splits == 1) return;
+        __syncthreads();
+        if (R.splits > 1) cluster_barrier(), cluster_barrier();
+        return;
     }
 
-    // ---- this warp's 16 rows: g and g + 8
+    // ------------------------------------------------------------------------------------------------ this warp's 16 rows: g and g + 8
+    int rb, b, h;
+    const bool there = unit_of(kg, rb, b, h);
+    const int r0 = rb * R.block_rows, r1 = there ? min(A.rows, r0 + R.block_rows) : 0;
+    const bool live = r0 + 16 * wm < r1;                           // a warp without a row only keeps the barriers going
     u32 q[KS][4];
     {
         const int ra = r0 + 16 * wm + g, rc = ra + 8;
@@ -211,31 +249,40 @@ k_cross_rows(const CrossArgs A, const __grid_constant__ CUtensorMap kmap, const 
             for (int e = 0; e < 2; ++e) {
                 const int d = 16 * k + 8 * e + 2 * t;
                 const bool in = d < A.D;
-                q[k][2 * e] = in && ra < r1 ? *reinterpret_cast<const u32*>(qa + d) & keep ^ flip : 0u;
-                q[k][2 * e + 1] = in && rc < r1 ? *reinterpret_cast<const u32*>(qc + d) & keep ^ flip : 0u;
+                q[k][2 * e] = in && ra < r1 ? *reinterpret_cast<const u32*>(qa + d) : 0u;
+                q[k][2 * e + 1] = in && rc < r1 ? *reinterpret_cast<const u32*>(qc + d) : 0u;
             }
+        if (flip || !keep) {
+#pragma unroll
+            for (int k = 0; k < KS; ++k)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) q[k][e] = q[k][e] & keep ^ flip;
+        }
     }
     const float c = score_scale(A);
     float o[NT][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < NT; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
 
-    // One chunk: 32 scores of each row, weights, O += P V. Matrices of 8 x 8 are read from the swizzled tiles: 16-byte piece p of row r
-    // lies at p ^ (r & 7).
+    // One chunk: the scores of its states, weights, O += P V. Matrices of 8 x 8 are read from the swizzled tiles: 16-byte piece p of row r
+    // lies at p ^ (r & 7). Products that add to the same registers are issued as far apart as they can be.
+    const int row8 = lane & 7, row16 = lane & 15;
     auto chunk = [&](auto masked_c, u32 bits, u32 kt, u32 vt) {
         constexpr bool MASKED = decltype(masked_c)::value;
         float s[NK][4];
 #pragma unroll
-        for (int n = 0; n < NK; ++n) {
-            s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
-            const int r = 8 * n + (lane & 7);
+        for (int n = 0; n < NK; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
 #pragma unroll
-            for (int k = 0; k < KS; k += 2) {
-                u32 f[4];
-                const int p = 2 * k + (lane >> 3);                 // pieces of 8 elements: two of step k, two of step k + 1
-                ldsm4(kt + (p >> 3) * (kChunk * 128) + r * 128 + (((p & 7) ^ (r & 7)) << 4), f);
-                mma16816<DT>(s[n], q[k][0], q[k][1], q[k][2], q[k][3], f[0], f[1]);
-                if (k + 1 < KS) mma16816<DT>(s[n], q[k + 1][0], q[k + 1][1], q[k + 1][2], q[k + 1][3], f[2], f[3]);
+        for (int k = 0; k < KS; k += 2) {
+            const int p = 2 * k + (lane >> 3);                     // pieces of 8 elements: two of step k, two of step k + 1
+            u32 f[NK][4];
+#pragma unroll
+            for (int n = 0; n < NK; ++n) ldsm4(kt + (p >> 3) * (P::CHUNK * 128) + (8 * n + row8) * 128 + (((p & 7) ^ row8) << 4), f[n]);
+#pragma unroll
+            for (int n = 0; n < NK; ++n) mma16816<DT>(s[n], q[k][0], q[k][1], q[k][2], q[k][3], f[n][0], f[n][1]);
+            if (k + 1 < KS) {
+#pragma unroll
+                for (int n = 0; n < NK; ++n) mma16816<DT>(s[n], q[k + 1][0], q[k + 1][1], q[k + 1][2], q[k + 1][3], f[n][2], f[n][3]);
             }
         }
         if (MASKED) {
@@ -251,7 +298,7 @@ k_cross_rows(const CrossArgs A, const __grid_constant__ CUtensorMap kmap, const 
         for (int e = 0; e < 2; ++e) {
             top[e] = fmaxf(s[0][2 * e], s[0][2 * e + 1]);
 #pragma unroll
-            for (int n = 1; n < NK; ++n) top[e] = fmaxf(top[e], fmaxf(s[n][2 * e], s[n][2 * e + 1]));
+            for (int n = 1; n < NK; ++n) top[e] = max3(top[e], s[n][2 * e], s[n][2 * e + 1]);
         }
         top[0] *= c, top[1] *= c;
         if (__any_sync(0xffffffffu, top[0] > m[0] + kSlack || top[1] > m[1] + kSlack)) {
@@ -268,116 +315,171 @@ k_cross_rows(const CrossArgs A, const __grid_constant__ CUtensorMap kmap, const 
 #pragma unroll
             for (int i = 0; i < NT; ++i) o[i][0] *= f[0], o[i][1] *= f[0], o[i][2] *= f[1], o[i][3] *= f[1];
         }
-        const float base[2] = {kRef - (m[0] == -INFINITY ? 0.f : m[0]), kRef - (m[1] == -INFINITY ? 0.f : m[1])};
+        const float ba = kRef - (m[0] == -INFINITY ? 0.f : m[0]), bc = kRef - (m[1] == -INFINITY ? 0.f : m[1]);
+        const u64 c2 = pair(c, c), ba2 = pair(ba, ba), bc2 = pair(bc, bc);
+        u64 sum[2] = {0, 0};
+        u32 w[NK][2];                                              // weights of rows g and g + 8
 #pragma unroll
         for (int n = 0; n < NK; ++n)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[n][e] = ex2(__fmaf_rn(s[n][e], c, base[e >> 1]));
+            for (int e = 0; e < 2; ++e) {
+                float lo, hi;
+                unpair(fma2(pair(s[n][2 * e], s[n][2 * e + 1]), c2, e ? bc2 : ba2), lo, hi);
+                lo = ex2(lo), hi = ex2(hi);
+                sum[e] = add2(sum[e], pair(lo, hi));
+                w[n][e] = weights2<DT>(lo, hi);
+            }
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-            float sum = 0.f;
-#pragma unroll
-            for (int n = 0; n < NK; ++n) sum += s[n][2 * e] + s[n][2 * e + 1];
-            l[e] += sum;
+            float lo, hi;
+            unpair(sum[e], lo, hi);
+            l[e] += lo + hi;
         }
 #pragma unroll
         for (int k = 0; k < NK / 2; ++k) {
-            const u32 a0 = weights2<DT>(s[2 * k][0], s[2 * k][1]), a1 = weights2<DT>(s[2 * k][2], s[2 * k][3]),
-                      a2 = weights2<DT>(s[2 * k + 1][0], s[2 * k + 1][1]), a3 = weights2<DT>(s[2 * k + 1][2], s[2 * k + 1][3]);
             // what lies where no state is may be anything, NaN too: this lane's keys 16 k + 2 t, + 1 and 8 further
             u32 z0 = 0xffffffffu, z1 = 0xffffffffu;
             if (MASKED) {
-                const u32 w = bits >> (16 * k + 2 * t);
-                z0 = (w & 1 ? 0xffffu : 0u) | (w & 2 ? 0xffff0000u : 0u);
-                z1 = (w & 256 ? 0xffffu : 0u) | (w & 512 ? 0xffff0000u : 0u);
+                const u32 x = bits >> (16 * k + 2 * t);
+                z0 = (x & 1 ? 0xffffu : 0u) | (x & 2 ? 0xffff0000u : 0u);
+                z1 = (x & 256 ? 0xffffu : 0u) | (x & 512 ? 0xffff0000u : 0u);
             }
-            const int r = 16 * k + (lane & 15);
 #pragma unroll
             for (int i = 0; i < NT; i += 2) {
                 u32 f[4];
                 const int p = i + (lane >> 4);
-                ldsm4t(vt + (p >> 3) * (kChunk * 128) + r * 128 + (((p & 7) ^ (r & 7)) << 4), f);
-                mma16816<DT>(o[i], a0, a1, a2, a3, MASKED ? f[0] & z0 : f[0], MASKED ? f[1] & z1 : f[1]);
-                mma16816<DT>(o[i + 1], a0, a1, a2, a3, MASKED ? f[2] & z0 : f[2], MASKED ? f[3] & z1 : f[3]);
+                ldsm4t(vt + (p >> 3) * (P::CHUNK * 128) + (16 * k + row16) * 128 + (((p & 7) ^ row8) << 4), f);
+                mma16816<DT>(o[i], w[2 * k][0], w[2 * k][1], w[2 * k + 1][0], w[2 * k + 1][1], MASKED ? f[0] & z0 : f[0], MASKED ? f[1] & z1 : f[1]);
+                mma16816<DT>(o[i + 1], w[2 * k][0], w[2 * k][1], w[2 * k + 1][0], w[2 * k + 1][1], MASKED ? f[2] & z0 : f[2], MASKED ? f[3] & z1 : f[3]);
             }
         }
     };
-    int slot = 0, use = 0;
+    int slot = kg * stages;
+    u32 phase = 0;
     for (;;) {
-        if (!mbar_wait_suspended(full(slot), use & 1, abort_flag, &g_tcq_cross_error)) break;
-        const int2 what = meta[kg * stages + slot];
+        if (!mbar_wait_suspended(bars + 16 * slot, phase, abort_flag, &g_tcq_cross_error)) break;
+        const int2 what = meta[slot];
         if (what.x < 0) break;
-        if (wm == 0) issue();                                      // into the stage that was used last
-        const u32 kt = sbase + (kg * stages + slot) * P::STAGE, vt = kt + P::HALF;
+        const u32 kt = sbase + slot * P::STAGE;
         if (live) {
-            if ((u32)what.y == kAll) chunk(std::false_type(), kAll, kt, vt);
-            else chunk(std::true_type(), (u32)what.y, kt, vt);
+            if ((u32)what.y == kAll) chunk(std::false_type(), kAll, kt, kt + P::HALF);
+            else chunk(std::true_type(), (u32)what.y, kt, kt + P::HALF);
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive(empty(slot));
-        if (++slot == stages) slot = 0, ++use;
-    }
-    if (wm == 0 && *abort_flag) {                                  // copies on their way land before their stages are left
-        volatile int never = 0;
-        for (; use < puse || (use == puse && slot < ps); use += slot + 1 == stages, slot = slot + 1 == stages ? 0 : slot + 1)
-            mbar_wait_suspended(full(slot), use & 1, &never, &g_tcq_cross_error, kWaitNs / 20);
+        if (lane == 0) mbar_arrive(bars + 16 * slot + 8);
+        if (++slot == (kg + 1) * stages) slot = kg * stages, phase ^= 1;
     }
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
         l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
         l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
     }
-    if (rings * splits == 1) {
-        if (!live) return;
+    const i64 out_st = (i64)A.heads * A.D, out_sb = (i64)A.T * out_st;
+    if (R.whole || rings * R.splits == 1) {
+        // four lanes hold 8 elements of a row in pairs: turned among them into 16-byte pieces, of which each lane stores every fourth
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
             const int r = r0 + 16 * wm + g + 8 * e;
-            if (r >= r1) continue;
             const float f = l[e] != 0.f ? 1.f / l[e] : 0.f;
-            u32* dst = reinterpret_cast<u32*>(A.out + row_at(A, b, h, r, (i64)A.T * A.heads * A.D, (i64)A.heads * A.D));
+            uint4* dst = reinterpret_cast<uint4*>(A.out + row_at(A, b, h, min(r, A.rows - 1), out_sb, out_st));
 #pragma unroll
-            for (int i = 0; i < NT; ++i)
-                if (8 * i < A.D) dst[4 * i + t] = pack2<DT>(o[i][2 * e] * f, o[i][2 * e + 1] * f);
+            for (int i = 0; i < NT; i += 4) {
+                u32 y[4], z[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) y[j] = i + j < NT ? pack2<DT>(o[i + j < NT ? i + j : 0][2 * e] * f, o[i + j < NT ? i + j : 0][2 * e + 1] * f) : 0u;
+                // lane t gets piece i + t: word j of it is lane j's y[t]
+#pragma unroll
+                for (int d = 0; d < 4; ++d) {
+                    const int mine = t ^ d;                        // give y[t ^ d] to lane t ^ d, take its y[t]
+                    const u32 give = mine == 0 ? y[0] : mine == 1 ? y[1] : mine == 2 ? y[2] : y[3];
+                    const u32 got = d ? __shfl_xor_sync(0xffffffffu, give, d) : give;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        if (j == mine) z[j] = got;
+                }
+                if (r < r1 && 8 * (i + t) < A.D) dst[i + t] = make_uint4(z[0], z[1], z[2], z[3]);
+            }
         }
         return;
     }
-    // ---- parts to shared memory (every chunk has arrived), added by all warps: rows of the CTA, one pair of elements a thread
+    // ---- parts to shared memory (every chunk has arrived), then added: four elements of a row a thread
     __syncthreads();
-    float* part = reinterpret_cast<float*>(smem_rows) + (size_t)warp * 16 * P::PITCH;
+    float* const parts = reinterpret_cast<float*>(smem_rows);
+    {
+        float* part = parts + (size_t)(kg * WM + wm) * 16 * P::PITCH;
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-        float* row = part + (g + 8 * e) * P::PITCH;
+        for (int e = 0; e < 2; ++e) {
+            float* row = part + (g + 8 * e) * P::PITCH;
 #pragma unroll
-        for (int i = 0; i < NT; ++i) *reinterpret_cast<float2*>(row + 8 * i + 2 * t) = make_float2(o[i][2 * e], o[i][2 * e + 1]);
-        if (t == 0) row[DP] = m[e], row[DP + 1] = l[e];
-    }
-    if (splits > 1) cluster_barrier();
-    else __syncthreads();
-    const int rows = r1 - r0, f0 = rows * rank / splits, f1 = rows * (rank + 1) / splits, half = A.D / 2;
-    for (int i = tid; i < (f1 - f0) * half; i += kRowWarps * 32) {
-        const int rr = f0 + i / half, d = 2 * (i % half), w = rr >> 4;
-        const u32 at = sbase + (((u32)w * 16 + (rr & 15)) * P::PITCH) * 4;
-        float top = -INFINITY;
-        for (int k = 0; k < splits; ++k) {
-            const u32 p = peer_addr(at, k);
-            for (int j = 0; j < rings; ++j) top = fmaxf(top, peer_ld(p + (j * WM * 16 * P::PITCH + DP) * 4));
+            for (int i = 0; i < NT; ++i) *reinterpret_cast<float2*>(row + 8 * i + 2 * t) = make_float2(o[i][2 * e], o[i][2 * e + 1]);
+            if (t == 0) *reinterpret_cast<float2*>(row + DP) = make_float2(m[e], l[e]);
         }
-        float sum = 0.f, a0 = 0.f, a1 = 0.f;
-        for (int k = 0; k < splits; ++k) {
-            const u32 p = peer_addr(at, k);
-            for (int j = 0; j < rings; ++j) {
-                const u32 pj = p + j * WM * 16 * P::PITCH * 4;
-                const float2 ml = peer_ld2(pj + DP * 4), v = peer_ld2(pj + d * 4);
-                const float f = top == -INFINITY ? (ml.y == ml.y ? 0.f : 1.f) : ex2(ml.x - top);
-                // a part without weight adds nothing, unless its sum is NaN: the row has to say so
-                if (f == 0.f && ml.y == ml.y) continue;
-                sum = __fmaf_rn(ml.y, f, sum), a0 = __fmaf_rn(v.x, f, a0), a1 = __fmaf_rn(v.y, f, a1);
+    }
+    const int rows = r1 - r0;
+    // the factor of a part with reference m and sum l next to others of reference up to top: a part without weight adds nothing, unless its
+    // sum is NaN (scores that are NaN move no reference): the row has to say so
+    auto factor = [](float2 ml, float top) { return top == -INFINITY ? (ml.y == ml.y ? 0.f : 1.f) : ml.y != ml.y ? 1.f : ex2(ml.x - top); };
+    auto store = [&](int row, int d, const float4& y, float sum) {
+        const float f = sum != 0.f ? 1.f / sum : 0.f;
+        if (d < A.D)
+            *reinterpret_cast<uint2*>(A.out + row_at(A, b, h, r0 + row, out_sb, out_st) + d) = make_uint2(pack2<DT>(y.x * f, y.y * f), pack2<DT>(y.z * f, y.w * f));
+    };
+    asm volatile("barrier.cta.sync 1, %0;" ::"n"(32 * kRowWarps) : "memory");
+    for (int i = tid; i < rows * (DP / 4); i += 32 * kRowWarps) {
+        const int row = i / (DP / 4), d = 4 * (i - row * (DP / 4));
+        const float* p = parts + row * P::PITCH;
+        float2 ml[RINGS];
+        float4 v[RINGS], y = make_float4(0.f, 0.f, 0.f, 0.f);
+        float top = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int k = 0; k < RINGS; ++k) {
+            ml[k] = make_float2(-INFINITY, 0.f), v[k] = y;
+            if (k < rings) {
+                ml[k] = *reinterpret_cast<const float2*>(p + k * WM * 16 * P::PITCH + DP);
+                v[k] = *reinterpret_cast<const float4*>(p + k * WM * 16 * P::PITCH + d);
+            }
+            top = fmaxf(top, ml[k].x);
+        }
+#pragma unroll
+        for (int k = 0; k < RINGS; ++k) {
+            const float f = factor(ml[k], top);
+            sum = __fmaf_rn(ml[k].y, f, sum);
+            y.x = __fmaf_rn(v[k].x, f, y.x), y.y = __fmaf_rn(v[k].y, f, y.y), y.z = __fmaf_rn(v[k].z, f, y.z), y.w = __fmaf_rn(v[k].w, f, y.w);
+        }
+        if (R.splits == 1) {
+            store(row, d, y, sum);
+        } else {
+            *reinterpret_cast<float4*>(parts + row * P::PITCH + d) = y;             // read by no other thread before
+            if (d == 0) *reinterpret_cast<float2*>(smem_rows + P::PARTS + 8 * row) = make_float2(top, sum);
+        }
+    }
+    if (R.splits == 1) return;
+    cluster_barrier();
+    for (int i = rank * (32 * kRowWarps) + tid; i < rows * (DP / 4); i += R.splits * (32 * kRowWarps)) {
+        const int row = i / (DP / 4), d = 4 * (i - row * (DP / 4));
+        float2 ml[8];
+        float4 v[8], y = make_float4(0.f, 0.f, 0.f, 0.f);
+        float top = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            ml[k] = make_float2(-INFINITY, 0.f), v[k] = y;
+            if (k < R.splits) {
+                const u32 p = peer_addr(sbase, k);
+                ml[k] = peer_ld2(p + P::PARTS + 8 * row);
+                v[k] = peer_ld4(p + (row * P::PITCH + d) * 4);
             }
         }
-        const float f = sum != 0.f ? 1.f / sum : 0.f;
-        *reinterpret_cast<u32*>(A.out + row_at(A, b, h, r0 + rr, (i64)A.T * A.heads * A.D, (i64)A.heads * A.D) + d) = pack2<DT>(a0 * f, a1 * f);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) top = fmaxf(top, ml[k].x);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const float f = factor(ml[k], top);
+            sum = __fmaf_rn(ml[k].y, f, sum);
+            y.x = __fmaf_rn(v[k].x, f, y.x), y.y = __fmaf_rn(v[k].y, f, y.y), y.z = __fmaf_rn(v[k].z, f, y.z), y.w = __fmaf_rn(v[k].w, f, y.w);
+        }
+        store(row, d, y, sum);
     }
-    if (splits > 1) cluster_barrier();                             // a part may be read until here
+    cluster_barrier();                                             // a part may be read until here
 }
 
 // ------------------------------------------------------------------------------------------------ tiles of 128 rows
@@ -396,19 +498,23 @@ k_cross_rows(const CrossArgs A, const __grid_constant__ CUtensorMap kmap, const 
 // up to the tile before. The reference m of a row moves only when a score passes it by kSlack; O (in TMEM) is then
 // rescaled by its own row's thread.
 constexpr int kTile = 128;
-
 template <int DP, bool ROWS>
 struct Tiles {
     static constexpr int ATOMS = (DP + 63) / 64;                       // 64-element columns of a tile
     static constexpr int TB = ATOMS * kTile * 128;                     // bytes of a tile: a group's queries, keys, values
     static constexpr int QN = ROWS ? 2 : 1;
     static constexpr int FIT = (226 * 1024 - QN * TB) / TB, RING = FIT < 8 ? FIT : 8;      // tiles of keys and values on their way
-    static constexpr int THREADS = 11 * 32;                            // eight softmax warps, product, load, clean
+    // Eight softmax warps; product, load and clean warps and one that only makes the warpgroup whole. The CTA is launched with 168 registers
+    // a thread (384 x 168 = 64,512); the softmax warps take 208 and the others keep 88: 256 x 208 + 128 x 88 = 64,512.
+    static constexpr int THREADS = 384, LAUNCH_REGS = 168;
     static constexpr int Q0 = 0, RING0 = QN * TB, BAR0 = RING0 + RING * TB;
     static constexpr int META = 8;                                     // tiles whose truth values are kept
-    static constexpr int META0 = BAR0 + 288, ML0 = META0 + META * 32;  // m, l of every row
+    static constexpr int META0 = BAR0 + 304, ML0 = META0 + META * 32;  // m, l of every row
     static constexpr int BYTES = ML0 + 2 * kTile * 8;
-    static constexpr u32 COLS = 512, S0 = 0, O0 = 256;                 // TMEM columns: scores (128 each), outputs
+    // TMEM columns: scores (128 each), outputs. Up to head width 64 the weights have columns of their own, so that the next tile's scores
+    // may be formed while the weights of this one are; else they lie over the scores.
+    static constexpr bool EARLY = DP <= 64;
+    static constexpr u32 COLS = 512, S0 = 0, P0 = EARLY ? 256 : 0, PG = EARLY ? 64 : 128, O0 = EARLY ? 384 : 256, OG = EARLY ? 64 : 128;
     static constexpr int PARTS = 2 * kTile * DP * 4;
     static_assert(RING >= 5, "two tiles in use, the next keys on their way");
     static_assert(PARTS <= BAR0 && BYTES <= 227 * 1024, "the parts overlay the tiles");
@@ -418,9 +524,10 @@ struct TileMeta {
     int at, whole, pad[2];
     u32 bits[4];
 };
-// Barriers, 8 bytes each from BAR0: ring slot i full and empty, values of tile t cleaned (t mod META), of group g scores and weights (two
-// halves), queries, the end.
-enum { TBAR_FULL = 0, TBAR_EMPTY = 8, TBAR_CLEAN = 16, TBAR_S = 24, TBAR_P = 26, TBAR_Q = 30, TBAR_END = 31, TBAR_COUNT = 32 };
+// Barriers, 8 bytes each from BAR0: ring slot i full and empty, values of tile t cleaned (t mod META), of group g scores, weights
+// (two halves), scores read and outputs (EARLY), queries, the end.
+enum { TBAR_FULL = 0, TBAR_EMPTY = 8, TBAR_CLEAN = 16, TBAR_S = 24, TBAR_P = 26, TBAR_READ = 30, TBAR_O = 32, TBAR_Q = 34, TBAR_END = 35, TBAR_COUNT = 36 };
+
 
 template <int DT, int DP, bool ROWS>
 __global__ void __launch_bounds__(Tiles<DP, ROWS>::THREADS, 1)
@@ -447,8 +554,10 @@ k_cross_tiles(const CrossArgs A, const __grid_constant__ CUtensorMap kmap, const
         for (int i = 0; i < P::META; ++i) mbar_init(bar(TBAR_CLEAN + i), 1);
         for (int i = 0; i < 2; ++i) {
             mbar_init(bar(TBAR_S + i), 1);
-            mbar_init(bar(TBAR_P + i), 4);                    // per softmax warp; group and half at 2 g + half
-            mbar_init(bar(TBAR_P + 2 + i), 4);
+            mbar_init(bar(TBAR_READ + i), 4);
+            mbar_init(bar(TBAR_O + i), 1);
+            mbar_init(bar(TBAR_P + 2 * i), 4);                // per softmax warp; group and half at 2 g + half
+            mbar_init(bar(TBAR_P + 2 * i + 1), 4);
         }
         mbar_init(bar(TBAR_Q), 256);
         mbar_init(bar(TBAR_END), 1);
@@ -475,14 +584,17 @@ k_cross_tiles(const CrossArgs A, const __grid_constant__ CUtensorMap kmap, const
     const bool parts = splits > 1 || !ROWS;                   // rows have more than one part
     const bool ragged = A.lens || A.mask;
 
+    if (warp < W_MMA) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    else asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     if (warp < W_MMA) {
         // ------------------------------------------------------------------------------------------------ softmax
         const int g = warp >> 2, gl = tid & 127, row = ROWS ? g * kTile + gl : gl;
         const bool idle = r0 + (row & ~31) >= r1;             // a warp without a row only keeps the barriers going
         const float c = score_scale(A);
+        constexpr int SEG = DP <= 32 ? 4 : DP <= 64 ? 8 : 16, RPP = 32 / SEG;      // lanes to a row of 16-byte pieces, rows a pass
         if (k1 > k0) {
-            // Queries to shared memory: SEG lanes to a row, 16 bytes each
-            constexpr int SEG = DP <= 32 ? 4 : DP <= 64 ? 8 : 16, RPP = 32 / SEG, WROWS = ROWS ? 32 : 16, NP = WROWS / RPP;
+            // queries to shared memory, all of a thread's requested at once
+            constexpr int WROWS = ROWS ? 32 : 16, NP = WROWS / RPP;
             const int sl = lane % SEG, first = warp * WROWS;
             const u32 flip = query_flip(A), keep = query_keep(A);
             uint4 w[NP];
@@ -490,40 +602,57 @@ k_cross_tiles(const CrossArgs A, const __grid_constant__ CUtensorMap kmap, const
             for (int n = 0; n < NP; ++n) {
                 const int rr = r0 + first + n * RPP + lane / SEG;
                 w[n] = make_uint4(0, 0, 0, 0);
-                if (rr < r1 && 8 * sl < A.D) {
-                    w[n] = *reinterpret_cast<const uint4*>(A.q + row_at(A, b, h, rr, A.q_sb, A.q_st) + 8 * sl);
-                    w[n].x = w[n].x & keep ^ flip, w[n].y = w[n].y & keep ^ flip, w[n].z = w[n].z & keep ^ flip, w[n].w = w[n].w & keep ^ flip;
-                }
+                if (rr < r1 && 8 * sl < A.D) w[n] = *reinterpret_cast<const uint4*>(A.q + row_at(A, b, h, rr, A.q_sb, A.q_st) + 8 * sl);
             }
 #pragma unroll
             for (int n = 0; n < NP; ++n) {
                 const int q = first + n * RPP + lane / SEG, qg = q >> 7, qr = q & 127;
+                w[n].x = w[n].x & keep ^ flip, w[n].y = w[n].y & keep ^ flip, w[n].z = w[n].z & keep ^ flip, w[n].w = w[n].w & keep ^ flip;
                 if (8 * sl < DP)
                     *reinterpret_cast<uint4*>(smem + P::Q0 + qg * P::TB + (sl >> 3) * (kTile * 128) + qr * 128 + (((sl & 7) ^ (qr & 7)) << 4)) = w[n];
             }
             async_proxy_fence();
         }
         mbar_arrive(bar(TBAR_Q));
-        const u32 lanes = (u32)((warp & 3) * 32) << 16, ts = tmem + lanes + P::S0 + g * kTile, to = tmem + lanes + P::O0 + g * kTile;
+        const u32 lanes = (u32)((warp & 3) * 32) << 16, ts = tmem + lanes + P::S0 + g * kTile, tp = tmem + lanes + P::P0 + g * P::PG,
+                  to = tmem + lanes + P::O0 + g * P::OG;
         float m = -INFINITY, l = 0.f;
         // One tile: 128 scores of this thread's row, their largest, weights over them. Nothing of the scores is read after the first
         // store; the product of a half is issued when its four warps have handed it over.
-        auto tile = [&](auto masked_c, int i, const u32 (&bits)[4]) {
+        auto tile = [&](auto masked_c, int i, const u32 (&bits)[4]) -> bool {
             constexpr bool MASKED = decltype(masked_c)::value;
             u32 v[4][32];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) tmem_ld32(ts + 32 * j, v[j]);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) tmem_ld_wait(v[j]);
-            if (MASKED) {
-#pragma unroll
-                for (int j = 0; j < 128; ++j)
-                    if (!(bits[j >> 5] >> (j & 31) & 1)) v[j >> 5][j & 31] = 0xff800000u;
-            }
             float raw[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            tmem_ld32(ts, v[0]);
+            tmem_ld32(ts + 32, v[1]);
+            tmem_ld_wait(v[0]);
+            tmem_ld_wait(v[1]);
+            tmem_ld32(ts + 64, v[2]);
+            tmem_ld32(ts + 96, v[3]);
 #pragma unroll
-            for (int j = 0; j < 128; j += 2)
-                raw[(j >> 1) & 3] = max3(raw[(j >> 1) & 3], __uint_as_float(v[j >> 5][j & 31]), __uint_as_float(v[j >> 5][(j & 31) + 1]));
+            for (int half = 0; half < 2; ++half) {
+                if (half) {
+                    tmem_ld_wait(v[2]);
+                    tmem_ld_wait(v[3]);
+                    if (P::EARLY) {
+                        tc_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(bar(TBAR_READ + g));
+                    }
+                }
+                if (MASKED) {
+#pragma unroll
+                    for (int j = 64 * half; j < 64 * half + 64; ++j)
+                        if (!(bits[j >> 5] >> (j & 31) & 1)) v[j >> 5][j & 31] = 0xff800000u;
+                }
+#pragma unroll
+                for (int j = 64 * half; j < 64 * half + 64; j += 2)
+                    raw[(j >> 1) & 3] = max3(raw[(j >> 1) & 3], __uint_as_float(v[j >> 5][j & 31]), __uint_as_float(v[j >> 5][(j & 31) + 1]));
+            }
+            if (P::EARLY && i > 0) {                          // the outputs up to the tile before are complete, its weights used
+                if (!wait(TBAR_O + g, i - 1)) return false;
+                tc_after();
+            }
             float top = fmaxf(fmaxf(raw[0], raw[1]), fmaxf(raw[2], raw[3]));
             top *= c;
             if (__any_sync(0xffffffffu, top > m + kSlack)) {
@@ -555,14 +684,14 @@ k_cross_tiles(const CrossArgs A, const __grid_constant__ CUtensorMap kmap, const
                 u32 w[16];
 #pragma unroll
                 for (int j = 0; j < 16; ++j) {
-                    const u32 x = v[q][2 * j], y = v[q][2 * j + 1];
+                    const u64 x = fma2(pair(__uint_as_float(v[q][2 * j]), __uint_as_float(v[q][2 * j + 1])), c2, a2);
                     float lo, hi;
-                    unpair(fma2(pair(__uint_as_float(x), __uint_as_float(y)), c2, a2), lo, hi);
+                    unpair(x, lo, hi);
                     lo = ex2(lo), hi = ex2(hi);
                     sum[j & 1] = add2(sum[j & 1], pair(lo, hi));
                     w[j] = weights2<DT>(lo, hi);
                 }
-                tmem_st16(ts + 16 * q, w);
+                tmem_st16(tp + 16 * q, w);
                 if (q & 1) {
                     tmem_st_wait();
                     tc_before();
@@ -573,6 +702,7 @@ k_cross_tiles(const CrossArgs A, const __grid_constant__ CUtensorMap kmap, const
             float lo, hi;
             unpair(add2(sum[0], sum[1]), lo, hi);
             l += lo + hi;
+            return true;
         };
         bool ok = true;
         for (int i = 0; k1 > k0; ++i) {
@@ -583,17 +713,24 @@ k_cross_tiles(const CrossArgs A, const __grid_constant__ CUtensorMap kmap, const
             const int4 head = *reinterpret_cast<const int4*>(&t);
             if (head.x < 0) break;
             if (idle) {
-                if (lane == 0) mbar_arrive(bar(TBAR_P + 2 * g)), mbar_arrive(bar(TBAR_P + 2 * g + 1));
+                // the next scores may come before the other warps have handed this tile's weights over: not before its outputs
+                if (P::EARLY && i > 0) ok = wait(TBAR_O + g, i - 1);
+                if (!ok) break;
+                if (lane == 0) {
+                    if (P::EARLY) mbar_arrive(bar(TBAR_READ + g));
+                    mbar_arrive(bar(TBAR_P + 2 * g)), mbar_arrive(bar(TBAR_P + 2 * g + 1));
+                }
                 continue;
             }
             u32 bits[4] = {};
             if (head.y) {
-                tile(std::false_type(), i, bits);
+                ok = tile(std::false_type(), i, bits);
             } else {
                 const uint4 w = *reinterpret_cast<const uint4*>(t.bits);
                 bits[0] = w.x, bits[1] = w.y, bits[2] = w.z, bits[3] = w.w;
-                tile(std::true_type(), i, bits);
+                ok = tile(std::true_type(), i, bits);
             }
+            if (!ok) break;
         }
         // every product has ended: the rows' outputs, or their parts, over the tiles, 16-byte pieces permuted within a row
         const bool got = ok && l != 0.f;
@@ -601,23 +738,27 @@ k_cross_tiles(const CrossArgs A, const __grid_constant__ CUtensorMap kmap, const
         if (parts) asm volatile("barrier.cta.sync 15, 256;" ::: "memory");
         constexpr int XP = (DP / 4) % 8 == 0 ? 7 : 3, XO = (DP / 8) % 8 == 0 ? 7 : (DP / 8) % 4 == 0 ? 3 : 1;
         if (!idle) {
-#pragma unroll 1
-            for (int d = 0; d < DP; d += 8) {
-                u32 o[8] = {};
+#pragma unroll
+            for (int d0 = 0; d0 < DP; d0 += 32) {
+                u32 o[32] = {};
                 if (ok && k1 > k0) {
-                    tmem_ld8(to + d, o);
+                    if (d0 + 32 <= DP) tmem_ld32(to + d0, o);
+                    else tmem_ld16(to + d0, o);
                     tmem_ld_wait(o);
                 }
-                float y[8];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) y[j] = got ? __uint_as_float(o[j]) * f : 0.f;
-                if (parts) {
-                    float4* part = reinterpret_cast<float4*>(smem) + (g * kTile + gl) * (DP / 4);
-                    part[(d / 4) ^ (gl & XP)] = make_float4(y[0], y[1], y[2], y[3]);
-                    part[(d / 4 + 1) ^ (gl & XP)] = make_float4(y[4], y[5], y[6], y[7]);
-                } else {
-                    reinterpret_cast<uint4*>(smem + P::Q0 + g * P::TB)[gl * (DP / 8) + ((d / 8) ^ (gl & XO))] =
-                        make_uint4(pack2<DT>(y[0], y[1]), pack2<DT>(y[2], y[3]), pack2<DT>(y[4], y[5]), pack2<DT>(y[6], y[7]));
+                for (int d = d0; d < d0 + 32 && d < DP; d += 8) {
+                    float y[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) y[j] = got ? __uint_as_float(o[d - d0 + j]) * f : 0.f;
+                    if (parts) {
+                        float4* part = reinterpret_cast<float4*>(smem) + (g * kTile + gl) * (DP / 4);
+                        part[(d / 4) ^ (gl & XP)] = make_float4(y[0], y[1], y[2], y[3]);
+                        part[(d / 4 + 1) ^ (gl & XP)] = make_float4(y[4], y[5], y[6], y[7]);
+                    } else {
+                        reinterpret_cast<uint4*>(smem + P::Q0 + g * P::TB)[gl * (DP / 8) + ((d / 8) ^ (gl & XO))] =
+                            make_uint4(pack2<DT>(y[0], y[1]), pack2<DT>(y[2], y[3]), pack2<DT>(y[4], y[5]), pack2<DT>(y[6], y[7]));
+                    }
                 }
             }
         }
@@ -625,12 +766,14 @@ k_cross_tiles(const CrossArgs A, const __grid_constant__ CUtensorMap kmap, const
             reinterpret_cast<float2*>(smem + P::ML0)[g * kTile + gl] = make_float2(ok && !idle ? m : -INFINITY, ok && !idle ? l : 0.f);
         } else if (!idle) {
             __syncwarp();
-            const int w0 = gl & ~31, rows = min(32, r1 - r0 - (row & ~31)), pieces = A.D / 8;
-            for (int e = lane; e < rows * pieces; e += 32) {
-                const int rr = e / pieces, ch = e - rr * pieces;
-                u16* dst = A.out + row_at(A, b, h, r0 + (row & ~31) + rr, (i64)A.T * A.heads * A.D, (i64)A.heads * A.D);
-                reinterpret_cast<uint4*>(dst)[ch] =
-                    reinterpret_cast<const uint4*>(smem + P::Q0 + g * P::TB)[(w0 + rr) * (DP / 8) + (ch ^ ((w0 + rr) & XO))];
+            const int sl = lane % SEG;
+#pragma unroll 4
+            for (int n = 0; n < 32; n += RPP) {
+                const int rr = (gl & ~31) + n + lane / SEG, rg = r0 + (row & ~31) + n + lane / SEG;
+                if (rg < r1 && 8 * sl < A.D) {
+                    u16* dst = A.out + row_at(A, b, h, rg, (i64)A.T * A.heads * A.D, (i64)A.heads * A.D);
+                    reinterpret_cast<uint4*>(dst)[sl] = reinterpret_cast<const uint4*>(smem + P::Q0 + g * P::TB)[rr * (DP / 8) + (sl ^ (rr & XO))];
+                }
             }
         }
     } else if (k1 > k0 && warp == W_LOAD) {
@@ -721,7 +864,7 @@ k_cross_tiles(const CrossArgs A, const __grid_constant__ CUtensorMap kmap, const
         bool ok = true;
         auto scores = [&](int g, int i) {
             const int t = ROWS ? i : 2 * i + g, item = 2 * t, s = item % P::RING;
-            ok = ok && wait(TBAR_FULL + s, item / P::RING);
+            ok = ok && wait(TBAR_FULL + s, item / P::RING) && (!P::EARLY || i == 0 || wait(TBAR_READ + g, i - 1));
             if (!ok) return;
             if (meta[t & (P::META - 1)].at < 0) {
                 ended[g] = true;
@@ -749,13 +892,16 @@ k_cross_tiles(const CrossArgs A, const __grid_constant__ CUtensorMap kmap, const
                 if (elect_one()) {
 #pragma unroll
                     for (int k = 4 * half; k < 4 * half + 4; ++k)
-                        mma_ts(tmem + P::O0 + g * kTile, tmem + P::S0 + g * kTile + 8 * k, vd + (u32)(s * tb + k * (16 * 128 / 16)), idesc_f16(DP) | IDESC | kIdescBAlongN,
+                        mma_ts(tmem + P::O0 + g * P::OG, tmem + P::P0 + g * P::PG + 8 * k, vd + (u32)(s * tb + k * (16 * 128 / 16)), idesc_f16(DP) | IDESC | kIdescBAlongN,
                                k > 0 ? 1u : (u32)(i > 0));
                 }
                 __syncwarp();
             }
-            if (!ROWS || g == 1) {
-                if (elect_one()) mma_commit(bar(TBAR_EMPTY + s));
+            if (P::EARLY || !ROWS || g == 1) {
+                if (elect_one()) {
+                    if (P::EARLY) mma_commit(bar(TBAR_O + g));
+                    if (!ROWS || g == 1) mma_commit(bar(TBAR_EMPTY + s));
+                }
                 __syncwarp();
             }
         };
@@ -766,8 +912,9 @@ k_cross_tiles(const CrossArgs A, const __grid_constant__ CUtensorMap kmap, const
 #pragma unroll
             for (int g = 0; g < 2; ++g)
                 if (ok && !ended[g]) {
+                    if (P::EARLY) scores(g, i + 1);
                     outputs(g, i);
-                    scores(g, i + 1);
+                    if (!P::EARLY) scores(g, i + 1);
                 }
         // The end of both groups: complete when every product is. After an expired wait too, products in flight end before TMEM is
         // freed.
@@ -781,6 +928,9 @@ k_cross_tiles(const CrossArgs A, const __grid_constant__ CUtensorMap kmap, const
     tc_before();
     __syncthreads();
     tc_after();
+    // Back to the launch's registers for the code that all warps share, behind the barrier: every softmax warp has had its larger share.
+    if (warp < W_MMA) asm volatile("setmaxnreg.dec.sync.aligned.u32 168;");
+    else asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
     if (warp == W_MMA) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(P::COLS) : "memory");
     if (!parts) return;
 
@@ -843,6 +993,9 @@ int launch_tiles(const CrossArgs& A, const CUtensorMap& km, const CUtensorMap& v
     if (cudaGetDevice(&dev) != cudaSuccess || dev > 63) return TCQ_ERR_DEVICE;
     if (!held[dev][1].load(std::memory_order_acquire)) {
         if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, P::BYTES) != cudaSuccess) return TCQ_ERR_LAUNCH;
+        // the register shares of the roles are taken from what the launch gives the CTA: less would leave them waiting
+        cudaFuncAttributes fa;
+        if (cudaFuncGetAttributes(&fa, kern) != cudaSuccess || fa.numRegs != P::LAUNCH_REGS) return TCQ_ERR_LAUNCH;
         for (int s = 8; s >= 1; --s) {
             int n = 0;
             cfg.gridDim = dim3(s);
@@ -897,38 +1050,44 @@ template <int DT, int DP>
 int launch_rows(const CrossArgs& A, const CUtensorMap& km, const CUtensorMap& vm, void* stream) {
     typedef Rows<DP> P;
     const auto kern = k_cross_rows<DT, DP>;
-    int wm = 0;
-    while (wm < 3 && (16 << wm) < A.rows) ++wm;
-    const int rings = kRowWarps >> wm, row_blocks = (A.rows + (16 << wm) - 1) / (16 << wm);
-    const int block_rows = (((A.rows + row_blocks - 1) / row_blocks) + 15) & ~15;
-    const i64 units = (i64)A.B * A.kv_heads * row_blocks;
+    RowsPlan R = {};
+    while (R.wm_log2 < 2 && (16 << R.wm_log2) < A.rows) ++R.wm_log2;
+    const int rings = kRowWarps >> R.wm_log2;
+    R.row_blocks = (A.rows + (16 << R.wm_log2) - 1) / (16 << R.wm_log2);
+    R.block_rows = (((A.rows + R.row_blocks - 1) / R.row_blocks) + 15) & ~15;
+    const i64 units = (i64)A.B * A.kv_heads * R.row_blocks;
+    if (units > 0x7fffffff / 8) return TCQ_ERR_SHAPE;
     const int chunks = (A.N + P::CHUNK - 1) / P::CHUNK, sms = tcq_sm_count();
-    int splits = 1;
-    while (splits < 8 && units * splits < 2 * sms && chunks >= 2 * rings * splits * 2) splits *= 2;
-    const int each = (chunks + rings * splits - 1) / (rings * splits);
-    const int stages = each + 1 < 3 ? each + 1 : 3;
-    if (units * splits > 0x7fffffff) return TCQ_ERR_SHAPE;
+    R.units = (int)units;
+    // whole units where they are enough for two CTAs on every SM
+    R.whole = units >= (i64)2 * sms * rings;
+    R.splits = 1;
+    if (!R.whole)
+        while (R.splits < 8 && units * R.splits < 2 * sms && chunks >= 2 * rings * R.splits * 2) R.splits *= 2;
+    const int each = R.whole ? chunks : (chunks + rings * R.splits - 1) / (rings * R.splits);
+    const int most = rings == 1 ? P::MOST : 3;
+    R.stages = each + 1 < most ? each + 1 : most;
+    R.by_blocks = make_fastdiv((unsigned)R.row_blocks), R.by_heads = make_fastdiv((unsigned)A.kv_heads), R.by_splits = make_fastdiv((unsigned)R.splits);
     static std::atomic<unsigned long long> set{0};
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev > 63) return TCQ_ERR_DEVICE;
     if (!(set.load(std::memory_order_relaxed) >> dev & 1)) {
-        if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, P::bytes(kRowWarps, 3)) != cudaSuccess)
-            return TCQ_ERR_LAUNCH;
+        if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, P::bytes(kRowWarps, 3)) != cudaSuccess) return TCQ_ERR_LAUNCH;
         set.fetch_or(1ull << dev, std::memory_order_relaxed);
     }
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(units * splits));
-    cfg.blockDim = dim3(kRowWarps * 32);
-    cfg.dynamicSmemBytes = P::bytes(rings, stages);
+    cfg.gridDim = dim3((unsigned)(R.whole ? (units + rings - 1) / rings : units * R.splits));
+    cfg.blockDim = dim3(kRowThreads);
+    cfg.dynamicSmemBytes = P::bytes(rings, R.stages);
     cfg.stream = (cudaStream_t)stream;
     cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = splits, attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = R.splits, attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 2;
-    return cudaLaunchKernelEx(&cfg, kern, A, km, vm, wm, stages, splits, row_blocks, block_rows) == cudaSuccess ? TCQ_OK : TCQ_ERR_LAUNCH;
+    cfg.numAttrs = R.splits > 1 ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, kern, A, km, vm, R) == cudaSuccess ? TCQ_OK : TCQ_ERR_LAUNCH;
 }
 
 // Call f(integral_constant<int, DP>) for the head width rounded up to one that is built.
