@@ -120,11 +120,11 @@ struct Rows {
 };
 struct RowsPlan {
     int wm_log2, stages, splits, whole, row_blocks, block_rows, units;
-    FastDiv by_blocks, by_heads, by_splits;
+    FastDiv by_blocks, by_heads, by_splits, by_workers;
 };
 
 template <int DT, int DP>
-__global__ void __launch_bounds__(kRowThreads, DP <= 64 ? 3 : 2)
+__global__ void __launch_bounds__(kRowThreads, DP <= 48 ? 4 : DP <= 64 ? 3 : 2)
 k_cross_rows(const CrossArgs A, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const RowsPlan R) {
     typedef Rows<DP> P;
     constexpr int KS = DP / 16, NT = DP / 8, NK = P::CHUNK / 8, RINGS = kRowWarps;
@@ -158,74 +158,70 @@ k_cross_rows(const CrossArgs A, const __grid_constant__ CUtensorMap kmap, const 
 
     if (warp == kRowWarps) {
         // ------------------------------------------------------------------------------------------------ the requests
-        int pc[RINGS] = {}, c1[RINGS] = {}, ub[RINGS] = {}, uh[RINGS] = {}, ulen[RINGS] = {};
-        unsigned char pm[RINGS] = {};
-        auto look = [&](int k) {                                   // the truth values of chunk pc
-            if (A.mask && pc[k] < c1[k]) {
-                const int j = pc[k] * P::CHUNK + lane;
-                pm[k] = lane < P::CHUNK && j < ulen[k] ? A.mask[ub[k] * A.mask_sb + j] : 0;
-            }
-        };
-#pragma unroll
-        for (int k = 0; k < RINGS; ++k) {
-            int rb;
-            const bool there = k < rings && unit_of(k, rb, ub[k], uh[k]);
-            ulen[k] = there ? states_of(A, ub[k]) : 0;
-        }
-#pragma unroll
-        for (int k = 0; k < RINGS; ++k) {
+        // Lane k serves ring k, so that a pass over the rings costs as much as one of them.
+        int rb, b = 0, h = 0, len = 0, pc = 0, c1 = 0;
+        if (lane < rings && unit_of(lane, rb, b, h)) {
+            len = states_of(A, b);
             // this ring's chunks: all, or its run of the cluster's
-            const int chunks = (ulen[k] + P::CHUNK - 1) / P::CHUNK, workers = R.whole ? 1 : R.splits * rings, w = R.whole ? 0 : rank * rings + k;
-            const int each = chunks / workers, more = chunks - each * workers;
-            pc[k] = w * each + min(w, more), c1[k] = k < rings ? pc[k] + each + (w < more) : pc[k];
-            look(k);
+            c1 = (len + P::CHUNK - 1) / P::CHUNK;
+            if (!R.whole) {
+                const int w = rank * rings + lane, each = (int)fdiv((unsigned)c1, R.by_workers), more = c1 - each * (R.splits * rings);
+                pc = w * each + min(w, more), c1 = pc + each + (w < more);
+            }
         }
-        u32 ended = 0;
-        bool ok = true;
+        bool more = lane < rings, ok = true;
         int slot = 0, use = 0;
-        for (; ok && ended != (1u << rings) - 1; ++slot) {
-            if (slot == stages) slot = 0, ++use;
-#pragma unroll
-            for (int k = 0; k < RINGS; ++k) {
-                if (k >= rings || (ended >> k & 1) || !ok) continue;
-                const int s = k * stages + slot;
-                u32 bits = 0;
-                int at = -1;
-                while (pc[k] < c1[k]) {
-                    const int n = ulen[k] - pc[k] * P::CHUNK;
-                    bits = A.mask ? __ballot_sync(0xffffffffu, pm[k] != 0) : n >= P::CHUNK ? kAll : (1u << n) - 1u;
-                    at = pc[k]++;
-                    look(k);
-                    if (bits) break;
+        u32 s = lane * stages, dst = sbase + s * P::STAGE, full = bars + 16 * s;      // of this lane's ring and the pass's stage
+        while (ok && __any_sync(0xffffffffu, more)) {
+            u32 bits = 0;
+            if (!A.mask) {
+                const int n = len - pc * P::CHUNK;
+                bits = n >= P::CHUNK ? kAll : n <= 0 ? 0u : (1u << n) - 1u;
+                if (pc >= c1) bits = 0;
+            } else {
+                // all lanes look at a ring's next chunks until one holds a state
+                for (int k = 0; k < rings; ++k) {
+                    int at = __shfl_sync(0xffffffffu, pc, k);
+                    const int end = __shfl_sync(0xffffffffu, c1, k), n = __shfl_sync(0xffffffffu, len, k);
+                    const unsigned char* row = A.mask + __shfl_sync(0xffffffffu, b, k) * A.mask_sb;
+                    u32 x = 0;
+                    for (; at < end; ++at) {
+                        const int j = at * P::CHUNK + lane;
+                        x = __ballot_sync(0xffffffffu, lane < P::CHUNK && j < n && row[j] != 0);
+                        if (x) break;
+                    }
+                    if (lane == k) pc = at, bits = x;
                 }
-                if (!bits) at = -1, ended |= 1u << k;
-                if (use) ok = mbar_wait_suspended(bars + 16 * s + 8, (use - 1) & 1, abort_flag, &g_tcq_cross_error);
-                if (ok && elect_one()) {
-                    meta[s] = make_int2(at, (int)bits);
-                    if (at < 0) {
-                        mbar_arrive(bars + 16 * s);
+            }
+            if (more) {
+                if (use) ok = mbar_wait_suspended(full + 8, (use - 1) & 1, abort_flag, &g_tcq_cross_error);
+                if (ok) {
+                    meta[s] = make_int2(bits ? pc : -1, (int)bits);
+                    if (!bits) {
+                        mbar_arrive(full);
+                        more = false;
                     } else {
-                        const u32 dst = sbase + s * P::STAGE;
-                        mbar_expect_tx(bars + 16 * s, P::STAGE);
+                        mbar_expect_tx(full, P::STAGE);
 #pragma unroll
-                        for (int a = 0; a < P::ATOMS; ++a)
-                            tma_load_4d(dst + a * (P::CHUNK * 128), &kmap, bars + 16 * s, 64 * a, at * P::CHUNK, uh[k], ub[k] * A.kb);
+                        for (int a = 0; a < P::ATOMS; ++a) tma_load_4d(dst + a * (P::CHUNK * 128), &kmap, full, 64 * a, pc * P::CHUNK, h, b * A.kb);
 #pragma unroll
-                        for (int a = 0; a < P::ATOMS; ++a)
-                            tma_load_4d(dst + P::HALF + a * (P::CHUNK * 128), &vmap, bars + 16 * s, 64 * a, at * P::CHUNK, uh[k], ub[k] * A.vb);
+                        for (int a = 0; a < P::ATOMS; ++a) tma_load_4d(dst + P::HALF + a * (P::CHUNK * 128), &vmap, full, 64 * a, pc * P::CHUNK, h, b * A.vb);
+                        ++pc;
                     }
                 }
-                __syncwarp();
+            }
+            ok = __all_sync(0xffffffffu, ok);
+            ++s, dst += P::STAGE, full += 16;
+            if (++slot == stages) slot = 0, ++use, s -= stages, dst -= stages * P::STAGE, full -= 16 * stages;
+        }
+        if (*abort_flag && lane < rings) {                         // copies on their way land before their stages are left
+            volatile int never = 0;
+            for (int i = 0; i < stages; ++i) {
+                const int uses = use + (i < slot);                 // at most: a barrier that saw fewer is waited for in vain, within the limit
+                if (uses) mbar_wait_suspended(bars + 16 * (lane * stages + i), (uses - 1) & 1, &never, &g_tcq_cross_error, kWaitNs / 100);
             }
         }
-        if (*abort_flag) {                                         // copies on their way land before their stages are left
-            volatile int never = 0;
-            for (int k = 0; k < rings; ++k)
-                for (int s = 0; s < stages; ++s) {
-                    const int uses = use + (s < slot);             // at most: a barrier that saw fewer is waited for in vain, within the limit
-                    if (uses) mbar_wait_suspended(bars + 16 * (k * stages + s), (uses - 1) & 1, &never, &g_tcq_cross_error, kWaitNs / 100);
-                }
-        }
+        __syncwarp();
         if (R.whole || rings * R.splits == 1) return;
         __syncthreads();
         if (R.splits > 1) cluster_barrier(), cluster_barrier();
@@ -376,29 +372,16 @@ k_cross_rows(const CrossArgs A, const __grid_constant__ CUtensorMap kmap, const 
     }
     const i64 out_st = (i64)A.heads * A.D, out_sb = (i64)A.T * out_st;
     if (R.whole || rings * R.splits == 1) {
-        // four lanes hold 8 elements of a row in pairs: turned among them into 16-byte pieces, of which each lane stores every fourth
+        // (sixteen bytes a lane, turned among the four of a row by shuffles, took ten times as long)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
             const int r = r0 + 16 * wm + g + 8 * e;
             const float f = l[e] != 0.f ? 1.f / l[e] : 0.f;
-            uint4* dst = reinterpret_cast<uint4*>(A.out + row_at(A, b, h, min(r, A.rows - 1), out_sb, out_st));
+            u32* dst = reinterpret_cast<u32*>(A.out + row_at(A, b, h, min(r, A.rows - 1), out_sb, out_st));
+            if (r < r1)
 #pragma unroll
-            for (int i = 0; i < NT; i += 4) {
-                u32 y[4], z[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) y[j] = i + j < NT ? pack2<DT>(o[i + j < NT ? i + j : 0][2 * e] * f, o[i + j < NT ? i + j : 0][2 * e + 1] * f) : 0u;
-                // lane t gets piece i + t: word j of it is lane j's y[t]
-#pragma unroll
-                for (int d = 0; d < 4; ++d) {
-                    const int mine = t ^ d;                        // give y[t ^ d] to lane t ^ d, take its y[t]
-                    const u32 give = mine == 0 ? y[0] : mine == 1 ? y[1] : mine == 2 ? y[2] : y[3];
-                    const u32 got = d ? __shfl_xor_sync(0xffffffffu, give, d) : give;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        if (j == mine) z[j] = got;
-                }
-                if (r < r1 && 8 * (i + t) < A.D) dst[i + t] = make_uint4(z[0], z[1], z[2], z[3]);
-            }
+                for (int i = 0; i < NT; ++i)
+                    if (8 * i < A.D) dst[4 * i + t] = weights2<DT>(o[i][2 * e] * f, o[i][2 * e + 1] * f);
         }
         return;
     }
@@ -1067,7 +1050,7 @@ int launch_rows(const CrossArgs& A, const CUtensorMap& km, const CUtensorMap& vm
     const int each = R.whole ? chunks : (chunks + rings * R.splits - 1) / (rings * R.splits);
     const int most = rings == 1 ? P::MOST : 3;
     R.stages = each + 1 < most ? each + 1 : most;
-    R.by_blocks = make_fastdiv((unsigned)R.row_blocks), R.by_heads = make_fastdiv((unsigned)A.kv_heads), R.by_splits = make_fastdiv((unsigned)R.splits);
+    R.by_blocks = make_fastdiv((unsigned)R.row_blocks), R.by_heads = make_fastdiv((unsigned)A.kv_heads), R.by_splits = make_fastdiv((unsigned)R.splits), R.by_workers = make_fastdiv((unsigned)(R.splits * rings));
     static std::atomic<unsigned long long> set{0};
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev > 63) return TCQ_ERR_DEVICE;
