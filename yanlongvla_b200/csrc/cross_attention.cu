@@ -106,12 +106,13 @@ TCQ_HD void mma16816(float (&d)[4], u32 a0, u32 a1, u32 a2, u32 a3, u32 b0, u32 
 }
 
 // Shared memory of a CTA: the rings, then their barriers and what each stage holds. Parts overlay the rings.
-template <int DP>
+template <int DP, int MT>
 struct Rows {
     static constexpr int CHUNK = DP <= 64 ? 32 : 16;                                                 // states
     static constexpr int ATOMS = (DP + 63) / 64, HALF = ATOMS * CHUNK * 128, STAGE = 2 * HALF;       // bytes of a chunk's keys, of both: 8 KB
     static constexpr int PITCH = DP + 4;                                                             // floats of a part's row
-    static constexpr int PARTS = kRowWarps * 16 * PITCH * 4, ML = 16 * kRowWarps * 8;                // parts, then m and l of the CTA's rows
+    static constexpr int ROWS = 16 * MT;                                                             // of a warp
+    static constexpr int PARTS = kRowWarps * ROWS * PITCH * 4, ML = ROWS * kRowWarps * 8;               // parts, then m and l of the CTA's rows
     static constexpr int MOST = 6;                                                                   // stages of a ring, at most
     static constexpr int ring_bytes(int rings, int stages) {
         return rings * stages * STAGE > PARTS + ML ? rings * stages * STAGE : PARTS + ML;
@@ -123,10 +124,10 @@ struct RowsPlan {
     FastDiv by_blocks, by_heads, by_splits, by_workers;
 };
 
-template <int DT, int DP>
-__global__ void __launch_bounds__(kRowThreads, DP <= 48 ? 4 : DP <= 64 ? 3 : 2)
+template <int DT, int DP, int MT>
+__global__ void __launch_bounds__(kRowThreads, MT == 2 ? 2 : DP <= 48 ? 4 : DP <= 64 ? 3 : 2)
 k_cross_rows(const CrossArgs A, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const RowsPlan R) {
-    typedef Rows<DP> P;
+    typedef Rows<DP, MT> P;
     constexpr int KS = DP / 16, NT = DP / 8, NK = P::CHUNK / 8, RINGS = kRowWarps;
     constexpr u32 kAll = (u32)((1ull << P::CHUNK) - 1);
     extern __shared__ __align__(1024) char smem_rows[];
@@ -228,46 +229,56 @@ k_cross_rows(const CrossArgs A, const __grid_constant__ CUtensorMap kmap, const 
         return;
     }
 
-    // ------------------------------------------------------------------------------------------------ this warp's 16 rows: g and g + 8
+    // ------------------------------------------------------------------------------------------------ this warp's rows: 16 j + g, + 8
     int rb, b, h;
     const bool there = unit_of(kg, rb, b, h);
-    const int r0 = rb * R.block_rows, r1 = there ? min(A.rows, r0 + R.block_rows) : 0;
-    const bool live = r0 + 16 * wm < r1;                           // a warp without a row only keeps the barriers going
-    u32 q[KS][4];
+    const int w0 = P::ROWS * wm, r0 = rb * R.block_rows, r1 = there ? min(A.rows, r0 + R.block_rows) : 0;
+    const bool live = r0 + w0 < r1;                                // a warp without a row only keeps the barriers going
+    u32 q[MT][KS][4];
     {
-        const int ra = r0 + 16 * wm + g, rc = ra + 8;
-        const u16* qa = A.q + row_at(A, b, h, min(ra, A.rows - 1), A.q_sb, A.q_st);
-        const u16* qc = A.q + row_at(A, b, h, min(rc, A.rows - 1), A.q_sb, A.q_st);
         const u32 flip = query_flip(A), keep = query_keep(A);
 #pragma unroll
-        for (int k = 0; k < KS; ++k)
+        for (int j = 0; j < MT; ++j)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                const int d = 16 * k + 8 * e + 2 * t;
-                const bool in = d < A.D;
-                q[k][2 * e] = in && ra < r1 ? *reinterpret_cast<const u32*>(qa + d) : 0u;
-                q[k][2 * e + 1] = in && rc < r1 ? *reinterpret_cast<const u32*>(qc + d) : 0u;
+                const int r = r0 + w0 + 16 * j + 8 * e + g;
+                const u16* qr = A.q + row_at(A, b, h, min(r, A.rows - 1), A.q_sb, A.q_st);
+#pragma unroll
+                for (int k = 0; k < KS; ++k)
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        const int d = 16 * k + 8 * x + 2 * t;
+                        q[j][k][2 * x + e] = d < A.D && r < r1 ? *reinterpret_cast<const u32*>(qr + d) : 0u;
+                    }
             }
         if (flip || !keep) {
 #pragma unroll
-            for (int k = 0; k < KS; ++k)
+            for (int j = 0; j < MT; ++j)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) q[k][e] = q[k][e] & keep ^ flip;
+                for (int k = 0; k < KS; ++k)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) q[j][k][e] = q[j][k][e] & keep ^ flip;
         }
     }
     const float c = score_scale(A);
-    float o[NT][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    float o[MT][NT][4], m[MT][2], l[MT][2];
 #pragma unroll
-    for (int i = 0; i < NT; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+    for (int j = 0; j < MT; ++j) {
+        m[j][0] = m[j][1] = -INFINITY, l[j][0] = l[j][1] = 0.f;
+#pragma unroll
+        for (int i = 0; i < NT; ++i) o[j][i][0] = o[j][i][1] = o[j][i][2] = o[j][i][3] = 0.f;
+    }
 
     // One chunk: the scores of its states, weights, O += P V. Matrices of 8 x 8 are read from the swizzled tiles: 16-byte piece p of row r
     // lies at p ^ (r & 7). Products that add to the same registers are issued as far apart as they can be.
     const int row8 = lane & 7, row16 = lane & 15;
     auto chunk = [&](auto masked_c, u32 bits, u32 kt, u32 vt) {
         constexpr bool MASKED = decltype(masked_c)::value;
-        float s[NK][4];
+        float s[MT][NK][4];
 #pragma unroll
-        for (int n = 0; n < NK; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+        for (int j = 0; j < MT; ++j)
+#pragma unroll
+            for (int n = 0; n < NK; ++n) s[j][n][0] = s[j][n][1] = s[j][n][2] = s[j][n][3] = 0.f;
 #pragma unroll
         for (int k = 0; k < KS; k += 2) {
             const int p = 2 * k + (lane >> 3);                     // pieces of 8 elements: two of step k, two of step k + 1
@@ -275,11 +286,12 @@ k_cross_rows(const CrossArgs A, const __grid_constant__ CUtensorMap kmap, const 
 #pragma unroll
             for (int n = 0; n < NK; ++n) ldsm4(kt + (p >> 3) * (P::CHUNK * 128) + (8 * n + row8) * 128 + (((p & 7) ^ row8) << 4), f[n]);
 #pragma unroll
-            for (int n = 0; n < NK; ++n) mma16816<DT>(s[n], q[k][0], q[k][1], q[k][2], q[k][3], f[n][0], f[n][1]);
-            if (k + 1 < KS) {
+            for (int x = 0; x < 2 && k + x < KS; ++x)
 #pragma unroll
-                for (int n = 0; n < NK; ++n) mma16816<DT>(s[n], q[k + 1][0], q[k + 1][1], q[k + 1][2], q[k + 1][3], f[n][2], f[n][3]);
-            }
+                for (int n = 0; n < NK; ++n)
+#pragma unroll
+                    for (int j = 0; j < MT; ++j)
+                        mma16816<DT>(s[j][n], q[j][k + x][0], q[j][k + x][1], q[j][k + x][2], q[j][k + x][3], f[n][2 * x], f[n][2 * x + 1]);
         }
         if (MASKED) {
             const u32 w = bits >> (2 * t);
@@ -287,50 +299,61 @@ k_cross_rows(const CrossArgs A, const __grid_constant__ CUtensorMap kmap, const 
             for (int n = 0; n < NK; ++n)
 #pragma unroll
                 for (int e = 0; e < 2; ++e)
-                    if (!(w >> (8 * n + e) & 1)) s[n][e] = s[n][2 + e] = -INFINITY;
-        }
-        float top[2];
+                    if (!(w >> (8 * n + e) & 1)) {
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            top[e] = fmaxf(s[0][2 * e], s[0][2 * e + 1]);
-#pragma unroll
-            for (int n = 1; n < NK; ++n) top[e] = max3(top[e], s[n][2 * e], s[n][2 * e + 1]);
+                        for (int j = 0; j < MT; ++j) s[j][n][e] = s[j][n][2 + e] = -INFINITY;
+                    }
         }
-        top[0] *= c, top[1] *= c;
-        if (__any_sync(0xffffffffu, top[0] > m[0] + kSlack || top[1] > m[1] + kSlack)) {
-            float f[2];
+        float top[MT][2];
+        bool above = false;
+#pragma unroll
+        for (int j = 0; j < MT; ++j)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 1));
-                top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 2));
-                const bool move = top[e] > m[e] + kSlack;
-                f[e] = move ? ex2(m[e] - top[e]) : 1.f;
-                if (move) m[e] = top[e];
-                l[e] *= f[e];
+                top[j][e] = fmaxf(s[j][0][2 * e], s[j][0][2 * e + 1]);
+#pragma unroll
+                for (int n = 1; n < NK; ++n) top[j][e] = max3(top[j][e], s[j][n][2 * e], s[j][n][2 * e + 1]);
+                top[j][e] *= c;
+                above = above || top[j][e] > m[j][e] + kSlack;
             }
+        if (__any_sync(0xffffffffu, above)) {
 #pragma unroll
-            for (int i = 0; i < NT; ++i) o[i][0] *= f[0], o[i][1] *= f[0], o[i][2] *= f[1], o[i][3] *= f[1];
+            for (int j = 0; j < MT; ++j) {
+                float f[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    float x = top[j][e];
+                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+                    const bool move = x > m[j][e] + kSlack;
+                    f[e] = move ? ex2(m[j][e] - x) : 1.f;
+                    if (move) m[j][e] = x;
+                    l[j][e] *= f[e];
+                }
+#pragma unroll
+                for (int i = 0; i < NT; ++i) o[j][i][0] *= f[0], o[j][i][1] *= f[0], o[j][i][2] *= f[1], o[j][i][3] *= f[1];
+            }
         }
-        const float ba = kRef - (m[0] == -INFINITY ? 0.f : m[0]), bc = kRef - (m[1] == -INFINITY ? 0.f : m[1]);
-        const u64 c2 = pair(c, c), ba2 = pair(ba, ba), bc2 = pair(bc, bc);
-        u64 sum[2] = {0, 0};
-        u32 w[NK][2];                                              // weights of rows g and g + 8
+        const u64 c2 = pair(c, c);
+        u32 w[MT][NK][2];                                          // weights of rows g and g + 8
 #pragma unroll
-        for (int n = 0; n < NK; ++n)
+        for (int j = 0; j < MT; ++j)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
+                const float base = kRef - (m[j][e] == -INFINITY ? 0.f : m[j][e]);
+                const u64 b2 = pair(base, base);
+                u64 sum = 0;
                 float lo, hi;
-                unpair(fma2(pair(s[n][2 * e], s[n][2 * e + 1]), c2, e ? bc2 : ba2), lo, hi);
-                lo = ex2(lo), hi = ex2(hi);
-                sum[e] = add2(sum[e], pair(lo, hi));
-                w[n][e] = weights2<DT>(lo, hi);
-            }
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            float lo, hi;
-            unpair(sum[e], lo, hi);
-            l[e] += lo + hi;
-        }
+                for (int n = 0; n < NK; ++n) {
+                    unpair(fma2(pair(s[j][n][2 * e], s[j][n][2 * e + 1]), c2, b2), lo, hi);
+                    lo = ex2(lo), hi = ex2(hi);
+                    sum = add2(sum, pair(lo, hi));
+                    w[j][n][e] = weights2<DT>(lo, hi);
+                }
+                unpair(sum, lo, hi);
+                l[j][e] += lo + hi;
+            }
 #pragma unroll
         for (int k = 0; k < NK / 2; ++k) {
             // what lies where no state is may be anything, NaN too: this lane's keys 16 k + 2 t, + 1 and 8 further
@@ -345,8 +368,12 @@ k_cross_rows(const CrossArgs A, const __grid_constant__ CUtensorMap kmap, const 
                 u32 f[4];
                 const int p = i + (lane >> 4);
                 ldsm4t(vt + (p >> 3) * (P::CHUNK * 128) + (16 * k + row16) * 128 + (((p & 7) ^ row8) << 4), f);
-                mma16816<DT>(o[i], w[2 * k][0], w[2 * k][1], w[2 * k + 1][0], w[2 * k + 1][1], MASKED ? f[0] & z0 : f[0], MASKED ? f[1] & z1 : f[1]);
-                mma16816<DT>(o[i + 1], w[2 * k][0], w[2 * k][1], w[2 * k + 1][0], w[2 * k + 1][1], MASKED ? f[2] & z0 : f[2], MASKED ? f[3] & z1 : f[3]);
+                if (MASKED) f[0] &= z0, f[1] &= z1, f[2] &= z0, f[3] &= z1;
+#pragma unroll
+                for (int x = 0; x < 2; ++x)
+#pragma unroll
+                    for (int j = 0; j < MT; ++j)
+                        mma16816<DT>(o[j][i + x], w[j][2 * k][0], w[j][2 * k][1], w[j][2 * k + 1][0], w[j][2 * k + 1][1], f[2 * x], f[2 * x + 1]);
             }
         }
     };
@@ -366,37 +393,43 @@ k_cross_rows(const CrossArgs A, const __grid_constant__ CUtensorMap kmap, const 
         if (++slot == (kg + 1) * stages) slot = kg * stages, phase ^= 1;
     }
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-        l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
-        l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
-    }
+    for (int j = 0; j < MT; ++j)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            l[j][e] += __shfl_xor_sync(0xffffffffu, l[j][e], 1);
+            l[j][e] += __shfl_xor_sync(0xffffffffu, l[j][e], 2);
+        }
     const i64 out_st = (i64)A.heads * A.D, out_sb = (i64)A.T * out_st;
     if (R.whole || rings * R.splits == 1) {
         // (sixteen bytes a lane, turned among the four of a row by shuffles, took ten times as long)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            const int r = r0 + 16 * wm + g + 8 * e;
-            const float f = l[e] != 0.f ? 1.f / l[e] : 0.f;
-            u32* dst = reinterpret_cast<u32*>(A.out + row_at(A, b, h, min(r, A.rows - 1), out_sb, out_st));
-            if (r < r1)
+        for (int j = 0; j < MT; ++j)
 #pragma unroll
-                for (int i = 0; i < NT; ++i)
-                    if (8 * i < A.D) dst[4 * i + t] = weights2<DT>(o[i][2 * e] * f, o[i][2 * e + 1] * f);
-        }
+            for (int e = 0; e < 2; ++e) {
+                const int r = r0 + w0 + 16 * j + 8 * e + g;
+                const float f = l[j][e] != 0.f ? 1.f / l[j][e] : 0.f;
+                u32* dst = reinterpret_cast<u32*>(A.out + row_at(A, b, h, min(r, A.rows - 1), out_sb, out_st));
+                if (r < r1)
+#pragma unroll
+                    for (int i = 0; i < NT; ++i)
+                        if (8 * i < A.D) dst[4 * i + t] = weights2<DT>(o[j][i][2 * e] * f, o[j][i][2 * e + 1] * f);
+            }
         return;
     }
     // ---- parts to shared memory (every chunk has arrived), then added: four elements of a row a thread
     __syncthreads();
     float* const parts = reinterpret_cast<float*>(smem_rows);
     {
-        float* part = parts + (size_t)(kg * WM + wm) * 16 * P::PITCH;
+        float* part = parts + (size_t)(kg * WM + wm) * P::ROWS * P::PITCH;
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            float* row = part + (g + 8 * e) * P::PITCH;
+        for (int j = 0; j < MT; ++j)
 #pragma unroll
-            for (int i = 0; i < NT; ++i) *reinterpret_cast<float2*>(row + 8 * i + 2 * t) = make_float2(o[i][2 * e], o[i][2 * e + 1]);
-            if (t == 0) *reinterpret_cast<float2*>(row + DP) = make_float2(m[e], l[e]);
-        }
+            for (int e = 0; e < 2; ++e) {
+                float* row = part + (16 * j + 8 * e + g) * P::PITCH;
+#pragma unroll
+                for (int i = 0; i < NT; ++i) *reinterpret_cast<float2*>(row + 8 * i + 2 * t) = make_float2(o[j][i][2 * e], o[j][i][2 * e + 1]);
+                if (t == 0) *reinterpret_cast<float2*>(row + DP) = make_float2(m[j][e], l[j][e]);
+            }
     }
     const int rows = r1 - r0;
     // the factor of a part with reference m and sum l next to others of reference up to top: a part without weight adds nothing, unless its
@@ -418,8 +451,8 @@ k_cross_rows(const CrossArgs A, const __grid_constant__ CUtensorMap kmap, const 
         for (int k = 0; k < RINGS; ++k) {
             ml[k] = make_float2(-INFINITY, 0.f), v[k] = y;
             if (k < rings) {
-                ml[k] = *reinterpret_cast<const float2*>(p + k * WM * 16 * P::PITCH + DP);
-                v[k] = *reinterpret_cast<const float4*>(p + k * WM * 16 * P::PITCH + d);
+                ml[k] = *reinterpret_cast<const float2*>(p + k * WM * P::ROWS * P::PITCH + DP);
+                v[k] = *reinterpret_cast<const float4*>(p + k * WM * P::ROWS * P::PITCH + d);
             }
             top = fmaxf(top, ml[k].x);
         }
@@ -1029,21 +1062,27 @@ bool encode(CUtensorMap* map, const void* p, int dtype, int D, int N, int heads,
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int DT, int DP>
+template <int DT, int DP, int MT>
 int launch_rows(const CrossArgs& A, const CUtensorMap& km, const CUtensorMap& vm, void* stream) {
-    typedef Rows<DP> P;
-    const auto kern = k_cross_rows<DT, DP>;
+    typedef Rows<DP, MT> P;
+    const auto kern = k_cross_rows<DT, DP, MT>;
     RowsPlan R = {};
-    while (R.wm_log2 < 2 && (16 << R.wm_log2) < A.rows) ++R.wm_log2;
+    // as many warps to a unit as its rows want, up to four; of those block heights the one that leaves the fewest warps without rows (272
+    // rows of each of 256 units: nine blocks of 32 rows 17.1 us, three of 128 20.3)
+    int fewest = 1 << 30;
+    for (int w = 2; w >= 0; --w) {
+        const int warps = (A.rows + (P::ROWS << w) - 1) / (P::ROWS << w) << w;
+        if (warps < fewest || (w < 2 && warps == fewest && A.rows <= (P::ROWS << w))) fewest = warps, R.wm_log2 = w;
+    }
     const int rings = kRowWarps >> R.wm_log2;
-    R.row_blocks = (A.rows + (16 << R.wm_log2) - 1) / (16 << R.wm_log2);
-    R.block_rows = (((A.rows + R.row_blocks - 1) / R.row_blocks) + 15) & ~15;
+    R.row_blocks = (A.rows + (P::ROWS << R.wm_log2) - 1) / (P::ROWS << R.wm_log2);
+    R.block_rows = (((A.rows + R.row_blocks - 1) / R.row_blocks) + P::ROWS - 1) & ~(P::ROWS - 1);
     const i64 units = (i64)A.B * A.kv_heads * R.row_blocks;
     if (units > 0x7fffffff / 8) return TCQ_ERR_SHAPE;
     const int chunks = (A.N + P::CHUNK - 1) / P::CHUNK, sms = tcq_sm_count();
     R.units = (int)units;
-    // whole units where they are enough for two CTAs on every SM
-    R.whole = units >= (i64)2 * sms * rings;
+    // whole units where they are enough for a CTA on every SM
+    R.whole = units >= (i64)sms * rings;
     R.splits = 1;
     if (!R.whole)
         while (R.splits < 8 && units * R.splits < 2 * sms && chunks >= 2 * rings * R.splits * 2) R.splits *= 2;
@@ -1110,7 +1149,7 @@ int tcq_cross_attention(const void* q, int64_t q_sb, int64_t q_st, const void* k
     CUtensorMap km, vm;
     // few rows or few states: products of 16 rows; else tiles of 128 rows and 128 states
     const bool tiles = rows > 32 && N >= 512;
-    const int box = tiles ? kTile : by_width(head_dim, [](auto d) { return Rows<decltype(d)::value>::CHUNK; });
+    const int box = tiles ? kTile : by_width(head_dim, [](auto d) { return Rows<decltype(d)::value, 1>::CHUNK; });
     if (!encode(&km, k, dtype, head_dim, N, kv_heads, B, k_st, k_sb, box) || !encode(&vm, v, dtype, head_dim, N, kv_heads, B, v_st, v_sb, box))
         return TCQ_ERR_DEVICE;
     const int group = heads / kv_heads;
@@ -1122,7 +1161,10 @@ int tcq_cross_attention(const void* q, int64_t q_sb, int64_t q_st, const void* k
             if (dtype == TCQ_DT_BF16) return rows <= kTile ? launch_tiles<TCQ_DT_BF16, DP, false>(A, km, vm, stream) : launch_tiles<TCQ_DT_BF16, DP, true>(A, km, vm, stream);
             return rows <= kTile ? launch_tiles<TCQ_DT_F16, DP, false>(A, km, vm, stream) : launch_tiles<TCQ_DT_F16, DP, true>(A, km, vm, stream);
         }
-        return dtype == TCQ_DT_BF16 ? launch_rows<TCQ_DT_BF16, DP>(A, km, vm, stream) : launch_rows<TCQ_DT_F16, DP>(A, km, vm, stream);
+        if constexpr (DP <= 64) {
+            if (rows > 16) return dtype == TCQ_DT_BF16 ? launch_rows<TCQ_DT_BF16, DP, 2>(A, km, vm, stream) : launch_rows<TCQ_DT_F16, DP, 2>(A, km, vm, stream);
+        }
+        return dtype == TCQ_DT_BF16 ? launch_rows<TCQ_DT_BF16, DP, 1>(A, km, vm, stream) : launch_rows<TCQ_DT_F16, DP, 1>(A, km, vm, stream);
     });
 }
 
