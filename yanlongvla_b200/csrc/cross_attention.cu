@@ -65,7 +65,7 @@ TCQ_HD float score_scale(const CrossArgs& A) { return A.scale_log2 == 0.f ? 1.f 
 TCQ_HD u32 query_flip(const CrossArgs& A) { return A.scale_log2 < 0.f ? 0x80008000u : 0u; }
 TCQ_HD u32 query_keep(const CrossArgs& A) { return A.scale_log2 == 0.f ? 0u : ~0u; }
 
-// Two weights, rounded to nearest even (a NaN of any kind stays one); lo in the low half.
+// Two weights or outputs, rounded to nearest even (a NaN of any kind stays one); lo in the low half.
 template <int DT>
 TCQ_HD u32 weights2(float lo, float hi) {
     u32 r;
@@ -73,6 +73,10 @@ TCQ_HD u32 weights2(float lo, float hi) {
     else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
 }
+
+// The factor of a part with reference ml.x and sum ml.y next to others of reference up to top: a part without weight adds nothing, unless
+// its sum is NaN (scores that are NaN move no reference): the row has to say so.
+TCQ_HD float part_factor(float2 ml, float top) { return top == -INFINITY ? (ml.y == ml.y ? 0.f : 1.f) : ml.y != ml.y ? 1.f : ex2(ml.x - top); }
 
 // Weights are 2^(x - m + kRef), m the row's reference, moved only when a score passes it by more than kSlack: below 2^13, so
 // that FP16 holds them with 11 bits from there down to 2^-14.
@@ -432,13 +436,10 @@ k_cross_rows(const CrossArgs A, const __grid_constant__ CUtensorMap kmap, const 
             }
     }
     const int rows = r1 - r0;
-    // the factor of a part with reference m and sum l next to others of reference up to top: a part without weight adds nothing, unless its
-    // sum is NaN (scores that are NaN move no reference): the row has to say so
-    auto factor = [](float2 ml, float top) { return top == -INFINITY ? (ml.y == ml.y ? 0.f : 1.f) : ml.y != ml.y ? 1.f : ex2(ml.x - top); };
     auto store = [&](int row, int d, const float4& y, float sum) {
         const float f = sum != 0.f ? 1.f / sum : 0.f;
         if (d < A.D)
-            *reinterpret_cast<uint2*>(A.out + row_at(A, b, h, r0 + row, out_sb, out_st) + d) = make_uint2(pack2<DT>(y.x * f, y.y * f), pack2<DT>(y.z * f, y.w * f));
+            *reinterpret_cast<uint2*>(A.out + row_at(A, b, h, r0 + row, out_sb, out_st) + d) = make_uint2(weights2<DT>(y.x * f, y.y * f), weights2<DT>(y.z * f, y.w * f));
     };
     asm volatile("barrier.cta.sync 1, %0;" ::"n"(32 * kRowWarps) : "memory");
     for (int i = tid; i < rows * (DP / 4); i += 32 * kRowWarps) {
@@ -458,7 +459,7 @@ k_cross_rows(const CrossArgs A, const __grid_constant__ CUtensorMap kmap, const 
         }
 #pragma unroll
         for (int k = 0; k < RINGS; ++k) {
-            const float f = factor(ml[k], top);
+            const float f = part_factor(ml[k], top);
             sum = __fmaf_rn(ml[k].y, f, sum);
             y.x = __fmaf_rn(v[k].x, f, y.x), y.y = __fmaf_rn(v[k].y, f, y.y), y.z = __fmaf_rn(v[k].z, f, y.z), y.w = __fmaf_rn(v[k].w, f, y.w);
         }
@@ -489,7 +490,7 @@ k_cross_rows(const CrossArgs A, const __grid_constant__ CUtensorMap kmap, const 
         for (int k = 0; k < 8; ++k) top = fmaxf(top, ml[k].x);
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-            const float f = factor(ml[k], top);
+            const float f = part_factor(ml[k], top);
             sum = __fmaf_rn(ml[k].y, f, sum);
             y.x = __fmaf_rn(v[k].x, f, y.x), y.y = __fmaf_rn(v[k].y, f, y.y), y.z = __fmaf_rn(v[k].z, f, y.z), y.w = __fmaf_rn(v[k].w, f, y.w);
         }
@@ -545,10 +546,14 @@ struct TileMeta {
 enum { TBAR_FULL = 0, TBAR_EMPTY = 8, TBAR_CLEAN = 16, TBAR_S = 24, TBAR_P = 26, TBAR_READ = 30, TBAR_O = 32, TBAR_Q = 34, TBAR_END = 35, TBAR_COUNT = 36 };
 
 
+struct TilesPlan {
+    int row_tiles, tile_rows, splits;
+    FastDiv by_tiles, by_heads, by_splits;
+};
+
 template <int DT, int DP, bool ROWS>
 __global__ void __launch_bounds__(Tiles<DP, ROWS>::THREADS, 1)
-k_cross_tiles(const CrossArgs A, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, int row_tiles, int tile_rows,
-              int splits) {
+k_cross_tiles(const CrossArgs A, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const TilesPlan R) {
     typedef Tiles<DP, ROWS> P;
     constexpr int KS = DP / 16;
     constexpr u32 IDESC = DT == TCQ_DT_BF16 ? kIdescBf16 : 0u;
@@ -592,11 +597,11 @@ k_cross_tiles(const CrossArgs A, const __grid_constant__ CUtensorMap kmap, const
     pdl_wait();
 
     // ---- the unit: rows r0 .. r1 - 1 of key head h of sequence b, and this CTA's tiles [k0, k1) of its states
-    const int sp = blockIdx.x % splits, unit = blockIdx.x / splits, rt = unit % row_tiles, bh = unit / row_tiles, b = bh / A.kv_heads,
-              h = bh - b * A.kv_heads;
-    const int r0 = rt * tile_rows, r1 = min(A.rows, r0 + tile_rows);
+    const int splits = R.splits, unit = (int)fdiv(blockIdx.x, R.by_splits), sp = (int)blockIdx.x - unit * splits;
+    const int bh = (int)fdiv((unsigned)unit, R.by_tiles), b = (int)fdiv((unsigned)bh, R.by_heads), h = bh - b * A.kv_heads;
+    const int r0 = (unit - bh * R.row_tiles) * R.tile_rows, r1 = min(A.rows, r0 + R.tile_rows);
     const int len = states_of(A, b), tiles = (len + kTile - 1) / kTile;
-    const int k0 = (int)((i64)tiles * sp / splits), k1 = (int)((i64)tiles * (sp + 1) / splits);
+    const int each = (int)fdiv((unsigned)tiles, R.by_splits), more = tiles - each * splits, k0 = sp * each + min(sp, more), k1 = k0 + each + (sp < more);
     const bool parts = splits > 1 || !ROWS;                   // rows have more than one part
     const bool ragged = A.lens || A.mask;
 
@@ -773,7 +778,7 @@ k_cross_tiles(const CrossArgs A, const __grid_constant__ CUtensorMap kmap, const
                         part[(d / 4 + 1) ^ (gl & XP)] = make_float4(y[4], y[5], y[6], y[7]);
                     } else {
                         reinterpret_cast<uint4*>(smem + P::Q0 + g * P::TB)[gl * (DP / 8) + ((d / 8) ^ (gl & XO))] =
-                            make_uint4(pack2<DT>(y[0], y[1]), pack2<DT>(y[2], y[3]), pack2<DT>(y[4], y[5]), pack2<DT>(y[6], y[7]));
+                            make_uint4(weights2<DT>(y[0], y[1]), weights2<DT>(y[2], y[3]), weights2<DT>(y[4], y[5]), weights2<DT>(y[6], y[7]));
                     }
                 }
             }
@@ -957,28 +962,37 @@ k_cross_tiles(const CrossArgs A, const __grid_constant__ CUtensorMap kmap, const
         const int rows = r1 - r0, s0 = rows * sp / splits, s1 = rows * (sp + 1) / splits, pieces = A.D / 8;
         for (int e = tid; e < (s1 - s0) * pieces; e += P::THREADS) {
             const int row = s0 + e / pieces, c8 = e % pieces;
-            float top = -INFINITY;
-            for (int k = 0; k < splits; ++k)
+            // four parts at a time, all of their loads under way at once
+            constexpr int G = ROWS ? 1 : 2;
+            float top = -INFINITY, acc[8] = {}, sum = 0.f;
+            for (int k0 = 0; k0 < splits * G; k0 += 4) {
+                float2 ml[4];
+                float4 u[4], v[4];
 #pragma unroll
-                for (int g = 0; g < (ROWS ? 1 : 2); ++g) top = fmaxf(top, peer_ld2(peer_addr(sbase + P::ML0 + (g * kTile + row) * 8, k)).x);
-            float acc[8] = {}, sum = 0.f;
-            for (int k = 0; k < splits; ++k)
-#pragma unroll
-                for (int g = 0; g < (ROWS ? 1 : 2); ++g) {
-                    const float2 ml = peer_ld2(peer_addr(sbase + P::ML0 + (g * kTile + row) * 8, k));
-                    const float f = top == -INFINITY ? (ml.y == ml.y ? 0.f : 1.f) : ex2(ml.x - top);
-                    // a part without weight adds nothing, unless its sum is NaN: the row has to say so
-                    if (f == 0.f && ml.y == ml.y) continue;
-                    sum += ml.y * f;
-                    const u32 base = peer_addr(sbase, k) + (g * kTile + row) * (DP * 4);
-                    const float4 u = peer_ld4(base + (((2 * c8) ^ (row & XP)) << 4)), v = peer_ld4(base + (((2 * c8 + 1) ^ (row & XP)) << 4));
-                    acc[0] += u.x * f, acc[1] += u.y * f, acc[2] += u.z * f, acc[3] += u.w * f;
-                    acc[4] += v.x * f, acc[5] += v.y * f, acc[6] += v.z * f, acc[7] += v.w * f;
+                for (int k = 0; k < 4; ++k) {
+                    ml[k] = make_float2(-INFINITY, 0.f), u[k] = v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (k0 + k < splits * G) {
+                        const u32 p = peer_addr(sbase, (k0 + k) / G), at = ((k0 + k) % G) * kTile + row;
+                        ml[k] = peer_ld2(p + P::ML0 + at * 8);
+                        u[k] = peer_ld4(p + at * (DP * 4) + (((2 * c8) ^ (row & XP)) << 4)), v[k] = peer_ld4(p + at * (DP * 4) + (((2 * c8 + 1) ^ (row & XP)) << 4));
+                    }
                 }
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const float both = fmaxf(top, ml[k].x);
+                    const float old = both == -INFINITY ? 1.f : ex2(top - both), f = part_factor(ml[k], both);
+                    top = both;
+                    sum = __fmaf_rn(ml[k].y, f, sum * old);
+                    acc[0] = __fmaf_rn(u[k].x, f, acc[0] * old), acc[1] = __fmaf_rn(u[k].y, f, acc[1] * old);
+                    acc[2] = __fmaf_rn(u[k].z, f, acc[2] * old), acc[3] = __fmaf_rn(u[k].w, f, acc[3] * old);
+                    acc[4] = __fmaf_rn(v[k].x, f, acc[4] * old), acc[5] = __fmaf_rn(v[k].y, f, acc[5] * old);
+                    acc[6] = __fmaf_rn(v[k].z, f, acc[6] * old), acc[7] = __fmaf_rn(v[k].w, f, acc[7] * old);
+                }
+            }
             const float f = sum != 0.f ? 1.f / sum : 0.f;
             u32 w[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) w[j] = sum != 0.f ? pack2<DT>(acc[2 * j] * f, acc[2 * j + 1] * f) : 0u;
+            for (int j = 0; j < 4; ++j) w[j] = sum != 0.f ? weights2<DT>(acc[2 * j] * f, acc[2 * j + 1] * f) : 0u;
             u16* dst = A.out + row_at(A, b, h, r0 + row, (i64)A.T * A.heads * A.D, (i64)A.heads * A.D) + 8 * c8;
             *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
         }
@@ -990,9 +1004,11 @@ template <int DT, int DP, bool ROWS>
 int launch_tiles(const CrossArgs& A, const CUtensorMap& km, const CUtensorMap& vm, void* stream) {
     typedef Tiles<DP, ROWS> P;
     const auto kern = k_cross_tiles<DT, DP, ROWS>;
-    const int most = ROWS ? 2 * kTile : kTile, row_tiles = (A.rows + most - 1) / most;
-    const int tile_rows = (((A.rows + row_tiles - 1) / row_tiles) + 31) & ~31;     // even shares, in warps
-    const i64 units = (i64)A.B * A.kv_heads * row_tiles;
+    const int most = ROWS ? 2 * kTile : kTile;
+    TilesPlan R = {};
+    R.row_tiles = (A.rows + most - 1) / most;
+    R.tile_rows = (((A.rows + R.row_tiles - 1) / R.row_tiles) + 31) & ~31;         // even shares, in warps
+    const i64 units = (i64)A.B * A.kv_heads * R.row_tiles;
     cudaLaunchConfig_t cfg = {};
     cfg.blockDim = dim3(P::THREADS);
     cfg.dynamicSmemBytes = P::BYTES;
@@ -1036,10 +1052,12 @@ int launch_tiles(const CrossArgs& A, const CUtensorMap& km, const CUtensorMap& v
         }
     }
     if (units * splits > 0x7fffffff) return TCQ_ERR_SHAPE;
+    R.splits = splits;
+    R.by_tiles = make_fastdiv((unsigned)R.row_tiles), R.by_heads = make_fastdiv((unsigned)A.kv_heads), R.by_splits = make_fastdiv((unsigned)splits);
     cfg.gridDim = dim3((unsigned)(units * splits));
     attr[0].val.clusterDim.x = splits;
     cfg.numAttrs = 2;
-    return cudaLaunchKernelEx(&cfg, kern, A, km, vm, row_tiles, tile_rows, splits) == cudaSuccess ? TCQ_OK : TCQ_ERR_LAUNCH;
+    return cudaLaunchKernelEx(&cfg, kern, A, km, vm, R) == cudaSuccess ? TCQ_OK : TCQ_ERR_LAUNCH;
 }
 
 // Zeros for queries without states (N = 0).
