@@ -309,7 +309,7 @@ int tcq_kv8_attention(const tcq_kv8_cache* cache, const void* q, int dtype, int6
 /* Pages of the cache shared by several sequences. refs (pages,) int32 counts the table entries that name a page (0: the page is
  * free); a row of a table names its sequence's pages from block 0 on and holds -1 behind them. pages is below 2^30, the
  * sequences of a table number at most TCQ_KV8_MAX_SEQUENCES. Results do not depend on timing. */
-#define TCQ_KV8_MAX_SEQUENCES 8192
+#define TCQ_KV8_MAX_SEQUENCES 4096
 
 /* Sequence b becomes what sequence parent[b] was, all at once: row b names parent[b]'s pages of its lens tokens (pages it had only
  * reserved are not shared), lens[b] is its length. parent[b] = b: unchanged; below 0: empty. Pages that are named no more become free. */

@@ -37,7 +37,7 @@ def test_bookkeeping_refuses(L):
     for call in (fork, free, reserve):
         for name in ('refs', 'table', 'lens', 'more'):
             assert call(**{name: None}) == 4
-        assert call(pages=0) == 1 and call(pages=1 << 30) == 1 and call(blocks=0) == 1 and call(n=0) == 1 and call(n=8193) == 1
+        assert call(pages=0) == 1 and call(pages=1 << 30) == 1 and call(blocks=0) == 1 and call(n=0) == 1 and call(n=4097) == 1
     assert reserve(granted=None) == 4 and reserve(copies=None) == 4
 
 

@@ -133,7 +133,7 @@ def test_large_pools(K, pages, offset):
 
 
 def test_many_sequences(K):
-    n = 8192
+    n = 4096
     s = Both(K, 3 * n, n, 3)
     s.reserve([b % 130 for b in range(n)])
     s.fork([b ^ 1 if b % 3 else b for b in range(n)])
@@ -371,3 +371,15 @@ def test_refusals(K):
     with pytest.raises(K.TcqError):
         K.kv8_compact(c, table, lens, ints([[0], [0]]), table, kept=ints([1]))
     assert K.device_error() == 0
+
+
+def test_compact_bad_numbers_next_to_good_ones(K):
+    """A token of zeros where the number is past the sequence, the tokens next to it as they are."""
+    c = filled(K, 6, 9, 64, 8)                                                 # nine heads: more than a CTA takes at once
+    k0, v0 = c.k[0].clone(), c.v[0].clone()
+    K.kv8_compact(c, ints([[0]]), ints([60]), ints([[64, 1, 2, 3, 4, 5, 6, 60, 8, 9, 10, 11, -1, 13]]), ints([[3]]))
+    assert K.device_error() == 2
+    for j in (1, 2, 3, 4, 5, 6, 8, 9, 10, 11, 13):
+        assert torch.equal(c.k[3, :, j], k0[:, j]) and torch.equal(c.v[3, :, :, j], v0[:, :, j])
+    for j in (0, 7, 12, *range(14, 64)):
+        assert not c.k[3, :, j].any() and not c.v[3, :, :, j].any()

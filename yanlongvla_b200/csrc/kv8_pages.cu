@@ -4,6 +4,7 @@
 // refs[p] counts the table entries that name page p; 0 is a free page. A row of a table names its sequence's pages from block 0 on
 // and -1 behind them. The book-keeping kernels are bound by the chain of their dependent loads (0.6 to 0.8 us each), the copies by HBM.
 #include "memory.cuh"
+#include "tc.cuh"
 
 __device__ int g_tcq_pages_error;
 
@@ -33,18 +34,18 @@ TCQ_HD int clamped(int n, int lo, int hi) {
 TCQ_HD int blocks_of(int tokens) { return tokens / kBlk + (tokens % kBlk != 0); }
 
 // ------------------------------------------------------------------------------------------------ fork
-// Row b becomes what row parent[b] was, all rows at once. A cluster of eight CTAs takes the table's columns, C at a time: a tile of
-// all rows is staged in shared memory, so that rows may change places in the table itself. Lengths are read by every CTA before
-// the cluster's barrier and written by one behind it.
+// Row b becomes what row parent[b] was, all rows at once. A CTA takes C of the table's columns, all rows of them staged in shared memory, so
+// that rows may change places in the table itself. Every CTA reads the lengths; they are changed when all have: behind the barrier of
+// a cluster where eight CTAs hold the table (`alone`), else by a second launch.
 constexpr int kForkCtas = 8, kForkThreads = 512, kForkTile = 64 * 1024;
 
 __global__ void __launch_bounds__(kForkThreads, 1) k_kv8_fork(int* __restrict__ refs, int pages, int* __restrict__ table, int blocks,
-                                                              int* __restrict__ lens, const int* __restrict__ parent, int B, int shift) {
+                                                              int* __restrict__ lens, const int* __restrict__ parent, int B, int shift, int alone) {
     extern __shared__ int s_mem[];
     int *s_from = s_mem, *s_len = s_mem + B, *s_tile = s_mem + 2 * B;      // parent, tokens of the row's old sequence, a tile
     pdl_launch_dependents();
     pdl_wait();
-    const int tid = threadIdx.x, C = 1 << shift, rank = blockIdx.x;
+    const int tid = threadIdx.x, C = 1 << shift, c0 = blockIdx.x * C;
     for (int b = tid; b < B; b += kForkThreads) {
         int p = parent[b];
         if (p >= B) {
@@ -55,34 +56,44 @@ __global__ void __launch_bounds__(kForkThreads, 1) k_kv8_fork(int* __restrict__ 
         s_len[b] = clamped(lens[b], 0, (int)min((i64)blocks * kBlk, (i64)0x7fffffff));
     }
     __syncthreads();
-    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-#pragma unroll 1
-    for (int c0 = rank * C; c0 < blocks; c0 += kForkCtas * C) {
-        const int n = B << shift;
+    if (alone) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    const int n = c0 < blocks ? B << shift : 0;
 #pragma unroll 8
-        for (int i = tid; i < n; i += kForkThreads) {
-            const int b = i >> shift, c = c0 + (i & (C - 1));
-            s_tile[i] = c < blocks ? table[(i64)b * blocks + c] : -1;
-        }
-        __syncthreads();
-        for (int i = tid; i < n; i += kForkThreads) {
-            const int b = i >> shift, c = c0 + (i & (C - 1)), p = s_from[b];
-            if (p == b || c >= blocks) continue;
-            const int old = s_tile[i];
-            int now = p < 0 || c >= blocks_of(s_len[p]) ? -1 : s_tile[(p << shift) + (i & (C - 1))];
-            if (now >= pages) {
-                out_of_range();
-                now = -1;
-            }
-            if (old >= 0 && old < pages) atomicAdd(refs + old, -1);
-            if (now >= 0) atomicAdd(refs + now, 1);
-            if (now != old) table[(i64)b * blocks + c] = now < 0 ? -1 : now;
-        }
-        __syncthreads();
+    for (int i = tid; i < n; i += kForkThreads) {
+        const int b = i >> shift, c = c0 + (i & (C - 1));
+        s_tile[i] = c < blocks ? table[(i64)b * blocks + c] : -1;
     }
+    __syncthreads();
+    for (int i = tid; i < n; i += kForkThreads) {
+        const int b = i >> shift, c = c0 + (i & (C - 1)), p = s_from[b];
+        if (p == b || c >= blocks) continue;
+        const int old = s_tile[i];
+        int now = p < 0 || c >= blocks_of(s_len[p]) ? -1 : s_tile[(p << shift) + (i & (C - 1))];
+        if (now >= pages) {
+            out_of_range();
+            now = -1;
+        }
+        if (old >= 0 && old < pages) atomicAdd(refs + old, -1);
+        if (now >= 0) atomicAdd(refs + now, 1);
+        if (now != old) table[(i64)b * blocks + c] = now < 0 ? -1 : now;
+    }
+    if (!alone) return;
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-    if (rank == 0)
+    if (blockIdx.x == 0)
         for (int b = tid; b < B; b += kForkThreads) lens[b] = s_from[b] < 0 ? 0 : s_len[s_from[b]];
+}
+
+// The lengths after a fork whose table more CTAs have changed.
+__global__ void __launch_bounds__(kForkThreads, 1) k_kv8_fork_lens(int* __restrict__ lens, const int* __restrict__ parent, int B, int most) {
+    extern __shared__ int s_mem[];
+    pdl_launch_dependents();
+    pdl_wait();
+    for (int b = threadIdx.x; b < B; b += kForkThreads) s_mem[b] = min(max(lens[b], 0), most);
+    __syncthreads();
+    for (int b = threadIdx.x; b < B; b += kForkThreads) {
+        const int p = parent[b] >= B ? b : parent[b];
+        lens[b] = p < 0 ? 0 : s_mem[p];
+    }
 }
 
 // ------------------------------------------------------------------------------------------------ free
@@ -151,17 +162,35 @@ TCQ_HD u32 free_mask(const int* refs, int pages, i64 base) {
     return m;
 }
 
+// Where a page's writers are counted: open addressing in shared memory, at least two places to a sequence.
+struct Writers {
+    int *page, *count, *last;
+    u32 mask;
+    TCQ_HD u32 place(int p) const {
+        u32 i = ((u32)p * 2654435761u >> 7) & mask;
+        for (;;) {
+            const int seen = atomicCAS(page + i, -1, p);
+            if (seen == -1 || seen == p) return i;
+            i = (i + 1) & mask;
+        }
+    }
+};
+
 __global__ void __launch_bounds__(kResThreads, 1) k_kv8_reserve(int* refs, int pages, int* __restrict__ table, int blocks,
                                                                 const int* __restrict__ lens, const int* __restrict__ count,
-                                                                int* __restrict__ granted, int* __restrict__ copies, int B, int lanes) {
+                                                                int* __restrict__ granted, int* __restrict__ copies, int B, int lanes, int places) {
     extern __shared__ int s_mem[];
-    int *s_upto = s_mem, *s_first = s_mem + B, *s_begun = s_mem + 2 * B;   // missing pages up to a sequence, first missing block, begun page
+    // missing pages up to a sequence, its first missing block, its begun block's page
+    int *s_upto = s_mem, *s_first = s_mem + B, *s_begun = s_mem + 2 * B;
+    const Writers W = {s_mem + 3 * B, s_mem + 3 * B + places, s_mem + 3 * B + 2 * places, (u32)places - 1};
     __shared__ int s_warp[32];
+    const int tid = threadIdx.x, sub = tid & (lanes - 1), per_pass = kResThreads / lanes;
+    for (int i = tid; i < places; i += kResThreads) W.page[i] = W.last[i] = -1, W.count[i] = 0;
     pdl_launch_dependents();
     pdl_wait();
-    const int tid = threadIdx.x, sub = tid & (lanes - 1), per_pass = kResThreads / lanes;
     const int limit = (int)min((i64)blocks * kBlk, (i64)0x7fffffff);
     const u32 mask0 = free_mask(refs, pages, (i64)tid * kResPer);
+    __syncthreads();
     for (int b0 = 0; b0 < B; b0 += per_pass) {
         const int b = b0 + tid / lanes;
         int missing = 0, first = 0, last = 0, at = -1, cnt = 0;
@@ -174,11 +203,9 @@ __global__ void __launch_bounds__(kResThreads, 1) k_kv8_reserve(int* refs, int p
             if (cnt > 0 && fits) {
                 first = len / kBlk, last = blocks_of(len + cnt);
                 const bool begun = len % kBlk != 0;
-                if (begun) {
-                    at = table[(i64)b * blocks + first];
-                    if ((unsigned)at >= (unsigned)pages) fits = false, at = -1;
-                }
+                if (begun) at = table[(i64)b * blocks + first];
                 for (int j = first + begun + sub; j < last; j += lanes) missing += table[(i64)b * blocks + j] < 0;
+                if (begun && (unsigned)at >= (unsigned)pages) fits = false, at = -1;
             }
         }
         for (int o = 1; o < lanes; o <<= 1) missing += __shfl_xor_sync(0xffffffffu, missing, o);
@@ -187,32 +214,23 @@ __global__ void __launch_bounds__(kResThreads, 1) k_kv8_reserve(int* refs, int p
             const bool want = cnt > 0 && fits;
             s_upto[b] = want ? missing : -1;                                // -1: nothing asked for, or no room in the table
             s_first[b] = want ? last - missing : 0;
-            s_begun[b] = want && at >= 0 && __ldcg(refs + at) > 1 ? at : -1;
+            if (want && at >= 0) {
+                const u32 w = W.place(at);
+                atomicAdd(W.count + w, 1);
+                atomicMax(W.last + w, b);
+            }
+            s_begun[b] = want ? at : -1;
         }
     }
     __syncthreads();
-    // Writers of shared pages let them go; where that leaves none, the last of them (the highest number) keeps the page.
-    for (int b = tid; b < B; b += kResThreads)
-        if (s_begun[b] >= 0) atomicAdd(refs + s_begun[b], -1);
-    __syncthreads();
-    for (int b0 = 0; b0 < B; b0 += kResThreads) {
-        const int b = b0 + tid;
-        if (b < B && s_begun[b] >= 0 && __ldcg(refs + s_begun[b]) <= 0) s_begun[b] |= 1 << 30;
-    }
-    __syncthreads();
-    for (int b = tid; b < B; b += kResThreads)
-        if (s_begun[b] >= 0 && s_begun[b] >> 30) atomicMax(refs + (s_begun[b] & ~(1 << 30)), b + 1);
-    __syncthreads();
+    // A page that others name too is replaced for its writers; where the writers are all who name it, the last of them keeps it.
     for (int b = tid; b < B; b += kResThreads) {
         const int at = s_begun[b];
-        if (at >= 0 && at >> 30) s_begun[b] = __ldcg(refs + (at & ~(1 << 30))) == b + 1 ? -2 - (at & ~(1 << 30)) : at & ~(1 << 30);
+        if (at < 0) continue;
+        const int held = __ldcg(refs + at);
+        const u32 w = W.place(at);
+        if (held <= 1 || (held == W.count[w] && W.last[w] == b)) s_begun[b] = -1;
     }
-    __syncthreads();
-    for (int b = tid; b < B; b += kResThreads)
-        if (s_begun[b] <= -2) {
-            refs[-2 - s_begun[b]] = 1;
-            s_begun[b] = -1;
-        }
     __syncthreads();
     // sequences in order, a run of them to a thread: missing pages up to and with each
     const int run = (B + kResThreads - 1) / kResThreads, r0 = min(B, tid * run), r1 = min(B, r0 + run);
@@ -236,10 +254,8 @@ __global__ void __launch_bounds__(kResThreads, 1) k_kv8_reserve(int* refs, int p
         granted[b] = ok ? count[b] : 0;
         if (!(ok && copied)) copies[b] = copies[B + b] = -1;
         else copies[b] = s_begun[b];
-        if (asked && !ok) {
-            refused = 1;
-            if (copied) atomicAdd(refs + s_begun[b], 1);
-        }
+        if (ok && copied) atomicAdd(refs + s_begun[b], -1);
+        refused |= asked && !ok;
         s_upto[b] = upto;
     }
     if (refused) out_of_range();
@@ -317,36 +333,47 @@ __global__ void __launch_bounds__(256) k_kv8_copy(const __grid_constant__ Layers
 }
 
 // ------------------------------------------------------------------------------------------------ compact
-// A CTA writes one head of one block of new pages, keys (blockIdx.z even) or values, in one layer: for its up to 64 tokens the page
-// and slot they come from, s = the largest of their pages' scales, q' = rint(q (s_old / s)) (a token whose page has that scale
-// keeps its integers). Keys are rows of a token: 16 bytes of one a thread. Values lie token by token along a row, so the source
-// pages' tiles pass through shared memory, from which four tokens' bytes make a word.
+// A CTA writes one block of new pages, keys (blockIdx.z even) or values, in one layer, hg heads one after the other (so that the chain
+// number -> page -> scale is walked once for them): for its up to 64 tokens the page and slot they come from, per head s = the
+// largest of their pages' scales, q' = rint(q (s_old / s)) (a token whose page has that scale keeps its integers). Keys are rows of a
+// token: a thread moves 16 bytes. Values lie token by token along a row: a thread makes words of four tokens, of one or two
+// words where its warp's tokens lie four in a row (whole runs kept), else byte by byte.
 //
 // Quotients of integers q' = q r with 0 <= r <= 1: the byte in a float's low bits (2^23 + 128 + q), its offset taken off, times r,
-// rounded to nearest even by adding 1.5 * 2^23.
-TCQ_HD u32 scaled4(u32 w, const float (&r)[4]) {
-    const u32 u = w ^ 0x80808080u;
-    u32 b[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) b[i] = __float_as_uint((__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7440 + i)) - 8388736.f) * r[i] + 12582912.f);
-    return __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
+// rounded to nearest even by adding 1.5 * 2^23; each step one rounding.
+TCQ_HD u32 scaled4(u32 w, u64 r01, u64 r23) {
+    const u32 u = w ^ 0x80808080u, c = 0x4b000000u;
+    const u64 off = pair(-8388736.f, -8388736.f), big = pair(12582912.f, 12582912.f);
+    const u64 a = pair(__uint_as_float(__byte_perm(u, c, 0x7440)), __uint_as_float(__byte_perm(u, c, 0x7441)));
+    const u64 b = pair(__uint_as_float(__byte_perm(u, c, 0x7442)), __uint_as_float(__byte_perm(u, c, 0x7443)));
+    float x, y, z, v;
+    unpair(add2(mul2(add2(a, off), r01), big), x, y);
+    unpair(add2(mul2(add2(b, off), r23), big), z, v);
+    return __byte_perm(__byte_perm(__float_as_uint(x), __float_as_uint(y), 0x0040), __byte_perm(__float_as_uint(z), __float_as_uint(v), 0x0040), 0x5410);
 }
+
+constexpr int kCompactHeads = 8;
 
 template <int D>
 __global__ void __launch_bounds__(128) k_kv8_compact(const __grid_constant__ Layers L, const int* __restrict__ table, int blocks,
                                                      const int* __restrict__ lens, const int* __restrict__ index, int M,
                                                      const int* __restrict__ kept, const int* __restrict__ new_table, int new_blocks,
-                                                     int pages, int heads, int NB) {
+                                                     int pages, int heads, int NB, int hg, FastDiv by_groups, FastDiv by_blocks) {
     constexpr int TH = 128, PAGE = kBlk * D;
-    __shared__ __align__(16) char tile[2 * PAGE];          // up to two source pages' values
     __shared__ int s_page[kBlk], s_slot[kBlk];
-    __shared__ float s_ratio[kBlk];
-    __shared__ float s_top[2];
+    __shared__ __align__(16) float s_ratio[kCompactHeads][kBlk];
+    __shared__ float s_top[kCompactHeads][2];
     pdl_launch_dependents();
     pdl_wait();
-    const int h = blockIdx.x % heads, bn = blockIdx.x / heads, n = bn % NB, b = bn / NB, tid = threadIdx.x;
+    const int bn = (int)fdiv(blockIdx.x, by_groups), hq = (int)blockIdx.x - bn * (int)by_groups.d, b = (int)fdiv((unsigned)bn, by_blocks),
+              n = bn - b * NB, tid = threadIdx.x;
+    const int h0 = hq * hg, hn = min(hg, heads - h0);
     const bool is_v = blockIdx.z & 1;
     const auto& l = L.at[blockIdx.y];
+    const int slot0 = tid & (kBlk - 1), first = n * kBlk;
+    // the block's tokens: numbers, pages
+    int number = first + slot0 < M ? index[(i64)b * M + first + slot0] : -1;
+    const int to = n < new_blocks ? new_table[(i64)b * new_blocks + n] : -1;
     int m = M;
     if (kept) {
         m = kept[b];
@@ -355,113 +382,119 @@ __global__ void __launch_bounds__(128) k_kv8_compact(const __grid_constant__ Lay
             m = m < 0 ? 0 : M;
         }
     }
-    const int live = min(m - n * kBlk, kBlk);
+    const int len = min(lens[b], (int)min((i64)blocks * kBlk, (i64)0x7fffffff));
+    const int live = min(m - first, kBlk);
     if (live <= 0) return;
-    const int to = n < new_blocks ? new_table[(i64)b * new_blocks + n] : -1;
     if ((unsigned)to >= (unsigned)pages) {
         if (tid == 0) out_of_range();
         return;
     }
+    int page = -1;
+    if (slot0 < live) {
+        if (number >= 0 && number < len) page = table[(i64)b * blocks + number / kBlk];
+        if ((unsigned)page >= (unsigned)pages) page = -1, out_of_range();
+    }
+    // scales of the heads: the first 64 threads take those of even number, the others those of odd
     const float* scale = is_v ? l.vs : l.ks;
-    if (tid < kBlk) {
-        int page = -1, slot = 0;
-        float s = 0.f;
-        if (tid < live) {
-            const int len = min(lens[b], (int)min((i64)blocks * kBlk, (i64)0x7fffffff));
-            int i = index[(i64)b * M + n * kBlk + tid];
-            bool ok = (unsigned)i < (unsigned)max(len, 0);
-            if (ok) {
-                slot = i % kBlk;
-                page = table[(i64)b * blocks + i / kBlk];
-                ok = (unsigned)page < (unsigned)pages;
-            }
-            if (ok) s = scale[(i64)page * heads + h];
-            else page = -1, out_of_range();
-        }
-        float top = s;
+    float sc[kCompactHeads / 2];
+#pragma unroll
+    for (int i = 0; i < kCompactHeads / 2; ++i) {
+        const int hh = 2 * i + (tid >> 6);
+        sc[i] = page >= 0 && hh < hn ? scale[(i64)page * heads + h0 + hh] : 0.f;
+    }
+    if (tid < kBlk) s_page[tid] = page, s_slot[tid] = number & (kBlk - 1);
+#pragma unroll
+    for (int i = 0; i < kCompactHeads / 2; ++i) {
+        float top = sc[i];
 #pragma unroll
         for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        if ((tid & 31) == 0) s_top[tid >> 5] = top;
-        s_page[tid] = page, s_slot[tid] = slot;
-        s_ratio[tid] = s;
+        if ((tid & 31) == 0) s_top[2 * i + (tid >> 6)][tid >> 5 & 1] = top;
     }
     __syncthreads();
-    const float top = fmaxf(s_top[0], s_top[1]);
-    if (tid < kBlk) s_ratio[tid] = top > 0.f ? s_ratio[tid] / top : 0.f;
-    if (tid == 0) (is_v ? l.vs : l.ks)[(i64)to * heads + h] = top;
-    const i64 dst = ((i64)to * heads + h) * PAGE;
+#pragma unroll
+    for (int i = 0; i < kCompactHeads / 2; ++i) {
+        const int hh = 2 * i + (tid >> 6);
+        const float top = fmaxf(s_top[hh][0], s_top[hh][1]);
+        s_ratio[hh][slot0] = top > 0.f ? sc[i] / top : 0.f;
+        if (slot0 == 0 && hh < hn) (is_v ? l.vs : l.ks)[(i64)to * heads + h0 + hh] = top;
+    }
+    const i64 dst = ((i64)to * heads + h0) * PAGE;
     __syncthreads();
     if (!is_v) {
         constexpr int C = D / 16, NU = (kBlk * C + TH - 1) / TH;
-        uint4 w[NU];
+        const i8* src[NU];
+        bool there[NU];
 #pragma unroll
         for (int i = 0; i < NU; ++i) {
-            const int u = tid + TH * i, t = u / C, c = u - t * C;
-            if (kBlk * C % TH != 0 && u >= kBlk * C) break;
-            const int page = s_page[t];
-            w[i] = page < 0 ? make_uint4(0, 0, 0, 0) : *reinterpret_cast<const uint4*>(l.k + ((i64)page * heads + h) * PAGE + s_slot[t] * D + 16 * c);
+            const int u = tid + TH * i, t = min(u / C, kBlk - 1), c = u - u / C * C, p = s_page[t];
+            there[i] = p >= 0 && u < kBlk * C;
+            src[i] = l.k + ((i64)max(p, 0) * heads + h0) * PAGE + s_slot[t] * D + 16 * c;
         }
+#pragma unroll 2
+        for (int hh = 0; hh < hn; ++hh) {
+            uint4 w[NU];
 #pragma unroll
-        for (int i = 0; i < NU; ++i) {
-            const int u = tid + TH * i, t = u / C;
-            if (kBlk * C % TH != 0 && u >= kBlk * C) break;
-            const float r = s_ratio[t];
-            if (r != 1.f) {
-                const float r4[4] = {r, r, r, r};
-                w[i].x = scaled4(w[i].x, r4), w[i].y = scaled4(w[i].y, r4), w[i].z = scaled4(w[i].z, r4), w[i].w = scaled4(w[i].w, r4);
+            for (int i = 0; i < NU; ++i) w[i] = there[i] ? *reinterpret_cast<const uint4*>(src[i] + hh * PAGE) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+            for (int i = 0; i < NU; ++i) {
+                const int u = tid + TH * i, t = u / C;
+                if (kBlk * C % TH != 0 && u >= kBlk * C) break;
+                const float r = s_ratio[hh][t];
+                if (r != 1.f) {
+                    const u64 r2 = pair(r, r);
+                    w[i].x = scaled4(w[i].x, r2, r2), w[i].y = scaled4(w[i].y, r2, r2), w[i].z = scaled4(w[i].z, r2, r2), w[i].w = scaled4(w[i].w, r2, r2);
+                }
+                *reinterpret_cast<uint4*>(l.k + dst + hh * PAGE + 16 * u) = w[i];
             }
-            *reinterpret_cast<uint4*>(l.k + dst + 16 * u) = w[i];
         }
         return;
     }
-    // Values: word (d, g) holds tokens 4 g .. 4 g + 3 of element d. Sixteen lanes to a row, so that bytes of neighbouring tokens
-    // come from neighbouring words.
+    // Values: word (d, g) holds tokens 4 g .. 4 g + 3 of element d; sixteen lanes to a row.
     constexpr int NW = D * 16 / TH, ROWS = TH / 16;
     const int g = tid & 15, d0 = tid >> 4;
-    u32 out[NW];
+    const i8* src[4];
+    bool there[4], run = true;
 #pragma unroll
-    for (int i = 0; i < NW; ++i) out[i] = 0;
-    int mypage[4], myslot[4];
-    float r4[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) mypage[e] = s_page[4 * g + e], myslot[e] = s_slot[4 * g + e], r4[e] = s_ratio[4 * g + e];
-    // runs of tokens of one page, two at a time
-    for (int t = 0; t < live;) {
-        int page[2] = {-1, -1}, from[2], end = t;
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            from[k] = end;
-            if (end >= live) continue;
-            page[k] = s_page[end];
-            while (end < live && s_page[end] == page[k]) ++end;
-        }
-        __syncthreads();
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-            if (page[k] >= 0) {
-                const char* src = reinterpret_cast<const char*>(l.v + ((i64)page[k] * heads + h) * PAGE);
-#pragma unroll
-                for (int i = 0; i < (PAGE / 16 + TH - 1) / TH; ++i)
-                    if (PAGE / 16 % TH == 0 || tid + TH * i < PAGE / 16) cp_async16(tile + k * PAGE + (tid + TH * i) * 16, src + (tid + TH * i) * 16);
-            }
-        cp_async_wait_all();
-        __syncthreads();
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int p = 4 * g + e;
-            if (p >= t && p < end && mypage[e] >= 0) {
-                const char* src = tile + (p >= from[1] && page[1] >= 0 ? PAGE : 0) + myslot[e];
-#pragma unroll
-                for (int i = 0; i < NW; ++i) out[i] |= (u32)(unsigned char)src[(d0 + ROWS * i) * kBlk] << (8 * e);
-            }
-        }
-        t = end;
+    for (int e = 0; e < 4; ++e) {
+        const int p = s_page[4 * g + e], s = s_slot[4 * g + e];
+        there[e] = p >= 0;
+        src[e] = l.v + ((i64)max(p, 0) * heads + h0) * PAGE + d0 * kBlk + s;
+        run = run && src[e] == src[0] + e && there[e] == there[0];
     }
-    const bool same = r4[0] == 1.f && r4[1] == 1.f && r4[2] == 1.f && r4[3] == 1.f;
+    run = run || !(there[0] || there[1] || there[2] || there[3]);
+    const u32 skew = (u32)(reinterpret_cast<uintptr_t>(src[0]) & 3);
+    const u32* word = reinterpret_cast<const u32*>(src[0] - skew);
+    const bool words = __all_sync(0xffffffffu, run);
+#pragma unroll 1
+    for (int hh = 0; hh < hn; ++hh) {
+        u32 out[NW];
+        if (words) {
+            u32 more[NW];
 #pragma unroll
-    for (int i = 0; i < NW; ++i) {
-        if (!same) out[i] = scaled4(out[i], r4);
-        reinterpret_cast<u32*>(l.v + dst)[(d0 + ROWS * i) * 16 + g] = out[i];
+            for (int i = 0; i < NW; ++i) {
+                out[i] = there[0] ? word[hh * (PAGE / 4) + ROWS * i * (kBlk / 4)] : 0u;
+                more[i] = there[0] && skew ? word[hh * (PAGE / 4) + ROWS * i * (kBlk / 4) + 1] : 0u;
+            }
+#pragma unroll
+            for (int i = 0; i < NW; ++i) out[i] = __funnelshift_r(out[i], more[i], 8 * skew);
+        } else {
+#pragma unroll
+            for (int i = 0; i < NW; ++i) {
+                u32 x[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[e] = there[e] ? (unsigned char)src[e][hh * PAGE + ROWS * i * kBlk] : 0u;
+                out[i] = __byte_perm(x[0] | x[1] << 8, x[2] | x[3] << 8, 0x5410);
+            }
+        }
+        const float4 r = *reinterpret_cast<const float4*>(&s_ratio[hh][4 * g]);
+        if (r.x != 1.f || r.y != 1.f || r.z != 1.f || r.w != 1.f) {
+            const u64 r01 = pair(r.x, r.y), r23 = pair(r.z, r.w);
+#pragma unroll
+            for (int i = 0; i < NW; ++i) out[i] = scaled4(out[i], r01, r23);
+        }
+        u32* const to_v = reinterpret_cast<u32*>(l.v + dst + hh * PAGE) + d0 * 16 + g;
+#pragma unroll
+        for (int i = 0; i < NW; ++i) to_v[ROWS * 16 * i] = out[i];
     }
 }
 
@@ -501,10 +534,10 @@ int tcq_kv8_fork(int32_t* refs, int pages, int32_t* table, int blocks, int32_t* 
     const int e = check_table(refs, pages, table, blocks, lens, B);
     if (e) return e;
     if (!parent) return TCQ_ERR_ARG;
-    // columns of a tile: 32 (a line of the table), fewer where all rows' would not fit; no more than the eight CTAs share evenly
-    int shift = 5;
+    // columns of a CTA: eight (a sector of the table), four where eight CTAs hold the whole table then, fewer where all rows' would not fit
+    int shift = blocks <= 4 * kForkCtas ? 2 : 3;
     while (shift > 0 && ((i64)B << shift) * 4 > kForkTile) --shift;
-    while (shift > 2 && blocks <= (kForkCtas << (shift - 1))) --shift;
+    const int ctas = (blocks + (1 << shift) - 1) >> shift, alone = ctas <= kForkCtas;
     static std::atomic<unsigned long long> set{0};
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev > 63) return TCQ_ERR_DEVICE;
@@ -514,19 +547,22 @@ int tcq_kv8_fork(int32_t* refs, int pages, int32_t* table, int blocks, int32_t* 
         set.fetch_or(1ull << dev, std::memory_order_relaxed);
     }
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(kForkCtas);
+    cfg.gridDim = dim3(ctas);
     cfg.blockDim = dim3(kForkThreads);
     cfg.dynamicSmemBytes = (size_t)4 * (((size_t)B << shift) + 2 * B);
     cfg.stream = (cudaStream_t)stream;
     cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = kForkCtas, attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = ctas, attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 2;
-    return cudaLaunchKernelEx(&cfg, k_kv8_fork, (int*)refs, pages, (int*)table, blocks, (int*)lens, (const int*)parent, B, shift) == cudaSuccess
-               ? TCQ_OK : TCQ_ERR_LAUNCH;
+    cfg.numAttrs = alone ? 2 : 1;
+    if (cudaLaunchKernelEx(&cfg, k_kv8_fork, (int*)refs, pages, (int*)table, blocks, (int*)lens, (const int*)parent, B, shift, alone) != cudaSuccess)
+        return TCQ_ERR_LAUNCH;
+    const i64 tokens = (i64)blocks * kBlk;
+    return alone ? TCQ_OK : launch_pdl(k_kv8_fork_lens, dim3(1), kForkThreads, (size_t)4 * B, stream, (int*)lens, (const int*)parent, B,
+                                       (int)(tokens < 0x7fffffff ? tokens : 0x7fffffff));
 }
 
 int tcq_kv8_free(int32_t* refs, int pages, int32_t* table, int blocks, int32_t* lens, const int32_t* keep, int B, void* stream) {
@@ -545,7 +581,9 @@ int tcq_kv8_reserve(int32_t* refs, int pages, int32_t* table, int blocks, const 
     // lanes that look through a sequence's entries side by side: what 1024 threads allow
     int lanes = 32;
     while (lanes > 1 && B * lanes > kResThreads) lanes >>= 1;
-    constexpr int most = 12 * TCQ_KV8_MAX_SEQUENCES;
+    int places = 64;
+    while (places < 2 * B) places <<= 1;
+    constexpr int most = 36 * TCQ_KV8_MAX_SEQUENCES;
     static std::atomic<unsigned long long> set{0};
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev > 63) return TCQ_ERR_DEVICE;
@@ -553,8 +591,8 @@ int tcq_kv8_reserve(int32_t* refs, int pages, int32_t* table, int blocks, const 
         if (cudaFuncSetAttribute(k_kv8_reserve, cudaFuncAttributeMaxDynamicSharedMemorySize, most) != cudaSuccess) return TCQ_ERR_LAUNCH;
         set.fetch_or(1ull << dev, std::memory_order_relaxed);
     }
-    return launch_pdl(k_kv8_reserve, dim3(1), kResThreads, (size_t)12 * B, stream, (int*)refs, pages, (int*)table, blocks, (const int*)lens,
-                      (const int*)count, (int*)granted, (int*)copies, B, lanes);
+    return launch_pdl(k_kv8_reserve, dim3(1), kResThreads, (size_t)12 * (B + places), stream, (int*)refs, pages, (int*)table, blocks, (const int*)lens,
+                      (const int*)count, (int*)granted, (int*)copies, B, lanes, places);
 }
 
 int tcq_kv8_copy(const tcq_kv8_cache* caches, int layers, const int32_t* copies, int n, void* stream) {
@@ -577,13 +615,18 @@ int tcq_kv8_compact(const tcq_kv8_cache* caches, int layers, const int32_t* tabl
     if (!table || !lens || !index || !new_table) return TCQ_ERR_ARG;
     if (B < 1 || tokens < 1 || blocks < 1 || new_blocks < 1) return TCQ_ERR_SHAPE;
     const int NB = (tokens + kBlk - 1) / kBlk, heads = caches->kv_heads;
-    const i64 ctas = (i64)B * NB * heads;
+    // heads that a CTA takes one after the other: fewer where the launch would be short of CTAs
+    int hg = kCompactHeads;
+    while (hg > 1 && (i64)B * NB * ((heads + hg - 1) / hg) * (layers < TCQ_KV8_MAX_LAYERS ? layers : TCQ_KV8_MAX_LAYERS) * 2 < (i64)16 * tcq_sm_count()) hg >>= 1;
+    const int groups = (heads + hg - 1) / hg;
+    const i64 ctas = (i64)B * NB * groups;
     if (ctas > 0x7fffffff) return TCQ_ERR_SHAPE;
+    const FastDiv by_groups = make_fastdiv((unsigned)groups), by_blocks = make_fastdiv((unsigned)NB);
     return by_layers(caches, layers, [&](int count, const Layers& L) {
         return by_head_dim(caches->head_dim, [&](auto d) {
             return launch_pdl(k_kv8_compact<decltype(d)::value>, dim3((unsigned)ctas, count, 2), 128, 0, stream, L, (const int*)table, blocks,
                               (const int*)lens, (const int*)index, tokens, (const int*)kept, (const int*)new_table, new_blocks,
-                              caches->pages, heads, NB);
+                              caches->pages, heads, NB, hg, by_groups, by_blocks);
         });
     });
 }
