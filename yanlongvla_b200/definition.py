@@ -188,6 +188,21 @@ def add_norm(x, delta, weight, bias, eps, kind, mod=None, mod_rows=1):
     return h, n.to(torch.bfloat16).view(h.shape)
 
 
+def cross_attention(q, k, v, heads, lens=None):
+    """softmax(q k^T / sqrt(D)) v over the states that are there, in FP32: q (B * S, T, heads * D), k, v (B, N, heads * D), lens (B,);
+    the S batches of q next to each other read the states of one sequence. Rows that see no state are zero."""
+    B, N, W = k.shape
+    D = W // heads
+    q_, k_, v_ = (x.float().reshape(B, -1, heads, D).transpose(1, 2) for x in (q, k, v))
+    score = (q_ @ k_.transpose(2, 3)) * D ** -0.5
+    if lens is not None:
+        there = torch.arange(N, device=k.device) < lens[:, None]
+        score = score.masked_fill(~there[:, None, None], float('-inf'))
+        v_ = v_.masked_fill(~there[:, None, :, None], 0.0)
+    p = torch.softmax(score, -1).nan_to_num(0.0)
+    return (p @ v_).transpose(1, 2).reshape(q.shape).to(q.dtype)
+
+
 def rope(x, cos, sin, heads):
     """Half-split rotary embedding of x (B, T, heads * D) BF16 with cos / sin (T, D/2) FP32: for each head,
     (a, b) -> (a cos - b sin, a sin + b cos), rounded to BF16."""

@@ -306,14 +306,20 @@ class DitBlock(torch.nn.Module):
         """Cross-attention keys / values of the backbone features: computed once per action chunk."""
         return self.attn1.k_proj(feats), self.attn1.v_proj(feats)
 
-    def forward(self, x, delta, silu_temb, kv=None):
+    def forward(self, x, delta, silu_temb, kv=None, lens=None):
+        """kv: the cross-attention's keys and values, of one batch each observation; x may hold several candidates of each (the
+        candidates of one observation next to each other). lens (observations,) int32: states that are there."""
         d = x.shape[-1]
         mod = self.adaln(silu_temb)                           # (B, 1, 2d): AdaLN scale, shift
         x, h = self.norm1(x, delta, mod=(mod[:, 0, :d], mod[:, 0, d:]), mod_rows=x.shape[1])
         a = self.attn1
         if self.cross:
             k, v = kv
-            o = _attention(a.q_proj(h), k, v, self.heads)
+            if lens is None and k.shape[0] == x.shape[0]:
+                o = _attention(a.q_proj(h), k, v, self.heads)
+            else:
+                cross = definition.cross_attention if getattr(self, 'torch_ops', False) else K.cross_attention
+                o = cross(a.q_proj(h), k, v, self.heads, lens=lens)
         else:
             o = _attention(a.q_proj(h), a.k_proj(h), a.v_proj(h), self.heads)
         x, h = self.norm3(x, a.o_proj(o))
@@ -363,13 +369,14 @@ class GrootStylePolicy(torch.nn.Module):
         img = img.view(B, c.cameras * c.image_tokens, -1)
         return torch.cat((img, self.embed_tokens(lang_ids)), 1)
 
-    def backbone(self, prefix, memory=None):
+    def backbone(self, prefix, memory=None, lens=None):
         """prefix (B, T, 2048) -> features of the same shape. memory: a stream.StreamMemory, to which the prefix is added as the
-        next frame and all of which its tokens attend to."""
+        next frame and all of which its tokens attend to; with lens (B,) int32 only the first lens[b] tokens are. (Without a memory
+        padding needs no care here: it comes last, and no token sees a later one.)"""
         c = self.c
         x, d = prefix, None
         if memory is not None:
-            memory.begin_frame(prefix)
+            memory.begin_frame(prefix, lens)
             for i, blk in enumerate(self.llm):
                 x, d = blk(x, d, None, memory, i)
             return self.llm_norm(x, d)[1]
@@ -385,12 +392,18 @@ class GrootStylePolicy(torch.nn.Module):
         emb = torch.cat((ang.sin(), ang.cos()))[None, None, :].expand(B, 1, 256).to(torch.bfloat16)
         return self.time2(F.silu(self.time1(emb)))
 
-    def action_head(self, feats, state, noise):
-        """feats (B, T, 2048), state (B, 64), noise (B, chunk, action_dim) -> actions (B, chunk, action_dim)."""
+    def action_head(self, feats, state, noise, lens=None):
+        """feats (B, T, 2048), state (B, 64), noise (B * S, chunk, action_dim) -> actions (B * S, chunk, action_dim): S candidate chunks
+        for each observation, b * S .. b * S + S - 1 from the features of observation b, whose keys and values are formed and
+        read once for all of them. lens (B,) int32: features that are there (None: all T)."""
         c = self.c
-        B = feats.shape[0]
+        if noise.shape[0] % feats.shape[0]:
+            raise ValueError(f'action_head: {noise.shape[0]} noise batches for {feats.shape[0]} observations')
         kvs = [blk.kv(feats) if blk.cross else None for blk in self.dit]
         st = self.state_enc2(F.silu(self.state_enc1(state.to(torch.bfloat16))))[:, None, :]
+        B, candidates = noise.shape[0], noise.shape[0] // feats.shape[0]
+        if candidates > 1:
+            st = st.repeat_interleave(candidates, 0)
         a = noise.float()
         dt = 1.0 / c.flow_steps
         ts = torch.arange(c.flow_steps, device=feats.device, dtype=torch.float32) * dt   # on device: graph-capturable
@@ -399,13 +412,16 @@ class GrootStylePolicy(torch.nn.Module):
             x = torch.cat((st, self.action_enc(a.to(torch.bfloat16)) + temb), 1)
             silu_temb, d = F.silu(temb), None
             for blk, kv in zip(self.dit, kvs):
-                x, d = blk(x, d, silu_temb, kv)
+                x, d = blk(x, d, silu_temb, kv, lens)
             v = self.proj_out(self.out_norm(x, d)[1][:, 1:])
             a = a + dt * v.float()
         return a
 
-    def forward(self, images, lang_ids, state, noise, memory=None):
-        return self.action_head(self.backbone(self.embed(images, lang_ids), memory), state, noise)
+    def forward(self, images, lang_ids, state, noise, memory=None, lang_lens=None):
+        """lang_lens (B,) int32: language tokens of each observation, the rest of lang_ids is padding; noise may hold several
+        candidates of each observation (see action_head)."""
+        lens = None if lang_lens is None else lang_lens + self.c.cameras * self.c.image_tokens
+        return self.action_head(self.backbone(self.embed(images, lang_ids), memory, lens), state, noise, lens)
 
 
 # ---------------------------------------------------------------------------------------------------- weights
@@ -483,7 +499,7 @@ def build_policy(device='cuda', runtime='fly', c=PolicyConfig(), seed=0, layers=
     info['chains'] = wire_chains(model) if runtime != 'reference' and modules.FUSE['chain'] else 0
     if runtime == 'reference':
         for m in model.modules():
-            if isinstance(m, (RMSNorm, LayerNorm, LlmBlock)):
+            if isinstance(m, (RMSNorm, LayerNorm, LlmBlock, DitBlock)):
                 m.torch_ops = True
     model.eval()
     return model, layers, info

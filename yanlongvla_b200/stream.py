@@ -1,11 +1,13 @@
 """A policy that acts on a stream of frames: every LLM layer keeps the keys and values of past frames in an 8-bit paged cache
 (kernels.KV8Cache), positions have three axes (time, row, column), and a new frame's tokens attend to all that is remembered.
 
-    python -m yanlongvla_b200.stream --robots 2 --frames 8 [--llm-layers 24]
+    python -m yanlongvla_b200.stream --robots 2 --frames 8 [--llm-layers 24] [--window 4] [--candidates 8]
 
-runs the policy of `policy` (random weights, synthetic frames) with a memory and prints the time per frame. The kernels:
-rope_axes turns the queries, kv8_append turns and stores the keys and stores the values, kv8_attention reads the cache. All
-lengths and positions live on the device, so a step can be captured in a CUDA graph: what a capture records moves them on at each
+runs the policy of `policy` (random weights, synthetic frames) with a memory and prints the time per frame; with a window it
+remembers no more than that many frames, with candidates it forms several action chunks of each observation. The kernels:
+rope_axes turns the queries, kv8_append turns and stores the keys and stores the values, kv8_attention reads the cache; of a memory
+with a pool of pages kv8_fork shares, kv8_reserve and kv8_copy give pages, kv8_compact and kv8_free forget. All lengths and
+positions live on the device, so a step can be captured in a CUDA graph: what a capture records moves them on at each
 replay, and StreamMemory.reserve(), called before each replay, keeps the host's count and checks the capacity.
 """
 import argparse
@@ -16,16 +18,22 @@ from . import kernels as K
 
 
 class StreamMemory:
-    """Caches of every LLM layer for `robots` sequences of up to `max_tokens` tokens. Pages are assigned once: block i of robot b
-    is page b * blocks + i of each layer. Its operators are the kernels in every runtime of the policy, the one of PyTorch
-    operations among them."""
+    """Caches of every LLM layer for `robots` sequences of up to `max_tokens` tokens. Without `pages`, pages are assigned once: block i
+    of robot b is page b * blocks + i of each layer. With it, all robots share a pool of that many pages and get them as
+    they remember more; such a memory can be forked and thinned out (fork, keep, keep_recent). Its operators are the kernels in
+    every runtime of the policy, the one of PyTorch operations among them."""
 
-    def __init__(self, c, robots, max_tokens, device='cuda', theta=10000.0, max_frames=4096):
+    def __init__(self, c, robots, max_tokens, device='cuda', theta=10000.0, max_frames=4096, pages=None):
         D = c.llm_hidden // c.llm_heads
         self.c, self.robots, self.max_tokens, self.tokens = c, robots, max_tokens, 0
         blocks = -(-max_tokens // K.KV8_BLOCK)
-        self.caches = [K.KV8Cache.empty(robots * blocks, c.llm_kv_heads, D, device) for _ in range(c.llm_layers)]
-        self.table = torch.arange(robots * blocks, dtype=torch.int32, device=device).view(robots, blocks)
+        self.pages = None if pages is None else K.KV8Pages.empty(pages, device)
+        self.caches = [K.KV8Cache.empty(robots * blocks if pages is None else pages, c.llm_kv_heads, D, device) for _ in range(c.llm_layers)]
+        if pages is None:
+            self.table = torch.arange(robots * blocks, dtype=torch.int32, device=device).view(robots, blocks)
+        else:
+            self.table = self.pages.table(robots, blocks)
+        self.count = None                                                        # tokens of the current frame, where not all of it
         # a quarter of the frequencies for time, the rest split between rows and columns
         time = D // 8
         row = (D // 2 - time + 1) // 2
@@ -51,9 +59,11 @@ class StreamMemory:
         self.frames += 1
         self.tokens += n
 
-    def begin_frame(self, frame=None):
+    def begin_frame(self, frame=None, count=None):
         """Make room for the next frame: its tokens follow those remembered. On the device but for the check of the capacity.
-        frame: the (B, T, ...) tensor that the layers will get; one of another batch or length is refused before anything moves."""
+        frame: the (B, T, ...) tensor that the layers will get; one of another batch or length is refused before anything moves.
+        count (robots,) int32: each robot's tokens of the frame, the rest is padding (None: all). A robot that the pool of pages does
+        not serve remembers nothing of the frame (device_error reports flag 2)."""
         n = self.pos.shape[2]
         if frame is not None and tuple(frame.shape[:2]) != (self.robots, n):
             raise K.TcqError(f'StreamMemory: a frame of {self.robots} robots with {n} tokens each expected, got {tuple(frame.shape[:2])}')
@@ -61,18 +71,66 @@ class StreamMemory:
             self.reserve()
         self.pos[0] += 1
         self.start.copy_(self.lens)
-        self.lens += n
+        self.count = count
+        if self.pages is not None:
+            want = torch.full_like(self.lens, n) if count is None else count
+            self.count, copies = K.kv8_reserve(self.pages, self.table, self.lens, want)
+            K.kv8_copy(self.caches, copies)
+        self.lens += n if self.count is None else self.count
 
     def attend(self, layer, q, k, v):
         """The attention of one layer over everything remembered and the current frame (causal): q (B, T, heads * D) is turned in
         place, k and v (B, T, kv_heads * D) go into the layer's cache."""
         cache = self.caches[layer]
-        K.kv8_append(cache, k, v, self.table, self.start, rope=self.rope, pos=self.pos)
+        K.kv8_append(cache, k, v, self.table, self.start, count=self.count, rope=self.rope, pos=self.pos)
         K.rope_axes(q, self.pos, self.rope, out=q)
-        return K.kv8_attention(q, cache, self.table, self.lens)
+        return K.kv8_attention(q, cache, self.table, self.lens, count=self.count)
+
+    def _pooled(self, what):
+        if self.pages is None:
+            raise K.TcqError(f'StreamMemory: {what} needs a pool of pages (pages=)')
+
+    def fork(self, parent):
+        """Robot b's memory becomes what robot parent[b]'s is (parent (robots,) int32; below 0: empty), without copying it: pages are shared
+        until one of the robots goes on in a begun block. For several continuations of one past."""
+        self._pooled('fork')
+        K.kv8_fork(self.pages, self.table, self.lens, parent)
+
+    def keep(self, index, kept=None):
+        """Remember only the tokens index[b, j], j < kept[b] (index (robots, n) int32, kept (robots,) int32 or None: all n), packed into
+        pages of the pool, which takes the old ones back; positions in time and space stay what they were. A robot whose tokens
+        the pool's free pages do not hold next to the old ones keeps its memory (device_error reports flag 2)."""
+        self._pooled('keep')
+        n = index.shape[1]
+        if n > self.table.shape[1] * K.KV8_BLOCK:
+            raise K.TcqError(f'StreamMemory: {n} tokens do not fit {self.max_tokens}')
+        kept = torch.full_like(self.lens, n) if kept is None else kept
+        table = self.pages.table(*self.table.shape)
+        granted, _ = K.kv8_reserve(self.pages, table, torch.zeros_like(self.lens), kept)
+        K.kv8_compact(self.caches, self.table, self.lens, index, table, kept=granted)
+        stays = granted < kept
+        K.kv8_free(self.pages, self.table, self.lens, torch.where(stays, self.lens, 0))
+        self.table.copy_(torch.where(stays[:, None], self.table, table))
+        self.lens.copy_(torch.where(stays, self.lens, granted))
+        if not torch.cuda.is_current_stream_capturing():
+            self.tokens = min(self.tokens, n)
+
+    def keep_recent(self, tokens):
+        """Remember only the newest `tokens` tokens of each robot (0: none). Positions go on as if the others were still there."""
+        self._pooled('keep_recent')
+        if tokens < 1:
+            K.kv8_free(self.pages, self.table, self.lens, torch.zeros_like(self.lens))
+            if not torch.cuda.is_current_stream_capturing():
+                self.tokens = 0
+            return
+        kept = self.lens.clamp(max=tokens)
+        at = torch.arange(tokens, dtype=torch.int32, device=self.lens.device)
+        self.keep((self.lens - kept)[:, None] + at.minimum((kept - 1).clamp(min=0)[:, None]), kept)
 
     def forget(self):
         self.tokens = self.frames = 0
+        if self.pages is not None:
+            K.kv8_free(self.pages, self.table, self.lens, torch.zeros_like(self.lens))
         self.lens.zero_()
         self.start.zero_()
         self.pos[0].fill_(-1)
@@ -87,19 +145,31 @@ def main(argv=None):
     ap = argparse.ArgumentParser(description='run the policy on a stream of synthetic frames with an 8-bit memory')
     ap.add_argument('--robots', type=int, default=1)
     ap.add_argument('--frames', type=int, default=16)
+    ap.add_argument('--window', type=int, default=0, help='frames remembered (0: all)')
+    ap.add_argument('--candidates', type=int, default=1, help='action chunks formed of each observation')
     ap.add_argument('--vit-layers', type=int, default=P.PolicyConfig.vit_layers)
     ap.add_argument('--llm-layers', type=int, default=P.PolicyConfig.llm_layers)
     ap.add_argument('--dit-layers', type=int, default=P.PolicyConfig.dit_layers)
     a = ap.parse_args(argv)
     c = P.PolicyConfig(vit_layers=a.vit_layers, llm_layers=a.llm_layers, dit_layers=a.dit_layers)
     model, _, _ = P.build_policy(runtime='resident', c=c)
-    memory = StreamMemory(c, a.robots, a.frames * c.prefix_tokens)
+    n, window = c.prefix_tokens, a.window if 0 < a.window < a.frames else 0
+    if window:
+        # full and next to it what is kept of it
+        blocks = -(-window * n // K.KV8_BLOCK) + -(-(window - 1) * n // K.KV8_BLOCK)
+        memory = StreamMemory(c, a.robots, window * n, pages=a.robots * blocks)
+    else:
+        memory = StreamMemory(c, a.robots, a.frames * n)
     ev = [torch.cuda.Event(enable_timing=True) for _ in range(2)]
     with torch.no_grad():
         for f in range(a.frames):
-            obs = P.synthetic_observations(a.robots, c, seed=f)
+            images, lang, state, noise = P.synthetic_observations(a.robots, c, seed=f)
+            if a.candidates > 1:
+                noise = torch.randn(a.robots * a.candidates, *noise.shape[1:], device=noise.device)
             ev[0].record()
-            actions = model(*obs, memory=memory)
+            if window and memory.tokens == window * n:
+                memory.keep_recent((window - 1) * n)
+            actions = model(images, lang, state, noise, memory=memory)
             ev[1].record()
             ev[1].synchronize()
             print(f'frame {f}: {memory.tokens} tokens remembered, {ev[0].elapsed_time(ev[1]):.2f} ms, actions {tuple(actions.shape)}')
