@@ -363,10 +363,10 @@ PyObject* kv8_reserve(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const char* me = "kv8_reserve";
         const Rows r = paged(me, a[0], a[1], a[2], a[3], "count");
         void* st = stream_of(me, r.dev);
-        at::Tensor granted = at::empty({r.B}, r.options), copies = at::empty({2, r.B}, r.options);
-        done(f_reserve(r.refs, r.pages, r.table, r.blocks, r.lens, r.more, granted.data_ptr<int32_t>(), copies.data_ptr<int32_t>(), r.B, st),
-             "tcq_kv8_reserve", me);
-        return Py_BuildValue("(NN)", THPVariable_Wrap(granted), THPVariable_Wrap(copies));
+        at::Tensor made = at::empty({3, r.B}, r.options);             // one allocation: granted, then copies
+        int32_t* granted = made.data_ptr<int32_t>();
+        done(f_reserve(r.refs, r.pages, r.table, r.blocks, r.lens, r.more, granted, granted + r.B, r.B, st), "tcq_kv8_reserve", me);
+        return Py_BuildValue("(NN)", THPVariable_Wrap(made.select(0, 0)), THPVariable_Wrap(made.narrow(0, 1, 2)));
     });
 }
 

@@ -474,25 +474,29 @@ k_cross_rows(const CrossArgs A, const __grid_constant__ CUtensorMap kmap, const 
     cluster_barrier();
     for (int i = rank * (32 * kRowWarps) + tid; i < rows * (DP / 4); i += R.splits * (32 * kRowWarps)) {
         const int row = i / (DP / 4), d = 4 * (i - row * (DP / 4));
-        float2 ml[8];
-        float4 v[8], y = make_float4(0.f, 0.f, 0.f, 0.f);
+        // four parts at a time, all of their loads under way at once
+        float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
         float top = -INFINITY, sum = 0.f;
+        for (int k0 = 0; k0 < R.splits; k0 += 4) {
+            float2 ml[4];
+            float4 v[4];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            ml[k] = make_float2(-INFINITY, 0.f), v[k] = y;
-            if (k < R.splits) {
-                const u32 p = peer_addr(sbase, k);
-                ml[k] = peer_ld2(p + P::PARTS + 8 * row);
-                v[k] = peer_ld4(p + (row * P::PITCH + d) * 4);
+            for (int k = 0; k < 4; ++k) {
+                ml[k] = make_float2(-INFINITY, 0.f), v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (k0 + k < R.splits) {
+                    const u32 p = peer_addr(sbase, k0 + k);
+                    ml[k] = peer_ld2(p + P::PARTS + 8 * row);
+                    v[k] = peer_ld4(p + (row * P::PITCH + d) * 4);
+                }
             }
-        }
 #pragma unroll
-        for (int k = 0; k < 8; ++k) top = fmaxf(top, ml[k].x);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            const float f = part_factor(ml[k], top);
-            sum = __fmaf_rn(ml[k].y, f, sum);
-            y.x = __fmaf_rn(v[k].x, f, y.x), y.y = __fmaf_rn(v[k].y, f, y.y), y.z = __fmaf_rn(v[k].z, f, y.z), y.w = __fmaf_rn(v[k].w, f, y.w);
+            for (int k = 0; k < 4; ++k) {
+                const float both = fmaxf(top, ml[k].x), old = both == -INFINITY ? 1.f : ex2(top - both), f = part_factor(ml[k], both);
+                top = both;
+                sum = __fmaf_rn(ml[k].y, f, sum * old);
+                y.x = __fmaf_rn(v[k].x, f, y.x * old), y.y = __fmaf_rn(v[k].y, f, y.y * old);
+                y.z = __fmaf_rn(v[k].z, f, y.z * old), y.w = __fmaf_rn(v[k].w, f, y.w * old);
+            }
         }
         store(row, d, y, sum);
     }
@@ -1085,13 +1089,16 @@ int launch_rows(const CrossArgs& A, const CUtensorMap& km, const CUtensorMap& vm
     typedef Rows<DP, MT> P;
     const auto kern = k_cross_rows<DT, DP, MT>;
     RowsPlan R = {};
-    // as many warps to a unit as its rows want, up to four; of those block heights the one that leaves the fewest warps without rows (272
-    // rows of each of 256 units: nine blocks of 32 rows 17.1 us, three of 128 20.3)
-    int fewest = 1 << 30;
-    for (int w = 2; w >= 0; --w) {
-        const int warps = (A.rows + (P::ROWS << w) - 1) / (P::ROWS << w) << w;
-        if (warps < fewest || (w < 2 && warps == fewest && A.rows <= (P::ROWS << w))) fewest = warps, R.wm_log2 = w;
-    }
+    // As many warps to a unit as its rows want, up to four. Up to head width 64, of those block heights the one that leaves the fewest warps
+    // without rows (272 rows of each of 256 units over 160 states: nine blocks of 32 rows 17.1 us, three of 128 20.3); wider heads of many
+    // units want every state read for as many rows as there are (33 rows of 512 units over 640 states of 128: three blocks of 16 73 us,
+    // one of 64 48; of 8 units over 160 states 5.4 and 9.1).
+    while (R.wm_log2 < 2 && (P::ROWS << R.wm_log2) < A.rows) ++R.wm_log2;
+    if (DP <= 64 || (i64)A.B * A.kv_heads <= tcq_sm_count())
+        for (int w = R.wm_log2 - 1, fewest = (A.rows + (P::ROWS << R.wm_log2) - 1) / (P::ROWS << R.wm_log2) << R.wm_log2; w >= 0; --w) {
+            const int warps = (A.rows + (P::ROWS << w) - 1) / (P::ROWS << w) << w;
+            if (warps < fewest) fewest = warps, R.wm_log2 = w;
+        }
     const int rings = kRowWarps >> R.wm_log2;
     R.row_blocks = (A.rows + (P::ROWS << R.wm_log2) - 1) / (P::ROWS << R.wm_log2);
     R.block_rows = (((A.rows + R.row_blocks - 1) / R.row_blocks) + P::ROWS - 1) & ~(P::ROWS - 1);
@@ -1102,8 +1109,10 @@ int launch_rows(const CrossArgs& A, const CUtensorMap& km, const CUtensorMap& vm
     // whole units where they are enough for a CTA on every SM
     R.whole = units >= (i64)sms * rings;
     R.splits = 1;
+    // Else a unit's states are divided while there are SMs to spare and a ring keeps more chunks than adding its parts is worth: four, and one
+    // for every eight rows.
     if (!R.whole)
-        while (R.splits < 8 && units * R.splits < 2 * sms && chunks >= 2 * rings * R.splits * 2) R.splits *= 2;
+        while (R.splits < 8 && units * R.splits < 2 * sms && chunks >= rings * R.splits * (4 + R.block_rows / 8)) R.splits *= 2;
     const int each = R.whole ? chunks : (chunks + rings * R.splits - 1) / (rings * R.splits);
     const int most = rings == 1 ? P::MOST : 3;
     R.stages = each + 1 < most ? each + 1 : most;
@@ -1141,6 +1150,22 @@ int by_width(int d, F f) {
     return f(std::integral_constant<int, 128>());
 }
 
+// Products of 16 rows or tiles of 128? A tile's CTA costs about 5 us before and behind its states, and computes 128 or 256 rows whatever
+// there are; a row costs three times as much in the other kernel. Where tiles give every unit an SM of its own (and its states
+// are divided over a cluster), they win from 256 states on if the rows are not few (us, products of 16 / tiles, heads of 64: 8 units of
+// 33 rows over 160 states 6.5 / 6.3, over 640 12.7 / 8.8; of 17 rows 7.8 / 8.5; heads of 128: 33 rows over 640 8.4 / 11.0, 64 rows 12.8 /
+// 11.8; 64 units of 17 rows over 1280 17.4 / 12.7). Else by what the states of a unit cost in either, in picoseconds of the device (heads of 64: 1.15 a row and state against
+// 0.35, 50,000 a tile of rows; of 128: 1.95, 0.43, 60,000): 512 units of 64 rows over 640 states 27.8 / 37.3, over 2560 98.4 / 83.0; of 256
+// rows over 160 states 34 / 38, over 320 55 / 44; heads of 128, 256 rows over 160 states 58 / 48.
+bool prefer_tiles(i64 rows, int N, int D, i64 units) {
+    const bool wide = D > 64;
+    if (N < (wide ? 128 : 256)) return false;
+    const i64 row_tiles = (rows + 255) / 256;
+    if (units * row_tiles <= tcq_sm_count()) return N >= 256 && (rows > (wide ? 48 : 32) || (wide && rows > 16 && units * N >= 65536));
+    const i64 small = !wide && rows > 16 ? (rows + 31) / 32 * 32 : (rows + 15) / 16 * 16, padded = rows <= 128 ? 128 : 256 * row_tiles;
+    return (double)N * (wide ? 1.95 * (double)small - 0.43 * (double)padded : 1.15 * (double)small - 0.35 * (double)padded) > (wide ? 60000.0 : 50000.0) * (double)row_tiles;
+}
+
 }  // namespace
 
 extern "C" {
@@ -1165,8 +1190,7 @@ int tcq_cross_attention(const void* q, int64_t q_sb, int64_t q_st, const void* k
     // sequences that share one batch of states (stride 0) have one in the tensor map
     if (B == 1) k_sb = v_sb = 0;
     CUtensorMap km, vm;
-    // few rows or few states: products of 16 rows; else tiles of 128 rows and 128 states
-    const bool tiles = rows > 32 && N >= 512;
+    const bool tiles = prefer_tiles(rows, N, head_dim, (i64)B * kv_heads);
     const int box = tiles ? kTile : by_width(head_dim, [](auto d) { return Rows<decltype(d)::value, 1>::CHUNK; });
     if (!encode(&km, k, dtype, head_dim, N, kv_heads, B, k_st, k_sb, box) || !encode(&vm, v, dtype, head_dim, N, kv_heads, B, v_st, v_sb, box))
         return TCQ_ERR_DEVICE;
