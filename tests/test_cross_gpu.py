@@ -249,5 +249,9 @@ def test_refusals(K):
     refused(TypeError, heads='2')
     refused(TypeError, scale='a')
     refused(TypeError, lens=[1, 2])
+    refused(q=q.clone().requires_grad_())
+    refused(v=k.clone().requires_grad_())
+    with torch.no_grad():
+        K.cross_attention(q.clone().requires_grad_(), k, k, 2, 1)
     K.cross_attention(q, k, k, 2, 1)
     assert K.device_error() == 0

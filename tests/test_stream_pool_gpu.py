@@ -120,6 +120,20 @@ def test_frames_of_differing_length(P, setup, K, Memory):
     assert K.device_error() == 0
 
 
+def test_counts_of_a_frame(P, setup, K, Memory):
+    """A count that is none of the frame's is refused before anything moves; one past the frame is the whole frame."""
+    c, _ = setup
+    n = c.prefix_tokens
+    for pages in (None, 8):
+        memory = Memory(c, 2, n, pages=pages)
+        for bad in (ints([n, n]).long(), ints([n]), torch.tensor([n, n], dtype=torch.int32)):
+            with pytest.raises(K.TcqError, match='count'):
+                memory.begin_frame(count=bad)
+        assert memory.tokens == memory.frames == 0 and memory.pos[0].eq(-1).all() and not memory.lens.any()
+        memory.begin_frame(count=ints([n + 1, -1]))
+        assert memory.lens.tolist() == [n, 0]
+
+
 def test_a_pool_without_pages_left(P, setup, K, Memory):
     """The robot that is not served remembers nothing of the frame, the other all of it."""
     c, model = setup

@@ -6,6 +6,7 @@
 #include <Python.h>
 
 #include <ATen/core/Tensor.h>
+#include <ATen/core/grad_mode.h>
 #include <ATen/ops/empty.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
@@ -450,6 +451,8 @@ PyObject* cross_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
         if (v.sizes() != k.sizes()) refuse(me, "k and v must have the same shape");
         if (k.scalar_type() != q.scalar_type() || v.scalar_type() != q.scalar_type()) refuse(me, "q, k and v must have one type");
         if (B < 1 || q.size(0) < 1 || q.size(0) % B) refuse(me, "q must have a multiple of the batches of k and v");
+        if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad()))
+            refuse(me, "it forms no gradient: call it under torch.no_grad(), or on detached tensors");
         const int dt = dtype_code(me, q, false);
         const int32_t* lp = a[5] == Py_None ? nullptr : ints(me, "lens", tensor(me, a[5], "lens"), {B}, dev);
         const uint8_t* mp = nullptr;

@@ -199,7 +199,9 @@ def cross_attention(q, k, v, heads, lens=None):
         there = torch.arange(N, device=k.device) < lens[:, None]
         score = score.masked_fill(~there[:, None, None], float('-inf'))
         v_ = v_.masked_fill(~there[:, None, :, None], 0.0)
-    p = torch.softmax(score, -1).nan_to_num(0.0)
+    p = torch.softmax(score, -1)
+    if lens is not None:
+        p = p.masked_fill((lens <= 0)[:, None, None, None], 0.0)
     return (p @ v_).transpose(1, 2).reshape(q.shape).to(q.dtype)
 
 

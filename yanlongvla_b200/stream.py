@@ -62,18 +62,20 @@ class StreamMemory:
     def begin_frame(self, frame=None, count=None):
         """Make room for the next frame: its tokens follow those remembered. On the device but for the check of the capacity.
         frame: the (B, T, ...) tensor that the layers will get; one of another batch or length is refused before anything moves.
-        count (robots,) int32: each robot's tokens of the frame, the rest is padding (None: all). A robot that the pool of pages does
+        count (robots,) int32: each robot's tokens of the frame (0 .. its length), the rest is padding (None: all). A robot that the pool of pages does
         not serve remembers nothing of the frame (device_error reports flag 2)."""
         n = self.pos.shape[2]
         if frame is not None and tuple(frame.shape[:2]) != (self.robots, n):
             raise K.TcqError(f'StreamMemory: a frame of {self.robots} robots with {n} tokens each expected, got {tuple(frame.shape[:2])}')
+        if count is not None and (count.dtype != torch.int32 or count.shape != self.lens.shape or count.device != self.lens.device):
+            raise K.TcqError(f'StreamMemory: count must be int32 ({self.robots},) on {self.lens.device}, got {count.dtype} {tuple(count.shape)}')
         if not torch.cuda.is_current_stream_capturing():
             self.reserve()
         self.pos[0] += 1
         self.start.copy_(self.lens)
-        self.count = count
+        self.count = None if count is None else count.clamp(0, n)
         if self.pages is not None:
-            want = torch.full_like(self.lens, n) if count is None else count
+            want = torch.full_like(self.lens, n) if count is None else self.count
             self.count, copies = K.kv8_reserve(self.pages, self.table, self.lens, want)
             K.kv8_copy(self.caches, copies)
         self.lens += n if self.count is None else self.count
