@@ -199,7 +199,7 @@ k_cross_rows(const CrossArgs A, const __grid_constant__ CUtensorMap kmap, const 
                 }
             }
             if (more) {
-                if (use) ok = mbar_wait_suspended(full + 8, (use - 1) & 1, abort_flag, &g_tcq_cross_error);
+                if (use) ok = mbar_wait_ready(full + 8, (use - 1) & 1, abort_flag, &g_tcq_cross_error);
                 if (ok) {
                     meta[s] = make_int2(bits ? pc : -1, (int)bits);
                     if (!bits) {
@@ -384,7 +384,7 @@ k_cross_rows(const CrossArgs A, const __grid_constant__ CUtensorMap kmap, const 
     int slot = kg * stages;
     u32 phase = 0;
     for (;;) {
-        if (!mbar_wait_suspended(bars + 16 * slot, phase, abort_flag, &g_tcq_cross_error)) break;
+        if (!mbar_wait_ready(bars + 16 * slot, phase, abort_flag, &g_tcq_cross_error)) break;
         const int2 what = meta[slot];
         if (what.x < 0) break;
         const u32 kt = sbase + slot * P::STAGE;
@@ -570,7 +570,7 @@ k_cross_tiles(const CrossArgs A, const __grid_constant__ CUtensorMap kmap, const
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     constexpr int W_MMA = 8, W_LOAD = 9, W_CLEAN = 10;
     auto bar = [&](int i) -> u32 { return bars + 8 * i; };
-    auto wait = [&](int i, u32 parity) -> bool { return mbar_wait_suspended(bar(i), parity & 1, abort_flag, &g_tcq_cross_error); };
+    auto wait = [&](int i, u32 parity) -> bool { return mbar_wait_ready(bar(i), parity & 1, abort_flag, &g_tcq_cross_error); };
     if (tid == 0) {
         for (int i = 0; i < P::RING; ++i) {
             mbar_init(bar(TBAR_FULL + i), 1);

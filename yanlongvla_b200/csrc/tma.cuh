@@ -96,6 +96,21 @@ __device__ __forceinline__ bool mbar_wait_suspended(u32 bar, u32 parity, volatil
     }
 }
 
+// The same where the phase is mostly complete when it is asked for: a look that does not suspend and one that may, in straight code,
+// before the loop, whose entry alone costs some 150 clocks.
+__device__ __forceinline__ bool mbar_wait_ready(u32 bar, u32 parity, volatile int* abort_flag, int* err, unsigned long long limit = kWaitNs) {
+    u32 ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    if (ok || mbar_try(bar, parity)) return true;
+    return mbar_wait_suspended(bar, parity, abort_flag, err, limit);
+}
+
 __device__ __forceinline__ void tma_load_2d(u32 dst, const CUtensorMap* map, u32 bar, int x, int y) {
     asm volatile(
         "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
