@@ -383,3 +383,27 @@ def test_compact_bad_numbers_next_to_good_ones(K):
         assert torch.equal(c.k[3, :, j], k0[:, j]) and torch.equal(c.v[3, :, :, j], v0[:, :, j])
     for j in (0, 7, 12, *range(14, 64)):
         assert not c.k[3, :, j].any() and not c.v[3, :, :, j].any()
+
+
+def test_compact_rounds_the_product_first(K):
+    """rint(fl(q r)), not rint(q r): of some 10^8 products a few tens lie so near a half that the two differ."""
+    P, g = 3000, torch.Generator(device='cuda').manual_seed(1)
+    c = K.KV8Cache.empty(3 * P, 8, 64)
+    for cells, scale in ((c.k, c.k_scale), (c.v, c.v_scale)):
+        cells.copy_(torch.randint(-127, 128, cells.shape, device='cuda', generator=g))
+        scale.copy_(torch.rand(scale.shape, device='cuda', generator=g) + 0.02)
+    at = torch.arange(64, device='cuda')
+    index = (2 * torch.arange(P, device='cuda')[:, None] + at // 32) * 64 + at % 32 + 8         # half of each of two pages
+    pages = torch.arange(3 * P, device='cuda', dtype=torch.int32)[None]
+    K.kv8_compact(c, pages[:, :2 * P].contiguous(), ints([2 * P * 64]), index.view(1, -1).int(), pages[:, 2 * P:].contiguous())
+    differ = 0
+    for cells, scale, transposed in ((c.k, c.k_scale, False), (c.v, c.v_scale, True)):
+        old = scale[:2 * P].view(P, 2, 8)
+        ratio = (old / old.amax(1, keepdim=True))[..., None, None]
+        q = (cells[:2 * P, :, :, 8:40] if transposed else cells[:2 * P, :, 8:40].transpose(2, 3)).reshape(P, 2, 8, 64, 32)
+        got = cells[2 * P:] if transposed else cells[2 * P:].transpose(2, 3)
+        got = got.reshape(P, 8, 64, 2, 32).permute(0, 3, 1, 2, 4)
+        want = (q.float() * ratio).round()
+        assert torch.equal(got.float(), want)
+        differ += (want != (q.double() * ratio.double()).round()).sum().item()
+    assert differ > 0

@@ -341,14 +341,17 @@ __global__ void __launch_bounds__(256) k_kv8_copy(const __grid_constant__ Layers
 //
 // Quotients of integers q' = q r with 0 <= r <= 1: the byte in a float's low bits (2^23 + 128 + q), its offset taken off, times r,
 // rounded to nearest even by adding 1.5 * 2^23; each step one rounding.
-TCQ_HD u32 scaled4(u32 w, u64 r01, u64 r23) {
+// (The product stands alone: a packed one was contracted with the addition behind it, which rounds once and now and then to the other side.)
+TCQ_HD u32 scaled4(u32 w, const float4& r) {
     const u32 u = w ^ 0x80808080u, c = 0x4b000000u;
     const u64 off = pair(-8388736.f, -8388736.f), big = pair(12582912.f, 12582912.f);
     const u64 a = pair(__uint_as_float(__byte_perm(u, c, 0x7440)), __uint_as_float(__byte_perm(u, c, 0x7441)));
     const u64 b = pair(__uint_as_float(__byte_perm(u, c, 0x7442)), __uint_as_float(__byte_perm(u, c, 0x7443)));
     float x, y, z, v;
-    unpair(add2(mul2(add2(a, off), r01), big), x, y);
-    unpair(add2(mul2(add2(b, off), r23), big), z, v);
+    unpair(add2(a, off), x, y);
+    unpair(add2(b, off), z, v);
+    unpair(add2(pair(__fmul_rn(x, r.x), __fmul_rn(y, r.y)), big), x, y);
+    unpair(add2(pair(__fmul_rn(z, r.z), __fmul_rn(v, r.w)), big), z, v);
     return __byte_perm(__byte_perm(__float_as_uint(x), __float_as_uint(y), 0x0040), __byte_perm(__float_as_uint(z), __float_as_uint(v), 0x0040), 0x5410);
 }
 
@@ -441,8 +444,8 @@ __global__ void __launch_bounds__(128) k_kv8_compact(const __grid_constant__ Lay
                 if (kBlk * C % TH != 0 && u >= kBlk * C) break;
                 const float r = s_ratio[hh][t];
                 if (r != 1.f) {
-                    const u64 r2 = pair(r, r);
-                    w[i].x = scaled4(w[i].x, r2, r2), w[i].y = scaled4(w[i].y, r2, r2), w[i].z = scaled4(w[i].z, r2, r2), w[i].w = scaled4(w[i].w, r2, r2);
+                    const float4 r4 = make_float4(r, r, r, r);
+                    w[i].x = scaled4(w[i].x, r4), w[i].y = scaled4(w[i].y, r4), w[i].z = scaled4(w[i].z, r4), w[i].w = scaled4(w[i].w, r4);
                 }
                 *reinterpret_cast<uint4*>(l.k + dst + hh * PAGE + 16 * u) = w[i];
             }
@@ -488,9 +491,8 @@ __global__ void __launch_bounds__(128) k_kv8_compact(const __grid_constant__ Lay
         }
         const float4 r = *reinterpret_cast<const float4*>(&s_ratio[hh][4 * g]);
         if (r.x != 1.f || r.y != 1.f || r.z != 1.f || r.w != 1.f) {
-            const u64 r01 = pair(r.x, r.y), r23 = pair(r.z, r.w);
 #pragma unroll
-            for (int i = 0; i < NW; ++i) out[i] = scaled4(out[i], r01, r23);
+            for (int i = 0; i < NW; ++i) out[i] = scaled4(out[i], r);
         }
         u32* const to_v = reinterpret_cast<u32*>(l.v + dst + hh * PAGE) + d0 * 16 + g;
 #pragma unroll

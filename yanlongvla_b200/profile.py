@@ -211,6 +211,36 @@ def _case_memory(kind, robots, tokens, length, width, launches):
             K.kv8_read(cache, table, zero, lens, length)
 
 
+def _case_cross(robots, tokens, length, width, kv_heads, launches):
+    """Cross attention of `tokens` queries (32 heads of `width`) to `length` states of each of `robots` sequences."""
+    from . import kernels as K
+    g = torch.Generator(device='cuda').manual_seed(17)
+    q = torch.randn(robots, tokens, 32 * width, device='cuda', generator=g).bfloat16()
+    k, v = (torch.randn(robots, length, kv_heads * width, device='cuda', generator=g).bfloat16() for _ in range(2))
+    for _ in range(launches):
+        K.cross_attention(q, k, v, 32, kv_heads)
+
+
+def _case_compact(robots, length, width, chosen, launches):
+    """Tokens of `robots` sequences of `length` in four layers of 8 key heads packed into other pages: every second one, or the newest
+    three quarters."""
+    from . import kernels as K
+    blocks = -(-length // K.KV8_BLOCK)
+    caches = [K.KV8Cache.empty(2 * robots * blocks, 8, width) for _ in range(4)]
+    g = torch.Generator(device='cuda').manual_seed(18)
+    for c in caches:
+        for x in (c.k, c.v):
+            x.copy_(torch.randint(-127, 128, x.shape, device='cuda', generator=g, dtype=torch.int8))
+        for x in (c.k_scale, c.v_scale):
+            x.copy_(0.01 + 0.01 * torch.rand(x.shape, device='cuda', generator=g))
+    pages = torch.randperm(2 * robots * blocks, device='cuda', generator=g).to(torch.int32).view(2, robots, blocks)
+    at = torch.arange(0, length, 2, device='cuda') if chosen else torch.arange(length // 4, length, device='cuda')
+    index = at.to(torch.int32).expand(robots, -1).contiguous()
+    lens = torch.full((robots,), length, dtype=torch.int32, device='cuda')
+    for _ in range(launches):
+        K.kv8_compact(caches, pages[0], lens, index, pages[1])
+
+
 def _case_policy(batch):
     """replay_breakdown of one CUDA-graph replay of the fly policy's action chunk for `batch` observations."""
     import json
@@ -233,15 +263,17 @@ def _case_policy(batch):
 def main(argv=None):
     import argparse
     ap = argparse.ArgumentParser(description='one kernel case for a profiler')
-    ap.add_argument('case', choices=['gemv', 'gemv_tc', 'gemm', 'pre', 'rotate', 'chain', 'attend', 'append', 'read', 'policy'])
+    ap.add_argument('case', choices=['gemv', 'gemv_tc', 'gemm', 'pre', 'rotate', 'chain', 'attend', 'append', 'read', 'cross', 'compact', 'policy'])
     ap.add_argument('--m', type=int, default=4096)
     ap.add_argument('--n', type=int, default=None)
     ap.add_argument('--k', type=int, default=None)
     ap.add_argument('--tokens', type=int, default=1)
     ap.add_argument('--launches', type=int, default=4)
-    ap.add_argument('--robots', type=int, default=1, help='attend / append / read: sequences')
-    ap.add_argument('--length', type=int, default=4096, help='attend / read: cached tokens of a sequence')
-    ap.add_argument('--width', type=int, default=64, help='attend / append / read: head width')
+    ap.add_argument('--robots', type=int, default=1, help='attend / append / read / cross / compact: sequences')
+    ap.add_argument('--length', type=int, default=4096, help='attend / read / compact: cached tokens of a sequence; cross: states')
+    ap.add_argument('--width', type=int, default=64, help='attend / append / read / cross / compact: head width')
+    ap.add_argument('--kv-heads', type=int, default=8, help='cross: key heads')
+    ap.add_argument('--chosen', action='store_true', help='compact: every second token instead of the newest three quarters')
     ap.add_argument('--out', choices=['i32', 'bf16'], default='i32', help='gemm case: INT32 or BF16 (scaled) output')
     a = ap.parse_args(argv)
     if a.case == 'gemv':
@@ -254,6 +286,10 @@ def main(argv=None):
         _case_policy(a.tokens)
     elif a.case in ('attend', 'append', 'read'):
         _case_memory(a.case, a.robots, a.tokens, a.length, a.width, a.launches)
+    elif a.case == 'cross':
+        _case_cross(a.robots, a.tokens, a.length, a.width, a.kv_heads, a.launches)
+    elif a.case == 'compact':
+        _case_compact(a.robots, a.length, a.width, a.chosen, a.launches)
     elif a.case == 'chain':
         _case_chain(a.m, a.k or 1536, a.launches)
     else:
