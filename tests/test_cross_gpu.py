@@ -255,3 +255,45 @@ def test_refusals(K):
         K.cross_attention(q.clone().requires_grad_(), k, k, 2, 1)
     K.cross_attention(q, k, k, 2, 1)
     assert K.device_error() == 0
+
+
+def test_first_call_in_a_capture():
+    """What the first call asks the device works in a capture too, and with two threads at once."""
+    import subprocess
+    import sys
+    from pathlib import Path
+    code = '''
+import threading, torch
+from yanlongvla_b200 import kernels as K
+x = {n: torch.randn(2, n, 256, device='cuda').bfloat16() for n in (1, 300, 700, 9000)}
+def calls():
+    return [K.cross_attention(x[t], x[n], x[n], 4) for t, n in ((1, 9000), (1, 300), (300, 300), (300, 700), (700, 9000))]
+owner = K.KV8Pages.empty(300)
+table, lens = owner.table(2, 100), torch.zeros(2, dtype=torch.int32, device='cuda')
+ints = lambda v: torch.tensor(v, dtype=torch.int32, device='cuda')
+n, p = ints([70, 0]), ints([0, 0])
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    a = calls()
+    granted, copies = K.kv8_reserve(owner, table, lens, n)
+    lens += granted
+    K.kv8_fork(owner, table, lens, p)
+g.replay()
+torch.cuda.synchronize()
+assert lens.tolist() == [70, 70] and owner.refs[:3].tolist() == [2, 2, 0]
+got = [None] * 4
+def work(i):
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        for _ in range(20):
+            got[i] = calls()
+    s.synchronize()
+t = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+[y.start() for y in t]; [y.join() for y in t]
+for b in got:
+    assert all(torch.equal(u, v) for u, v in zip(a, b))
+assert K.device_error() == 0
+'''
+    r = subprocess.run([sys.executable, '-c', code], cwd=Path(__file__).resolve().parent.parent, capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0, r.stderr[-2000:]

@@ -1103,38 +1103,52 @@ int launch_rows(const CrossArgs& A, const CUtensorMap& km, const CUtensorMap& vm
     R.row_blocks = (A.rows + (P::ROWS << R.wm_log2) - 1) / (P::ROWS << R.wm_log2);
     R.block_rows = (((A.rows + R.row_blocks - 1) / R.row_blocks) + P::ROWS - 1) & ~(P::ROWS - 1);
     const i64 units = (i64)A.B * A.kv_heads * R.row_blocks;
-    if (units > 0x7fffffff / 8) return TCQ_ERR_SHAPE;
+    if (units > 0x7fffffff / 16) return TCQ_ERR_SHAPE;
     const int chunks = (A.N + P::CHUNK - 1) / P::CHUNK, sms = tcq_sm_count();
     R.units = (int)units;
     // whole units where they are enough for a CTA on every SM
     R.whole = units >= (i64)sms * rings;
     R.splits = 1;
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[2];
+    cfg.blockDim = dim3(kRowThreads);
+    cfg.stream = (cudaStream_t)stream;
+    cfg.attrs = attr;
+    // Clusters of sixteen CTAs that the device holds at a time, and one more; asked once per device.
+    static std::atomic<int> sixteens[64];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev > 63) return TCQ_ERR_DEVICE;
+    if (!sixteens[dev].load(std::memory_order_acquire)) {
+        if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, P::bytes(kRowWarps, 3)) != cudaSuccess) return TCQ_ERR_LAUNCH;
+        int n = 0;
+        cfg.gridDim = dim3(16);
+        cfg.dynamicSmemBytes = P::bytes(kRowWarps, 3);
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = 16, attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        cfg.numAttrs = 1;
+        if (cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess ||
+            cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess)
+            n = 0, cudaGetLastError();
+        sixteens[dev].store(n + 1, std::memory_order_release);
+    }
     // Else a unit's states are divided while there are SMs to spare and a ring keeps more chunks than adding its parts is worth: four, and one
-    // for every eight rows.
+    // for every eight rows. Into sixteen only where all those clusters run at once (one token over 16411 states, 8 key heads of 64: one
+    // sequence, 8 clusters, 13.6 -> 10.8 us; four sequences 26 us with eight CTAs to a cluster, 37 with sixteen).
     if (!R.whole)
-        while (R.splits < 8 && units * R.splits < 2 * sms && chunks >= rings * R.splits * (4 + R.block_rows / 8)) R.splits *= 2;
+        while (R.splits < (units < sixteens[dev].load(std::memory_order_relaxed) && units * 16 <= sms ? 16 : 8) && units * R.splits < 2 * sms &&
+               chunks >= rings * R.splits * (4 + R.block_rows / 8))
+            R.splits *= 2;
     const int each = R.whole ? chunks : (chunks + rings * R.splits - 1) / (rings * R.splits);
     const int most = rings == 1 ? P::MOST : 3;
     R.stages = each + 1 < most ? each + 1 : most;
-    R.by_blocks = make_fastdiv((unsigned)R.row_blocks), R.by_heads = make_fastdiv((unsigned)A.kv_heads), R.by_splits = make_fastdiv((unsigned)R.splits), R.by_workers = make_fastdiv((unsigned)(R.splits * rings));
-    static std::atomic<unsigned long long> set{0};
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev > 63) return TCQ_ERR_DEVICE;
-    if (!(set.load(std::memory_order_relaxed) >> dev & 1)) {
-        if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, P::bytes(kRowWarps, 3)) != cudaSuccess) return TCQ_ERR_LAUNCH;
-        set.fetch_or(1ull << dev, std::memory_order_relaxed);
-    }
-    cudaLaunchConfig_t cfg = {};
+    R.by_blocks = make_fastdiv((unsigned)R.row_blocks), R.by_heads = make_fastdiv((unsigned)A.kv_heads);
+    R.by_splits = make_fastdiv((unsigned)R.splits), R.by_workers = make_fastdiv((unsigned)(R.splits * rings));
     cfg.gridDim = dim3((unsigned)(R.whole ? (units + rings - 1) / rings : units * R.splits));
-    cfg.blockDim = dim3(kRowThreads);
     cfg.dynamicSmemBytes = P::bytes(rings, R.stages);
-    cfg.stream = (cudaStream_t)stream;
-    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     attr[1].id = cudaLaunchAttributeClusterDimension;
     attr[1].val.clusterDim.x = R.splits, attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-    cfg.attrs = attr;
     cfg.numAttrs = R.splits > 1 ? 2 : 1;
     return cudaLaunchKernelEx(&cfg, kern, A, km, vm, R) == cudaSuccess ? TCQ_OK : TCQ_ERR_LAUNCH;
 }
