@@ -297,3 +297,19 @@ assert K.device_error() == 0
 '''
     r = subprocess.run([sys.executable, '-c', code], cwd=Path(__file__).resolve().parent.parent, capture_output=True, text=True, timeout=120)
     assert r.returncode == 0, r.stderr[-2000:]
+
+
+@pytest.mark.parametrize('T,heads', [(300, 2), (100, 2), (17, 4)])
+@pytest.mark.parametrize('D', [64, 72, 128])
+def test_blocks_left_out(K, T, heads, D):
+    """Blocks of 64 states of which the mask leaves all, some or none: neighbours, far ones, an odd number of them, the ragged last one."""
+    N = 64 * 19 + 37
+    keep = [[0, 1, 2, 3], [0, 2, 4, 6, 8], [18, 19], [19], [1], [3, 4, 9, 17], list(range(20)), [0, 19], [5, 6, 7]]
+    block = torch.arange(N, device='cuda') // 64
+    mask = torch.stack([torch.isin(block, torch.tensor(b, device='cuda')) for b in keep])
+    mask[3:, ::5] = False
+    B = len(keep)
+    q, k, v = rand(B, T, heads * D), rand(B, N, heads * D, seed=1), rand(B, N, heads * D, seed=2)
+    k[~mask], v[~mask] = math.nan, math.inf
+    check(K, q, k, v, heads, mask=mask)
+    check(K, q, k, v, heads, mask=mask, lens=ints([N, N, N - 30, N, 64, 64 * 17 + 1, 64 * 11, N - 1, 64 * 6 + 3]))

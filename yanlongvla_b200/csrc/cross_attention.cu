@@ -90,7 +90,12 @@ constexpr float kRef = 5.f, kSlack = 8.f;
 //   - the same unit, its states divided among the rings of a cluster's CTAs (few units). A row's parts are added in shared memory, a
 //     cluster's through distributed shared memory, always in the same order.
 // A ring holds chunks of 32 states (16 above head width 64): TMA, 128-byte swizzle, zeros past D and N. The requesting warp
-// passes over chunks of which the mask leaves nothing, and tells what each stage holds.
+// passes over chunks of which the mask leaves nothing, and tells what each stage holds. Up to head width 64 a warp takes two tiles of 16
+// rows where there are more than 16 (fragments of K and V read once for both).
+//
+// One token of four sequences over 16411 states of 8 heads of 64: 26 us, 5.1 TB/s. 32 x 17 queries over 160 states, 32 heads of 48: 8.0 us
+// (requests by the computing warps 24.5, by a warp ring after ring 15.6, by a lane for each ring 8.5), bound by five chunks in a
+// row of 700 to 1,000 clocks in each of eight warps an SM, which 168 registers leave.
 constexpr int kRowWarps = 4, kRowThreads = 32 * (kRowWarps + 1);
 
 TCQ_HD void ldsm4(u32 addr, u32 (&r)[4]) {
@@ -518,6 +523,13 @@ k_cross_rows(const CrossArgs A, const __grid_constant__ CUtensorMap kmap, const 
 // of the tile before, and a commit covers every product issued before it: scores that have arrived mean that O is complete
 // up to the tile before. The reference m of a row moves only when a score passes it by kSlack; O (in TMEM) is then
 // rescaled by its own row's thread.
+//
+// Bound by the products' shared-memory operands (a tile for both groups at head width 128 takes 3,100 clocks, with the exponentials left out 2,900,
+// where its products alone should take 2,048) and, below that width, by the chain scores - maximum - weights (a warp alone gets an
+// exponential in 11 clocks of the unit's 8; 2,830 clocks a tile at width 64): 2 x 4096 x 4096, 32 heads of 128 over 8 (F16) 449 to 455 us,
+// 1,208 to 1,224 TFLOP/s; heads of 64 374 us. Measured on the way, the first of these: queries requested one by one 544 us, the waits' loop
+// entered for complete barriers 468. No faster: scores in two halves 521, two threads to a row 464 (against 465), a product warp for each group
+// 459 (454), an eighth of the exponentials by polynomial 466 (454), the groups taking turns at the exponentials 474 (454).
 constexpr int kTile = 128;
 template <int DP, bool ROWS>
 struct Tiles {
@@ -550,6 +562,11 @@ struct TileMeta {
 enum { TBAR_FULL = 0, TBAR_EMPTY = 8, TBAR_CLEAN = 16, TBAR_S = 24, TBAR_P = 26, TBAR_READ = 30, TBAR_O = 32, TBAR_Q = 34, TBAR_END = 35, TBAR_COUNT = 36 };
 
 
+// Boxes of a whole tile's states, and of half a tile's (only where a mask may leave blocks out between two that are wanted: a tile in two
+// boxes costs 7 % of the whole call, 2 x 4096 x 4096, heads of 128, 456 -> 488 us).
+struct TileMaps {
+    CUtensorMap k, v, k_half, v_half;
+};
 struct TilesPlan {
     int row_tiles, tile_rows, splits;
     FastDiv by_tiles, by_heads, by_splits;
@@ -557,7 +574,7 @@ struct TilesPlan {
 
 template <int DT, int DP, bool ROWS>
 __global__ void __launch_bounds__(Tiles<DP, ROWS>::THREADS, 1)
-k_cross_tiles(const CrossArgs A, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const TilesPlan R) {
+k_cross_tiles(const CrossArgs A, const __grid_constant__ TileMaps maps, const TilesPlan R) {
     typedef Tiles<DP, ROWS> P;
     constexpr int KS = DP / 16;
     constexpr u32 IDESC = DT == TCQ_DT_BF16 ? kIdescBf16 : 0u;
@@ -600,12 +617,13 @@ k_cross_tiles(const CrossArgs A, const __grid_constant__ CUtensorMap kmap, const
     pdl_launch_dependents();
     pdl_wait();
 
-    // ---- the unit: rows r0 .. r1 - 1 of key head h of sequence b, and this CTA's tiles [k0, k1) of its states
+    // ---- the unit: rows r0 .. r1 - 1 of key head h of sequence b, and this CTA's half tiles [k0, k1) of its states
     const int splits = R.splits, unit = (int)fdiv(blockIdx.x, R.by_splits), sp = (int)blockIdx.x - unit * splits;
     const int bh = (int)fdiv((unsigned)unit, R.by_tiles), b = (int)fdiv((unsigned)bh, R.by_heads), h = bh - b * A.kv_heads;
     const int r0 = (unit - bh * R.row_tiles) * R.tile_rows, r1 = min(A.rows, r0 + R.tile_rows);
     const int len = states_of(A, b), tiles = (len + kTile - 1) / kTile;
-    const int each = (int)fdiv((unsigned)tiles, R.by_splits), more = tiles - each * splits, k0 = sp * each + min(sp, more), k1 = k0 + each + (sp < more);
+    const int each = (int)fdiv((unsigned)tiles, R.by_splits), more = tiles - each * splits, first = sp * each + min(sp, more);
+    const int k0 = 2 * first, k1 = min(2 * (first + each + (sp < more)), (len + kTile / 2 - 1) / (kTile / 2));
     const bool parts = splits > 1 || !ROWS;                   // rows have more than one part
     const bool ragged = A.lens || A.mask;
 
@@ -803,43 +821,63 @@ k_cross_tiles(const CrossArgs A, const __grid_constant__ CUtensorMap kmap, const
         }
     } else if (k1 > k0 && warp == W_LOAD) {
         // ------------------------------------------------------------------------------------------------ load
-        // Item 2 t of the ring is the keys of the t-th tile that holds a state, item 2 t + 1 its values.
+        // A tile is made of the next two blocks of 64 states that hold one, so that what a mask leaves out in such blocks (an image) costs
+        // nothing. Item 2 t of the ring is the keys of tile t, item 2 t + 1 its values.
+        constexpr int H = kTile / 2;
         const unsigned char* mrow = A.mask ? A.mask + b * A.mask_sb : nullptr;
-        unsigned char mb[4] = {};
-        auto look = [&](int i) {
+        unsigned char mb[2] = {};
+        int i = k0;
+        auto look = [&]() {                                   // the truth values of block i
             if (mrow && i < k1)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) mb[j] = i * kTile + 32 * j + lane < len ? mrow[i * kTile + 32 * j + lane] : 0;
+                for (int j = 0; j < 2; ++j) mb[j] = i * H + 32 * j + lane < len ? mrow[i * H + 32 * j + lane] : 0;
         };
-        look(k0);
+        auto next = [&](u32& w0, u32& w1) -> int {            // the next block with a state, its truth values; below 0: none
+            w0 = w1 = 0;
+            while (i < k1) {
+                const int n = len - i * H;
+                w0 = mrow ? __ballot_sync(0xffffffffu, mb[0] != 0) : n >= 32 ? 0xffffffffu : (1u << n) - 1u;
+                w1 = mrow ? __ballot_sync(0xffffffffu, mb[1] != 0) : n >= 64 ? 0xffffffffu : n > 32 ? (1u << (n - 32)) - 1u : 0u;
+                ++i;
+                look();
+                if (w0 | w1) return i - 1;
+            }
+            return -1;
+        };
+        look();
         bool ok = true;
         int t = 0;
         auto slot_free = [&](int item) { return item < P::RING || wait(TBAR_EMPTY + item % P::RING, item / P::RING - 1); };
-        for (int i = k0; i < k1 && ok; ++i) {
-            u32 bits[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int n = len - i * kTile - 32 * j;
-                bits[j] = mrow ? __ballot_sync(0xffffffffu, mb[j] != 0) : n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u;
-            }
-            look(i + 1);
-            if (!(bits[0] | bits[1] | bits[2] | bits[3])) continue;
-            const bool whole = (bits[0] & bits[1] & bits[2] & bits[3]) == 0xffffffffu;
+        while (ok) {
+            u32 w[4];
+            const int b0 = next(w[0], w[1]);
+            if (b0 < 0) break;
+            const int b1 = next(w[2], w[3]);
+            // Neighbours, or the last block alone, are one box: what it has too much is not there, rows past the last state arrive as zeros.
+            const bool one = b1 < 0 || b1 == b0 + 1;
             ok = slot_free(2 * t);
             if (ok && lane == 0) {
                 TileMeta& e = meta[t & (P::META - 1)];
-                e.at = i, e.whole = whole;
-                e.bits[0] = bits[0], e.bits[1] = bits[1], e.bits[2] = bits[2], e.bits[3] = bits[3];
+                e.at = b0, e.whole = (w[0] & w[1] & w[2] & w[3]) == 0xffffffffu;
+                e.bits[0] = w[0], e.bits[1] = w[1], e.bits[2] = w[2], e.bits[3] = w[3];
             }
             for (int vals = 0; vals < 2 && ok; ++vals) {
                 const int item = 2 * t + vals, s = item % P::RING;
                 if (vals) ok = slot_free(item);
                 if (ok && lane == 0) {
+                    const u32 dst = sbase + P::RING0 + s * P::TB;
+                    const int sequence = b * (vals ? A.vb : A.kb);
                     mbar_expect_tx(bar(TBAR_FULL + s), P::TB);
 #pragma unroll
-                    for (int a = 0; a < P::ATOMS; ++a)
-                        tma_load_4d(sbase + P::RING0 + s * P::TB + a * (kTile * 128), vals ? &vmap : &kmap, bar(TBAR_FULL + s), 64 * a, i * kTile, h,
-                                    b * (vals ? A.vb : A.kb));
+                    for (int a = 0; a < P::ATOMS; ++a) {
+                        const u32 to = dst + a * (kTile * 128);
+                        if (one) {
+                            tma_load_4d(to, vals ? &maps.v : &maps.k, bar(TBAR_FULL + s), 64 * a, b0 * H, h, sequence);
+                        } else {
+                            tma_load_4d(to, vals ? &maps.v_half : &maps.k_half, bar(TBAR_FULL + s), 64 * a, b0 * H, h, sequence);
+                            tma_load_4d(to + H * 128, vals ? &maps.v_half : &maps.k_half, bar(TBAR_FULL + s), 64 * a, b1 * H, h, sequence);
+                        }
+                    }
                 }
                 __syncwarp();
             }
@@ -1005,7 +1043,7 @@ k_cross_tiles(const CrossArgs A, const __grid_constant__ CUtensorMap kmap, const
 }
 
 template <int DT, int DP, bool ROWS>
-int launch_tiles(const CrossArgs& A, const CUtensorMap& km, const CUtensorMap& vm, void* stream) {
+int launch_tiles(const CrossArgs& A, const TileMaps& maps, void* stream) {
     typedef Tiles<DP, ROWS> P;
     const auto kern = k_cross_tiles<DT, DP, ROWS>;
     const int most = ROWS ? 2 * kTile : kTile;
@@ -1061,7 +1099,7 @@ int launch_tiles(const CrossArgs& A, const CUtensorMap& km, const CUtensorMap& v
     cfg.gridDim = dim3((unsigned)(units * splits));
     attr[0].val.clusterDim.x = splits;
     cfg.numAttrs = 2;
-    return cudaLaunchKernelEx(&cfg, kern, A, km, vm, R) == cudaSuccess ? TCQ_OK : TCQ_ERR_LAUNCH;
+    return cudaLaunchKernelEx(&cfg, kern, A, maps, R) == cudaSuccess ? TCQ_OK : TCQ_ERR_LAUNCH;
 }
 
 // Zeros for queries without states (N = 0).
@@ -1203,20 +1241,26 @@ int tcq_cross_attention(const void* q, int64_t q_sb, int64_t q_st, const void* k
     }
     // sequences that share one batch of states (stride 0) have one in the tensor map
     if (B == 1) k_sb = v_sb = 0;
-    CUtensorMap km, vm;
-    const bool tiles = prefer_tiles(rows, N, head_dim, (i64)B * kv_heads);
-    const int box = tiles ? kTile : by_width(head_dim, [](auto d) { return Rows<decltype(d)::value, 1>::CHUNK; });
-    if (!encode(&km, k, dtype, head_dim, N, kv_heads, B, k_st, k_sb, box) || !encode(&vm, v, dtype, head_dim, N, kv_heads, B, v_st, v_sb, box))
-        return TCQ_ERR_DEVICE;
+    const auto maps_of = [&](CUtensorMap& km, CUtensorMap& vm, int box) {
+        return encode(&km, k, dtype, head_dim, N, kv_heads, B, k_st, k_sb, box) && encode(&vm, v, dtype, head_dim, N, kv_heads, B, v_st, v_sb, box);
+    };
     const int group = heads / kv_heads;
     const CrossArgs A = {(const u16*)q, q_sb, q_st, (u16*)out, lens, mask, mask_sb, B, S, T, N, heads, kv_heads, group, head_dim, (int)rows,
                          k_sb != 0, v_sb != 0, make_fastdiv((unsigned)group), make_fastdiv((unsigned)T), scale * 1.4426950408889634f};
+    if (prefer_tiles(rows, N, head_dim, (i64)B * kv_heads)) {
+        TileMaps maps;
+        if (!maps_of(maps.k, maps.v, kTile) || (mask && !maps_of(maps.k_half, maps.v_half, kTile / 2))) return TCQ_ERR_DEVICE;
+        if (!mask) maps.k_half = maps.k, maps.v_half = maps.v;
+        return by_width(head_dim, [&](auto d) {
+            constexpr int DP = decltype(d)::value;
+            if (dtype == TCQ_DT_BF16) return rows <= kTile ? launch_tiles<TCQ_DT_BF16, DP, false>(A, maps, stream) : launch_tiles<TCQ_DT_BF16, DP, true>(A, maps, stream);
+            return rows <= kTile ? launch_tiles<TCQ_DT_F16, DP, false>(A, maps, stream) : launch_tiles<TCQ_DT_F16, DP, true>(A, maps, stream);
+        });
+    }
     return by_width(head_dim, [&](auto d) {
         constexpr int DP = decltype(d)::value;
-        if (tiles) {
-            if (dtype == TCQ_DT_BF16) return rows <= kTile ? launch_tiles<TCQ_DT_BF16, DP, false>(A, km, vm, stream) : launch_tiles<TCQ_DT_BF16, DP, true>(A, km, vm, stream);
-            return rows <= kTile ? launch_tiles<TCQ_DT_F16, DP, false>(A, km, vm, stream) : launch_tiles<TCQ_DT_F16, DP, true>(A, km, vm, stream);
-        }
+        CUtensorMap km, vm;
+        if (!maps_of(km, vm, Rows<DP, 1>::CHUNK)) return (int)TCQ_ERR_DEVICE;
         if constexpr (DP <= 64) {
             if (rows > 16) return dtype == TCQ_DT_BF16 ? launch_rows<TCQ_DT_BF16, DP, 2>(A, km, vm, stream) : launch_rows<TCQ_DT_F16, DP, 2>(A, km, vm, stream);
         }
