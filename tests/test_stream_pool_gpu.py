@@ -150,6 +150,32 @@ def test_a_pool_without_pages_left(P, setup, K, Memory):
         named(memory)
 
 
+def test_what_keep_refuses_and_cuts(P, setup, K, Memory):
+    """An index or a number of tokens that keep refuses costs no page of the pool; more tokens than a robot remembers are cut, on the
+    host's count too."""
+    c, model = setup
+    n = c.prefix_tokens
+    memory = Memory(c, 2, 2 * n, pages=16)
+    with torch.no_grad():
+        model(*frames(P, c, 2, 1)[0], memory=memory)
+    refs, index = memory.pages.refs.clone(), ints([[0] * 8] * 2)
+    for bad in (index.long(), index[:1], index[0], index[:, :0], index.cpu()):
+        with pytest.raises(K.TcqError, match='index'):
+            memory.keep(bad)
+    for bad in (ints([8, 8]).long(), ints([8]), torch.tensor([8, 8], dtype=torch.int32)):
+        with pytest.raises(K.TcqError, match='kept'):
+            memory.keep(index, bad)
+    assert torch.equal(memory.pages.refs, refs) and memory.lens.tolist() == [n, n] and memory.tokens == n
+    named(memory)
+    memory.keep(index[:, ::2], ints([9, -1]))                                   # the same token four times; a view of every other number
+    assert memory.lens.tolist() == [4, 0] and memory.tokens == 4
+    named(memory)
+    memory.keep(ints([[3, 2, 1, 0, 0, 0, 0]] * 2))
+    assert memory.lens.tolist() == [4, 0] and memory.tokens == 4
+    named(memory)
+    assert K.device_error() == 0
+
+
 def test_a_window_in_a_graph(P, K, Memory):
     """A frame with what goes before it forgotten, captured once: replays give what the steps outside a graph give."""
     c = P.PolicyConfig(vit_layers=1, llm_layers=2, dit_layers=1)

@@ -62,13 +62,13 @@ class StreamMemory:
     def begin_frame(self, frame=None, count=None):
         """Make room for the next frame: its tokens follow those remembered. On the device but for the check of the capacity.
         frame: the (B, T, ...) tensor that the layers will get; one of another batch or length is refused before anything moves.
-        count (robots,) int32: each robot's tokens of the frame (0 .. its length), the rest is padding (None: all). A robot that the pool of pages does
-        not serve remembers nothing of the frame (device_error reports flag 2)."""
+        count (robots,) int32: each robot's tokens of the frame (0 .. its length), the rest is padding (None: all). A robot that the
+        pool of pages does not serve remembers nothing of the frame (device_error reports flag 2)."""
         n = self.pos.shape[2]
         if frame is not None and tuple(frame.shape[:2]) != (self.robots, n):
             raise K.TcqError(f'StreamMemory: a frame of {self.robots} robots with {n} tokens each expected, got {tuple(frame.shape[:2])}')
-        if count is not None and (count.dtype != torch.int32 or count.shape != self.lens.shape or count.device != self.lens.device):
-            raise K.TcqError(f'StreamMemory: count must be int32 ({self.robots},) on {self.lens.device}, got {count.dtype} {tuple(count.shape)}')
+        if count is not None:
+            self._ints('count', count, (self.robots,))
         if not torch.cuda.is_current_stream_capturing():
             self.reserve()
         self.pos[0] += 1
@@ -88,6 +88,10 @@ class StreamMemory:
         K.rope_axes(q, self.pos, self.rope, out=q)
         return K.kv8_attention(q, cache, self.table, self.lens, count=self.count)
 
+    def _ints(self, name, t, shape):
+        if t.dtype != torch.int32 or tuple(t.shape) != shape or t.device != self.lens.device:
+            raise K.TcqError(f'StreamMemory: {name} must be int32 {shape} on {self.lens.device}, got {t.dtype} {tuple(t.shape)} on {t.device}')
+
     def _pooled(self, what):
         if self.pages is None:
             raise K.TcqError(f'StreamMemory: {what} needs a pool of pages (pages=)')
@@ -99,14 +103,20 @@ class StreamMemory:
         K.kv8_fork(self.pages, self.table, self.lens, parent)
 
     def keep(self, index, kept=None):
-        """Remember only the tokens index[b, j], j < kept[b] (index (robots, n) int32, kept (robots,) int32 or None: all n), packed into
-        pages of the pool, which takes the old ones back; positions in time and space stay what they were. A robot whose tokens
-        the pool's free pages do not hold next to the old ones keeps its memory (device_error reports flag 2)."""
+        """Remember only the tokens index[b, j], j < kept[b] (index (robots, n) int32, kept (robots,) int32 or None: all n; at most as
+        many as robot b remembers), packed into pages of the pool, which takes the old ones back; positions in time and space
+        stay what they were. A robot whose tokens the pool's free pages do not hold next to the old ones keeps its memory
+        (device_error reports flag 2)."""
         self._pooled('keep')
-        n = index.shape[1]
+        n = index.shape[-1] if index.dim() else 0
+        self._ints('index', index, (self.robots, max(n, 1)))
+        if kept is not None:
+            self._ints('kept', kept, (self.robots,))
         if n > self.table.shape[1] * K.KV8_BLOCK:
             raise K.TcqError(f'StreamMemory: {n} tokens do not fit {self.max_tokens}')
-        kept = torch.full_like(self.lens, n) if kept is None else kept
+        most = self.lens.clamp(max=n)
+        kept = most if kept is None else kept.clamp(min=0).minimum(most)
+        index = index.contiguous()
         table = self.pages.table(*self.table.shape)
         granted, _ = K.kv8_reserve(self.pages, table, torch.zeros_like(self.lens), kept)
         K.kv8_compact(self.caches, self.table, self.lens, index, table, kept=granted)
