@@ -34,6 +34,9 @@ def test_refuses(L):
         assert cross(**{name: A + 8}) == 2
     for name in ('q_sb', 'q_st', 'k_sb', 'k_st', 'v_sb', 'v_st'):
         assert cross(**{name: 4100}) == 2
+    for at in (A + 64, B, B + 64, C + 4096, D_):                                                # out in the queries, keys or values
+        assert cross(out=at, **({'q': D_ + 64} if at == D_ else {})) == 4
+    assert cross(q=D_, q_sb=8192, out=D_) == 4                                                   # q with gaps: its rows would move
     assert cross(k_st=0) == 4 and cross(v_st=0) == 4 and cross(k_sb=-4096) == 4                  # states on one another, backwards
 
 

@@ -206,6 +206,20 @@ def test_graphs_and_streams(K, T, N):
     assert K.device_error() == 0
 
 
+@pytest.mark.parametrize('T,heads,kv_heads,N', [(1, 8, 2, 9000), (1, 4, 4, 5), (17, 4, 4, 160), (150, 2, 2, 300), (130, 2, 2, 3000), (300, 4, 2, 700)])
+def test_output_in_place_of_the_queries(K, T, heads, kv_heads, N):
+    for D in (48, 128):
+        q, k, v = rand(3, T, heads * D), rand(3, N, kv_heads * D, seed=1), rand(3, N, kv_heads * D, seed=2)
+        for lens in (None, ints([N, 0, N // 2])):
+            want, own = K.cross_attention(q, k, v, heads, kv_heads, lens=lens), q.clone()
+            assert K.cross_attention(own, k, v, heads, kv_heads, lens=lens, out=own) is own
+            assert torch.equal(own, want)
+        wide = rand(6, T, heads * D)
+        with pytest.raises(K.TcqError):
+            K.cross_attention(wide[:3], k, v, heads, kv_heads, out=wide[1:4])
+    assert K.device_error() == 0
+
+
 def test_refusals(K):
     q, k = rand(2, 3, 128), rand(2, 50, 64, seed=1)
     ok = dict(q=q, k=k, v=k, heads=2, kv_heads=1)

@@ -1204,11 +1204,12 @@ int by_width(int d, F f) {
 
 // Products of 16 rows or tiles of 128? A tile's CTA costs about 5 us before and behind its states, and computes 128 or 256 rows whatever
 // there are; a row costs three times as much in the other kernel. Where tiles give every unit an SM of its own (and its states
-// are divided over a cluster), they win from 256 states on if the rows are not few (us, products of 16 / tiles, heads of 64: 8 units of
-// 33 rows over 160 states 6.5 / 6.3, over 640 12.7 / 8.8; of 17 rows 7.8 / 8.5; heads of 128: 33 rows over 640 8.4 / 11.0, 64 rows 12.8 /
-// 11.8; 64 units of 17 rows over 1280 17.4 / 12.7). Else by what the states of a unit cost in either, in picoseconds of the device (heads of 64: 1.15 a row and state against
-// 0.35, 50,000 a tile of rows; of 128: 1.95, 0.43, 60,000): 512 units of 64 rows over 640 states 27.8 / 37.3, over 2560 98.4 / 83.0; of 256
-// rows over 160 states 34 / 38, over 320 55 / 44; heads of 128, 256 rows over 160 states 58 / 48.
+// are divided over a cluster), they win from 256 states on if the rows are not few (us, products of 16 / tiles, heads of 64: 8 units
+// of 33 rows over 160 states 6.5 / 6.3, over 640 12.7 / 8.8; of 17 rows 7.8 / 8.5; heads of 128: 33 rows over 640 8.4 / 11.0, 64
+// rows 12.8 / 11.8; 64 units of 17 rows over 1280 17.4 / 12.7). Else by what the states of a unit cost in either, in picoseconds of
+// the device (heads of 64: 1.15 a row and state against 0.35, 50,000 a tile of rows; of 128: 1.95, 0.43, 60,000): 512 units of 64
+// rows over 640 states 27.8 / 37.3, over 2560 98.4 / 83.0; of 256 rows over 160 states 34 / 38, over 320 55 / 44; heads of 128, 256
+// rows over 160 states 58 / 48.
 bool prefer_tiles(i64 rows, int N, int D, i64 units) {
     const bool wide = D > 64;
     if (N < (wide ? 128 : 256)) return false;
@@ -1234,6 +1235,14 @@ int tcq_cross_attention(const void* q, int64_t q_sb, int64_t q_st, const void* k
     if (!tcq_aligned(q, 16) || !tcq_aligned(k, 16) || !tcq_aligned(v, 16) || !tcq_aligned(out, 16)) return TCQ_ERR_ALIGN;
     if ((q_sb | q_st | k_sb | k_st | v_sb | v_st) & 7) return TCQ_ERR_ALIGN;
     if (k_sb < 0 || k_st < 0 || v_sb < 0 || v_st < 0 || (N > 1 && (k_st < 8 || v_st < 8))) return TCQ_ERR_ARG;
+    // out may be q itself (a row's queries are read before it is written); beyond that it shares no byte with what is read
+    const i64 width = (i64)heads * head_dim, all = (i64)B * S * T * width;
+    const auto meets = [&](const void* p, i64 n) { return (const u16*)p < (const u16*)out + all && (const u16*)out < (const u16*)p + n; };
+    const bool same = q == out && (T == 1 || q_st == width) && ((i64)B * S == 1 || q_sb == T * width);
+    if (!same && q_sb >= 0 && q_st >= 0 && meets(q, ((i64)B * S - 1) * q_sb + (T - 1) * q_st + width)) return TCQ_ERR_ARG;
+    if (N > 0 && (meets(k, (B - 1) * k_sb + (N - 1) * k_st + (i64)kv_heads * head_dim) ||
+                  meets(v, (B - 1) * v_sb + (N - 1) * v_st + (i64)kv_heads * head_dim)))
+        return TCQ_ERR_ARG;
     if (N == 0) {
         const i64 n = (i64)B * S * T * heads * head_dim / 8;
         const i64 blocks = (n + 255) / 256, most = (i64)tcq_sm_count() * 8;

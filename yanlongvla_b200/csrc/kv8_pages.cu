@@ -343,9 +343,9 @@ __global__ void __launch_bounds__(256) k_kv8_copy(const __grid_constant__ Layers
 // Quotients of integers q' = q r with 0 <= r <= 1: the byte in a float's low bits (2^23 + 128 + q), its offset taken off, times r,
 // rounded to nearest even by adding 1.5 * 2^23; each step one rounding.
 //
-// Bound by HBM: three quarters of 2 x 65531 tokens, 8 heads of 128, four layers: 240 us of the 614 with the read back, 6.6 TB/s of what is kept and
-// written; half of 4 x 16411, eight layers, 8 heads of 64: 100 us (whole rows of values are read for the half of them). With source tiles in
-// shared memory and a CTA for each head 340 and 166 us.
+// Bound by HBM: three quarters of 2 x 65531 tokens, 8 heads of 128, four layers: 240 us of the 614 with the read back, 6.6 TB/s of what
+// is kept and written; half of 4 x 16411, eight layers, 8 heads of 64: 100 us (whole rows of values are read for the half of
+// them). With source tiles in shared memory and a CTA for each head about 350 and 170 us.
 // (The product stands alone: a packed one was contracted with the addition behind it, which rounds once and now and then to the other side.)
 TCQ_HD u32 scaled4(u32 w, const float4& r) {
     const u32 u = w ^ 0x80808080u, c = 0x4b000000u;
