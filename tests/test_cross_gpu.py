@@ -100,6 +100,20 @@ def test_masks(K, T, heads, kv_heads, N, dtype):
     assert not o[0].any() and not o[7].any()
 
 
+@pytest.mark.parametrize('B,T,heads,N', [(1, 1, 2, 9000), (40, 1, 16, 700), (40, 17, 16, 700), (3, 40, 2, 230)])
+@pytest.mark.parametrize('D', [64, 96])
+def test_masks_of_few_states(K, B, T, heads, N, D):
+    """Single states far apart, at the ends of what is read of a mask at a time (128 or 256 states), none at all."""
+    q, k, v = rand(B, T, heads * D), rand(B, N, heads * D, seed=1), rand(B, N, heads * D, seed=2)
+    mask = torch.zeros(B, N, dtype=torch.bool, device='cuda')
+    for b in range(B):
+        mask[b, [[127], [128], [0, N - 1], [255, 256], [N - 1], [15, 16, 144], [31, 32, 160], []][b % 8]] = True
+    if B == 1:
+        mask[0, [127, 2175, N - 1]] = True
+    check(K, q, k, v, heads, mask=mask)
+    check(K, q, k, v, heads, mask=mask, lens=torch.arange(B, dtype=torch.int32, device='cuda') * 37 % N)
+
+
 @pytest.mark.parametrize('T', [1, 17, 150, 300])
 def test_strides(K, T):
     """Keys and values as columns of one projection's output, queries of a wider one, tokens of every second row, batches shared."""
