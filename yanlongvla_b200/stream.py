@@ -8,9 +8,11 @@ remembers no more than that many frames, with candidates it forms several action
 rope_axes turns the queries, kv8_append turns and stores the keys and stores the values, kv8_attention reads the cache; of a memory
 with a pool of pages kv8_fork shares, kv8_reserve and kv8_copy give pages, kv8_compact and kv8_free forget. All lengths and
 positions live on the device, so a step can be captured in a CUDA graph: what a capture records moves them on at each
-replay, and StreamMemory.reserve(), called before each replay, keeps the host's count and checks the capacity.
+replay, and StreamMemory.reserve(), called before each replay (with what the step keeps of the past, where it forgets), keeps the
+host's count and checks the capacity.
 """
 import argparse
+import operator
 
 import torch
 
@@ -50,14 +52,20 @@ class StreamMemory:
         pos = torch.stack((torch.full_like(rows, -1), rows, cols)).to(device)          # begin_frame moves the time on
         self.pos = pos[:, None].expand(3, robots, pos.shape[1]).contiguous()
 
-    def reserve(self):
+    def reserve(self, kept=None):
         """Count the next frame in on the host; refused where it does not fit. begin_frame calls it, except in a capture, which runs
-        nothing: call it before each replay of a captured step."""
-        n = self.pos.shape[2]
-        if self.tokens + n > self.max_tokens or self.frames >= self.max_frames:
-            raise K.TcqError(f'StreamMemory: a frame of {n} tokens does not fit behind {self.tokens} of {self.max_tokens} tokens, {self.frames} frames')
+        nothing: call it before each replay of a captured step. kept: that step first keeps at most so many tokens of each robot (keep,
+        keep_recent; 0: none), which a capture does not count either."""
+        n, held = self.pos.shape[2], self.tokens
+        if kept is not None:
+            kept = operator.index(kept)
+            if kept < 0:
+                raise K.TcqError(f'StreamMemory: {kept} tokens cannot be kept')
+            held = min(held, kept)
+        if held + n > self.max_tokens or self.frames >= self.max_frames:
+            raise K.TcqError(f'StreamMemory: a frame of {n} tokens does not fit behind {held} of {self.max_tokens} tokens, {self.frames} frames')
         self.frames += 1
-        self.tokens += n
+        self.tokens = held + n
 
     def begin_frame(self, frame=None, count=None):
         """Make room for the next frame: its tokens follow those remembered. On the device but for the check of the capacity.
