@@ -31,3 +31,16 @@ def test_a_captured_window_goes_on(monkeypatch):
         with pytest.raises((K.TcqError, TypeError)):
             m.reserve(kept=kept)
     assert m.tokens == 360 and m.frames == 12
+
+
+def test_a_captured_forget_leaves_the_counts(monkeypatch):
+    """A capture runs nothing: what it records does not empty the memory on the host while the device still holds it."""
+    m, K = memory(monkeypatch, 1, 2 * N + 8)
+    m.begin_frame()
+    m.replay(lambda: (m.forget(), m.begin_frame()))                            # the capture of a step; on this machine it has run
+    assert (m.tokens, m.frames) == (N, 1)
+    m.begin_frame()
+    with pytest.raises(K.TcqError, match='does not fit'):
+        m.begin_frame()
+    m.forget()
+    assert (m.tokens, m.frames) == (0, 0) and not m.lens.any()

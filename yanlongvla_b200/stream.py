@@ -148,7 +148,10 @@ class StreamMemory:
         self.keep((self.lens - kept)[:, None] + at.minimum((kept - 1).clamp(min=0)[:, None]), kept)
 
     def forget(self):
-        self.tokens = self.frames = 0
+        """Remember nothing, time starts anew. (In a capture the host's counts stay: reserve(kept=0) before a replay, and max_frames counts
+        the frames of all replays.)"""
+        if not torch.cuda.is_current_stream_capturing():
+            self.tokens = self.frames = 0
         if self.pages is not None:
             K.kv8_free(self.pages, self.table, self.lens, torch.zeros_like(self.lens))
         self.lens.zero_()
