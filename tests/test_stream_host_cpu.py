@@ -44,3 +44,66 @@ def test_a_captured_forget_leaves_the_counts(monkeypatch):
         m.begin_frame()
     m.forget()
     assert (m.tokens, m.frames) == (0, 0) and not m.lens.any()
+
+
+@pytest.mark.parametrize('way', ['keep', 'keep_recent'])
+def test_the_count_is_not_below_what_is_there(monkeypatch, way):
+    """Robots whose tokens the pool does not hold next to the old ones keep their memory, and the host's count with it."""
+    m, K = memory(monkeypatch, 2, 2 * N, pages=10)                              # five pages a robot for two frames: none is left
+    m.begin_frame()
+    m.begin_frame()
+
+    def keep(n):
+        if way == 'keep':
+            m.keep(ints([list(range(n))] * 2))
+        else:
+            m.keep_recent(n)
+    keep(100)
+    assert K.flag == 2 and m.lens.tolist() == [2 * N] * 2 and m.tokens == 2 * N
+    with pytest.raises(K.TcqError, match='does not fit'):
+        m.begin_frame()
+    named(m)
+    m.forget()
+    m.begin_frame(count=ints([N, 10]))                                          # four pages; two more for robot 0, one for robot 1
+    keep(100)
+    assert m.lens.tolist() == [100, 10] and m.tokens == 100
+    named(m)
+
+
+def test_no_look_at_the_device_where_the_pool_is_large(monkeypatch):
+    """A window as the command sizes it is kept without reading a length back; where the pool might be too small, one is read."""
+    for pages, reads in ((2 * (6 + 4), 0), (2 * (6 + 4) - 1, 3)):
+        m, K = memory(monkeypatch, 2, 360, pages=pages)
+        seen = []
+        monkeypatch.setattr(m, '_longest', lambda own=m._longest: (seen.append(1), own())[1])
+        for _ in range(6):
+            m.keep_recent(200)
+            m.begin_frame(count=ints([N, 10]))
+            assert m.tokens == int(m.lens.max())
+            named(m)
+        assert len(seen) == reads
+
+
+def test_what_a_replay_keeps_in_a_small_pool(monkeypatch):
+    """Whether a pool that may be too small serves the keep of a replay is not known before it: the count stays."""
+    m, K = memory(monkeypatch, 2, 360, pages=2 * (5 + 4) - 1)
+
+    def step():
+        m.keep_recent(200)
+        m.begin_frame()
+    m.begin_frame()
+    m.begin_frame()
+    with pytest.raises(K.TcqError, match='does not fit'):
+        m.reserve(kept=200)
+    assert (m.tokens, m.frames) == (2 * N, 2)
+    m.forget()
+    m.begin_frame()
+    m.reserve(kept=200)                                                        # four pages a robot at most before it, three kept
+    m.replay(step)
+    assert m.lens.tolist() == [2 * N] * 2 and m.tokens == 2 * N
+    m, K = memory(monkeypatch, 1, N)                                            # without a pool nothing is kept, all may be forgotten
+    m.begin_frame()
+    with pytest.raises(K.TcqError, match='pool'):
+        m.reserve(kept=10)
+    m.reserve(kept=0)
+    assert (m.tokens, m.frames) == (N, 2)

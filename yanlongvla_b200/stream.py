@@ -55,17 +55,29 @@ class StreamMemory:
     def reserve(self, kept=None):
         """Count the next frame in on the host; refused where it does not fit. begin_frame calls it, except in a capture, which runs
         nothing: call it before each replay of a captured step. kept: that step first keeps at most so many tokens of each robot (keep,
-        keep_recent; 0: none), which a capture does not count either."""
+        keep_recent; 0: none), which a capture does not count either; where the pool might not hold them next to the old ones (see keep), the
+        count stays."""
         n, held = self.pos.shape[2], self.tokens
         if kept is not None:
             kept = operator.index(kept)
             if kept < 0:
                 raise K.TcqError(f'StreamMemory: {kept} tokens cannot be kept')
-            held = min(held, kept)
+            if kept:
+                self._pooled('keep')
+            if self._holds(kept):
+                held = min(held, kept)
         if held + n > self.max_tokens or self.frames >= self.max_frames:
             raise K.TcqError(f'StreamMemory: a frame of {n} tokens does not fit behind {held} of {self.max_tokens} tokens, {self.frames} frames')
         self.frames += 1
         self.tokens = held + n
+
+    def _holds(self, n):
+        """Whether the pool surely holds n tokens of every robot next to all that they may remember."""
+        blocks = lambda tokens: -(-tokens // K.KV8_BLOCK)
+        return n < 1 or self.robots * (blocks(self.tokens) + blocks(min(n, self.tokens))) <= self.pages.pages
+
+    def _longest(self):
+        return int(self.lens.max())
 
     def begin_frame(self, frame=None, count=None):
         """Make room for the next frame: its tokens follow those remembered. On the device but for the check of the capacity.
@@ -113,8 +125,9 @@ class StreamMemory:
     def keep(self, index, kept=None):
         """Remember only the tokens index[b, j], j < kept[b] (index (robots, n) int32, kept (robots,) int32 or None: all n; at most as
         many as robot b remembers), packed into pages of the pool, which takes the old ones back; positions in time and space
-        stay what they were. A robot whose tokens the pool's free pages do not hold next to the old ones keeps its memory
-        (device_error reports flag 2)."""
+        stay what they were. A robot whose tokens the pool's free pages do not hold next to the old ones keeps its memory, and so do all
+        behind it (device_error reports flag 2). A pool of robots * (blocks of all that they remember + blocks of n) pages serves all;
+        where it may be smaller, the call reads a length back to know whether it did (not in a capture)."""
         self._pooled('keep')
         n = index.shape[-1] if index.dim() else 0
         self._ints('index', index, (self.robots, max(n, 1)))
@@ -133,7 +146,7 @@ class StreamMemory:
         self.table.copy_(torch.where(stays[:, None], self.table, table))
         self.lens.copy_(torch.where(stays, self.lens, granted))
         if not torch.cuda.is_current_stream_capturing():
-            self.tokens = min(self.tokens, n)
+            self.tokens = min(self.tokens, n) if self._holds(n) else self._longest()
 
     def keep_recent(self, tokens):
         """Remember only the newest `tokens` tokens of each robot (0: none). Positions go on as if the others were still there."""
