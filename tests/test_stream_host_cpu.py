@@ -107,3 +107,37 @@ def test_what_a_replay_keeps_in_a_small_pool(monkeypatch):
         m.reserve(kept=10)
     m.reserve(kept=0)
     assert (m.tokens, m.frames) == (N, 2)
+
+
+@pytest.mark.parametrize('pages', [None, 16])
+def test_short_frames_count_what_they_hold(monkeypatch, pages):
+    """Frames of which padding is not remembered count in full until that is too much; then what is there counts."""
+    m, K = memory(monkeypatch, 2, 2 * N, pages=pages)
+    seen = []
+    monkeypatch.setattr(m, '_longest', lambda own=m._longest: (seen.append(1), own())[1])
+    for f in range(1, 9):
+        m.begin_frame(count=ints([20, 3]))
+        assert m.lens.tolist() == [20 * f, 3 * f] and m.tokens >= 20 * f and m.frames == f
+    assert m.tokens == 140 + N and len(seen) == 6
+    with pytest.raises(K.TcqError, match='does not fit behind 160'):
+        m.max_tokens = 2 * N - 1
+        m.begin_frame()
+    assert m.lens.tolist() == [160, 24] and m.frames == 8 and m.pos[0].eq(7).all()
+
+
+def test_frames_that_were_counted_and_not_run_count(monkeypatch):
+    """What is read from the device lacks the frames that have been counted in for replays to come."""
+    m, K = memory(monkeypatch, 1, 4 * N)
+    m.begin_frame(count=ints([20]))
+    m.reserve()
+    m.reserve()
+    m.reserve()                                                                # 20 on the device, three frames to come
+    assert m.tokens == 4 * N
+    with pytest.raises(K.TcqError, match=f'does not fit behind {20 + 3 * N} '):
+        m.reserve()
+    m.replay(m.begin_frame)
+    m.replay(m.begin_frame)
+    with pytest.raises(K.TcqError, match=f'does not fit behind {20 + 3 * N} '):
+        m.reserve()
+    m.replay(m.begin_frame)
+    assert m.lens.tolist() == [20 + 3 * N] == [m.tokens] and m.frames == 4

@@ -56,20 +56,24 @@ class StreamMemory:
         """Count the next frame in on the host; refused where it does not fit. begin_frame calls it, except in a capture, which runs
         nothing: call it before each replay of a captured step. kept: that step first keeps at most so many tokens of each robot (keep,
         keep_recent; 0: none), which a capture does not count either; where the pool might not hold them next to the old ones (see keep), the
-        count stays."""
-        n, held = self.pos.shape[2], self.tokens
+        count stays. Frames of which a count was remembered (begin_frame) are counted in full; where that is too much, the longest
+        memory's length is read from the device, behind the work of the current stream."""
+        n = self.pos.shape[2]
         if kept is not None:
             kept = operator.index(kept)
             if kept < 0:
                 raise K.TcqError(f'StreamMemory: {kept} tokens cannot be kept')
             if kept:
                 self._pooled('keep')
-            if self._holds(kept):
-                held = min(held, kept)
-        if held + n > self.max_tokens or self.frames >= self.max_frames:
-            raise K.TcqError(f'StreamMemory: a frame of {n} tokens does not fit behind {held} of {self.max_tokens} tokens, {self.frames} frames')
+
+        def held():
+            return min(self.tokens, kept) if kept is not None and self._holds(kept) else self.tokens
+        if held() + n > self.max_tokens and not torch.cuda.is_current_stream_capturing():
+            self.tokens = self._longest()                                        # frames with a count held less than was counted
+        if held() + n > self.max_tokens or self.frames >= self.max_frames:
+            raise K.TcqError(f'StreamMemory: a frame of {n} tokens does not fit behind {held()} of {self.max_tokens} tokens, {self.frames} frames')
+        self.tokens = held() + n
         self.frames += 1
-        self.tokens = held + n
 
     def _holds(self, n):
         """Whether the pool surely holds n tokens of every robot next to all that they may remember."""
@@ -77,7 +81,9 @@ class StreamMemory:
         return n < 1 or self.robots * (blocks(self.tokens) + blocks(min(n, self.tokens))) <= self.pages.pages
 
     def _longest(self):
-        return int(self.lens.max())
+        """The longest memory's tokens, read from the device, and those of frames that were counted and are not there yet."""
+        longest, last = torch.stack((self.lens.max(), self.pos[0, 0, 0])).tolist()
+        return min(self.tokens, longest + (self.frames - 1 - last) * self.pos.shape[2])
 
     def begin_frame(self, frame=None, count=None):
         """Make room for the next frame: its tokens follow those remembered. On the device but for the check of the capacity.
