@@ -141,3 +141,44 @@ def test_frames_that_were_counted_and_not_run_count(monkeypatch):
         m.reserve()
     m.replay(m.begin_frame)
     assert m.lens.tolist() == [20 + 3 * N] == [m.tokens] and m.frames == 4
+
+
+def test_robots_that_are_not_served_are_told(monkeypatch):
+    """served says of each robot whether the memory took what it was given of the last frame, in a replay too."""
+    m, K = memory(monkeypatch, 3, 3 * N, pages=10)
+    assert m.served.tolist() == [True] * 3
+    served = m.served
+    for counts, want in ((None, [True] * 3), (ints([0, 32, N]), [True, True, False]), (ints([0, 0, 0]), [True] * 3), (ints([N + 9, -1, 0]), [False, True, True]),
+                         (ints([0, 0, 1]), [True] * 3)):
+        before = m.lens.tolist()
+        m.replay(lambda: m.begin_frame(count=counts))
+        assert m.served is served
+        assert served.tolist() == want, counts
+        for b in range(3):
+            took = m.lens[b].item() - before[b]
+            assert took == (min(max(counts[b].item(), 0), N) if counts is not None else N) * want[b]
+        named(m)
+    m.forget()
+    assert served.tolist() == [True] * 3
+    plain, _ = memory(monkeypatch, 2, N)
+    plain.begin_frame(count=ints([3, 0]))
+    assert plain.served.tolist() == [True] * 2
+
+
+def test_a_robot_that_is_not_served_gets_no_actions(monkeypatch):
+    """Its features have seen nothing; the actions of all its candidates are zeros, those of the others what they were."""
+    from yanlongvla_b200 import policy
+    m, K = memory(monkeypatch, 3, N, pages=9)
+    m.served.copy_(torch.tensor([True, False, True]))
+    actions = torch.arange(1.0, 3 * 2 * 4 * 5 + 1).view(6, 4, 5)
+    p = policy.GrootStylePolicy.__new__(policy.GrootStylePolicy)
+    torch.nn.Module.__init__(p)
+    p.c = policy.PolicyConfig()
+    monkeypatch.setattr(policy.GrootStylePolicy, 'embed', lambda *a: torch.zeros(3, 1))
+    monkeypatch.setattr(policy.GrootStylePolicy, 'backbone', lambda *a: torch.zeros(3, 1))
+    monkeypatch.setattr(policy.GrootStylePolicy, 'action_head', lambda *a: actions)
+    noise = torch.zeros(6, 4, 5)
+    for memory_, want in ((None, actions), (m, actions * torch.tensor([1, 1, 0, 0, 1, 1.0])[:, None, None])):
+        assert torch.equal(p(None, None, None, noise, memory=memory_), want)
+    actions[2] = float('nan')                                                  # whatever the head made of it
+    assert not p(None, None, None, noise, memory=m)[2:4].any()

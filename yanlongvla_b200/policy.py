@@ -419,9 +419,14 @@ class GrootStylePolicy(torch.nn.Module):
 
     def forward(self, images, lang_ids, state, noise, memory=None, lang_lens=None):
         """lang_lens (B,) int32: language tokens of each observation, the rest of lang_ids is padding; noise may hold several
-        candidates of each observation (see action_head)."""
+        candidates of each observation (see action_head). A robot whose memory had no pages for the frame (memory.served) has seen
+        nothing: its actions are zeros."""
         lens = None if lang_lens is None else lang_lens + self.c.cameras * self.c.image_tokens
-        return self.action_head(self.backbone(self.embed(images, lang_ids), memory, lens), state, noise, lens)
+        actions = self.action_head(self.backbone(self.embed(images, lang_ids), memory, lens), state, noise, lens)
+        if memory is None or memory.pages is None:
+            return actions
+        served = memory.served.repeat_interleave(actions.shape[0] // memory.robots, output_size=actions.shape[0])
+        return torch.where(served[:, None, None], actions, 0)
 
 
 # ---------------------------------------------------------------------------------------------------- weights

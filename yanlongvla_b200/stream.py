@@ -36,6 +36,7 @@ class StreamMemory:
         else:
             self.table = self.pages.table(robots, blocks)
         self.count = None                                                        # tokens of the current frame, where not all of it
+        self.served = torch.ones(robots, dtype=torch.bool, device=device)        # which robots the pool had pages for in the current frame
         # a quarter of the frequencies for time, the rest split between rows and columns
         time = D // 8
         row = (D // 2 - time + 1) // 2
@@ -89,7 +90,8 @@ class StreamMemory:
         """Make room for the next frame: its tokens follow those remembered. On the device but for the check of the capacity.
         frame: the (B, T, ...) tensor that the layers will get; one of another batch or length is refused before anything moves.
         count (robots,) int32: each robot's tokens of the frame (0 .. its length), the rest is padding (None: all). A robot that the
-        pool of pages does not serve remembers nothing of the frame (device_error reports flag 2)."""
+        pool of pages does not serve remembers nothing of the frame, and its tokens attend to nothing (served (robots,) bool says which
+        robots were served, device_error reports flag 2)."""
         n = self.pos.shape[2]
         if frame is not None and tuple(frame.shape[:2]) != (self.robots, n):
             raise K.TcqError(f'StreamMemory: a frame of {self.robots} robots with {n} tokens each expected, got {tuple(frame.shape[:2])}')
@@ -103,6 +105,7 @@ class StreamMemory:
         if self.pages is not None:
             want = torch.full_like(self.lens, n) if count is None else self.count
             self.count, copies = K.kv8_reserve(self.pages, self.table, self.lens, want)
+            torch.eq(self.count, want, out=self.served)
             K.kv8_copy(self.caches, copies)
         self.lens += n if self.count is None else self.count
 
@@ -175,6 +178,7 @@ class StreamMemory:
             K.kv8_free(self.pages, self.table, self.lens, torch.zeros_like(self.lens))
         self.lens.zero_()
         self.start.zero_()
+        self.served.fill_(True)
         self.pos[0].fill_(-1)
 
     @property
