@@ -178,7 +178,29 @@ def test_a_robot_that_is_not_served_gets_no_actions(monkeypatch):
     monkeypatch.setattr(policy.GrootStylePolicy, 'backbone', lambda *a: torch.zeros(3, 1))
     monkeypatch.setattr(policy.GrootStylePolicy, 'action_head', lambda *a: actions)
     noise = torch.zeros(6, 4, 5)
+    state = torch.zeros(3, 64)
     for memory_, want in ((None, actions), (m, actions * torch.tensor([1, 1, 0, 0, 1, 1.0])[:, None, None])):
-        assert torch.equal(p(None, None, None, noise, memory=memory_), want)
+        assert torch.equal(p(None, None, state, noise, memory=memory_), want)
     actions[2] = float('nan')                                                  # whatever the head made of it
-    assert not p(None, None, None, noise, memory=m)[2:4].any()
+    assert not p(None, None, state, noise, memory=m)[2:4].any()
+
+
+def test_inputs_that_do_not_fit_leave_the_memory(monkeypatch):
+    """Noise or states of another batch are refused before the memory has moved."""
+    from yanlongvla_b200 import policy
+    m, K = memory(monkeypatch, 2, N, pages=9)
+    p = policy.GrootStylePolicy.__new__(policy.GrootStylePolicy)
+    torch.nn.Module.__init__(p)
+    p.c = policy.PolicyConfig()
+    monkeypatch.setattr(policy.GrootStylePolicy, 'embed', lambda *a: torch.zeros(2, N, 8))
+    monkeypatch.setattr(policy.GrootStylePolicy, 'backbone', lambda self, prefix, memory, lens: memory.begin_frame(prefix))
+    monkeypatch.setattr(policy.GrootStylePolicy, 'action_head', lambda self, feats, state, noise, lens: noise)
+    state = torch.zeros(2, 64)
+    for noise in (torch.zeros(3, 4, 5), torch.zeros(1, 4, 5), torch.zeros(0, 4, 5)):
+        with pytest.raises(ValueError, match='noise'):
+            p(None, None, state, noise, memory=m)
+    with pytest.raises(ValueError, match='state'):
+        p(None, None, state[:1], torch.zeros(4, 4, 5), memory=m)
+    assert m.frames == m.tokens == 0 and not m.lens.any()
+    p(None, None, state, torch.zeros(4, 4, 5), memory=m)
+    assert m.frames == 1

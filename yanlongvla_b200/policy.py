@@ -392,13 +392,19 @@ class GrootStylePolicy(torch.nn.Module):
         emb = torch.cat((ang.sin(), ang.cos()))[None, None, :].expand(B, 1, 256).to(torch.bfloat16)
         return self.time2(F.silu(self.time1(emb)))
 
+    @staticmethod
+    def _batches(observations, state, noise):
+        if state.shape[0] != observations:
+            raise ValueError(f'{state.shape[0]} state batches for {observations} observations')
+        if noise.shape[0] < 1 or noise.shape[0] % observations:
+            raise ValueError(f'{noise.shape[0]} noise batches for {observations} observations')
+
     def action_head(self, feats, state, noise, lens=None):
         """feats (B, T, 2048), state (B, 64), noise (B * S, chunk, action_dim) -> actions (B * S, chunk, action_dim): S candidate chunks
         for each observation, b * S .. b * S + S - 1 from the features of observation b, whose keys and values are formed and
         read once for all of them. lens (B,) int32: features that are there (None: all T)."""
         c = self.c
-        if noise.shape[0] % feats.shape[0]:
-            raise ValueError(f'action_head: {noise.shape[0]} noise batches for {feats.shape[0]} observations')
+        self._batches(feats.shape[0], state, noise)
         kvs = [blk.kv(feats) if blk.cross else None for blk in self.dit]
         st = self.state_enc2(F.silu(self.state_enc1(state.to(torch.bfloat16))))[:, None, :]
         B, candidates = noise.shape[0], noise.shape[0] // feats.shape[0]
@@ -422,7 +428,9 @@ class GrootStylePolicy(torch.nn.Module):
         candidates of each observation (see action_head). A robot whose memory had no pages for the frame (memory.served) has seen
         nothing: its actions are zeros."""
         lens = None if lang_lens is None else lang_lens + self.c.cameras * self.c.image_tokens
-        actions = self.action_head(self.backbone(self.embed(images, lang_ids), memory, lens), state, noise, lens)
+        prefix = self.embed(images, lang_ids)
+        self._batches(prefix.shape[0], state, noise)                             # before the memory moves
+        actions = self.action_head(self.backbone(prefix, memory, lens), state, noise, lens)
         if memory is None or memory.pages is None:
             return actions
         served = memory.served.repeat_interleave(actions.shape[0] // memory.robots, output_size=actions.shape[0])
