@@ -204,3 +204,33 @@ def test_inputs_that_do_not_fit_leave_the_memory(monkeypatch):
     assert m.frames == m.tokens == 0 and not m.lens.any()
     p(None, None, state, torch.zeros(4, 4, 5), memory=m)
     assert m.frames == 1
+
+
+def test_robots_within_the_window_stay_where_they_are(monkeypatch):
+    """keep_recent packs what is longer than the window: the others' tokens keep their pages, need no second ones and refuse no one."""
+    m, K = memory(monkeypatch, 4, 400, pages=3 + 3 + 5 + 2 + 4)                 # room next to the old ones for the long robot's tokens alone
+    m.begin_frame(count=ints([N, 130, N, 100]))
+    m.begin_frame(count=ints([0, 0, N, 0]))
+    before = m.table.clone()
+    m.keep_recent(200)
+    assert K.flag == 0 and m.lens.tolist() == [N, 130, 200, 100] and m.tokens == 200
+    for b in (0, 1, 3):
+        assert torch.equal(m.table[b], before[b])
+    named(m)
+    m.fork(ints([0, 1, 2, 2]))
+    refs = m.pages.refs.clone()
+    m.keep_recent(200)                                                         # nothing to forget: nothing moves
+    assert torch.equal(m.pages.refs, refs) and m.lens.tolist() == [N, 130, 200, 200]
+    m.keep_recent(130)                                                         # three pages each for three robots, seven free
+    assert K.flag == 2 and m.lens.tolist() == [130, 130, 130, 200]
+    named(m)
+
+
+def test_a_window_longer_than_the_memory(monkeypatch):
+    m, K = memory(monkeypatch, 2, 2 * N, pages=10)
+    m.begin_frame()
+    before = m.table.clone()
+    for tokens in (N, 2 * N, 10 ** 6, 1 << 40):
+        m.keep_recent(tokens)
+        assert m.lens.tolist() == [N, N] and m.tokens == N and torch.equal(m.table, before)
+    assert K.flag == 0

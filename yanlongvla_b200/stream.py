@@ -146,9 +146,13 @@ class StreamMemory:
             raise K.TcqError(f'StreamMemory: {n} tokens do not fit {self.max_tokens}')
         most = self.lens.clamp(max=n)
         kept = most if kept is None else kept.clamp(min=0).minimum(most)
-        index = index.contiguous()
+        self._pack(index.contiguous(), kept, kept)
+
+    def _pack(self, index, kept, move):
+        """move (robots,): kept, or 0 for robots whose memory may stay as it is."""
+        n = index.shape[1]
         table = self.pages.table(*self.table.shape)
-        granted, _ = K.kv8_reserve(self.pages, table, torch.zeros_like(self.lens), kept)
+        granted, _ = K.kv8_reserve(self.pages, table, torch.zeros_like(self.lens), move)
         K.kv8_compact(self.caches, self.table, self.lens, index, table, kept=granted)
         stays = granted < kept
         K.kv8_free(self.pages, self.table, self.lens, torch.where(stays, self.lens, 0))
@@ -158,16 +162,19 @@ class StreamMemory:
             self.tokens = min(self.tokens, n) if self._holds(n) else self._longest()
 
     def keep_recent(self, tokens):
-        """Remember only the newest `tokens` tokens of each robot (0: none). Positions go on as if the others were still there."""
+        """Remember only the newest `tokens` tokens of each robot (0: none). Positions go on as if the others were still there. Robots that
+        remember no more stay as they are; of the others' pages holds what keep says."""
         self._pooled('keep_recent')
         if tokens < 1:
             K.kv8_free(self.pages, self.table, self.lens, torch.zeros_like(self.lens))
             if not torch.cuda.is_current_stream_capturing():
                 self.tokens = 0
             return
+        tokens = min(tokens, self.table.shape[1] * K.KV8_BLOCK)
         kept = self.lens.clamp(max=tokens)
         at = torch.arange(tokens, dtype=torch.int32, device=self.lens.device)
-        self.keep((self.lens - kept)[:, None] + at.minimum((kept - 1).clamp(min=0)[:, None]), kept)
+        index = (self.lens - kept)[:, None] + at.minimum((kept - 1).clamp(min=0)[:, None])
+        self._pack(index, kept, torch.where(self.lens > tokens, kept, 0))
 
     def forget(self):
         """Remember nothing, time starts anew. (In a capture the host's counts stay: reserve(kept=0) before a replay, and max_frames counts
