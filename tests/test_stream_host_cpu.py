@@ -234,3 +234,19 @@ def test_a_window_longer_than_the_memory(monkeypatch):
         m.keep_recent(tokens)
         assert m.lens.tolist() == [N, N] and m.tokens == N and torch.equal(m.table, before)
     assert K.flag == 0
+
+
+@pytest.mark.parametrize('window', ['0', '3'])
+def test_the_command_has_positions_for_all_its_frames(monkeypatch, window):
+    from yanlongvla_b200 import policy, stream
+    made = []
+
+    def memory(c, robots, max_tokens, max_frames=4096, pages=None):
+        made.append(max_frames)
+        raise KeyboardInterrupt
+    monkeypatch.setattr(policy, 'build_policy', lambda runtime, c: (None, None, None))
+    monkeypatch.setattr(stream, 'StreamMemory', memory)
+    for frames in ('5000', '8'):
+        with pytest.raises(KeyboardInterrupt):
+            stream.main(['--frames', frames, '--window', window])
+    assert made == [5000, 4096]

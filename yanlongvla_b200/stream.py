@@ -207,12 +207,13 @@ def main(argv=None):
     c = P.PolicyConfig(vit_layers=a.vit_layers, llm_layers=a.llm_layers, dit_layers=a.dit_layers)
     model, _, _ = P.build_policy(runtime='resident', c=c)
     n, window = c.prefix_tokens, a.window if 0 < a.window < a.frames else 0
+    most = max(a.frames, 4096)                                                   # frames that positions are there for
     if window:
         # full and next to it what is kept of it
         blocks = -(-window * n // K.KV8_BLOCK) + -(-(window - 1) * n // K.KV8_BLOCK)
-        memory = StreamMemory(c, a.robots, window * n, pages=a.robots * blocks)
+        memory = StreamMemory(c, a.robots, window * n, max_frames=most, pages=a.robots * blocks)
     else:
-        memory = StreamMemory(c, a.robots, a.frames * n)
+        memory = StreamMemory(c, a.robots, a.frames * n, max_frames=most)
     ev = [torch.cuda.Event(enable_timing=True) for _ in range(2)]
     with torch.no_grad():
         for f in range(a.frames):
