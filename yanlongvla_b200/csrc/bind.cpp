@@ -436,6 +436,15 @@ PyObject* cross_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return guarded(n, 9, [&]() -> PyObject* {
         const char* me = "cross_attention";
         const at::Tensor &q = tensor(me, a[0], "q"), &k = tensor(me, a[1], "k"), &v = tensor(me, a[2], "v");
+        at::Tensor made;
+        const at::Tensor& given = a[8] == Py_None ? made : tensor(me, a[8], "out");
+        for (const at::Tensor* t : {&q, &k, &v, &given}) {
+            if (!t->defined()) continue;
+            if (at::GradMode::is_enabled() && t->requires_grad())
+                refuse(me, "it forms no gradient: call it under torch.no_grad(), or on detached tensors");
+            if (t->_fw_grad(0).defined())       // torch.no_grad() leaves forward mode on; there is one level
+                refuse(me, "it forms no tangent: call it on the primal tensors (torch.autograd.forward_ad.unpack_dual)");
+        }
         const int64_t heads = PyLong_AsLongLong(a[3]);
         if (heads == -1 && PyErr_Occurred()) return nullptr;
         const int64_t kv_heads = a[4] == Py_None ? heads : PyLong_AsLongLong(a[4]);
@@ -451,8 +460,6 @@ PyObject* cross_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
         if (v.sizes() != k.sizes()) refuse(me, "k and v must have the same shape");
         if (k.scalar_type() != q.scalar_type() || v.scalar_type() != q.scalar_type()) refuse(me, "q, k and v must have one type");
         if (B < 1 || q.size(0) < 1 || q.size(0) % B) refuse(me, "q must have a multiple of the batches of k and v");
-        if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad()))
-            refuse(me, "it forms no gradient: call it under torch.no_grad(), or on detached tensors");
         const int dt = dtype_code(me, q, false);
         const int32_t* lp = a[5] == Py_None ? nullptr : ints(me, "lens", tensor(me, a[5], "lens"), {B}, dev);
         const uint8_t* mp = nullptr;
@@ -468,9 +475,8 @@ PyObject* cross_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
         }
         const double scale = a[7] == Py_None ? 1.0 / std::sqrt((double)D) : PyFloat_AsDouble(a[7]);
         if (scale == -1.0 && PyErr_Occurred()) return nullptr;
-        at::Tensor made;
         if (a[8] == Py_None) made = at::empty(q.sizes(), q.options());
-        const at::Tensor& out = a[8] == Py_None ? made : tensor(me, a[8], "out");
+        const at::Tensor& out = given;
         if (out.sizes() != q.sizes() || out.scalar_type() != q.scalar_type() || !out.is_contiguous() || !out.is_cuda() || out.get_device() != dev)
             refuse(me, "out must be contiguous and have the shape, type and device of q");
         done(f_cross(q.const_data_ptr(), step(q, 0), step(q, 1), k.const_data_ptr(), step(k, 0), step(k, 1), v.const_data_ptr(), step(v, 0),
