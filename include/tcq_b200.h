@@ -43,7 +43,8 @@ enum tcq_status {
     TCQ_ERR_ARG = 4,       /* a required pointer is NULL, or an argument is out of range                        */
     TCQ_ERR_LAUNCH = 5,    /* the CUDA launch failed (cudaGetLastError after the launch)                        */
     TCQ_ERR_DEVICE = 6,    /* no usable device, or not an sm_100 device                                         */
-    TCQ_ERR_WORKSPACE = 7  /* the workspace is missing or smaller than the *_workspace() query returned           */
+    TCQ_ERR_WORKSPACE = 7, /* the workspace is missing or smaller than the *_workspace() query returned           */
+    TCQ_ERR_BUILD = 8      /* the kernel was compiled with other registers than its warps divide (the build warned) */
 };
 
 enum tcq_dtype { TCQ_DT_BF16 = 0, TCQ_DT_F32 = 1, TCQ_DT_F16 = 2, TCQ_DT_I32 = 3 };

@@ -10,6 +10,7 @@ compiled by g++ against the installed PyTorch's headers.
 """
 import argparse
 import os
+import re
 import subprocess
 import sys
 from concurrent.futures import ThreadPoolExecutor
@@ -24,17 +25,31 @@ BIND = PKG / '_bind.so'
 NVCC = os.environ.get('NVCC', 'nvcc')
 ARCH = ['-gencode', 'arch=compute_100a,code=sm_100a']
 FLAGS = ['-lineinfo', '-O3', '-std=c++17', '-fmad=false', '-Xcompiler', '-fPIC', '--expt-relaxed-constexpr',
-         f'-I{ROOT / "include"}', f'-I{CSRC}']
+         f'-I{ROOT / "include"}', f'-I{CSRC}', '-Xptxas', '-v']
+# Kernels whose warps divide the launch's registers among themselves (setmaxnreg), and the registers a thread that their shares are written
+# down for (LAUNCH_REGS in the source). The library does not launch one that was compiled with another number.
+LAUNCH_REGS = {r'k_cross_tiles': 168, r'k_attention_many\w*Li2EE': 80}
 
 
 def _headers():
     return list(CSRC.glob('*.cuh')) + list((ROOT / 'include').glob('*.h'))
 
 
+def registers(log):
+    """(kernel, registers a thread, what its shares are written down for) of the kernels of LAUNCH_REGS in what `ptxas -v` has printed."""
+    found = re.findall(r"Compiling entry function '(\w+)'.*?Used (\d+) registers", log, re.S)
+    return [(name, int(n), want) for name, n in found for pattern, want in LAUNCH_REGS.items() if re.search(pattern, name)]
+
+
+def wrong_registers(log):
+    return [x for x in registers(log) if x[1] != x[2]]
+
+
 def _compile(src, verbose=False, extra=()):
     obj = OBJ / (src.stem + '.o')
     newest = max(p.stat().st_mtime for p in [src] + _headers())
-    if obj.exists() and obj.stat().st_mtime >= newest:
+    log = OBJ / (src.stem + '.ptxas')
+    if obj.exists() and log.exists() and obj.stat().st_mtime >= newest:
         return obj, None
     cmd = [NVCC, *ARCH, *FLAGS, *extra, '-c', str(src), '-o', str(obj)]
     r = subprocess.run(cmd, capture_output=True, text=True)
@@ -42,6 +57,9 @@ def _compile(src, verbose=False, extra=()):
         sys.stderr.write(' '.join(cmd) + '\n' + r.stdout + r.stderr)
     if r.returncode:
         raise RuntimeError(f'nvcc failed on {src.name}')
+    log.write_text(r.stdout + r.stderr)
+    for name, n, want in wrong_registers(r.stdout + r.stderr):
+        sys.stderr.write(f'warning: {src.name}: {name} has {n} registers a thread, its warps divide {want}: it will not be launched\n')
     return obj, r.stderr
 
 
@@ -96,4 +114,4 @@ if __name__ == '__main__':
     ap.add_argument('--verbose', action='store_true')
     ap.add_argument('--ptxas', action='store_true', help='print register / shared-memory use (-Xptxas -v)')
     a = ap.parse_args()
-    print(build(force=a.force or a.ptxas, verbose=a.verbose or a.ptxas, extra=('-Xptxas', '-v') if a.ptxas else ()))
+    print(build(force=a.force or a.ptxas, verbose=a.verbose or a.ptxas))

@@ -1092,7 +1092,8 @@ int launch_tiles(const CrossArgs& A, const TileMaps& maps, void* stream) {
         if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, P::BYTES) != cudaSuccess) return TCQ_ERR_LAUNCH;
         // the register shares of the roles are taken from what the launch gives the CTA: less would leave them waiting
         cudaFuncAttributes fa;
-        if (cudaFuncGetAttributes(&fa, kern) != cudaSuccess || fa.numRegs != P::LAUNCH_REGS) return TCQ_ERR_LAUNCH;
+        if (cudaFuncGetAttributes(&fa, kern) != cudaSuccess) return TCQ_ERR_LAUNCH;
+        if (fa.numRegs != P::LAUNCH_REGS) return TCQ_ERR_BUILD;
         for (int s = 8; s >= 1; --s) {
             int n = 0;
             cfg.gridDim = dim3(s);

@@ -1208,7 +1208,8 @@ int launch_many(const AttnArgs& A, void* stream) {
         if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, P::BYTES) != cudaSuccess) return TCQ_ERR_LAUNCH;
         // the register shares of the roles are taken from what the launch gives the CTA: less would leave them waiting
         cudaFuncAttributes fa;
-        if (cudaFuncGetAttributes(&fa, kern) != cudaSuccess || (NG == 2 && fa.numRegs != P::LAUNCH_REGS)) return TCQ_ERR_LAUNCH;
+        if (cudaFuncGetAttributes(&fa, kern) != cudaSuccess) return TCQ_ERR_LAUNCH;
+        if (NG == 2 && fa.numRegs != P::LAUNCH_REGS) return TCQ_ERR_BUILD;
         for (int s = 8; s >= 1; --s) {
             int n = 0;
             cfg.gridDim = dim3(s);

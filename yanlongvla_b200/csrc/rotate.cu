@@ -930,6 +930,7 @@ const char* tcq_status_string(int status) {
         case TCQ_ERR_LAUNCH: return "CUDA launch failed";
         case TCQ_ERR_DEVICE: return "no usable sm_100 device";
         case TCQ_ERR_WORKSPACE: return "workspace missing or too small";
+        case TCQ_ERR_BUILD: return "the kernel was compiled with another number of registers than its warps divide (see the build's warnings)";
         default: return "unknown status";
     }
 }
