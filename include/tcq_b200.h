@@ -348,7 +348,8 @@ int tcq_kv8_compact(const tcq_kv8_cache* caches, int layers, const int32_t* tabl
  * 16-byte aligned; a k_sb or v_sb of 0 shares one batch of states), out contiguous: q itself, or memory apart from q, k and v. Query head h reads key head h / (heads /
  * kv_heads); head_dim is a multiple of 8, at most 128. State j of sequence b is there if j < lens[b] (lens NULL: N) and
  * mask[b * mask_sb + j] != 0 (mask NULL: yes); what lies in k and v where none is has no effect, NaN neither. Rows that see no
- * state are zero. Scores, sums and maxima are FP32; weights are rounded to the type once. No workspace; the same call gives the same bits. */
+ * state are zero. Scores, sums and maxima are FP32; weights are rounded to the type once. Scores scale * q k may be up to 2^23 in size; a row
+ * whose largest is further out is undefined (flag 2). No workspace; the same call gives the same bits. */
 int tcq_cross_attention(const void* q, int64_t q_sb, int64_t q_st, const void* k, int64_t k_sb, int64_t k_st, const void* v, int64_t v_sb,
                         int64_t v_st, int dtype, void* out, const int32_t* lens, const uint8_t* mask, int64_t mask_sb, float scale, int B,
                         int S, int T, int N, int heads, int kv_heads, int head_dim, void* stream);
@@ -362,7 +363,7 @@ int tcq_selftest_wait_expiry(unsigned limit_us, void* stream);
 int tcq_capture_id(void* stream, unsigned long long* id);
 
 /* Device error flags: 1 = a bounded pipeline wait expired and the kernel stopped early, 2 = a position, page number or
- * length given to a streaming-memory operator or to the cross attention was out of range (see there). Synchronizes the current device. reset != 0 clears the flags. Returns -1 if the flags cannot be read. */
+ * length given to a streaming-memory operator or to the cross attention, or a score there, was out of range (see there). Synchronizes the current device. reset != 0 clears the flags. Returns -1 if the flags cannot be read. */
 int tcq_device_error(int reset);
 
 #ifdef __cplusplus

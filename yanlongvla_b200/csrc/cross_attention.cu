@@ -80,7 +80,13 @@ TCQ_HD float part_factor(float2 ml, float top) { return top == -INFINITY ? (ml.y
 
 // Weights are 2^(x - m + kRef), m the row's reference, moved only when a score passes it by more than kSlack: below 2^13, so
 // that FP16 holds them with 11 bits from there down to 2^-14.
-constexpr float kRef = 5.f, kSlack = 8.f;
+// The weights come of one fused step, s c + (kRef - m): m, and the difference, are off by half a step of FP32 at |m| each, one in the
+// exponent together at 2^24. Past that the weights would leave the type's range, either way: a row whose reference ends there is
+// reported. (Scores less their reference before the scaling are right at any size, but cost 4 to 13 %: 17 queries
+// over 160 states 4.45 -> 4.83 us, 8 x 16 candidates
+// 14.7 -> 16.7, 2 x 4096 x 4096 with heads of 128 514 -> 533.)
+constexpr float kRef = 5.f, kSlack = 8.f, kMost = 16777216.f;
+TCQ_HD bool past_range(float m) { return fabsf(m) > kMost && fabsf(m) != INFINITY; }
 
 // ------------------------------------------------------------------------------------------------ products of 16 rows
 // Warps of 16 query rows on m16n8k16 products, for few rows or few states: bound by HBM where the states are many, by latency where
@@ -446,6 +452,10 @@ k_cross_rows(const CrossArgs A, const __grid_constant__ CUtensorMap kmap, const 
                     for (int i = 0; i < NT; ++i)
                         if (8 * i < A.D) dst[4 * i + t] = weights2<DT>(o[j][i][2 * e] * f, o[j][i][2 * e + 1] * f);
             }
+        bool past = false;                                         // behind the stores, which do not wait for it
+#pragma unroll
+        for (int j = 0; j < MT; ++j) past = past || past_range(m[j][0]) || past_range(m[j][1]);
+        if (past) atomicOr(&g_tcq_cross_error, 2);
         return;
     }
     // ---- parts to shared memory (every chunk has arrived), then added: four elements of a row a thread
@@ -464,10 +474,12 @@ k_cross_rows(const CrossArgs A, const __grid_constant__ CUtensorMap kmap, const 
             }
     }
     const int rows = r1 - r0;
-    auto store = [&](int row, int d, const float4& y, float sum) {
+    bool past = false;
+    auto store = [&](int row, int d, const float4& y, float top, float sum) {
         const float f = sum != 0.f ? 1.f / sum : 0.f;
         if (d < A.D)
             *reinterpret_cast<uint2*>(A.out + row_at(A, b, h, r0 + row, out_sb, out_st) + d) = make_uint2(weights2<DT>(y.x * f, y.y * f), weights2<DT>(y.z * f, y.w * f));
+        past = past || past_range(top);
     };
     asm volatile("barrier.cta.sync 1, %0;" ::"n"(32 * kRowWarps) : "memory");
     for (int i = tid; i < rows * (DP / 4); i += 32 * kRowWarps) {
@@ -492,13 +504,16 @@ k_cross_rows(const CrossArgs A, const __grid_constant__ CUtensorMap kmap, const 
             y.x = __fmaf_rn(v[k].x, f, y.x), y.y = __fmaf_rn(v[k].y, f, y.y), y.z = __fmaf_rn(v[k].z, f, y.z), y.w = __fmaf_rn(v[k].w, f, y.w);
         }
         if (R.splits == 1) {
-            store(row, d, y, sum);
+            store(row, d, y, top, sum);
         } else {
             *reinterpret_cast<float4*>(parts + row * P::PITCH + d) = y;             // read by no other thread before
             if (d == 0) *reinterpret_cast<float2*>(smem_rows + P::PARTS + 8 * row) = make_float2(top, sum);
         }
     }
-    if (R.splits == 1) return;
+    if (R.splits == 1) {
+        if (past) atomicOr(&g_tcq_cross_error, 2);
+        return;
+    }
     cluster_barrier();
     for (int i = rank * (32 * kRowWarps) + tid; i < rows * (DP / 4); i += R.splits * (32 * kRowWarps)) {
         const int row = i / (DP / 4), d = 4 * (i - row * (DP / 4));
@@ -526,8 +541,10 @@ k_cross_rows(const CrossArgs A, const __grid_constant__ CUtensorMap kmap, const 
                 y.z = __fmaf_rn(v[k].z, f, y.z * old), y.w = __fmaf_rn(v[k].w, f, y.w * old);
             }
         }
-        store(row, d, y, sum);
+        store(row, d, y, top, sum);
     }
+    if (past) atomicOr(&g_tcq_cross_error, 2);
+    __syncwarp();
     cluster_barrier();                                             // a part may be read until here
 }
 
@@ -842,6 +859,7 @@ k_cross_tiles(const CrossArgs A, const __grid_constant__ TileMaps maps, const Ti
                 }
             }
         }
+        if (past_range(m)) atomicOr(&g_tcq_cross_error, 2);
     } else if (k1 > k0 && warp == W_LOAD) {
         // ------------------------------------------------------------------------------------------------ load
         // A tile is made of the next two blocks of 64 states that hold one, so that what a mask leaves out in such blocks (an image) costs
