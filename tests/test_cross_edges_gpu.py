@@ -72,3 +72,17 @@ def test_large_scores_and_larger_ones(K, T, N, D, dtype):
     k.view(2, N, heads, D)[0, 0, 0] = math.inf                                 # infinite scores are what they are: NaN, and not reported
     K.cross_attention(q, k, v, heads)
     assert K.device_error() == 0
+
+
+@pytest.mark.parametrize('T,heads,kv_heads,N', [(1, 4, 4, 5000), (17, 4, 4, 160), (40, 4, 4, 200), (150, 2, 2, 300), (300, 4, 2, 900), (130, 2, 2, 3000)])
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float16])
+def test_random_masks(K, T, heads, kv_heads, N, dtype):
+    """States left out one by one at random, from few to nearly all; the masks are made from a seed."""
+    D, shares = 64, (0.0, 0.01, 0.5, 0.9, 0.99, 0.999)
+    B = len(shares)
+    g = torch.Generator(device='cuda').manual_seed(T + N)
+    q, k, v = rand(B, T, heads * D, dtype=dtype), rand(B, N, kv_heads * D, dtype=dtype, seed=1), rand(B, N, kv_heads * D, dtype=dtype, seed=2)
+    mask = torch.rand(B, N, device='cuda', generator=g) >= torch.tensor(shares, device='cuda')[:, None]
+    k[~mask], v[~mask] = math.inf, math.nan
+    check(K, q, k, v, heads, kv_heads, mask=mask)
+    check(K, q, k, v, heads, kv_heads, mask=mask, lens=ints([N, N - 1, N // 2, N, N, N // 3]))

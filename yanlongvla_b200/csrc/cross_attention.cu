@@ -82,9 +82,8 @@ TCQ_HD float part_factor(float2 ml, float top) { return top == -INFINITY ? (ml.y
 // that FP16 holds them with 11 bits from there down to 2^-14.
 // The weights come of one fused step, s c + (kRef - m): m, and the difference, are off by half a step of FP32 at |m| each, one in the
 // exponent together at 2^24. Past that the weights would leave the type's range, either way: a row whose reference ends there is
-// reported. (Scores less their reference before the scaling are right at any size, but cost 4 to 13 %: 17 queries
-// over 160 states 4.45 -> 4.83 us, 8 x 16 candidates
-// 14.7 -> 16.7, 2 x 4096 x 4096 with heads of 128 514 -> 533.)
+// reported. (Scores less their reference before the scaling are right at any size, but cost 4 to 13 %: 17 queries over 160 states
+// 4.45 -> 4.83 us, 8 x 16 candidates 14.7 -> 16.7, 2 x 4096 x 4096 with heads of 128 514 -> 533.)
 constexpr float kRef = 5.f, kSlack = 8.f, kMost = 16777216.f;
 TCQ_HD bool past_range(float m) { return fabsf(m) > kMost && fabsf(m) != INFINITY; }
 
