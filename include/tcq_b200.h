@@ -345,7 +345,7 @@ int tcq_kv8_compact(const tcq_kv8_cache* caches, int layers, const int32_t* tabl
  * out (B S, T, heads * head_dim) = softmax(scale * q k^T) v over an encoder's states (the action head's attention to the backbone's
  * features, in the reference a library call of its model code). q (B S, T, heads * head_dim): the S batches b S .. b S + S - 1 read the states of
  * sequence b, S candidates that share them; k, v (B, N, kv_heads * head_dim); all BF16 or all F16, strides *_sb, *_st in elements (rows
- * 16-byte aligned; a k_sb or v_sb of 0 shares one batch of states), out contiguous: q itself, or memory apart from q, k and v. Query head h reads key head h / (heads /
+ * 16-byte aligned; a k_sb or v_sb of 0 shares one batch of states), out contiguous: q itself, or memory apart from the inputs. Query head h reads key head h / (heads /
  * kv_heads); head_dim is a multiple of 8, at most 128. State j of sequence b is there if j < lens[b] (lens NULL: N) and
  * mask[b * mask_sb + j] != 0 (mask NULL: yes); what lies in k and v where none is has no effect, NaN neither. Rows that see no
  * state are zero. Scores, sums and maxima are FP32; weights are rounded to the type once. Scores scale * q k may be up to 2^23 in size; a row

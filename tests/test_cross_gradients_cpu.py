@@ -24,3 +24,6 @@ def test_tangents_and_gradients_are_refused():
             K.cross_attention(*a[:3], 1, out=a[3] if len(a) > 3 else None)
     with torch.no_grad(), pytest.raises(K.TcqError, match='CUDA'):
         K.cross_attention(leaf, leaf, leaf, 1)
+    with torch.inference_mode(), pytest.raises(K.TcqError, match='CUDA'):
+        y = torch.zeros(2, 3, 64, dtype=torch.bfloat16)
+        K.cross_attention(y, x, leaf, 1, out=y)

@@ -38,3 +38,23 @@ def test_against_all_addresses():
         assert (status != 4) == apart, (B, S, T, N, W, row, q_sb, q_st, k_sb, k_st, v_sb, v_st, q, k, v, out)
         outcomes[apart] += 1
     assert min(outcomes.values()) > 300
+
+
+def test_lengths_and_masks():
+    """The output shares no byte with the lengths and the mask's rows either."""
+    if torch.cuda.is_available():
+        pytest.skip('made-up addresses')
+    from yanlongvla_b200 import _lib as L
+    B, T, N, W = 3, 2, 20, 16
+    out, far, size = 1 << 24, 1 << 28, 2 * B * T * W                           # bytes
+
+    def cross(lens=None, mask=None, mask_sb=0, states=N):
+        return L.lib.tcq_cross_attention(far, T * W, W, 2 * far, N * W, W, 3 * far, N * W, W, L.DT_BF16, out, lens, mask, mask_sb, 1.0, B, 1, T, states, 2, 2, 8, None)
+    for at, apart in ((out - 4 * B, True), (out - 4 * B + 4, False), (out, False), (out + size - 4, False), (out + size, True)):
+        assert (cross(lens=at) != 4) == apart
+        assert (cross(lens=at, states=0) != 4)                                 # without states nothing is read
+    for sb in (N, N + 1, 0, size + N):
+        span = (B - 1) * sb + N
+        for at in range(out - span - 2, out + size + 3):
+            apart = not any(at + i * sb < out + size and at + i * sb + N > out for i in range(B))
+            assert (cross(mask=at, mask_sb=sb) != 4) == apart, (sb, at - out)

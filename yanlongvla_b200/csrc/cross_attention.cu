@@ -1243,8 +1243,8 @@ int by_width(int d, F f) {
     return f(std::integral_constant<int, 128>());
 }
 
-// Whether one of `batches` x n rows of w elements, the first at `from`, sb from batch to batch and st from row to row (none negative), has
-// an element in [0, all). The batches are looked at one by one only where the rows' whole extent reaches into it.
+// Whether one of `batches` x n rows of w bytes, the first at `from`, sb from batch to batch and st from row to row (none negative), has
+// a byte in [0, all). The batches are looked at one by one only where the rows' whole extent reaches into it.
 bool rows_meet(i64 from, i64 all, i64 batches, i64 sb, int n, i64 st, i64 w) {
     const auto extent_meets = [&](i64 a, i64 length) { return a < all && a + length > 0; };
     if (!extent_meets(from, (batches - 1) * sb + (n - 1) * st + w)) return false;
@@ -1291,14 +1291,15 @@ int tcq_cross_attention(const void* q, int64_t q_sb, int64_t q_st, const void* k
     if (!tcq_aligned(q, 16) || !tcq_aligned(k, 16) || !tcq_aligned(v, 16) || !tcq_aligned(out, 16)) return TCQ_ERR_ALIGN;
     if ((q_sb | q_st | k_sb | k_st | v_sb | v_st) & 7) return TCQ_ERR_ALIGN;
     if (k_sb < 0 || k_st < 0 || v_sb < 0 || v_st < 0 || (N > 1 && (k_st < 8 || v_st < 8))) return TCQ_ERR_ARG;
-    // out may be q itself (a row's queries are read before it is written); beyond that it shares no byte with the rows that are read
+    // out may be q itself (a row's queries are read before it is written); beyond that it shares no byte with what is read
     const i64 width = (i64)heads * head_dim, all = (i64)B * S * T * width, row = (i64)kv_heads * head_dim;
-    const auto meets = [&](const void* p, i64 batches, i64 sb, int n, i64 st, i64 w) {
-        return rows_meet(((intptr_t)p - (intptr_t)out) / 2, all, batches, sb, n, st, w);
+    const auto meets = [&](const void* p, i64 batches, i64 sb, int n, i64 st, i64 w, int size = 2) {
+        return rows_meet((intptr_t)p - (intptr_t)out, 2 * all, batches, sb * size, n, st * size, w * size);
     };
     const bool same = q == out && (T == 1 || q_st == width) && ((i64)B * S == 1 || q_sb == T * width);
     if (!same && q_sb >= 0 && q_st >= 0 && meets(q, (i64)B * S, q_sb, T, q_st, width)) return TCQ_ERR_ARG;
     if (N > 0 && (meets(k, B, k_sb, N, k_st, row) || meets(v, B, v_sb, N, v_st, row))) return TCQ_ERR_ARG;
+    if (N > 0 && ((lens && meets(lens, 1, 0, 1, 0, B, 4)) || (mask && mask_sb >= 0 && meets(mask, B, mask_sb, 1, 0, N, 1)))) return TCQ_ERR_ARG;
     if (N == 0) {
         const i64 n = (i64)B * S * T * heads * head_dim / 8;
         const i64 blocks = (n + 255) / 256, most = (i64)tcq_sm_count() * 8;

@@ -532,7 +532,7 @@ def cross_attention(q, k, v, heads, kv_heads=None, lens=None, mask=None, scale=N
     of q read the states of sequence b (S candidates that share them); query head h reads key head h // (heads / kv_heads). A
     state j is there if j < lens[b] ((B,) int32; None: all N) and mask[b, j] ((B, N) bool; None: yes); what lies elsewhere in k
     and v has no effect. scale None: D^-0.5. Scores scale q k
-    may be up to 2^23 in size; a row whose largest is further out is undefined (device_error reports flag 2). Returns out (B * S, T, heads * D) of q's type (q itself, or memory apart from q, k and v); rows that see no state are zero. It
+    may be up to 2^23 in size; a row whose largest is further out is undefined (device_error reports flag 2). Returns out (B * S, T, heads * D) of q's type (q itself, or memory apart from the inputs); rows that see no state are zero. It
     forms no gradient and refuses tensors that ask for one or carry a tangent; the same call gives the same bits every time."""
     return _bind.cross_attention(q, k, v, heads, kv_heads, lens, mask, scale, out)
 
