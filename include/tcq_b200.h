@@ -336,7 +336,7 @@ int tcq_kv8_copy(const tcq_kv8_cache* caches, int layers, const int32_t* copies,
 
 /* Pack tokens into other pages, in each of `layers` caches: token j < kept[b] (NULL: tokens) of a new sequence is token
  * index[b * tokens + j] of sequence b, in any order. table (B, blocks) and lens name the old tokens, new_table (B, new_blocks) the
- * pages that are written, none of which may be among those read. A new block's scale is the largest of the scales its tokens
+ * pages that are written, each of them once and none of those read. A new block's scale is the largest of the scales its tokens
  * come with, q' = rint(q * (s_old / s)); its unused slots are zero. A number past the sequence gives a token of zeros (flag 2). */
 int tcq_kv8_compact(const tcq_kv8_cache* caches, int layers, const int32_t* table, int blocks, const int32_t* lens, const int32_t* index,
                     int tokens, const int32_t* kept, const int32_t* new_table, int new_blocks, int B, void* stream);
@@ -348,8 +348,8 @@ int tcq_kv8_compact(const tcq_kv8_cache* caches, int layers, const int32_t* tabl
  * 16-byte aligned; a k_sb or v_sb of 0 shares one batch of states), out contiguous: q itself, or memory apart from the inputs. Query head h reads key head h / (heads /
  * kv_heads); head_dim is a multiple of 8, at most 128. State j of sequence b is there if j < lens[b] (lens NULL: N) and
  * mask[b * mask_sb + j] != 0 (mask NULL: yes); what lies in k and v where none is has no effect, NaN neither. Rows that see no
- * state are zero. Scores, sums and maxima are FP32; weights are rounded to the type once. Scores scale * q k may be up to 2^23 in size; a row
- * whose largest is further out is undefined (flag 2). No workspace; the same call gives the same bits. */
+ * state are zero. Scores, sums and maxima are FP32; weights are rounded to the type once. Scores scale * q k of states that are there
+ * may be up to 2^23 in size; rows with others are undefined (flag 2 where the largest is one). No workspace; the same call gives the same bits. */
 int tcq_cross_attention(const void* q, int64_t q_sb, int64_t q_st, const void* k, int64_t k_sb, int64_t k_st, const void* v, int64_t v_sb,
                         int64_t v_st, int dtype, void* out, const int32_t* lens, const uint8_t* mask, int64_t mask_sb, float scale, int B,
                         int S, int T, int N, int heads, int kv_heads, int head_dim, void* stream);

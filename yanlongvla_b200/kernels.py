@@ -519,8 +519,8 @@ def kv8_copy(caches, copies):
 
 def kv8_compact(caches, table, lens, index, new_table, kept=None):
     """Tokens packed into other pages, in every cache of `caches`: token j < kept[b] (None: all) of a new sequence is token index[b, j]
-    (B, n) int32 of sequence b, in any order; new_table (B, blocks) int32 names the pages that are written, none of which may be
-    among those that table names. A new block's scale is the largest its tokens come with, q' = rint(q * (s_old / s)): a
+    (B, n) int32 of sequence b, in any order; new_table (B, blocks) int32 names the pages that are written, each of them once and none
+    that table names. A new block's scale is the largest its tokens come with, q' = rint(q * (s_old / s)): a
     token that comes with that scale keeps its integers, any other is off by at most half of it more. Positions turned into
     the keys stay what they were. kv8_reserve gives the pages, kv8_free takes the old ones back."""
     return _bind.kv8_compact(caches, table, lens, index, new_table, kept)
@@ -531,9 +531,10 @@ def cross_attention(q, k, v, heads, kv_heads=None, lens=None, mask=None, scale=N
     contiguous rows (column views of wider tensors will do: rows 16-byte aligned); D a multiple of 8, at most 128. The S batches b * S ..
     of q read the states of sequence b (S candidates that share them); query head h reads key head h // (heads / kv_heads). A
     state j is there if j < lens[b] ((B,) int32; None: all N) and mask[b, j] ((B, N) bool; None: yes); what lies elsewhere in k
-    and v has no effect. scale None: D^-0.5. Scores scale q k
-    may be up to 2^23 in size; a row whose largest is further out is undefined (device_error reports flag 2). Returns out (B * S, T, heads * D) of q's type (q itself, or memory apart from the inputs); rows that see no state are zero. It
-    forms no gradient and refuses tensors that ask for one or carry a tangent; the same call gives the same bits every time."""
+    and v has no effect. scale None: D^-0.5. Scores scale q k of states that are there may be up to 2^23 in size; rows with others are
+    undefined (where the largest is one, device_error reports flag 2). Returns out (B * S, T, heads * D) of q's type (q itself, or memory
+    apart from the inputs); rows that see no state are zero. It forms no gradient and refuses tensors that ask for one or carry a
+    tangent; the same call gives the same bits every time."""
     return _bind.cross_attention(q, k, v, heads, kv_heads, lens, mask, scale, out)
 
 
