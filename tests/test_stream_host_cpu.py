@@ -250,3 +250,50 @@ def test_the_command_has_positions_for_all_its_frames(monkeypatch, window):
         with pytest.raises(KeyboardInterrupt):
             stream.main(['--frames', frames, '--window', window])
     assert made == [5000, 4096]
+
+
+@pytest.mark.parametrize('seed', range(12))
+def test_random_histories(monkeypatch, seed):
+    """Frames, forks and keeps in pools of any size: the count is never below what is there, a frame is refused only where the longest memory
+    leaves no room, pages are counted, and the flag is raised where a robot was not served."""
+    import random
+    rng = random.Random(seed)
+    robots, most = rng.choice((1, 2, 5)), rng.choice((N, 3 * N + 5, 700))
+    m, K = memory(monkeypatch, robots, most, pages=rng.choice((4, 9, 20, 60)))
+    refused = 0
+    for _ in range(60):
+        K.flag = 0
+        before, n = m.lens.tolist(), rng.choice((0, 1, 64, 100, 200, 500))
+        kind = rng.choice(('frame', 'frame', 'frame', 'fork', 'keep', 'recent', 'replay', 'forget'))
+        if kind == 'frame':
+            count = ints([rng.randint(0, N) for _ in range(robots)]) if rng.random() < 0.5 else None
+            try:
+                m.begin_frame(count=count)
+            except K.TcqError:
+                refused += 1
+                assert max(before) + N > most and m.lens.tolist() == before
+                continue
+            want = [N] * robots if count is None else count.tolist()
+            assert m.served.tolist() == [a - b == w for a, b, w in zip(m.lens.tolist(), before, want)]
+            assert m.served.all() == (K.flag == 0)
+        elif kind == 'fork':
+            m.fork(ints([rng.randrange(-1, robots) for _ in range(robots)]))
+        elif kind == 'keep' and n:
+            n = min(n, m.table.shape[1] * 64)
+            m.keep(torch.randint(0, 50, (robots, n), dtype=torch.int32), ints([rng.randint(-1, n) for _ in range(robots)]))
+        elif kind == 'recent':
+            m.keep_recent(n)
+            if K.flag == 0:
+                assert m.lens.tolist() == [min(n, b) for b in before]
+        elif kind == 'replay':
+            try:
+                m.reserve(kept=n)
+            except K.TcqError:
+                continue
+            m.replay(lambda: (m.keep_recent(n), m.begin_frame()))
+        elif kind == 'forget':
+            m.forget()
+        named(m)
+        assert m.lens.max() <= m.tokens <= most
+        assert all(blocks == -(-length // 64) for blocks, length in zip((m.table >= 0).sum(1).tolist(), m.lens.tolist()))
+    assert refused or most > N
